@@ -40,7 +40,7 @@ HIP_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 
-HIP_SOURCES = ["quant.hip", "gemm.hip", "gemm_blockscale.hip", "moe.hip", "moe_blockscale.hip", "routing.hip",
+HIP_SOURCES = ["gemm_fused.hip", "quant.hip", "gemm.hip", "gemm_blockscale.hip", "moe.hip", "moe_blockscale.hip", "routing.hip",
                "norm_quant.hip"]
 CPP_SOURCES = ["hkq_error.cpp"]
 # Per-source code generation options. The block-scale GEMM promotes every
@@ -62,6 +62,9 @@ MODULES = {
     "batched_gemm_bf16_tk": "bind_batched_gemm_bf16.cpp",
     "fused_gemm_a8w8_blockscale_mul_add_tk": "bind_fused_gemm_a8w8_blockscale_mul_add.cpp",
     "fused_gemm_a8w8_blockscale_a16w16_tk": "bind_fused_gemm_a8w8_blockscale_a16w16.cpp",
+    "fused_gemm_a8w8_epilogue_tk": "bind_fused_gemm_a8w8_epilogue.cpp",
+    "fused_gemm_a16w16_epilogue_tk": "bind_fused_gemm_a16w16_epilogue.cpp",
+    "gated_ffn_tk": "bind_gated_ffn.cpp",
     "moe_op_gemm_a8w8_tk": "bind_moe_op_gemm_a8w8.cpp",
     "moe_op_gemm_a8w8_blockscale_tk": "bind_moe_op_gemm_a8w8_blockscale.cpp",
     "moe_op_mxfp4_tk": "bind_moe_op_mxfp4.cpp",

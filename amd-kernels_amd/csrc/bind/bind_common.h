@@ -103,6 +103,16 @@ inline Workspace workspace(size_t bytes, py::object like) {
     return w;
 }
 
+// HKQ_ACT_* of an activation's name.
+inline int activation(const std::string& act) {
+    if (act == "none") return HKQ_ACT_NONE;
+    if (act == "relu") return HKQ_ACT_RELU;
+    if (act == "silu") return HKQ_ACT_SILU;
+    if (act == "gelu_tanh") return HKQ_ACT_GELU_TANH;
+    if (act == "gelu") return HKQ_ACT_GELU;
+    throw py::value_error("act must be one of none, relu, silu, gelu_tanh, gelu; got '" + act + "'");
+}
+
 inline void check(int rc, const char* what) {
     if (rc != 0) throw std::runtime_error(std::string(what) + ": " + hkq_last_error() + " (code " + std::to_string(rc) + ")");
 }

@@ -92,6 +92,58 @@ inline void gemm_bf16(py::object A, py::object B, py::object C, const char* what
           what);
 }
 
+// The fused epilogue of both dense forms: C = act(product * scales + bias) +
+// residual; bias bf16 [N], residual bf16 [M, N] (may be C), either None;
+// a_scale / b_scale as gemm_a8w8 (FP8) or null objects (bf16).
+inline void gemm_epilogue(bool fp8, py::object A, py::object B, py::object a_scale, py::object b_scale, py::object C,
+                          py::object bias, py::object residual, const std::string& act, float alpha, const char* what) {
+    auto a = view(A, "A"), b = view(B, "B"), c = view(C, "C");
+    if (fp8) {
+        expect_dtype(a, "A", {kFP8, kU8});
+        expect_dtype(b, "B", {kFP8, kU8});
+    } else {
+        expect_dtype(a, "A", {kBF16});
+        expect_dtype(b, "B", {kBF16});
+    }
+    expect_dtype(c, "C", {kBF16});
+    const int64_t lda = row_stride(a, "A"), ldb = row_stride(b, "B"), ldc = row_stride(c, "C");
+    const int64_t M = a.dim(0), K = a.dim(1), N = b.dim(0);
+    expect(b.dim(1) == K, "A and B must have the same K");
+    expect(c.dim(0) == M && c.dim(1) == N, "C must be [M, N]");
+    const void *pb = nullptr, *pr = nullptr;
+    const float *sa = nullptr, *sb = nullptr;
+    int64_t ldr = 0;
+    if (fp8) {
+        auto x = view(a_scale, "a_scale"), y = view(b_scale, "b_scale");
+        expect_dtype(x, "a_scale", {kF32});
+        expect_dtype(y, "b_scale", {kF32});
+        expect(x.numel() == M && x.contiguous(), "a_scale must be contiguous with M elements");
+        expect(y.numel() == N && y.contiguous(), "b_scale must be contiguous with N elements");
+        sa = (const float*)x.ptr;
+        sb = (const float*)y.ptr;
+    }
+    if (!bias.is_none()) {
+        auto v = view(bias, "bias");
+        expect_dtype(v, "bias", {kBF16});
+        expect(v.numel() == N && v.contiguous(), "bias must be contiguous with N elements");
+        pb = (const void*)v.ptr;
+    }
+    if (!residual.is_none()) {
+        auto v = view(residual, "residual");
+        expect_dtype(v, "residual", {kBF16});
+        ldr = row_stride(v, "residual");
+        expect(v.dim(0) == M && v.dim(1) == N, "residual must be [M, N]");
+        pr = (const void*)v.ptr;
+    }
+    const int id = activation(act);
+    Workspace ws = workspace(fp8 ? hkq_gemm_a8w8_workspace(M, N, K) : hkq_gemm_bf16_workspace(M, N, K), A);
+    check(fp8 ? hkq_gemm_a8w8_epilogue((const void*)a.ptr, (const void*)b.ptr, sa, sb, pb, pr, (void*)c.ptr, M, N, K, lda,
+                                       ldb, ldr, ldc, id, alpha, ws.ptr, ws.bytes, current_stream())
+              : hkq_gemm_bf16_epilogue((const void*)a.ptr, (const void*)b.ptr, pb, pr, (void*)c.ptr, M, N, K, lda, ldb, ldr,
+                                       ldc, id, alpha, ws.ptr, ws.bytes, current_stream()),
+          what);
+}
+
 // A batch of row-major matrices: the reference's 4-D (1, B, R, C) layout or a
 // plain (B, R, C) tensor, last dimension contiguous.
 struct Batched {

@@ -64,7 +64,7 @@ int hkq_gemm_a8w8_ws(const void* A, const void* B, const float* sa, const float*
     p.sb = sb;
     p.M = (int)M; p.N = (int)N; p.K = (int)K; p.kbytes = (int)K;
     p.lda = lda; p.ldb = ldb; p.ldc = ldc;
-    return launch_dense<MODE_A8W8>(p, workspace, workspace_bytes, stream);
+    return launch_dense<PlainOp, MODE_A8W8>(p, workspace, workspace_bytes, stream);
 }
 
 int hkq_gemm_a8w8(const void* A, const void* B, const float* sa, const float* sb, void* C, int64_t M, int64_t N,
@@ -157,7 +157,7 @@ int hkq_gemm_mxfp4_ws(const void* A, const void* As, const void* B, const void* 
     p.M = (int)M; p.N = (int)N; p.K = (int)K; p.kbytes = (int)(K / 2);
     p.lda = lda; p.ldb = ldb; p.ldc = ldc;
     p.lsa = ldsa; p.lsb = ldsb;
-    return launch_dense<MODE_MXFP4>(p, workspace, workspace_bytes, stream);
+    return launch_dense<PlainOp, MODE_MXFP4>(p, workspace, workspace_bytes, stream);
 }
 
 int hkq_gemm_mxfp4(const void* A, const void* As, const void* B, const void* Bs, void* C, int64_t M, int64_t N,
@@ -196,7 +196,7 @@ int hkq_batched_gemm_a8w8(const void* A, const void* B, const float* sa, const f
     p.bias = static_cast<const uint16_t*>(bias);
     p.bs_a = batch_stride_a; p.bs_b = batch_stride_b; p.bs_c = batch_stride_c;
     p.bs_sa = batch_stride_sa; p.bs_sb = batch_stride_sb; p.bs_bias = batch_stride_bias;
-    return launch_dense<MODE_A8W8>(p, nullptr, 0, stream);
+    return launch_dense<PlainOp, MODE_A8W8>(p, nullptr, 0, stream);
 }
 
 size_t hkq_gemm_bf16_workspace(int64_t M, int64_t N, int64_t K) {
@@ -231,7 +231,7 @@ int hkq_batched_gemm_bf16(const void* A, const void* B, const void* bias, void* 
     p.bias = static_cast<const uint16_t*>(bias);
     p.bs_a = 2 * batch_stride_a; p.bs_b = 2 * batch_stride_b; p.bs_c = batch_stride_c;
     p.bs_bias = batch_stride_bias;
-    return launch_dense<MODE_BF16>(p, workspace, workspace_bytes, stream);
+    return launch_dense<PlainOp, MODE_BF16>(p, workspace, workspace_bytes, stream);
 }
 
 int hkq_gemm_bf16(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,

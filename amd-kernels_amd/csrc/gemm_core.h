@@ -124,6 +124,29 @@ __device__ __forceinline__ v2i lds_read_tr8(const HKQ_LDS uint8_t* p) {
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<HKQ_LDS v2i*>(const_cast<HKQ_LDS uint8_t*>(p)));
 }
 
+// bf16 operands that lie with their rows (or columns) contiguous and K across
+// memory rows: a K-tile is 64 rows of K, each holding the tile's COLS rows of
+// the operand (COLS * 2 bytes). Logical 16-byte chunk c of row r lives at
+// physical chunk c ^ (4 * (r & 3)): 32 lanes of a transposed read touch 4
+// consecutive rows at 64 aligned bytes each, which then fall on the 4 quarters
+// of the 64 banks.
+template <int COLS>
+struct KTileT16 {
+    static constexpr int ROW = COLS * 2, ROWS = 64;
+    static constexpr int ROWS_PER_LOAD = 1024 / ROW;  // rows written by one wave-wide 16-byte LDS-direct load
+    __device__ static __forceinline__ int phys(int r, int c) { return c ^ (4 * (r & 3)); }
+};
+
+// ds_read_b64_tr_b16: in each group of 16 lanes, lane j receives 16-bit word
+// (j & 3) of the 8-byte pieces addressed by lanes 4i + (j >> 2), i = 0..3, as
+// its words i. With lanes 4i .. 4i + 3 addressing the four pieces of row i's 16
+// columns, lane j receives column j of 4 consecutive rows.
+typedef short v4s __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v2i lds_read_tr16(const HKQ_LDS uint8_t* p) {
+    return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       reinterpret_cast<HKQ_LDS v4s*>(const_cast<HKQ_LDS uint8_t*>(p))));
+}
+
 template <bool FP4, int OPA, int OPB>
 __device__ __forceinline__ v16f mfma_sel(const v8i& a, const v8i& b, const v16f& c, int sa, int sb) {
     if (FP4) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, OPA, sa, OPB, sb);

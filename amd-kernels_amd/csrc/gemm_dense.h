@@ -7,6 +7,7 @@
 #pragma once
 #include <algorithm>
 #include <cstdlib>
+#include <type_traits>
 
 #include "gemm_kgroup.h"
 #include "gemm_stream.h"
@@ -64,6 +65,97 @@ __device__ __forceinline__ float4 bias4(const DenseParams& p, int n) {
                        bf16_to_f32(b.y >> 16));
 }
 
+// What a workgroup does besides the plain product, as a template argument of
+// the kernels:
+//   FUSED   bias, activation and residual in the epilogue (FusedParams);
+//   GATED   the columns of a tile are gate and up rows of the same features of
+//           one weight (gemm_mainloop); the epilogue forms act(gate) * up;
+//   AT, BT  the operand lies with its rows contiguous and K across memory rows
+//           (bf16; p.kbytes counts 2 bytes per value of K, rounded up to whole
+//           K-tiles, p.K the rows that there are).
+struct PlainOp {
+    using Params = DenseParams;
+    static constexpr bool FUSED = false, GATED = false, AT = false, BT = false;
+};
+
+// Activations: 0 max(v, lo) (lo -inf: none, 0: ReLU), 1 v * logistic(v (c1 + c3
+// v^2)) (SiLU with alpha: c1 = alpha; tanh GELU, whose 0.5 (1 + tanh z) is the
+// logistic function of 2z), 2 v * Phi(v), Phi the normal distribution function
+// (GELU). c1 and c3 hold a factor -log2(e).
+struct ActParams {
+    int form;
+    float lo, c1, c3;
+};
+
+// Phi(v) by Abramowitz & Stegun 7.1.26: erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2),
+// t = 1 / (1 + 0.3275911 z), z >= 0, absolute error at most 1.5e-7. *density:
+// exp(-v^2 / 2).
+__device__ __forceinline__ float normal_cdf(float v, float* density) {
+    const float e = __builtin_amdgcn_exp2f(v * v * -0.72134752f);
+    const float k = __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fabsf(v), 0.23164189f, 1.0f));
+    float a = __builtin_fmaf(k, 0.530702715f, -0.726576014f);
+    a = __builtin_fmaf(k, a, 0.710706871f);
+    a = __builtin_fmaf(k, a, -0.142248368f);
+    a = __builtin_fmaf(k, a, 0.127414796f);
+    const float tail = a * k * e;  // erfc(|v| / sqrt 2) / 2
+    *density = e;
+    return v < 0.0f ? tail : 1.0f - tail;
+}
+
+__device__ __forceinline__ float logistic_arg(const ActParams& a, float v) {
+    // v^2 is bounded only so that c3 = 0 never meets an infinity; the logistic
+    // function is long constant there
+    return v * __builtin_fmaf(a.c3, min_num(v * v, 1e8f), a.c1);
+}
+
+__device__ __forceinline__ float act1(const ActParams& a, float v) {
+    if (a.form == 0) return v < a.lo ? a.lo : v;
+    if (a.form == 1) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(logistic_arg(a, v)));
+    float d;
+    return v * normal_cdf(v, &d);
+}
+
+// The activation of four values: one uniform branch for all of them.
+__device__ __forceinline__ float4 act4(const ActParams& a, float4 v) {
+    if (a.form == 0) {
+        return make_float4(v.x < a.lo ? a.lo : v.x, v.y < a.lo ? a.lo : v.y, v.z < a.lo ? a.lo : v.z, v.w < a.lo ? a.lo : v.w);
+    }
+    return make_float4(act1(a, v.x), act1(a, v.y), act1(a, v.z), act1(a, v.w));
+}
+
+struct FusedParams : DenseParams {
+    ActParams act;
+    // FUSED: residual bf16 [M, N] (nullptr: none), rows ldr elements apart; r16:
+    // they are 16-byte aligned
+    const uint16_t* residual;
+    int64_t ldr;
+    int r16;
+    // GATED: B holds F gate and F up rows, the up rows from Bu, both p.ldb bytes
+    // apart; N = 2F. C is [M, F]. Column scales (A8W8) in the weight's row order:
+    // feature f's at f and F + f, or (interleaved) 2f and 2f + 1. Y: nullptr, or
+    // bf16 [M, 2F] in that order, the scaled sums themselves; y16: its rows are
+    // 16-byte aligned.
+    const uint8_t* Bu;
+    int F, interleaved, y16;
+    uint16_t* Y;
+    int64_t ldy;
+};
+__device__ __forceinline__ const FusedParams& batch_slice(const FusedParams& p) { return p; }
+
+struct FusedOp {
+    using Params = FusedParams;
+    static constexpr bool FUSED = true, GATED = false, AT = false, BT = false;
+};
+struct GatedOp {
+    using Params = FusedParams;
+    static constexpr bool FUSED = false, GATED = true, AT = false, BT = false;
+};
+template <bool AT_, bool BT_>
+struct TransOp {
+    using Params = DenseParams;
+    static constexpr bool FUSED = false, GATED = false, AT = AT_, BT = BT_;
+};
+
 // Tile geometry of the dense GEMMs: 256 x 256 tiles computed by 4 waves of
 // 128 x 128 (whole tiles) or 64 x 128 (M halves of a tile, 128 x 256). K-tiles
 // are 128 bytes per row (whole 128-byte lines per row and load: half the
@@ -90,8 +182,8 @@ constexpr int dense_lds() { return dense_ring_lds<MODE, KTB>() + (MODE == MODE_A
 // K loop of one (WM*TM*32) x (WN*TN*32) block of C at (m0, n0) over K-tiles
 // [kt0, kt1): the operand sources start kt0 K-tiles into the rows, so the
 // loop (and its scale-block schedule) counts K-tiles from 0.
-template <int MODE, int WM, int WN, int TM, int TN, int KTB, int NS = dense_ns<KTB>()>
-__device__ __forceinline__ void dense_kloop(const DenseParams& p, int m0, int n0, int kt0, int kt1, HKQ_LDS uint8_t* smem,
+template <class Op, int MODE, int WM, int WN, int TM, int TN, int KTB, int NS = dense_ns<KTB>()>
+__device__ __forceinline__ void dense_kloop(const typename Op::Params& p, int m0, int n0, int kt0, int kt1, HKQ_LDS uint8_t* smem,
                                             v16f (&acc)[TN][TM]) {
     using Cfg = DenseCfg<MODE, WM, WN, TM, TN, KTB>;
     constexpr int NW = Cfg::NW, BM = Cfg::BM, BN = Cfg::BN;
@@ -116,16 +208,214 @@ __device__ __forceinline__ void dense_kloop(const DenseParams& p, int m0, int n0
     src.lsa = p.lsa;
     src.lsb = p.lsb;
     src.KT = kt1 - kt0;
-    const auto a_off = dense_offs<NW, KTB, Cfg::LA>(wave, lane, p.lda);
-    const auto b_off = dense_offs<NW, KTB, Cfg::LB>(wave, lane, p.ldb);
-    gemm_mainloop<MODE, WM, WN, TM, TN, KTB, NS>(src, a_off, b_off, smem, lane, wave, acc);
+    auto a_off = dense_offs<NW, KTB, Cfg::LA>(wave, lane, p.lda);
+    auto b_off = dense_offs<NW, KTB, Cfg::LB>(wave, lane, p.ldb);
+    if constexpr (Op::GATED) {
+        // the tile's features [n0 / 2, n0 / 2 + BN / 2): gate and up rows alike
+        const int f0 = n0 / 2, rows_f = min(p.F - f0, BN / 2);
+        src.b = p.B + (int64_t)f0 * p.ldb + kb0;
+        src.b2 = p.Bu + (int64_t)f0 * p.ldb + kb0;
+        src.b_bytes = min((int64_t)(rows_f - 1) * p.ldb + p.kbytes - kb0, (int64_t)0x7FFFFFFF);
+        b_off = dense_offs_gated<NW, KTB, Cfg::LB, TN>(wave, lane, p.ldb);
+    }
+    // rows of K across memory: columns m0 / n0 of every row from kt0 K-tiles on
+    if constexpr (Op::AT) {
+        src.a = p.A + (int64_t)kt0 * 64 * p.lda + (int64_t)m0 * 2;
+        src.a_bytes = (int64_t)(p.K - kt0 * 64 - 1) * p.lda + rows_a * 2;
+        src.a_kstep = 64 * p.lda;
+        a_off = dense_offs_t16<NW, Cfg::LA, BM>(wave, lane, p.lda);
+    }
+    if constexpr (Op::BT) {
+        src.b = p.B + (int64_t)kt0 * 64 * p.ldb + (int64_t)n0 * 2;
+        src.b_bytes = (int64_t)(p.K - kt0 * 64 - 1) * p.ldb + rows_b * 2;
+        src.b_kstep = 64 * p.ldb;
+        b_off = dense_offs_t16<NW, Cfg::LB, BN>(wave, lane, p.ldb);
+    }
+    gemm_mainloop<MODE, WM, WN, TM, TN, KTB, NS, Op::BT, Op::AT, Op::GATED>(src, a_off, b_off, smem, lane, wave, acc);
+}
+
+// A staged tile to C: the wave's TM*32 rows of COLS bf16 columns, PITCH bytes
+// apart at ep, go to rows [mw, ..) and columns [nw, ..) of C inside M x N.
+template <int TM, int COLS, int PITCH>
+__device__ __forceinline__ void store_staged(const HKQ_LDS uint8_t* ep, int lane, uint16_t* C, int64_t ldc, int M, int N,
+                                             int mw, int nw, bool c16) {
+    constexpr int SEGS = COLS * 2 / 16, ROWS_PER_PASS = 64 / SEGS, PASSES = TM * 32 / ROWS_PER_PASS;
+    constexpr int BATCH = PASSES < 8 ? PASSES : 8;
+    int ln = lane;  // opaque copy: keeps rl / seg out of the kernel's prologue
+    asm volatile("" : "+v"(ln));
+    const int rl = ln / SEGS, seg = ln % SEGS;
+    const int n = nw + seg * 8;
+#pragma unroll
+    for (int b = 0; b < PASSES; b += BATCH) {
+        v4i v[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) v[k] = lds_read16(ep + ((b + k) * ROWS_PER_PASS + rl) * PITCH + seg * 16);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int m = mw + (b + k) * ROWS_PER_PASS + rl;
+            if (m < M) store_piece_bf16(C + (int64_t)m * ldc + n, v[k], N - n, c16);
+        }
+    }
+}
+
+// Residual of a wave's sub-tile in the accumulators' layout, for tiles small
+// enough to hold it in registers from before the K loop (nothing waits on it
+// after the sums).
+template <class Op, int TM, int TN>
+struct EpiResidual {
+    static constexpr bool HELD = Op::FUSED && (TM == 1 || TM * TN <= 2);
+    v2i v[HELD ? TN : 1][4][HELD ? TM : 1];
+    __device__ __forceinline__ void load(const typename Op::Params& p, int lane, int mw, int nw) {
+        if constexpr (HELD) {
+            const int khalf = lane >> 5;
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int j = 0; j < TM; ++j) {
+                        const int m = mw + j * 32 + (lane & 31), n = nw + i * 32 + 8 * g + 4 * khalf;
+                        v[i][g][j] = v2i{0, 0};
+                        if (p.residual && m < p.M && n < p.N)
+                            v[i][g][j] = *reinterpret_cast<const v2i*>(p.residual + (int64_t)m * p.ldr + n);
+                    }
+        }
+    }
+};
+__device__ __forceinline__ float4 add_bf16x4(float4 v, const v2i& r) {
+    const uint32_t lo = (uint32_t)r[0], hi = (uint32_t)r[1];
+    return make_float4(v.x + bf16_to_f32(lo & 0xFFFF), v.y + bf16_to_f32(lo >> 16), v.z + bf16_to_f32(hi & 0xFFFF),
+                       v.w + bf16_to_f32(hi >> 16));
+}
+
+// FUSED epilogue: act(sums * scales + bias) + residual in fp32, one rounding,
+// staged and stored as store_tile_bf16 does. A large tile's residual comes
+// through the staging area: whole row pieces (16 bytes per lane, full lines)
+// are put where the results will go, and each lane replaces its own values.
+// Read straight in the accumulators' layout, 32 rows x 8 bytes per load, they
+// would cost a line request per row and load.
+template <class Op, int TM, int TN, typename RowScale, typename ColScale4>
+__device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], const EpiResidual<Op, TM, TN>& res,
+                                                 HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw,
+                                                 RowScale row_scale, ColScale4 col_scale4) {
+    constexpr int PITCH = TN * 32 * 2 + 16;
+    constexpr bool HELD = EpiResidual<Op, TM, TN>::HELD;
+    HKQ_LDS uint8_t* ep = smem + wave * (TM * 32) * PITCH;
+    const int khalf = lane >> 5;
+    const bool staged = !HELD && p.residual != nullptr;
+    if (staged) {
+        constexpr int SEGS = TN * 4, ROWS_PER_PASS = 64 / SEGS, PASSES = TM * 32 / ROWS_PER_PASS;
+        constexpr int BATCH = PASSES < 16 ? PASSES : 16;
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int rl = ln / SEGS, seg = ln % SEGS, left = p.N - nw - seg * 8;
+        const uint16_t* src = p.residual + (int64_t)(mw + rl) * p.ldr + nw + seg * 8;
+#pragma unroll
+        for (int b = 0; b < PASSES; b += BATCH) {
+            v4i v[BATCH];
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const int r = (b + k) * ROWS_PER_PASS;
+                const uint16_t* at = src + (int64_t)r * p.ldr;
+                v[k] = v4i{0, 0, 0, 0};
+                if (mw + r + rl < p.M) {
+                    if (left >= 8 && p.r16) {
+                        v[k] = *reinterpret_cast<const v4i*>(at);
+                    } else if (left > 0) {
+                        const v2i lo = *reinterpret_cast<const v2i*>(at);
+                        const v2i hi = left >= 8 ? *reinterpret_cast<const v2i*>(at + 4) : v2i{0, 0};
+                        v[k] = v4i{lo[0], lo[1], hi[0], hi[1]};
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k)
+                *reinterpret_cast<HKQ_LDS v4i*>(ep + ((b + k) * ROWS_PER_PASS + rl) * PITCH + seg * 16) = v[k];
+        }
+    }
+    float rs[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) rs[j] = row_scale(j);
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int nl = i * 32 + 8 * g + 4 * khalf;
+            const float4 cs = col_scale4(i, g), cb = bias4(p, nw + nl);
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                const float a = rs[j];
+                float4 v = act4(p.act, make_float4(acc[i][j][4 * g + 0] * a * cs.x + cb.x, acc[i][j][4 * g + 1] * a * cs.y + cb.y,
+                                                   acc[i][j][4 * g + 2] * a * cs.z + cb.z, acc[i][j][4 * g + 3] * a * cs.w + cb.w));
+                HKQ_LDS v2i* at = reinterpret_cast<HKQ_LDS v2i*>(ep + (j * 32 + (lane & 31)) * PITCH + nl * 2);
+                if constexpr (HELD) {
+                    if (p.residual) v = add_bf16x4(v, res.v[i][g][j]);
+                } else {
+                    if (staged) v = add_bf16x4(v, v2i(*at));
+                }
+                *at = v2i{(int)pk_bf16(v.x, v.y), (int)pk_bf16(v.z, v.w)};
+            }
+        }
+    store_staged<TM, TN * 32, PITCH>(ep, lane, p.C, p.ldc, p.M, p.N, mw, nw, p.c16 != 0);
+}
+
+// GATED epilogue: n-tiles i and i + TN / 2 of a lane hold gate and up of the same
+// features; C gets act(gate) * up, Y (if kept) both. fw: the wave's first
+// feature. The halves of Y go out one after the other through the same staging
+// area (a wave's LDS operations complete in order); interleaved, as pairs.
+template <int TM, int TN, typename RowScale, typename ColScale4>
+__device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], HKQ_LDS uint8_t* smem, int wave,
+                                                 int lane, int mw, int fw, RowScale row_scale, ColScale4 col_scale4) {
+    constexpr int HN = TN / 2, PITCH = HN * 64 + 16, PITCH_Y = TN * 64 + 16;
+    HKQ_LDS uint8_t* ep = smem + wave * (TM * 32) * PITCH_Y;
+    const int khalf = lane >> 5;
+    float rs[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) rs[j] = row_scale(j);
+    auto value = [&](int i, int j, int g) {
+        const float4 cs = col_scale4(i, g);
+        const float a = rs[j];
+        return make_float4(acc[i][j][4 * g + 0] * a * cs.x, acc[i][j][4 * g + 1] * a * cs.y, acc[i][j][4 * g + 2] * a * cs.z,
+                           acc[i][j][4 * g + 3] * a * cs.w);
+    };
+    auto each = [&](auto put) {
+#pragma unroll
+        for (int i = 0; i < HN; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int j = 0; j < TM; ++j) put(i, g, j, j * 32 + (lane & 31), i * 32 + 8 * g + 4 * khalf);
+    };
+    each([&](int i, int g, int j, int r, int n) {
+        const float4 u = value(i + HN, j, g), a = act4(p.act, value(i, j, g));
+        *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) = v2i{(int)pk_bf16(a.x * u.x, a.y * u.y), (int)pk_bf16(a.z * u.z, a.w * u.w)};
+    });
+    store_staged<TM, HN * 32, PITCH>(ep, lane, p.C, p.ldc, p.M, p.F, mw, fw, p.c16 != 0);
+    if (!p.Y) return;
+    if (p.interleaved) {
+        each([&](int i, int g, int j, int r, int n) {
+            const float4 a = value(i, j, g), u = value(i + HN, j, g);
+            *reinterpret_cast<HKQ_LDS v4i*>(ep + r * PITCH_Y + n * 4) =
+                v4i{(int)pk_bf16(a.x, u.x), (int)pk_bf16(a.y, u.y), (int)pk_bf16(a.z, u.z), (int)pk_bf16(a.w, u.w)};
+        });
+        store_staged<TM, TN * 32, PITCH_Y>(ep, lane, p.Y, p.ldy, p.M, 2 * p.F, mw, 2 * fw, p.y16 != 0);
+        return;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        each([&](int i, int g, int j, int r, int n) {
+            const float4 v = value(i + half * HN, j, g);
+            *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) = v2i{(int)pk_bf16(v.x, v.y), (int)pk_bf16(v.z, v.w)};
+        });
+        store_staged<TM, HN * 32, PITCH>(ep, lane, p.Y + (half ? p.F : 0), p.ldy, p.M, p.F, mw, fw, p.y16 != 0);
+    }
 }
 
 // One (TM*64) x 256 block of C: rows [m0, m0 + TM*64) of tile (tm, tn) of the
 // 256 x 256 tile grid, starting `half` * 128 rows into the tile, on an NS-stage
 // K-tile ring (the tile's row and column scales follow the ring).
-template <int MODE, int TM, int KTB, int NS = dense_ns<KTB>()>
-__device__ __forceinline__ void dense_block(const DenseParams& p, int tm, int tn, int half, HKQ_LDS uint8_t* smem) {
+template <class Op, int MODE, int TM, int KTB, int NS = dense_ns<KTB>()>
+__device__ __forceinline__ void dense_block(const typename Op::Params& p, int tm, int tn, int half, HKQ_LDS uint8_t* smem) {
     constexpr int WAVES_M = DENSE_WAVES_M, WAVES_N = DENSE_WAVES_N, TN = DENSE_TN;
     using Cfg = DenseCfg<MODE, WAVES_M, WAVES_N, TM, TN, KTB>;
     constexpr int BM = Cfg::BM, BN = Cfg::BN;
@@ -149,11 +439,18 @@ __device__ __forceinline__ void dense_block(const DenseParams& p, int tm, int tn
         const float* sa = static_cast<const float*>(p.sa) + m0;
         const float* sb = static_cast<const float*>(p.sb) + n0;
         lds_load4(sa, (uint32_t)rows_a * 4u, scl + wave * 256, (uint32_t)(wave * 64 + lane) * 4u);
-        lds_load4(sb, (uint32_t)rows_b * 4u, scl + DENSE_BM * 4 + wave * 256, (uint32_t)(wave * 64 + lane) * 4u);
+        if constexpr (Op::GATED) {
+            // tile column c of wave column c / 128: a gate column where c % 128 < 64
+            const int c = wave * 64 + lane, f = n0 / 2 + gated_row<TN>(c), up = c % (TN * 32) >= TN * 16;
+            lds_load4(p.sb, (uint32_t)p.F * 8u, scl + DENSE_BM * 4 + wave * 256,
+                      f < p.F ? (uint32_t)(p.interleaved ? 2 * f + up : f + up * p.F) * 4u : OOB);
+        } else {
+            lds_load4(sb, (uint32_t)rows_b * 4u, scl + DENSE_BM * 4 + wave * 256, (uint32_t)(wave * 64 + lane) * 4u);
+        }
     }
 
     v16f acc[TN][TM];
-    dense_kloop<MODE, WAVES_M, WAVES_N, TM, TN, KTB, NS>(p, m0, n0, 0, p.kbytes / KTB, smem, acc);
+    dense_kloop<Op, MODE, WAVES_M, WAVES_N, TM, TN, KTB, NS>(p, m0, n0, 0, p.kbytes / KTB, smem, acc);
 
     // Epilogue (scales of A8W8 applied in registers; MXFP4 has none left)
     const int mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
@@ -169,7 +466,11 @@ __device__ __forceinline__ void dense_block(const DenseParams& p, int tm, int tn
         }
         return make_float4(1.f, 1.f, 1.f, 1.f);
     };
-    if (p.bias)
+    if constexpr (Op::FUSED)
+        fused_store_tile<Op, TM, TN>(p, acc, EpiResidual<Op, TM, TN>{}, smem, wave, lane, mw, nw, row_scale, col_scale4);
+    else if constexpr (Op::GATED)
+        gated_store_tile<TM, TN>(p, acc, smem, wave, lane, mw, nw / 2, row_scale, col_scale4);
+    else if (p.bias)
         store_tile_bf16<TM, TN>(acc, smem, wave, lane, p.C, p.ldc, p.M, p.N, mw, nw, p.c16 != 0, row_scale, col_scale4,
                                 [&](int i, int g) { return bias4(p, nw + i * 32 + 8 * g + 4 * khalf); });
     else
@@ -183,11 +484,11 @@ __device__ __forceinline__ void dense_block(const DenseParams& p, int tm, int tn
 // dispatcher assigns workgroups round-robin) computes half (v >> 3) & 1 of tile
 // n_whole + 8 * (v >> 4) + (v & 7), so both halves of a tile run on one XCD.
 // Tile ids then go through tile_coords' XCD-aware order.
-template <int MODE, int KTB>
-__global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_gemm_kernel(const DenseParams pb) {
+template <class Op, int MODE, int KTB>
+__global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_gemm_kernel(const typename Op::Params pb) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
     HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
-    const DenseParams p = batch_slice(pb);
+    const typename Op::Params p = batch_slice(pb);
     const int u = blockIdx.x;
     int whole = -1, t = -1, half = 0;
     if (u < p.n_whole) {
@@ -201,10 +502,10 @@ __global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_g
     int tm, tn;
     if (whole >= 0) {
         tile_coords(whole, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-        dense_block<MODE, DENSE_TM, KTB>(p, tm, tn, 0, smem);
+        dense_block<Op, MODE, DENSE_TM, KTB>(p, tm, tn, 0, smem);
     } else {
         tile_coords(p.n_whole + t, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-        dense_block<MODE, DENSE_TM / 2, KTB>(p, tm, tn, half, smem);
+        dense_block<Op, MODE, DENSE_TM / 2, KTB>(p, tm, tn, half, smem);
     }
 }
 
@@ -352,13 +653,13 @@ __global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_s
     int tm = 0, tn = 0;
     if (has_half) tile_coords(p.n_whole + t, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
     if (half_first && has_half) {
-        dense_block<MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
+        dense_block<PlainOp, MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
         // the stream's first loads overwrite the half tile's staging: every
         // wave's LDS reads are done first (its C stores may still drain)
         lds_barrier();
     }
     if (mine > 0) dense_stream<MODE, DENSE_TM>(p, mine, b, G, 0, smem);
-    if (!half_first && has_half) dense_block<MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
+    if (!half_first && has_half) dense_block<PlainOp, MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
 }
 
 // ---------------------------------------------------------------------------
@@ -377,11 +678,11 @@ __global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_s
 // The scales of a wave's (TM*32) x (TN*32) block (A8W8: rows past M and
 // columns past N read 1; other modes: 1), loaded into registers before the K
 // loop so that the epilogue waits on none of them.
-template <int MODE, int TM, int TN>
+template <class Op, int MODE, int TM, int TN>
 struct EpiScales {
     float r[TM];
     float4 c[TN][4];
-    __device__ __forceinline__ void load(const DenseParams& p, int lane, int mw, int nw) {
+    __device__ __forceinline__ void load(const typename Op::Params& p, int lane, int mw, int nw) {
         const int khalf = lane >> 5;
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
@@ -392,6 +693,20 @@ struct EpiScales {
         for (int i = 0; i < TN; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
+                if constexpr (Op::GATED) {
+                    c[i][g] = make_float4(1.f, 1.f, 1.f, 1.f);
+                    const int f = nw / 2 + i % (TN / 2) * 32 + 8 * g + 4 * khalf;
+                    const bool up = i >= TN / 2;
+                    if (MODE == MODE_A8W8 && f < p.F) {
+                        const float* s = static_cast<const float*>(p.sb) + (p.interleaved ? 2 * f : up ? p.F + f : f);
+                        c[i][g] = *reinterpret_cast<const float4*>(s);
+                        if (p.interleaved) {
+                            const float4 d = *reinterpret_cast<const float4*>(s + 4);
+                            c[i][g] = up ? make_float4(c[i][g].y, c[i][g].w, d.y, d.w) : make_float4(c[i][g].x, c[i][g].z, d.x, d.z);
+                        }
+                    }
+                    continue;
+                }
                 const int n = nw + i * 32 + 8 * g + 4 * khalf;
                 c[i][g] = (MODE == MODE_A8W8 && n < p.N)
                               ? *reinterpret_cast<const float4*>(static_cast<const float*>(p.sb) + n)
@@ -400,14 +715,19 @@ struct EpiScales {
     }
 };
 
-template <int MODE, int WM, int WN, int TM, int TN>
-__device__ __forceinline__ void dense_epilogue_global(const DenseParams& p, v16f (&acc)[TN][TM],
-                                                      const EpiScales<MODE, TM, TN>& sc, HKQ_LDS uint8_t* smem,
-                                                      int wave, int lane, int mw, int nw) {
+template <class Op, int MODE, int TM, int TN>
+__device__ __forceinline__ void dense_epilogue_global(const typename Op::Params& p, v16f (&acc)[TN][TM],
+                                                      const EpiScales<Op, MODE, TM, TN>& sc,
+                                                      const EpiResidual<Op, TM, TN>& res, HKQ_LDS uint8_t* smem, int wave,
+                                                      int lane, int mw, int nw) {
     const int khalf = lane >> 5;
     auto row_scale = [&](int j) { return sc.r[j]; };
     auto col_scale4 = [&](int i, int g) { return sc.c[i][g]; };
-    if (p.bias)
+    if constexpr (Op::FUSED)
+        fused_store_tile<Op, TM, TN>(p, acc, res, smem, wave, lane, mw, nw, row_scale, col_scale4);
+    else if constexpr (Op::GATED)
+        gated_store_tile<TM, TN>(p, acc, smem, wave, lane, mw, nw / 2, row_scale, col_scale4);
+    else if (p.bias)
         store_tile_bf16<TM, TN>(acc, smem, wave, lane, p.C, p.ldc, p.M, p.N, mw, nw, p.c16 != 0, row_scale, col_scale4,
                                 [&](int i, int g) { return bias4(p, nw + i * 32 + 8 * g + 4 * khalf); });
     else
@@ -455,14 +775,14 @@ __device__ __forceinline__ int split_ticket(uint64_t* cnt, int splits) {
     }
 }
 
-template <int MODE, int WM, int WN, int TM, int TN, int KTB, int MINB, int NS>
-__global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const DenseParams pb) {
+template <class Op, int MODE, int WM, int WN, int TM, int TN, int KTB, int MINB, int NS>
+__global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const typename Op::Params pb) {
     using Cfg = DenseCfg<MODE, WM, WN, TM, TN, KTB>;
     constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW;
     constexpr int NQ = TN * TM * 4;  // float4 of accumulators per lane
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
     HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
-    const DenseParams p = batch_slice(pb);
+    const typename Op::Params p = batch_slice(pb);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = p.tiles_m * p.tiles_n;
@@ -476,14 +796,16 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const De
     const int mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
 
     // older than the K-tile loads: the loop's vmcnt waits cover them
-    EpiScales<MODE, TM, TN> sc;
+    EpiScales<Op, MODE, TM, TN> sc;
     sc.load(p, lane, mw, nw);
+    EpiResidual<Op, TM, TN> res;
+    if (p.splits == 1) res.load(p, lane, mw, nw);
 
     v16f acc[TN][TM];
-    dense_kloop<MODE, WM, WN, TM, TN, KTB, NS>(p, m0, n0, kt0, kt1, smem, acc);
+    dense_kloop<Op, MODE, WM, WN, TM, TN, KTB, NS>(p, m0, n0, kt0, kt1, smem, acc);
 
     if (p.splits == 1) {
-        dense_epilogue_global<MODE, WM, WN, TM, TN>(p, acc, sc, smem, wave, lane, mw, nw);
+        dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wave, lane, mw, nw);
         return;
     }
     // this split's partial: float4 q of lane l of wave w at
@@ -517,6 +839,7 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const De
     }
     __syncthreads();
     if (!last_split) return;
+    res.load(p, lane, mw, nw);  // by the one split that adds it, under the partial sums' loads
     // sum in split order; the other splits' float4 come in chunks of RCH
     // splits, all loads of a chunk in flight together (three splits' worth of
     // registers where the budget allows: 8 float4 per lane, or one workgroup
@@ -556,7 +879,7 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const De
                     }
         }
     }
-    dense_epilogue_global<MODE, WM, WN, TM, TN>(p, sum, sc, smem, wave, lane, mw, nw);
+    dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, smem, wave, lane, mw, nw);
 }
 
 // ---------------------------------------------------------------------------
@@ -585,25 +908,33 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const De
 // read nothing and whose scales were fetched after the sums.
 constexpr int NARROW_WAVES = 4, NARROW_ROWS = 16, NARROW_MAX_STEPS = 32;
 
-template <int MODE>
-__global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const DenseParams pb) {
+template <class Op, int MODE>
+__global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const typename Op::Params pb) {
     constexpr bool FP4 = MODE == MODE_MXFP4;
     constexpr int SB = FP4 ? 64 : 128;                      // bytes of a row per K-step
     constexpr int DEPTH = NARROW_MAX_STEPS / NARROW_WAVES;  // K-steps of a wave at most, all in flight together
     struct Frag {
         v4i b0, b1, a0, a1;  // weight row, activation row (b1, a1: FP8 only)
         uint32_t sb, sa;     // FP4: e8m0 scales of the step's 4 blocks (byte q is the lane's)
+        v4i u0, u1;          // GATED (FP8): the up row
     };
-    __shared__ v4f red[NARROW_WAVES][64];
-    const DenseParams p = batch_slice(pb);
+    constexpr bool GATED = Op::GATED;
+    static_assert(!GATED || !FP4, "gated: FP8");
+    __shared__ v4f red[GATED ? 2 : 1][NARROW_WAVES][64];
+    const typename Op::Params p = batch_slice(pb);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * 16, m0 = blockIdx.z * NARROW_ROWS;
     const int S = p.kbytes / SB;
     const int s0 = wave * S / NARROW_WAVES, s1 = (wave + 1) * S / NARROW_WAVES;
-    const int rows_a = min(NARROW_ROWS, p.M - m0), rows_b = min(16, p.N - n0);
+    int cols = p.N;  // GATED: n counts features
+    if constexpr (GATED) cols = p.F;
+    const int rows_a = min(NARROW_ROWS, p.M - m0), rows_b = min(16, cols - n0);
     const auto rb = make_rsrc(p.B + (int64_t)n0 * p.ldb, (uint32_t)(rows_b * p.ldb));
+    const uint8_t* up = p.B;
+    if constexpr (GATED) up = p.Bu;
+    const auto ru = make_rsrc(up + (int64_t)n0 * p.ldb, (uint32_t)(rows_b * p.ldb));
     const auto ra = make_rsrc(p.A + (int64_t)m0 * p.lda, (uint32_t)(rows_a * p.lda));
     const uint32_t b_off = (uint32_t)(r * p.ldb + 16 * q), a_off = (uint32_t)(r * p.lda + 16 * q);
     const auto rsb = make_rsrc(FP4 ? static_cast<const uint8_t*>(p.sb) + (int64_t)n0 * p.lsb : p.B,
@@ -617,6 +948,10 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const De
         const uint32_t kill = s < s1 ? 0u : OOB, kb = (uint32_t)s * SB | kill;
         f.b0 = __builtin_amdgcn_raw_buffer_load_b128(rb, b_off + kb, 0, 0);
         if constexpr (!FP4) f.b1 = __builtin_amdgcn_raw_buffer_load_b128(rb, b_off + kb + 64, 0, 0);
+        if constexpr (GATED) {
+            f.u0 = __builtin_amdgcn_raw_buffer_load_b128(ru, b_off + kb, 0, 0);
+            f.u1 = __builtin_amdgcn_raw_buffer_load_b128(ru, b_off + kb + 64, 0, 0);
+        }
         f.a0 = __builtin_amdgcn_raw_buffer_load_b128(ra, a_off + kb, 0, 0);
         if constexpr (!FP4) f.a1 = __builtin_amdgcn_raw_buffer_load_b128(ra, a_off + kb + 64, 0, 0);
         if constexpr (FP4) {
@@ -624,7 +959,7 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const De
             f.sa = __builtin_amdgcn_raw_buffer_load_b32(rsa, (uint32_t)(r * p.lsa) + ((uint32_t)s * 4 | kill), 0, 0);
         }
     };
-    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
+    v4f acc = v4f{0.f, 0.f, 0.f, 0.f}, acc_up = acc;
     auto mma = [&](const Frag& f) {
         if constexpr (FP4) {
             const v8i a = v8i{f.b0[0], f.b0[1], f.b0[2], f.b0[3], 0, 0, 0, 0};
@@ -635,17 +970,35 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const De
             const v8i a = v8i{f.b0[0], f.b0[1], f.b0[2], f.b0[3], f.b1[0], f.b1[1], f.b1[2], f.b1[3]};
             const v8i b = v8i{f.a0[0], f.a0[1], f.a0[2], f.a0[3], f.a1[0], f.a1[1], f.a1[2], f.a1[3]};
             acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, 0, 127, 0, 127);
+            if constexpr (GATED) {
+                const v8i u = v8i{f.u0[0], f.u0[1], f.u0[2], f.u0[3], f.u1[0], f.u1[1], f.u1[2], f.u1[3]};
+                acc_up = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(u, b, acc_up, 0, 0, 0, 127, 0, 127);
+            }
         }
     };
     // the epilogue's scales go out before the operands: no memory latency
     // follows the K loop
     const int n = n0 + 4 * q, m = m0 + r;
-    const bool in = n < p.N && m < p.M;  // N % 4 == 0: n .. n+3 all in or all out
-    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f);
+    const bool in = n < cols && m < p.M;  // N % 4 == 0: n .. n+3 all in or all out
+    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), cu = cs;
     float a = 1.f;
+    v2i res = v2i{0, 0};
     if (!FP4 && in) {
-        cs = *reinterpret_cast<const float4*>(static_cast<const float*>(p.sb) + n);
+        const float* sb = static_cast<const float*>(p.sb);
         a = static_cast<const float*>(p.sa)[m];
+        if constexpr (GATED) {
+            cs = *reinterpret_cast<const float4*>(sb + (p.interleaved ? 2 * n : n));
+            cu = *reinterpret_cast<const float4*>(sb + (p.interleaved ? 2 * n + 4 : p.F + n));
+            if (p.interleaved) {
+                const float4 x = cs, y = cu;
+                cs = make_float4(x.x, x.z, y.x, y.z);
+                cu = make_float4(x.y, x.w, y.y, y.w);
+            }
+        } else {
+            cs = *reinterpret_cast<const float4*>(sb + n);
+        }
+        if constexpr (Op::FUSED)
+            if (p.residual) res = *reinterpret_cast<const v2i*>(p.residual + (int64_t)m * p.ldr + n);
     }
     const float4 c = bias4(p, n);
     Frag f[DEPTH];
@@ -653,12 +1006,29 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const De
     for (int d = 0; d < DEPTH; ++d) load(s0 + d, f[d]);
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) mma(f[d]);
-    red[wave][lane] = acc;
+    red[0][wave][lane] = acc;
+    if constexpr (GATED) red[1][wave][lane] = acc_up;
     __syncthreads();
     if (wave != 0 || !in) return;
-    v4f v = red[0][lane];
+    v4f v = red[0][0][lane];
 #pragma unroll
-    for (int w = 1; w < NARROW_WAVES; ++w) v += red[w][lane];
+    for (int w = 1; w < NARROW_WAVES; ++w) v += red[0][w][lane];
+    if constexpr (GATED) {
+        v4f u = red[1][0][lane];
+#pragma unroll
+        for (int w = 1; w < NARROW_WAVES; ++w) u += red[1][w][lane];
+        const float4 g = act4(p.act, make_float4(v[0] * a * cs.x, v[1] * a * cs.y, v[2] * a * cs.z, v[3] * a * cs.w));
+        *reinterpret_cast<v2i*>(p.C + (int64_t)m * p.ldc + n) =
+            v2i{(int)pk_bf16(g.x * (u[0] * a * cu.x), g.y * (u[1] * a * cu.y)),
+                (int)pk_bf16(g.z * (u[2] * a * cu.z), g.w * (u[3] * a * cu.w))};
+        return;
+    }
+    if constexpr (Op::FUSED) {
+        float4 o = act4(p.act, make_float4(v[0] * a * cs.x + c.x, v[1] * a * cs.y + c.y, v[2] * a * cs.z + c.z, v[3] * a * cs.w + c.w));
+        if (p.residual) o = add_bf16x4(o, res);
+        *reinterpret_cast<v2i*>(p.C + (int64_t)m * p.ldc + n) = v2i{(int)pk_bf16(o.x, o.y), (int)pk_bf16(o.z, o.w)};
+        return;
+    }
     *reinterpret_cast<v2i*>(p.C + (int64_t)m * p.ldc + n) =
         v2i{(int)pk_bf16(v[0] * a * cs.x + c.x, v[1] * a * cs.y + c.y),
             (int)pk_bf16(v[2] * a * cs.z + c.z, v[3] * a * cs.w + c.w)};
@@ -687,12 +1057,12 @@ static int set_lds(K kern, int lds, bool& done) {
 // 29.6 -> 13.6, 64x28672x4096 42 -> 26; MXFP4 64x8192x8192 19.9 -> 9.1,
 // 1x8192x8192 11.9 -> 8.0; bf16 64x4096x4096 25.8 -> 9.0, 1x4096x4096
 // 17.1 -> 7.9, 300x4096x4096 22.9 -> 19.1.
-template <class Cfg>
-__global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const DenseParams pb) {
+template <class Op, class Cfg>
+__global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typename Op::Params pb) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
     HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
     constexpr int MODE = Cfg::MODE, BM = Cfg::BM, BN = Cfg::BN, TN = Cfg::TN, TM = Cfg::TM;
-    const DenseParams p = batch_slice(pb);
+    const typename Op::Params p = batch_slice(pb);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wg = wave % Cfg::GW, kg = wave / Cfg::GW;
@@ -716,6 +1086,17 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const Den
     src.b_step = (uint32_t)(8 * Cfg::GW * Cfg::SWP * p.ldb);
     src.bs_step = 0;
     src.sc_shift = 0;
+    if constexpr (Op::GATED) {
+        constexpr int GW = Cfg::GW;
+        const int f0 = n0 / 2, rows_f = min(p.F - f0, BN / 2);
+        src.b = buffer_desc(p.B + (int64_t)f0 * p.ldb, clamp_bytes((int64_t)(rows_f - 1) * p.ldb + p.kbytes));
+        src.b2 = buffer_desc(p.Bu + (int64_t)f0 * p.ldb, clamp_bytes((int64_t)(rows_f - 1) * p.ldb + p.kbytes));
+        if (GW == 8 && wg >= 4) src.b = src.b2;
+#pragma unroll
+        for (int i = 0; i < Cfg::SWP; ++i)
+            src.b_off[i] = (uint32_t)(((i * GW + wg) * 8 % 32 + lane / 8) * p.ldb) + kg_chunk<Cfg>(kg_row<Cfg>(i, wg, lane), lane);
+        src.b_step = (uint32_t)((GW == 8 ? 32 : 8 * GW * Cfg::SWP) * p.ldb);
+    }
     if constexpr (Cfg::FP4) {
         src.as = buffer_desc(static_cast<const uint8_t*>(p.sa) + (int64_t)m0 * p.lsa,
                              clamp_bytes((int64_t)(rows_a - 1) * p.lsa + p.K / 32));
@@ -729,18 +1110,20 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const Den
         }
     }
     const int mw = m0 + wg / Cfg::WN * TM * 32, nw = n0 + wg % Cfg::WN * TN * 32;
-    EpiScales<MODE, TM, TN> sc;
+    EpiScales<Op, MODE, TM, TN> sc;
     sc.load(p, lane, mw, nw);
+    EpiResidual<Op, TM, TN> res;
+    if (kg == 0) res.load(p, lane, mw, nw);
 
     v16f acc[TN][TM];
-    kgroup_kloop<Cfg>(src, smem, lane, wg, kg, acc);
+    kgroup_kloop<Cfg, false, Op::GATED>(src, smem, lane, wg, kg, acc);
     if (kg != 0) return;
-    dense_epilogue_global<MODE, 0, 0, TM, TN>(p, acc, sc, smem, wg, lane, mw, nw);
+    dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wg, lane, mw, nw);
 }
 
-template <class Cfg>
-static int launch_dense_kgroup(DenseParams& p, hipStream_t stream) {
-    auto kern = dense_kgroup_kernel<Cfg>;
+template <class Op, class Cfg>
+static int launch_dense_kgroup(typename Op::Params& p, hipStream_t stream) {
+    auto kern = dense_kgroup_kernel<Op, Cfg>;
     static bool attr_set = false;
     if (int e = set_lds(kern, Cfg::LDS, attr_set)) return e;
     p.tiles_m = (p.M + Cfg::BM - 1) / Cfg::BM;
@@ -832,7 +1215,7 @@ struct TileCosts {
     float split64_us, split64_e;           // 128 x 64 tiles: per K-tile, constant
     float split_us, split_e, split_parts;  // 128 x 128 tiles: per K-tile, constant, per split
 };
-static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const DensePlan* split) {
+static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const DensePlan* split, bool gated = false) {
     const int64_t M = p.M, N = p.N, kbytes = p.kbytes;
     // Tile rows `ld` bytes apart that a 32-bit buffer offset reaches. The 256-row
     // kernels end their extents with the last live row, so only those count
@@ -859,7 +1242,8 @@ static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const 
     int best = DT_NONE;
     float best_us = 0.f;
     for (int t = DT_256; t >= 0; --t) {
-        if (T.tile[t].us < 0.f || (t == DT_128x128_PAIR && kbytes % 128 != 0) || (t == DT_32x256 && (M > 32 || KT > 8)))
+        if (T.tile[t].us < 0.f || (t == DT_128x128_PAIR && kbytes % 128 != 0) || (t == DT_32x256 && (M > 32 || KT > 8)) ||
+            (gated && t == DT_32x32))  // one n-tile per wave: no pair of them
             continue;
         if (!(t == DT_256 ? fits(std::min<int64_t>(M, 256), std::min<int64_t>(N, 256)) : fits(BM[t], BN[t]))) continue;
         const int64_t tiles = batch * ((M + BM[t] - 1) / BM[t]) * ((N + BN[t] - 1) / BN[t]);
@@ -880,12 +1264,12 @@ static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const 
     return best;
 }
 
-template <int MODE, int WM, int WN, int TM, int TN, int KTB, int MINB, int NS = dense_ns<KTB>()>
-static int launch_dense_tiles(DenseParams& p, int splits, int kt_split, void* ws, hipStream_t stream) {
+template <class Op, int MODE, int WM, int WN, int TM, int TN, int KTB, int MINB, int NS = dense_ns<KTB>()>
+static int launch_dense_tiles(typename Op::Params& p, int splits, int kt_split, void* ws, hipStream_t stream) {
     using Cfg = DenseCfg<MODE, WM, WN, TM, TN, KTB>;
     constexpr int LDS = Cfg::lds_bytes(NS);
     static_assert(LDS * MINB <= 160 * 1024, "LDS budget of a CDNA4 CU");
-    auto kern = dense_tile_kernel<MODE, WM, WN, TM, TN, KTB, MINB, NS>;
+    auto kern = dense_tile_kernel<Op, MODE, WM, WN, TM, TN, KTB, MINB, NS>;
     static bool attr_set = false;
     if (int e = set_lds(kern, LDS, attr_set)) return e;
     p.tiles_m = (p.M + Cfg::BM - 1) / Cfg::BM;
@@ -902,11 +1286,11 @@ static int launch_dense_tiles(DenseParams& p, int splits, int kt_split, void* ws
     return hkq_launch_status();
 }
 
-template <int MODE, int KTB>
-static int launch_dense_whole(DenseParams& p, hipStream_t stream) {
+template <class Op, int MODE, int KTB>
+static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
     constexpr int LDS = dense_lds<MODE, KTB>();
     static_assert(LDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
-    auto kern = dense_gemm_kernel<MODE, KTB>;
+    auto kern = dense_gemm_kernel<Op, MODE, KTB>;
     static bool attr_set = false;  // per instantiation; the attribute is per-process
     if (int e = set_lds(kern, LDS, attr_set)) return e;
     p.tiles_m = (p.M + DENSE_BM - 1) / DENSE_BM;
@@ -926,7 +1310,7 @@ static int launch_dense_whole(DenseParams& p, hipStream_t stream) {
     // MXFP4 stays on the one-tile kernel: its stream (the K loop below with
     // compile-time scale slots, C stored from registers since the ring and the
     // scale blocks fill the LDS) spills and measured 1.8x slower on MI355X.
-    if constexpr (KTB == 128 && MODE != MODE_MXFP4) {
+    if constexpr (KTB == 128 && MODE != MODE_MXFP4 && std::is_same<Op, PlainOp>::value) {
         // the persistent streaming kernel: one workgroup per CU, whole tiles as
         // a K-tile stream (needs K-tiles per tile % 8 == 0; one 2-D GEMM without
         // bias, C's rows 16-byte aligned); HKQ_DENSE_STREAM=0 selects the
@@ -982,8 +1366,8 @@ static bool use_narrow(int mode, const DenseParams& p, int64_t batch) {
     return mode == MODE_A8W8 && S >= 24 && p.M <= (wgs >= 3 * ncu ? 4 : wgs >= 2 * ncu ? 1 : 0);
 }
 
-template <int MODE>
-static int launch_dense(DenseParams& p, void* ws, size_t ws_bytes, hipStream_t stream) {
+template <class Op, int MODE>
+static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipStream_t stream) {
     p.c16 = (p.ldc % 8 == 0) && (reinterpret_cast<uintptr_t>(p.C) % 16 == 0);
     if (p.M == 0 || p.N == 0) return 0;
     const int64_t batch = std::max(1, p.batch);
@@ -993,8 +1377,9 @@ static int launch_dense(DenseParams& p, void* ws, size_t ws_bytes, hipStream_t s
     }
     if constexpr (MODE != MODE_BF16) {
         if (use_narrow(MODE, p, batch)) {
-            const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)batch, (unsigned)((p.M + NARROW_ROWS - 1) / NARROW_ROWS));
-            narrow_gemm_kernel<MODE><<<grid, 64 * NARROW_WAVES, 0, stream>>>(p);
+            const int cols = Op::GATED ? p.N / 2 : p.N;
+            const dim3 grid((unsigned)((cols + 15) / 16), (unsigned)batch, (unsigned)((p.M + NARROW_ROWS - 1) / NARROW_ROWS));
+            narrow_gemm_kernel<Op, MODE><<<grid, 64 * NARROW_WAVES, 0, stream>>>(p);
             return hkq_launch_status();
         }
     }
@@ -1003,38 +1388,40 @@ static int launch_dense(DenseParams& p, void* ws, size_t ws_bytes, hipStream_t s
     bool split = false;
     if constexpr (MODE != MODE_MXFP4) {
         pl = dense_plan(MODE, p.M, p.N, p.kbytes);
-        split = p.batch <= 1 && p.bias == nullptr && pl.geo != GEO_SKINNY && pl.splits > 1 && ws != nullptr &&
+        split = !Op::GATED && p.batch <= 1 && (Op::FUSED || p.bias == nullptr) && pl.geo != GEO_SKINNY && pl.splits > 1 && ws != nullptr &&
                 ws_bytes >= pl.ws_bytes;
     }
     constexpr int M4 = MODE == MODE_MXFP4;  // the e8m0 blocks take LDS from the ring
-    switch (dense_tile_plan(MODE, p, batch, split ? &pl : nullptr)) {
-        case DT_32x32: return launch_dense_kgroup<KgCfg<MODE, 1, 1, 4, 1, 1, 4>>(p, stream);
-        case DT_32x64: return launch_dense_kgroup<KgCfg<MODE, 1, 1, 4, 1, 2, 3 - M4>>(p, stream);
-        case DT_32x128: return launch_dense_kgroup<KgCfg<MODE, 1, 1, 4 - M4, 1, 4, 2>>(p, stream);
-        case DT_32x256: return launch_dense_kgroup<KgCfg<MODE, 1, 4, 1, 1, 2, 3>>(p, stream);
-        case DT_64x64: return launch_dense_kgroup<KgCfg<MODE, 1, 1, 4, 2, 2, 2>>(p, stream);
-        case DT_128x64: return launch_dense_kgroup<KgCfg<MODE, 4, 1, 2, 1, 2, 3 - M4>>(p, stream);
-        case DT_128x128: return launch_dense_kgroup<KgCfg<MODE, 4, 2, 1, 1, 2, 4>>(p, stream);
+    switch (dense_tile_plan(MODE, p, batch, split ? &pl : nullptr, Op::GATED)) {
+        case DT_32x32:
+            if constexpr (!Op::GATED) return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 1, 1, 4>>(p, stream);
+            break;
+        case DT_32x64: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 1, 2, 3 - M4>>(p, stream);
+        case DT_32x128: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4 - M4, 1, 4, 2>>(p, stream);
+        case DT_32x256: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 4, 1, 1, 2, 3>>(p, stream);
+        case DT_64x64: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 2, 2, 2>>(p, stream);
+        case DT_128x64: return launch_dense_kgroup<Op, KgCfg<MODE, 4, 1, 2, 1, 2, 3 - M4>>(p, stream);
+        case DT_128x128: return launch_dense_kgroup<Op, KgCfg<MODE, 4, 2, 1, 1, 2, 4>>(p, stream);
         case DT_128x256:
-            if constexpr (!M4) return launch_dense_kgroup<KgCfg<MODE, 2, 4, 1, 2, 2, 3>>(p, stream);
+            if constexpr (!M4) return launch_dense_kgroup<Op, KgCfg<MODE, 2, 4, 1, 2, 2, 3>>(p, stream);
             break;
         case DT_128x128_PAIR:
-            return launch_dense_tiles<MODE, 2, 2, 2, 2, 128, 2>(p, 1, p.kbytes / 128, nullptr, stream);
+            return launch_dense_tiles<Op, MODE, 2, 2, 2, 2, 128, 2>(p, 1, p.kbytes / 128, nullptr, stream);
         case DT_SPLIT:
             // one workgroup per CU where the splits allow, on a deeper ring
             // (two K-tiles of loads in flight or more)
-            if constexpr (!M4) {
+            if constexpr (!M4 && !Op::GATED) {
                 const int ncu = cu_count() > 0 ? cu_count() : 256;
                 const bool one_round = pl.tiles * pl.splits <= ncu;
                 const int S = pl.splits, kt = pl.kt_split;
                 if constexpr (MODE == MODE_A8W8)
                     if (pl.geo == GEO_128x64) {
-                        if (!one_round) return launch_dense_tiles<MODE, 4, 1, 1, 2, 128, 2>(p, S, kt, ws, stream);
-                        if (kt >= 6) return launch_dense_tiles<MODE, 4, 1, 1, 2, 128, 1, 6>(p, S, kt, ws, stream);
-                        return launch_dense_tiles<MODE, 4, 1, 1, 2, 128, 1, 3>(p, S, kt, ws, stream);
+                        if (!one_round) return launch_dense_tiles<Op, MODE, 4, 1, 1, 2, 128, 2>(p, S, kt, ws, stream);
+                        if (kt >= 6) return launch_dense_tiles<Op, MODE, 4, 1, 1, 2, 128, 1, 6>(p, S, kt, ws, stream);
+                        return launch_dense_tiles<Op, MODE, 4, 1, 1, 2, 128, 1, 3>(p, S, kt, ws, stream);
                     }
-                if (!one_round) return launch_dense_tiles<MODE, 2, 2, 2, 2, 128, 2>(p, S, kt, ws, stream);
-                return launch_dense_tiles<MODE, 2, 2, 2, 2, 128, 1, 4>(p, S, kt, ws, stream);
+                if (!one_round) return launch_dense_tiles<Op, MODE, 2, 2, 2, 2, 128, 2>(p, S, kt, ws, stream);
+                return launch_dense_tiles<Op, MODE, 2, 2, 2, 2, 128, 1, 4>(p, S, kt, ws, stream);
             }
             break;
         case DT_NONE:
@@ -1043,7 +1430,7 @@ static int launch_dense(DenseParams& p, void* ws, size_t ws_bytes, hipStream_t s
     }
     // 128-byte K-tiles of this kernel need whole ones in every row: a partial
     // last K-tile would read the next row's bytes instead of zeros
-    return p.kbytes % 128 == 0 ? launch_dense_whole<MODE, 128>(p, stream) : launch_dense_whole<MODE, 64>(p, stream);
+    return p.kbytes % 128 == 0 ? launch_dense_whole<Op, MODE, 128>(p, stream) : launch_dense_whole<Op, MODE, 64>(p, stream);
 }
 
 }  // namespace hkq

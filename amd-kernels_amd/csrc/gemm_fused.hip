@@ -1,0 +1,332 @@
+// gemm_fused.hip -- the products of a feed-forward layer with what follows them:
+//
+//   hkq_gemm_*_epilogue      C = bf16(act(sums * scales + bias) + residual), FP8
+//                            and bf16 operands;
+//   hkq_gated_ffn_*          H = bf16(act(X Wg^T) * (X Wu^T)) in one kernel, FP8
+//                            and bf16 operands (bf16 may keep both projections);
+//   hkq_gated_ffn_backward   the gradients of X and W from those of H.
+//
+// The K loops, tile sizes and their choice are the dense GEMMs' (gemm_dense.h);
+// this file adds the epilogues, the pairing of gate and up columns in a tile,
+// and for the backward products bf16 operands whose K runs across memory rows.
+#include <limits>
+
+#include "gemm_dense.h"
+
+namespace hkq {
+
+static bool make_act(int act, float alpha, ActParams& a) {
+    constexpr float LOG2E = 1.44269504089f, TANH_C1 = 1.59576912161f;  // 2 sqrt(2 / pi)
+    a = ActParams{0, -std::numeric_limits<float>::infinity(), 0.f, 0.f};
+    switch (act) {
+        case HKQ_ACT_NONE: return true;
+        case HKQ_ACT_RELU: a.lo = 0.f; return true;
+        case HKQ_ACT_SILU: a.form = 1; a.c1 = -LOG2E * alpha; return true;
+        case HKQ_ACT_GELU_TANH: a.form = 1; a.c1 = -LOG2E * TANH_C1; a.c3 = a.c1 * 0.044715f; return true;
+        case HKQ_ACT_GELU: a.form = 2; return true;
+    }
+    return false;
+}
+
+// --------------------------------------------------------------------------
+// Gradients of the projections, from dH [M, F] and the kept Y [M, 2F]:
+//   dgate = dH * up * act'(gate),  dup = dH * act(gate)
+// in fp32, rounded to bf16 (they are operands of bf16 matrix products) into
+// rows of P values in Y's column order; values 2F .. P - 1 are zeros, so that
+// the products take whole K-tiles. HBM-bound: 6 bytes read and 4 written per
+// feature; a thread owns 8 features.
+// --------------------------------------------------------------------------
+__device__ __forceinline__ void act_grad(const ActParams& p, float v, float& f, float& df) {
+    if (p.form == 0) {
+        f = v < p.lo ? p.lo : v;
+        df = v > p.lo ? 1.0f : 0.0f;
+    } else if (p.form == 1) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(logistic_arg(p, v)));
+        const float slope = -0.69314718056f * __builtin_fmaf(3.0f * p.c3, min_num(v * v, 1e8f), p.c1);
+        f = v * s;
+        df = __builtin_fmaf(f * (1.0f - s), slope, s);
+    } else {
+        float e;
+        const float phi = normal_cdf(v, &e);
+        f = v * phi;
+        df = __builtin_fmaf(v * 0.3989422804f, e, phi);
+    }
+}
+
+__device__ __forceinline__ void unpack_bf16x8(const v4i& v, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = bf16_to_f32((uint32_t)v[i] & 0xFFFF);
+        f[2 * i + 1] = bf16_to_f32((uint32_t)v[i] >> 16);
+    }
+}
+
+__global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restrict__ dh, const uint16_t* __restrict__ y,
+                                                         uint16_t* __restrict__ dy, int64_t M, int F, int64_t lddh,
+                                                         int64_t ldy, int64_t P, int segs, int interleaved, ActParams act) {
+    for (int64_t b = blockIdx.x; b < M * segs; b += gridDim.x) {
+        const int64_t row = b / segs;
+        const int f = ((int)(b - row * segs) * 256 + (int)threadIdx.x) * 8;
+        if (f >= F) continue;
+        const uint16_t* yr = y + row * ldy;
+        uint16_t* dr = dy + row * P;
+        const v4i hv = *reinterpret_cast<const v4i*>(dh + row * lddh + f);
+        const v4i y0 = *reinterpret_cast<const v4i*>(yr + (interleaved ? 2 * f : f));
+        const v4i y1 = *reinterpret_cast<const v4i*>(yr + (interleaved ? 2 * f + 8 : F + f));
+        float h[8], a[8], c[8], g[8], u[8];
+        unpack_bf16x8(hv, h);
+        unpack_bf16x8(y0, a);
+        unpack_bf16x8(y1, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            g[j] = interleaved ? (j < 4 ? a[2 * j & 7] : c[2 * j & 7]) : a[j];
+            u[j] = interleaved ? (j < 4 ? a[(2 * j & 7) + 1] : c[(2 * j & 7) + 1]) : c[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float v, dv;
+            act_grad(act, g[j], v, dv);
+            g[j] = h[j] * u[j] * dv;
+            u[j] = h[j] * v;
+        }
+        v4i o0, o1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o0[j] = (int)(interleaved ? pk_bf16(g[j], u[j]) : pk_bf16(g[2 * j], g[2 * j + 1]));
+            o1[j] = (int)(interleaved ? pk_bf16(g[j + 4], u[j + 4]) : pk_bf16(u[2 * j], u[2 * j + 1]));
+        }
+        *reinterpret_cast<v4i*>(dr + (interleaved ? 2 * f : f)) = o0;
+        *reinterpret_cast<v4i*>(dr + (interleaved ? 2 * f + 8 : F + f)) = o1;
+        if (f + 8 == F)
+            for (int64_t t = 2 * (int64_t)F; t < P; t += 8) *reinterpret_cast<v4i*>(dr + t) = v4i{0, 0, 0, 0};
+    }
+}
+
+// Plan of a backward product over `KT` K-tiles of 64: 256 x 256 tiles, 128 x 128
+// tiles on two workgroups per CU, or the latter with K split over workgroups
+// (partial sums in the workspace) where they fill at most half of the CUs. Costs
+// as in dense_tile_plan's bf16 table.
+struct TransPlan {
+    int tile;  // DT_256, DT_128x128_PAIR or DT_SPLIT
+    int splits, kt_split;
+    size_t ws_bytes;
+};
+static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT) {
+    const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
+    auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
+    auto rounds = [](int64_t n, int64_t d) { return (float)((n + d - 1) / d); };
+    const int64_t t128 = tiles(128);
+    const float us256 = rounds(tiles(256), ncu) * ((float)KT * 0.647f + 2.1f);
+    const float us128 = t128 <= ncu ? (float)KT * 0.559f + 0.6f : rounds(t128, 2 * ncu) * ((float)KT * 0.645f + 0.9f);
+    TransPlan p{us256 <= us128 ? DT_256 : DT_128x128_PAIR, 1, (int)KT, 0};
+    if (2 * t128 <= ncu && KT >= 8) {
+        const int64_t s = std::min<int64_t>((ncu + t128 - 1) / t128, KT / 4);
+        if (s > 1) {
+            const int64_t per = (KT + s - 1) / s, n = (KT + per - 1) / per;
+            if ((float)per * 0.494f + 5.5f + 1.2f * (float)n < std::min(us256, us128))
+                p = TransPlan{DT_SPLIT, (int)n, (int)per, SPLIT_CNT_BYTES + (size_t)(n * t128) * (128 * 128 * 4)};
+        }
+    }
+    return p;
+}
+
+// C [M, N] = A . B^T over K rows of memory (B, and A with AT), K-tiles of 64.
+template <bool AT>
+static int launch_trans(DenseParams& p, void* ws, hipStream_t stream) {
+    using Op = TransOp<AT, true>;
+    p.c16 = p.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
+    const TransPlan pl = trans_plan(p.M, p.N, p.kbytes / 128);
+    if (pl.tile == DT_256) return launch_dense_whole<Op, MODE_BF16, 128>(p, stream);
+    if (pl.tile == DT_128x128_PAIR) return launch_dense_tiles<Op, MODE_BF16, 2, 2, 2, 2, 128, 2>(p, 1, p.kbytes / 128, nullptr, stream);
+    return launch_dense_tiles<Op, MODE_BF16, 2, 2, 2, 2, 128, 1, 4>(p, pl.splits, pl.kt_split, ws, stream);
+}
+
+// Row pitch (values) of the projections' gradients, and their place in the
+// backward's workspace after the split counters and partial sums of either
+// product.
+static int64_t grad_pitch(int64_t F) { return (2 * F + 63) / 64 * 64; }
+static size_t grad_offset(int64_t M, int64_t F, int64_t K) {
+    const size_t dx = trans_plan(M, K, grad_pitch(F) / 64).ws_bytes, dw = trans_plan(2 * F, K, (M + 63) / 64).ws_bytes;
+    return ((dx > dw ? dx : dw) + 255) / 256 * 256;
+}
+
+}  // namespace hkq
+
+using namespace hkq;
+
+static int check_act(int act, float alpha, ActParams& a) {
+    HKQ_CHECK_ARG(make_act(act, alpha, a), "act must be one of HKQ_ACT_NONE, _RELU, _SILU, _GELU_TANH, _GELU");
+    HKQ_CHECK_ARG(act != HKQ_ACT_SILU || (alpha == alpha && alpha - alpha == 0.0f), "alpha must be finite");
+    return 0;
+}
+
+template <int MODE>
+static int gemm_epilogue(const void* A, const void* B, const float* sa, const float* sb, const void* bias,
+                         const void* residual, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldr,
+                         int64_t ldc, int act, float alpha, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    constexpr int ES = MODE == MODE_BF16 ? 2 : 1;  // bytes per value of A and B
+    HKQ_CHECK_ARG(M >= 0 && N >= 0 && K > 0, "M, N must be >= 0 and K > 0");
+    HKQ_CHECK_ARG(M < (1 << 30) && N < (1 << 30) && K < (1 << 30), "dimensions must be < 2^30");
+    HKQ_CHECK_ARG(N % 4 == 0, "N must be a multiple of 4");
+    HKQ_CHECK_ARG(ldc >= N && ldc % 4 == 0, "ldc must be >= N and a multiple of 4");
+    HKQ_CHECK_ARG(MODE == MODE_BF16 || K % 64 == 0, "K must be a multiple of 64");
+    HKQ_CHECK_ARG(MODE != MODE_BF16 || K % 32 == 0, "K must be a multiple of 32");
+    HKQ_CHECK_ARG(lda >= K && ldb >= K && lda * ES % 16 == 0 && ldb * ES % 16 == 0,
+                  "lda/ldb must be >= K and keep rows 16-byte aligned");
+    HKQ_CHECK_ARG(!residual || (ldr >= N && ldr % 4 == 0), "ldr must be >= N and a multiple of 4");
+    FusedParams p{};
+    if (int e = check_act(act, alpha, p.act)) return e;
+    HKQ_CHECK_ARG(residual != C || ldr == ldc || !residual, "a residual in place of C must have its pitch");
+    if (M == 0 || N == 0) return 0;
+    HKQ_CHECK_ARG(A && B && C && (MODE == MODE_BF16 || (sa && sb)), "A, B, C and the scales are required");
+    HKQ_CHECK_ALIGN(A, 16);
+    HKQ_CHECK_ALIGN(B, 16);
+    HKQ_CHECK_ALIGN(C, 8);
+    HKQ_CHECK_ALIGN(sa, 4);
+    HKQ_CHECK_ALIGN(sb, 16);
+    HKQ_CHECK_ALIGN(bias, 8);
+    HKQ_CHECK_ALIGN(residual, 8);
+    HKQ_CHECK_ALIGN(workspace, 16);
+    p.A = static_cast<const uint8_t*>(A);
+    p.B = static_cast<const uint8_t*>(B);
+    p.C = static_cast<uint16_t*>(C);
+    p.sa = sa;
+    p.sb = sb;
+    p.bias = static_cast<const uint16_t*>(bias);
+    p.M = (int)M; p.N = (int)N; p.K = (int)K; p.kbytes = (int)(K * ES);
+    p.lda = lda * ES; p.ldb = ldb * ES; p.ldc = ldc;
+    p.residual = static_cast<const uint16_t*>(residual);
+    p.ldr = ldr;
+    p.r16 = ldr % 8 == 0 && reinterpret_cast<uintptr_t>(residual) % 16 == 0;
+    return launch_dense<FusedOp, MODE>(p, workspace, workspace_bytes, stream);
+}
+
+template <int MODE>
+static int gated_ffn(const void* X, const void* W, const float* sx, const float* sw, void* H, void* Y, int64_t M, int64_t F,
+                     int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int64_t ldy, int act, float alpha, int interleaved,
+                     hipStream_t stream) {
+    constexpr int ES = MODE == MODE_BF16 ? 2 : 1;
+    HKQ_CHECK_ARG(M >= 0 && F >= 0 && K > 0, "M, F must be >= 0 and K > 0");
+    HKQ_CHECK_ARG(M < (1 << 30) && F < (1 << 29) && K < (1 << 30), "M and K must be < 2^30, F < 2^29");
+    HKQ_CHECK_ARG(F % 8 == 0, "F must be a multiple of 8");
+    HKQ_CHECK_ARG(MODE == MODE_BF16 || K % 64 == 0, "K must be a multiple of 64");
+    HKQ_CHECK_ARG(MODE != MODE_BF16 || K % 32 == 0, "K must be a multiple of 32");
+    HKQ_CHECK_ARG(ldx >= K && ldw >= K && ldx * ES % 16 == 0 && ldw * ES % 16 == 0,
+                  "ldx/ldw must be >= K and keep rows 16-byte aligned");
+    HKQ_CHECK_ARG(ldh >= F && ldh % 4 == 0, "ldh must be >= F and a multiple of 4");
+    HKQ_CHECK_ARG(!Y || (ldy >= 2 * F && ldy % 4 == 0), "ldy must be >= 2F and a multiple of 4");
+    FusedParams p{};
+    if (int e = check_act(act, alpha, p.act)) return e;
+    if (M == 0 || F == 0) return 0;
+    HKQ_CHECK_ARG(X && W && H && (MODE == MODE_BF16 || (sx && sw)), "X, W, H and the scales are required");
+    HKQ_CHECK_ALIGN(X, 16);
+    HKQ_CHECK_ALIGN(W, 16);
+    HKQ_CHECK_ALIGN(sx, 4);
+    HKQ_CHECK_ALIGN(sw, 16);
+    HKQ_CHECK_ALIGN(H, 8);
+    HKQ_CHECK_ALIGN(Y, 8);
+    p.A = static_cast<const uint8_t*>(X);
+    p.B = static_cast<const uint8_t*>(W);
+    p.Bu = p.B + (interleaved ? ldw : F * ldw) * ES;
+    p.C = static_cast<uint16_t*>(H);
+    p.sa = sx;
+    p.sb = sw;
+    p.M = (int)M; p.N = (int)(2 * F); p.F = (int)F; p.K = (int)K; p.kbytes = (int)(K * ES);
+    p.lda = ldx * ES; p.ldb = (interleaved ? 2 : 1) * ldw * ES; p.ldc = ldh;
+    p.interleaved = interleaved != 0;
+    p.Y = static_cast<uint16_t*>(Y);
+    p.ldy = ldy;
+    p.y16 = ldy % 8 == 0 && reinterpret_cast<uintptr_t>(Y) % 16 == 0;
+    return launch_dense<GatedOp, MODE>(p, nullptr, 0, stream);
+}
+
+extern "C" {
+
+int hkq_gemm_a8w8_epilogue(const void* A, const void* B, const float* sa, const float* sb, const void* bias,
+                           const void* residual, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
+                           int64_t ldr, int64_t ldc, int act, float alpha, void* workspace, size_t workspace_bytes,
+                           hipStream_t stream) {
+    return gemm_epilogue<MODE_A8W8>(A, B, sa, sb, bias, residual, C, M, N, K, lda, ldb, ldr, ldc, act, alpha, workspace,
+                                    workspace_bytes, stream);
+}
+
+int hkq_gemm_bf16_epilogue(const void* A, const void* B, const void* bias, const void* residual, void* C, int64_t M,
+                           int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldr, int64_t ldc, int act, float alpha,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    return gemm_epilogue<MODE_BF16>(A, B, nullptr, nullptr, bias, residual, C, M, N, K, lda, ldb, ldr, ldc, act, alpha,
+                                    workspace, workspace_bytes, stream);
+}
+
+int hkq_gated_ffn_a8w8(const void* X, const void* W, const float* sx, const float* sw, void* H, int64_t M, int64_t F,
+                       int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int act, float alpha, int interleaved,
+                       hipStream_t stream) {
+    return gated_ffn<MODE_A8W8>(X, W, sx, sw, H, nullptr, M, F, K, ldx, ldw, ldh, 0, act, alpha, interleaved, stream);
+}
+
+int hkq_gated_ffn_bf16(const void* X, const void* W, void* H, void* Y, int64_t M, int64_t F, int64_t K, int64_t ldx,
+                       int64_t ldw, int64_t ldh, int64_t ldy, int act, float alpha, int interleaved, hipStream_t stream) {
+    return gated_ffn<MODE_BF16>(X, W, nullptr, nullptr, H, Y, M, F, K, ldx, ldw, ldh, ldy, act, alpha, interleaved, stream);
+}
+
+size_t hkq_gated_ffn_backward_workspace(int64_t M, int64_t F, int64_t K) {
+    if (M <= 0 || F <= 0 || K <= 0) return 0;
+    return grad_offset(M, F, K) + (size_t)M * (size_t)grad_pitch(F) * 2;
+}
+
+int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const void* Y, void* dX, void* dW, int64_t M,
+                           int64_t F, int64_t K, int64_t lddh, int64_t ldx, int64_t ldw, int64_t ldy, int64_t lddx,
+                           int64_t lddw, int act, float alpha, int interleaved, void* workspace, size_t workspace_bytes,
+                           hipStream_t stream) {
+    HKQ_CHECK_ARG(M >= 0 && F >= 0 && K > 0, "M, F must be >= 0 and K > 0");
+    HKQ_CHECK_ARG(M < (1 << 30) && F <= (1 << 20) && K < (1 << 30), "M and K must be < 2^30, F <= 2^20");
+    HKQ_CHECK_ARG(F % 8 == 0, "F must be a multiple of 8");
+    HKQ_CHECK_ARG(K % 32 == 0, "K must be a multiple of 32");
+    HKQ_CHECK_ARG(lddh >= F && lddh % 8 == 0, "lddh must be >= F and a multiple of 8");
+    HKQ_CHECK_ARG(ldy >= 2 * F && ldy % 8 == 0, "ldy must be >= 2F and a multiple of 8");
+    HKQ_CHECK_ARG(!dW || (ldx >= K && ldx % 8 == 0 && ldx < (1 << 24)), "ldx must be >= K, a multiple of 8 and < 2^24");
+    HKQ_CHECK_ARG(!dX || (ldw >= K && ldw % 8 == 0 && ldw < (1 << 24)), "ldw must be >= K, a multiple of 8 and < 2^24");
+    HKQ_CHECK_ARG(!dX || (lddx >= K && lddx % 4 == 0), "lddx must be >= K and a multiple of 4");
+    HKQ_CHECK_ARG(!dW || (lddw >= K && lddw % 4 == 0), "lddw must be >= K and a multiple of 4");
+    ActParams a;
+    if (int e = check_act(act, alpha, a)) return e;
+    if (F == 0 && (M == 0 || !dX)) return 0;
+    HKQ_CHECK_ARG(M == 0 || F == 0 || (dH && Y), "dH and Y are required");
+    HKQ_CHECK_ARG(M == 0 || F == 0 || ((!dW || X) && (!dX || W)), "X is required for dW, W for dX");
+    HKQ_CHECK_ARG(workspace_bytes >= hkq_gated_ffn_backward_workspace(M, F, K) && (workspace || M == 0 || F == 0),
+                  "the workspace is smaller than hkq_gated_ffn_backward_workspace(M, F, K)");
+    HKQ_CHECK_ALIGN(dH, 16);
+    HKQ_CHECK_ALIGN(X, 16);
+    HKQ_CHECK_ALIGN(W, 16);
+    HKQ_CHECK_ALIGN(Y, 16);
+    HKQ_CHECK_ALIGN(dX, 8);
+    HKQ_CHECK_ALIGN(dW, 8);
+    HKQ_CHECK_ALIGN(workspace, 16);
+    const int64_t P = grad_pitch(F);
+    const uint8_t* dy = static_cast<const uint8_t*>(workspace);
+    if (M > 0 && F > 0) {
+        uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + grad_offset(M, F, K));
+        dy = reinterpret_cast<const uint8_t*>(out);
+        const int segs = (int)((F / 8 + 255) / 256);
+        gated_grad_kernel<<<(unsigned)std::min<int64_t>(M * segs, 1 << 20), 256, 0, stream>>>(
+            static_cast<const uint16_t*>(dH), static_cast<const uint16_t*>(Y), out, M, (int)F, lddh, ldy, P, segs,
+            interleaved != 0, a);
+        if (int e = hkq_launch_status()) return e;
+    }
+    if (dX && M > 0) {  // [M, K] = dY [M, 2F] . W [2F, K]
+        DenseParams p{};
+        p.A = dy; p.B = static_cast<const uint8_t*>(W); p.C = static_cast<uint16_t*>(dX);
+        p.M = (int)M; p.N = (int)K; p.K = (int)(2 * F); p.kbytes = (int)(2 * P);
+        p.lda = 2 * P; p.ldb = 2 * ldw; p.ldc = lddx;
+        if (int e = launch_trans<false>(p, workspace, stream)) return e;
+    }
+    if (dW && F > 0) {  // [2F, K] = dY^T . X [M, K]; without tokens zeros
+        DenseParams p{};
+        p.A = dy; p.B = static_cast<const uint8_t*>(X); p.C = static_cast<uint16_t*>(dW);
+        p.M = (int)(2 * F); p.N = (int)K; p.K = (int)M; p.kbytes = (int)((M + 63) / 64 * 128);
+        p.lda = 2 * P; p.ldb = 2 * ldx; p.ldc = lddw;
+        if (int e = launch_trans<true>(p, workspace, stream)) return e;
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -81,6 +81,7 @@ template <class Cfg, bool GATHER = false>
 struct KgSrc {
     static constexpr int NA = GATHER ? Cfg::LA : Cfg::SWP;
     v4i a, b, as, bs;
+    v4i b2;  // GATED: the up half's rows; b: the gate half's (8-wave groups: each wave's own half)
     uint32_t a_off[NA], b_off[Cfg::SWP];
     uint32_t a_step, b_step;  // bytes between load i and load i + SWP (linear operands)
     uint32_t s_off[Cfg::PW > 0 ? Cfg::PW : 1], c_off[Cfg::LC > 0 ? Cfg::LC : 1];
@@ -126,7 +127,10 @@ __device__ __forceinline__ void lds_load4_s(const v4i& desc, HKQ_LDS void* dst, 
 // The K loop. On return group 0 of the workgroup holds the sums in
 // out[n-tile][m-tile], the LDS is free and every load has landed.
 // wg: the wave's index in its group, kg: its group.
-template <class Cfg, bool GATHER>
+// GATED (see gemm_mainloop): with w = GW waves, loads idx of a wave alternate
+// between the halves every GP loads (8-wave groups: waves 4 .. 7 load the up
+// half); b_step is then the step between a half's own loads.
+template <class Cfg, bool GATHER, bool GATED = false>
 __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_LDS uint8_t* smem, int lane, int wg, int kg,
                                              v16f (&out)[Cfg::TN][Cfg::TM]) {
     using KT = typename Cfg::KT;
@@ -174,7 +178,15 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
         const uint32_t kb = live ? (uint32_t)kt * 128u : OOB;
         constexpr int SWP = Cfg::SWP;
         const uint32_t tail = src.half_tail && kt == src.KT - 1 ? OOB : 0u;
-        if (idx < LB) {
+        if (GATED && idx < LB) {
+            static_assert(!GATED || (!GATHER && !FP4 && !BS && TN % 2 == 0 && (GW <= 4 || (GW == 8 && TN == 2))), "gated tiles");
+            constexpr int GP = GW <= 4 && GATED ? TN / 2 * 4 / GW : 1;
+            const bool up = GW <= 4 && (idx / GP) % 2 != 0;
+            const int fi = GW <= 4 ? idx / (2 * GP) * GP + idx % GP : idx;
+            lds_load16_s(up ? src.b2 : src.b, st + Cfg::BM * 128 + (idx * GW + wg) * 1024,
+                         src.b_off[idx % SWP] | (upper[GATHER ? 0 : idx % SWP] & tail),
+                         live ? kb + (uint32_t)(fi / SWP) * src.b_step : OOB);
+        } else if (idx < LB) {
             const uint32_t off = GATHER ? src.b_off[idx % SWP] : src.b_off[idx % SWP] | (upper[GATHER ? 0 : idx % SWP] & tail);
             lds_load16_s(src.b, st + Cfg::BM * 128 + (idx * GW + wg) * 1024, off,
                          live ? kb + (uint32_t)(idx / SWP) * src.b_step : OOB);

@@ -79,9 +79,30 @@ struct LoopSrc {
     // scale row is at r * lsa.
     bool sa_gathered = false;
     uint32_t sa_row[4] = {0u, 0u, 0u, 0u};
-    // N-contiguous B (BT): bytes from one K-tile of B to the next (128 rows of K)
-    int64_t b_kstep = 0;
+    // N-contiguous B (BT) and M-contiguous A (AT): bytes from one K-tile to the
+    // next (FP8, FP4: 128 rows of K; bf16: 64, where the extents may pass 2^31
+    // as a whole)
+    int64_t a_kstep = 0, b_kstep = 0;
+    // GATED: first row of the up half; `b` is that of the gate half, b_bytes the
+    // extent of either
+    const uint8_t* b2 = nullptr;
 };
+
+// GATED tiles: the 32-column n-tiles of each wave are gate columns in the first
+// half and up columns of the same features in the second, so that a lane holds
+// both in the same accumulator registers. Tile row r (of TN * 32 per wave) is
+// row gated_row(r) of its half.
+template <int TN>
+__device__ __forceinline__ int gated_row(int r) {
+    return r / (TN * 32) * (TN * 16) + r % (TN * 16);
+}
+// Whether load i of a K-tile carries rows of the up half (RPL rows per load and
+// wave: the waves' loads i together cover whole 32-row n-tiles of one half).
+template <class Cfg, int TN>
+constexpr bool gated_up(int i) {
+    static_assert(Cfg::NW * Cfg::RPL % 32 == 0 && Cfg::NW * Cfg::RPL <= TN * 16, "a load of all waves stays in one half");
+    return i * Cfg::NW * Cfg::RPL / 32 % TN >= TN / 2;
+}
 
 // Byte offset (row and logical chunk, excluding the K position) of LDS-direct
 // load instruction i of `wave` for a plain row-major operand.
@@ -122,6 +143,34 @@ __device__ __forceinline__ TableOff<N> dense_offs_t(int wave, int lane, int64_t 
     return o;
 }
 
+// The same for a bf16 operand with its rows contiguous (KTileT16).
+template <int NW, int N, int COLS>
+__device__ __forceinline__ TableOff<N> dense_offs_t16(int wave, int lane, int64_t ld) {
+    using T = KTileT16<COLS>;
+    constexpr int CHUNKS = T::ROW / 16;
+    TableOff<N> o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = (i * NW + wave) * T::ROWS_PER_LOAD + lane / CHUNKS;
+        o.v[i] = (uint32_t)(r * ld) + (uint32_t)(T::phys(r, lane % CHUNKS) << 4);
+    }
+    return o;
+}
+
+// Load offsets of a GATED tile's B rows (row stride ld bytes), each relative to
+// the first row of its half.
+template <int NW, int KTB, int N, int TN>
+__device__ __forceinline__ TableOff<N> dense_offs_gated(int wave, int lane, int64_t ld) {
+    using KT = KTile<KTB>;
+    TableOff<N> o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = (i * NW + wave) * KT::ROWS_PER_LOAD + lane / KT::CHUNKS;
+        o.v[i] = (uint32_t)(gated_row<TN>(r) * ld) + (uint32_t)(KT::load_chunk(lane, r) << 4);
+    }
+    return o;
+}
+
 // LDS base addresses of the transposed B fragment reads (BT): per n-tile t
 // of the wave, the lane's row 64h + (j >> 1) (h = lane / 32, j = lane % 16)
 // and byte 8 (j & 1) of logical chunk (wave's first column)/16 + 2t + g
@@ -141,6 +190,24 @@ __device__ __forceinline__ TBase<TN> tr_bases(uint32_t b_region, int wave_col, i
     for (int t = 0; t < TN; ++t) {
         const int chunk = (wave_col >> 4) + 2 * t + g;
         o.v[t] = b_region + (uint32_t)(row * KTileT::ROW + (KTileT::phys(row, chunk) << 4) + 8 * (j & 1));
+        asm volatile("" : "+v"(o.v[t]));
+    }
+    return o;
+}
+
+// The same for a bf16 operand with its rows contiguous: per 32-row tile t the
+// lane's row of K 32h + (j >> 2) and piece j & 3 of columns 16g .. 16g + 15;
+// reads at rows +8 (2 ks + part) and +4 ride as immediates.
+template <int T, int COLS>
+__device__ __forceinline__ TBase<T> tr16_bases(uint32_t region, int wave_col, int lane) {
+    using K = KTileT16<COLS>;
+    TBase<T> o;
+    const int j = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
+    const int row = 32 * h + (j >> 2);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const int chunk = (wave_col >> 3) + 4 * t + 2 * g + ((j & 3) >> 1);
+        o.v[t] = region + (uint32_t)(row * K::ROW + (K::phys(row, chunk) << 4) + 8 * (j & 1));
         asm volatile("" : "+v"(o.v[t]));
     }
     return o;
@@ -169,8 +236,11 @@ __device__ __forceinline__ TBase<TN> tr_bases(uint32_t b_region, int wave_col, i
 // each load instruction (TableOff; out of bounds for rows that must read zero).
 // On return acc holds the tile's fp32 sums and every wave is past a vmcnt(0)
 // barrier, so the caller may reuse the LDS.
-template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, int KTB, int NS, bool BT = false, typename AOff,
-          typename BOff>
+//
+// BT / AT: B N-contiguous (FP8, FP4: KTileT; bf16: KTileT16) / A M-contiguous
+// (bf16); GATED: B rows from the two halves of a gate/up weight (src.b, src.b2).
+template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, int KTB, int NS, bool BT = false, bool AT = false,
+          bool GATED = false, typename AOff, typename BOff>
 __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_off, const BOff& b_off,
                                               HKQ_LDS uint8_t* smem, int lane, int wave, v16f (&acc)[TN][TM]) {
     using Cfg = DenseCfg<MODE, WAVES_M, WAVES_N, TM, TN, KTB>;
@@ -186,8 +256,11 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
     static_assert(NS >= 2 && (NS - 1) * NLD + 3 <= 63, "ring depth and vmcnt budget");
     static_assert(!Cfg::SBLK || NS == 2, "the scale-block schedule assumes a 2-stage ring");
     static_assert(Cfg::SB_KT <= 4 && LSA <= 4, "gathered scale rows: at most 4 load slots per lane");
-    static_assert(!BT || (KTB == 128 && Cfg::BN == KTileT::ROW && (MODE == MODE_A8W8 || MODE == MODE_MXFP4)),
+    constexpr bool BT16 = BT && MODE == MODE_BF16;  // AT is bf16 only
+    static_assert(!BT || BT16 || (KTB == 128 && Cfg::BN == KTileT::ROW && (MODE == MODE_A8W8 || MODE == MODE_MXFP4)),
                   "N-contiguous B: FP8 or FP4, 128-byte K-tiles of 256 columns");
+    static_assert(!(BT16 || AT) || (KTB == 128 && MODE == MODE_BF16), "transposed operands: bf16, 128-byte K-tiles");
+    static_assert(!GATED || (!FP4 && !BT && !AT), "gated tiles: K-contiguous FP8 or bf16 operands");
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
     const int KTN = src.KT;
 
@@ -241,6 +314,14 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
     // otherwise pull NS K-tiles of the next split's bytes).
     const v4i desc_a = buffer_desc(src.a, (uint32_t)(src.a_bytes < 0x7FFFFFFF ? (src.a_bytes > 0 ? src.a_bytes : 0) : 0x7FFFFFFF));
     const v4i desc_b = buffer_desc(src.b, (uint32_t)(src.b_bytes < 0x7FFFFFFF ? (src.b_bytes > 0 ? src.b_bytes : 0) : 0x7FFFFFFF));
+    const v4i desc_b2 = buffer_desc(src.b2, (uint32_t)(src.b_bytes < 0x7FFFFFFF ? (src.b_bytes > 0 ? src.b_bytes : 0) : 0x7FFFFFFF));
+    // bf16 AT / BT: a K-tile's rows start kt K-tiles into the operand, whose
+    // extent may pass 32 bits, so the base moves and the extent is what is left
+    auto load_t16 = [&](const uint8_t* base, int64_t bytes, int64_t kstep, int kt, HKQ_LDS uint8_t* dst, uint32_t off) {
+        const int64_t at = (int64_t)kt * kstep;
+        const int64_t left = kt < KTN && bytes > at ? bytes - at : 0;
+        lds_load16_u(base + at, (uint32_t)(left < 0x7FFFFFFF ? left : 0x7FFFFFFF), dst, off);
+    };
 
     // Load instruction idx of K-tile kt into `stage`: A rows, B rows, then (FP4)
     // scales: KTB 64: group g covers rows g*64 + lane; KTB 128: one scale unit,
@@ -260,11 +341,21 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
                 return;
             }
         }
-        if (idx < LA) {
+        if (AT && idx < LA) {
+            load_t16(src.a, src.a_bytes, src.a_kstep, kt, smem + Cfg::a_stage(NS, stage) + (idx * NW + wave) * 1024, a_off.v[idx]);
+        } else if (idx < LA) {
             lds_load16_d(desc_a, smem + Cfg::a_stage(NS, stage) + (idx * NW + wave) * 1024,
                          live ? a_off.v[idx] + (uint32_t)kb : 0x80000000u);
+        } else if (BT16 && idx < LA + LB) {
+            const int i = idx - LA;
+            load_t16(src.b, src.b_bytes, src.b_kstep, kt, smem + Cfg::b_stage(NS, stage) + (i * NW + wave) * 1024, b_off.v[i]);
         } else if (idx < LA + LB) {
             const int i = idx - LA;
+            if constexpr (GATED) {
+                lds_load16_d(gated_up<Cfg, TN>(i) ? desc_b2 : desc_b, smem + Cfg::b_stage(NS, stage) + (i * NW + wave) * 1024,
+                             live ? b_off.v[i] + (uint32_t)kb : 0x80000000u);
+                return;
+            }
             const uint32_t kbb = BT ? (uint32_t)(kt * src.b_kstep) : (uint32_t)kb;
             lds_load16_d(desc_b, smem + Cfg::b_stage(NS, stage) + (i * NW + wave) * 1024,
                          live ? b_off.v[i] + kbb : 0x80000000u);
@@ -305,8 +396,18 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
             asm volatile("" : "+v"(b_base[ks][part]));
         }
 
-    const TBase<TN> bt = BT ? tr_bases<TN>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::b_stage(NS, 0), wn * TN * 32, lane)
-                            : TBase<TN>{};
+    const TBase<TN> bt = BT16 ? tr16_bases<TN, BN>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::b_stage(NS, 0), wn * TN * 32, lane)
+                         : BT ? tr_bases<TN>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::b_stage(NS, 0), wn * TN * 32, lane)
+                              : TBase<TN>{};
+    const TBase<TM> at = AT ? tr16_bases<TM, BM>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::a_stage(NS, 0), wm * TM * 32, lane)
+                            : TBase<TM>{};
+    // the lane's 8 values of K 32h + 8 (2 ks + part) .. +7 of its column: two
+    // transposed reads of 4 rows each
+    auto read_t16 = [](uint32_t base, int row) {
+        const v2i lo = lds_read_tr16(reinterpret_cast<const HKQ_LDS uint8_t*>((uintptr_t)base));
+        const v2i hi = lds_read_tr16(reinterpret_cast<const HKQ_LDS uint8_t*>((uintptr_t)(base + (uint32_t)(4 * row))));
+        return v4i{lo[0], lo[1], hi[0], hi[1]};
+    };
 
     struct Frags {
         v4i a[TM][PARTS], b[TN][PARTS];
@@ -317,6 +418,17 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
     auto read_piece = [&](int stage, int ks, Frags& f, int idx) {
         const int t = idx / (2 * PARTS), isb = (idx / PARTS) & 1, part = idx % PARTS;
         if ((isb ? TN : TM) <= t) return;
+        if (BT16 && isb) {
+            f.b[t][part] = read_t16(bt.v[t] + (uint32_t)(Cfg::b_stage(NS, stage) - Cfg::b_stage(NS, 0)) +
+                                        (uint32_t)(8 * (2 * ks + part) * KTileT16<BN>::ROW),
+                                    KTileT16<BN>::ROW);
+            return;
+        }
+        if (AT && !isb) {
+            f.a[t][part] = read_t16(at.v[t] + (uint32_t)Cfg::a_stage(NS, stage) + (uint32_t)(8 * (2 * ks + part) * KTileT16<BM>::ROW),
+                                    KTileT16<BM>::ROW);
+            return;
+        }
         if (BT && isb) {
             // the lane's 16 bytes of K [64h + 32ks + 16part, +16) of its column:
             // two transposed reads of 8 rows each

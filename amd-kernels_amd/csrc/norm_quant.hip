@@ -5,14 +5,19 @@
 //                         quantization/fused_mxfp4_quant/kernel.cpp:40-243
 //                         (y = x * rsqrt(mean(x^2) + eps) * w, then the 1x128
 //                         per-block rule or the MX shared-exponent rule);
+//   add_rmsnorm_quant_kernel
+//                         residual addition + RMSNorm + per-token or 1x128 FP8 /
+//                         INT8 quantization;
 //   swiglu_quant_kernel   SiLU-and-mul of a gate/up GEMM output followed by
 //                         per-token or 1x128 FP8 quantization: the activation of
 //                         moe-gemm/moe_op_silu_fused/kernel.cpp:1-13 and the
 //                         silu of moe-gemm/moe_op_gemm_a8w8/kernel.cpp:57-59,
 //                         feeding the down projection.
 //
-// Both are HBM-bound: each input element is read once into registers, the
+// All are HBM-bound: each input element is read once into registers, the
 // row statistic is reduced, and the codes are encoded from registers.
+#include <type_traits>
+
 #include "hkq_device.h"
 #include "hkq_host.h"
 
@@ -145,6 +150,151 @@ __global__ __launch_bounds__(256) void rmsnorm_quant_kernel(const uint16_t* __re
 }
 
 // --------------------------------------------------------------------------
+// Residual addition + RMSNorm + 8-bit quantization. T threads per row (64: a
+// wave, four rows per workgroup; 256: a workgroup); thread t holds the 16-byte
+// chunks c = t + T i of the row in registers, read once:
+//   h    = bf16(x + res), stored (without a residual h = x and nothing is
+//          stored); the norm is that of the stored, rounded stream;
+//   sum  = fma-chain of h^2 over the thread's chunks (i, then element order),
+//          the xor butterfly over the wave's lanes, then the waves in order;
+//   r    = 1 / sqrt(sum / D + eps),  y = (h * r) * w   (as above);
+//   s    = max(amax / QMAX, 1e-10) over the row (GROUP 0) or 128 columns,
+//   q    = encode(clamp(y * (1/s), +-QMAX)).
+// Maxima are taken over the magnitudes' bit patterns, in which a NaN exceeds
+// every number: a NaN among a scale's values makes that scale NaN, so it does
+// not vanish in the codes.
+// --------------------------------------------------------------------------
+template <int KIND>
+__device__ __forceinline__ float quant_scale(float m) {
+    const float s = KIND == HKQ_KIND_FP8 ? fp8_group_scale(m) : max_num(m / 127.0f, 1e-10f);
+    return m != m ? m : s;
+}
+template <int KIND>
+__device__ __forceinline__ float quant_recip(float s) { return KIND == HKQ_KIND_FP8 ? recip_scale(s) : 1.0f / s; }
+template <int KIND>
+__device__ __forceinline__ uint32_t quant4(const float* y, float rc) {
+    constexpr float QMAX = KIND == HKQ_KIND_FP8 ? 448.0f : 127.0f;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = max_num(min_num(KIND == HKQ_KIND_FP8 ? y[j] * rc : __builtin_rintf(y[j] * rc), QMAX), -QMAX);
+    if (KIND == HKQ_KIND_FP8) return cvt_pk4_e4m3(v[0], v[1], v[2], v[3]);
+    uint32_t o = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o |= ((uint32_t)(int32_t)v[j] & 0xFFu) << (8 * j);
+    return o;
+}
+
+template <int KIND, int GROUP, int T, int NC>
+__global__ __launch_bounds__(256) void add_rmsnorm_quant_kernel(const uint16_t* x, const uint16_t* res,
+                                                                const uint16_t* __restrict__ w, uint16_t* h,
+                                                                uint8_t* __restrict__ q, float* __restrict__ s, int M,
+                                                                int D, int64_t ldx, int64_t ldr, int64_t ldh,
+                                                                int64_t ldq, int64_t lds, float eps) {
+    constexpr int WAVES = T / 64;  // of a row
+    const int t = threadIdx.x % T, wave = threadIdx.x >> 6;
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * (256 / T) + threadIdx.x / T);
+    if (T == 64 && row >= M) return;  // no barriers in this form
+    const int nch = D >> 3;
+    // chunks past D read zero and their stores are dropped by the buffer bounds
+    const auto rx = make_rsrc(x + (int64_t)row * ldx, (uint32_t)D * 2u);
+    const auto rw = make_rsrc(w, (uint32_t)D * 2u);
+    uint4 xv[NC], wv[NC];
+    auto load = [&](const __amdgpu_buffer_rsrc_t& rsrc, int i) {
+        const v4i v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (uint32_t)(t + T * i) * 16u, 0, 0);
+        return make_uint4((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]);
+    };
+#pragma unroll
+    for (int i = 0; i < NC; ++i) xv[i] = load(rx, i);
+    if (res) {
+        const auto rr = make_rsrc(res + (int64_t)row * ldr, (uint32_t)D * 2u);
+        const auto rh = make_rsrc(h + (int64_t)row * ldh, (uint32_t)D * 2u);
+        uint4 rv[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) rv[i] = load(rr, i);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) wv[i] = load(rw, i);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float a[8], b[8];
+            unpack8(xv[i], a);
+            unpack8(rv[i], b);
+            xv[i] = make_uint4(pk_bf16(a[0] + b[0], a[1] + b[1]), pk_bf16(a[2] + b[2], a[3] + b[3]),
+                               pk_bf16(a[4] + b[4], a[5] + b[5]), pk_bf16(a[6] + b[6], a[7] + b[7]));
+            __builtin_amdgcn_raw_buffer_store_b128(v4i{(int)xv[i].x, (int)xv[i].y, (int)xv[i].z, (int)xv[i].w}, rh,
+                                                   (uint32_t)(t + T * i) * 16u, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) wv[i] = load(rw, i);
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        float f[8];
+        unpack8(xv[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(f[j], f[j], ss);
+    }
+    ss = group_sum<64>(ss);
+    __shared__ float red[2][4];
+    if constexpr (WAVES == 4) {
+        if ((t & 63) == 0) red[0][wave] = ss;
+        __syncthreads();
+        ss = ((red[0][0] + red[0][1]) + red[0][2]) + red[0][3];
+    }
+    const float r = 1.0f / __builtin_sqrtf(ss / (float)D + eps);
+    const auto rq = make_rsrc(q + (int64_t)row * ldq, (uint32_t)D);
+    float* sr = s + (int64_t)row * lds;
+
+    // y over the registers of h and w: magnitudes' maxima as bit patterns
+    float y[NC][8];
+    uint32_t m[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        float f[8], g[8];
+        unpack8(xv[i], f);
+        unpack8(wv[i], g);
+        m[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            y[i][j] = (f[j] * r) * g[j];
+            m[i] = max(m[i], __float_as_uint(y[i][j]) & 0x7FFFFFFFu);
+        }
+        // chunks past D hold zeros, but 0 * r is NaN for an infinite r
+        if (t + T * i >= nch) m[i] = 0;
+    }
+    float sc = 0.0f, rc = 0.0f;
+    if constexpr (GROUP == 0) {
+        uint32_t mm = m[0];
+#pragma unroll
+        for (int i = 1; i < NC; ++i) mm = max(mm, m[i]);
+        float a = group_max_abs<64>(__uint_as_float(mm));
+        if constexpr (WAVES == 4) {
+            if ((t & 63) == 0) red[1][wave] = a;
+            __syncthreads();
+            mm = max(max(__float_as_uint(red[1][0]), __float_as_uint(red[1][1])),
+                     max(__float_as_uint(red[1][2]), __float_as_uint(red[1][3])));
+            a = __uint_as_float(mm);
+        }
+        sc = quant_scale<KIND>(a);
+        rc = quant_recip<KIND>(sc);
+        if (t == 0) sr[0] = sc;
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int c = t + T * i;
+        if (T * i >= nch) break;  // no thread has a chunk here
+        if constexpr (GROUP == 128) {
+            sc = quant_scale<KIND>(group_max_abs<16>(__uint_as_float(m[i])));
+            rc = quant_recip<KIND>(sc);
+            if ((t & 15) == 0 && c < nch) sr[c >> 4] = sc;
+        }
+        const v2i codes = v2i{(int)quant4<KIND>(y[i], rc), (int)quant4<KIND>(y[i] + 4, rc)};
+        __builtin_amdgcn_raw_buffer_store_b64(codes, rq, (uint32_t)c * 8u, 0, 0);
+    }
+}
+
+// --------------------------------------------------------------------------
 // SwiGLU + FP8 quantization. One workgroup (256 threads) per row of the
 // gate/up GEMM output y [M, 2F] (bf16); thread t owns the activation chunks
 // c = t + 256 i (8 columns each):
@@ -255,6 +405,27 @@ int rmsnorm_nc(const uint16_t* x, const uint16_t* w, uint8_t* q, void* s, int M,
     return launch_rmsnorm<MODE, 16>(x, w, q, s, M, D, ldx, ldq, lds, eps, st);
 }
 
+template <int KIND, int GROUP, int T, int NC>
+int launch_add_rmsnorm(const uint16_t* x, const uint16_t* res, const uint16_t* w, uint16_t* h, uint8_t* q, float* s, int M,
+                       int D, int64_t ldx, int64_t ldr, int64_t ldh, int64_t ldq, int64_t lds, float eps, hipStream_t st) {
+    constexpr int ROWS = 256 / T;
+    add_rmsnorm_quant_kernel<KIND, GROUP, T, NC>
+        <<<(unsigned)(((int64_t)M + ROWS - 1) / ROWS), 256, 0, st>>>(x, res, w, h, q, s, M, D, ldx, ldr, ldh, ldq, lds, eps);
+    return hkq_launch_status();
+}
+
+// Threads per row and chunks per thread by D alone, so that a row's sum, and
+// with it every code, does not depend on how many rows a call has.
+template <int KIND, int GROUP, typename... A>
+int add_rmsnorm_nc(int D, A... a) {
+    if (D <= 512) return launch_add_rmsnorm<KIND, GROUP, 64, 1>(a...);
+    if (D <= 1024) return launch_add_rmsnorm<KIND, GROUP, 64, 2>(a...);
+    if (D <= 2048) return launch_add_rmsnorm<KIND, GROUP, 64, 4>(a...);
+    if (D <= 4096) return launch_add_rmsnorm<KIND, GROUP, 256, 2>(a...);
+    if (D <= 8192) return launch_add_rmsnorm<KIND, GROUP, 256, 4>(a...);
+    return launch_add_rmsnorm<KIND, GROUP, 256, 8>(a...);
+}
+
 template <int IL, int GROUP, int NC>
 int launch_swiglu(const uint16_t* y, uint8_t* q, float* s, int M, int F, int64_t ldy, int64_t ldq, int64_t lds,
                   float alpha, hipStream_t st) {
@@ -301,6 +472,42 @@ extern "C" int hkq_rmsnorm_quant(const void* x, const void* w, void* q, void* s,
                                           ldq, lds, eps, st);
     return rmsnorm_nc<NQ_MXFP4>((const uint16_t*)x, (const uint16_t*)w, (uint8_t*)q, s, (int)M, (int)D, ldx, ldq,
                                 lds, eps, st);
+}
+
+extern "C" int hkq_add_rmsnorm_quant(const void* x, const void* res, const void* w, void* h, void* q, float* s, int64_t M,
+                                     int64_t D, int64_t ldx, int64_t ldr, int64_t ldh, int64_t ldq, int64_t lds, float eps,
+                                     int group, int kind, hkq_stream_t stream) {
+    HKQ_CHECK_ARG(kind == HKQ_KIND_FP8 || kind == HKQ_KIND_INT8, "kind must be HKQ_KIND_FP8 or HKQ_KIND_INT8");
+    HKQ_CHECK_ARG(group == 0 || group == 128, "group must be 0 (per token) or 128");
+    HKQ_CHECK_ARG(M >= 0 && M <= INT32_MAX, "M must be in [0, 2^31)");
+    HKQ_CHECK_ARG(D >= 8 && D <= 16384 && D % (group ? 128 : 8) == 0,
+                  "D must be a multiple of 8 (128 with groups) in [8, 16384]");
+    HKQ_CHECK_ARG(ldx >= D && ldx % 8 == 0, "ldx must be >= D and a multiple of 8");
+    HKQ_CHECK_ARG(!res || (ldr >= D && ldr % 8 == 0 && ldh >= D && ldh % 8 == 0),
+                  "ldr and ldh must be >= D and multiples of 8");
+    HKQ_CHECK_ARG(ldq >= D && ldq % 8 == 0, "ldq must be >= D and a multiple of 8");
+    HKQ_CHECK_ARG(lds >= (group ? D / 128 : 1), "lds must hold a row of scales");
+    HKQ_CHECK_ARG(eps >= 0.0f, "eps must be non-negative");
+    HKQ_CHECK_ARG((res != nullptr) == (h != nullptr), "res and h go together: both or neither");
+    if (M == 0) return 0;
+    HKQ_CHECK_ARG(x && w && q && s, "x, w, q and s are required");
+    HKQ_CHECK_ALIGN(x, 16);
+    HKQ_CHECK_ALIGN(res, 16);
+    HKQ_CHECK_ALIGN(w, 16);
+    HKQ_CHECK_ALIGN(h, 16);
+    HKQ_CHECK_ALIGN(q, 8);
+    HKQ_CHECK_ALIGN(s, 4);
+    auto run = [&](auto k, auto g) {
+        return add_rmsnorm_nc<decltype(k)::value, decltype(g)::value>(
+            (int)D, (const uint16_t*)x, (const uint16_t*)res, (const uint16_t*)w, (uint16_t*)h, (uint8_t*)q, s, (int)M,
+            (int)D, ldx, ldr, ldh, ldq, lds, eps, (hipStream_t)stream);
+    };
+    using Fp8 = std::integral_constant<int, HKQ_KIND_FP8>;
+    using Int8 = std::integral_constant<int, HKQ_KIND_INT8>;
+    using G0 = std::integral_constant<int, 0>;
+    using G128 = std::integral_constant<int, 128>;
+    if (kind == HKQ_KIND_FP8) return group ? run(Fp8{}, G128{}) : run(Fp8{}, G0{});
+    return group ? run(Int8{}, G128{}) : run(Int8{}, G0{});
 }
 
 extern "C" int hkq_swiglu_quant(const void* y, void* q, float* s, int64_t M, int64_t F, int64_t ldy, int64_t ldq,

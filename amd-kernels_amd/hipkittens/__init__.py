@@ -12,6 +12,8 @@ the modules this build provides:
     hk.batched_gemm.a8w8.dispatch(A, B, a_s, b_s, C, bias) # batched_gemm_a8w8_tk (also .bf16)
     hk.fused_gemm.a8w8_blockscale_mul_add.dispatch(a, b, c, a_s, b_s, c_a, c_b)
                                                            # (also .a8w8_blockscale_a16w16)
+    hk.fused_gemm.a8w8_epilogue.dispatch(A, B, a_s, b_s, C, bias, residual, act)   # (also .a16w16_epilogue)
+    hk.ffn.gated.gated_ffn_a8w8(X, W, x_s, w_s, H, act)    # (also gated_ffn_bf16, gated_ffn_backward)
     hk.moe_routing.quant.downcast_to_mxfp(...)             # quant_moe_tk
     hk.moe_routing.topk.moe_topk(X, ...)                   # moe_topk_tk (also bitmatrix,
                                                            # expt_data, align_block_size)
@@ -137,6 +139,12 @@ def fused_rmsnorm_mxfp4_quant_fwd(*args, **kwargs):
     return _call("fused_mxfp4_quant_tk", "fused_rmsnorm_mxfp4_quant_fwd", *args, **kwargs)
 
 
+def fused_add_rmsnorm_quant_fwd(*args, **kwargs):
+    """fused_add_rmsnorm_quant_fwd(input bf16 [M,D], residual, weight bf16 [D], hidden, output e4m3|int8 [M,D], scales
+    f32 [M] or [M,D/128], eps, group_size=0): hidden = input + residual, both None without one (extension)"""
+    return _call("fused_fp8_quant_tk", "fused_add_rmsnorm_quant_fwd", *args, **kwargs)
+
+
 def swiglu_quant_fwd(*args, **kwargs):
     """swiglu_quant_fwd(input bf16 [M,2F], output e4m3 [M,F], scales f32 [M] or [M,F/128], alpha=1.0,
     interleaved=False, group_size=0) (extension)"""
@@ -181,6 +189,14 @@ class _BatchedGemmNamespace:
 class _FusedGemmNamespace:
     a8w8_blockscale_a16w16 = _SubModule("fused_gemm_a8w8_blockscale_a16w16_tk")
     a8w8_blockscale_mul_add = _SubModule("fused_gemm_a8w8_blockscale_mul_add_tk")
+    # extensions: bias, activation and residual in the dense GEMMs' epilogue
+    a8w8_epilogue = _SubModule("fused_gemm_a8w8_epilogue_tk")
+    a16w16_epilogue = _SubModule("fused_gemm_a16w16_epilogue_tk")
+
+
+class _FeedForwardNamespace:
+    # extension: the gated projection pair and its backward pass
+    gated = _SubModule("gated_ffn_tk")
 
 
 class _MoeGemmNamespace:
@@ -202,5 +218,6 @@ class _MoeRoutingNamespace:
 gemm = _GemmNamespace()
 batched_gemm = _BatchedGemmNamespace()
 fused_gemm = _FusedGemmNamespace()
+ffn = _FeedForwardNamespace()
 moe = _MoeGemmNamespace()
 moe_routing = _MoeRoutingNamespace()

@@ -16,6 +16,9 @@ LIB_PATH = os.path.join(_PKG, "lib", "libhkq.so")
 KIND_FP8 = 0
 KIND_INT8 = 1
 
+# activations of the fused epilogues and the gated feed-forward (HKQ_ACT_*)
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu": 4}
+
 # Every entry point declared in include/hkq.h, with its ctypes signature.
 _P, _I64, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 SIGNATURES = {
@@ -50,6 +53,13 @@ SIGNATURES = {
                                      _P, _P, _P, _P] + [_I64] * 12 + [_P]),
     "hkq_moe_pack_kmajor": (_I, [_P, _P] + [_I64] * 7 + [_P]),
     "hkq_rmsnorm_quant": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float, _I, _P]),
+    "hkq_add_rmsnorm_quant": (_I, [_P] * 6 + [_I64] * 7 + [ctypes.c_float, _I, _I, _P]),
+    "hkq_gemm_a8w8_epilogue": (_I, [_P] * 7 + [_I64] * 7 + [_I, ctypes.c_float, _P, ctypes.c_size_t, _P]),
+    "hkq_gemm_bf16_epilogue": (_I, [_P] * 5 + [_I64] * 7 + [_I, ctypes.c_float, _P, ctypes.c_size_t, _P]),
+    "hkq_gated_ffn_a8w8": (_I, [_P] * 5 + [_I64] * 6 + [_I, ctypes.c_float, _I, _P]),
+    "hkq_gated_ffn_bf16": (_I, [_P] * 4 + [_I64] * 7 + [_I, ctypes.c_float, _I, _P]),
+    "hkq_gated_ffn_backward_workspace": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "hkq_gated_ffn_backward": (_I, [_P] * 6 + [_I64] * 9 + [_I, ctypes.c_float, _I, _P, ctypes.c_size_t, _P]),
     "hkq_swiglu_quant": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float, _I, _I, _P]),
     "hkq_moe_mxfp4": (_I, [_P] * 10 + [_I64, _I64, _I64, _I64, _I] + [_I64] * 10 + [_P]),
     "hkq_moe_mxfp4_kn": (_I, [_P] * 10 + [_I64, _I64, _I64, _I64, _I] + [_I64] * 10 + [_P]),
@@ -206,6 +216,35 @@ def rmsnorm_quant(x, w, eps: float = 1e-6, kind: int = 0, q=None, s=None, stream
     return q, s
 
 
+def add_rmsnorm_quant(x, w, residual=None, eps: float = 1e-6, kind: int = KIND_FP8, group: int = 0, h=None, q=None,
+                      s=None, stream=None):
+    """Residual addition + RMSNorm + 8-bit quantization of bf16 [M, D]:
+    h = bf16(x + residual) (x itself without one), then (q float8_e4m3fn / int8
+    [M, D], s fp32 [M] (group 0) or [M, D/128] (group 128), h bf16 [M, D] or
+    None without a residual). h may be x or residual."""
+    import torch
+
+    M, D = x.shape
+    bf16, codes = (torch.bfloat16,), (torch.int8,) if kind == KIND_INT8 else (torch.float8_e4m3fn, torch.uint8)
+    if residual is not None and h is None:
+        h = torch.empty((M, D), dtype=torch.bfloat16, device=x.device)
+    if residual is None and h is not None:
+        raise ValueError("h is written with a residual only")
+    if q is None:
+        q = torch.empty((M, D), dtype=codes[0], device=x.device)
+    if s is None:
+        s = torch.empty((M,) if group == 0 else (M, D // 128), dtype=torch.float32, device=x.device)
+    for t, name, shape, types in ((x, "x", (M, D), bf16), (w, "w", (D,), bf16), (residual, "residual", (M, D), bf16),
+                                  (h, "h", (M, D), bf16), (q, "q", (M, D), codes),
+                                  (s, "s", (M,) if group == 0 else (M, D // 128), (torch.float32,))):
+        if t is not None:
+            _expect(t, name, shape, types, x.device)
+    with torch.cuda.device(x.device):
+        call("hkq_add_rmsnorm_quant", _ptr(x), _opt_ptr(residual), _ptr(w), _opt_ptr(h), _ptr(q), _ptr(s), M, D, _pitch(x),
+             _pitch(residual), _pitch(h), _pitch(q), _pitch(s) if group else 1, eps, group, kind, _stream(stream))
+    return q, s, h
+
+
 def swiglu_quant(y, alpha: float = 1.0, interleaved: bool = False, group: int = 0, q=None, s=None, stream=None):
     """SiLU-and-mul of a gate/up output bf16 [M, 2F] + FP8 quantization:
     (q float8_e4m3fn [M, F], s fp32 [M] (group 0) or [M, F/128] (group 128))."""
@@ -222,9 +261,37 @@ def swiglu_quant(y, alpha: float = 1.0, interleaved: bool = False, group: int = 
     return q, s
 
 
-def _workspace(nbytes: int, like):
+def _pitch(t) -> int:
+    """Row pitch of a 2-D tensor (its row length where no pitch is stepped over, whatever its stride says); 0 for None."""
+    return 0 if t is None else t.shape[1] if t.shape[0] <= 1 or t.numel() == 0 else t.stride(0)
+
+
+def _activation(act: str) -> int:
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
+    return ACTIVATIONS[act]
+
+
+def _expect(t, name: str, shape, dtypes, device) -> None:
+    """A tensor operand of the feed-forward operators: its shape, type and
+    device, and a contiguous last dimension."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}; expected {' or '.join(str(d) for d in dtypes)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the first operand on {device}")
+    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+
+
+def _workspace(nbytes: int, like, stream=None):
+    """Scratch memory of `stream` (the current one): handed out again in that stream's order."""
     import torch
 
+    if stream is not None and nbytes:
+        with torch.cuda.stream(stream):
+            return _workspace(nbytes, like)
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
@@ -331,6 +398,135 @@ def gemm_bf16(A, B, C=None, bias=None, stream=None, split: bool = True):
          B3.stride(1), C3.stride(1), A3.stride(0), B3.stride(0), C3.stride(0), b2.stride(0) if b2 is not None else 0,
          _ptr(ws) if ws is not None else None, ws.numel() if ws is not None else 0, _stream(stream))
     return C
+
+
+def gemm_a8w8_epilogue(A, B, sa, sb, bias=None, act: str = "none", residual=None, alpha: float = 1.0, C=None,
+                       stream=None, split: bool = True):
+    """bf16(act((A . B^T) * sa[m] * sb[n] + bias[n]) + residual): A [M, K], B
+    [N, K] E4M3FN codes, sa [M], sb [N] fp32, bias bf16 [N], residual bf16
+    [M, N] (may be C) -> C bf16 [M, N]. act: a name of ACTIVATIONS; alpha: of
+    "silu". split=False runs without a workspace (no split-K)."""
+    import torch
+
+    M, K = A.shape
+    N = B.shape[0]
+    codes = (torch.float8_e4m3fn, torch.uint8)
+    _expect(A, "A", (M, K), codes, A.device)
+    _expect(B, "B", (N, K), codes, A.device)
+    _expect(sa.view(-1), "sa", (M,), (torch.float32,), A.device)
+    _expect(sb.view(-1), "sb", (N,), (torch.float32,), A.device)
+    return _gemm_epilogue("a8w8", A, B, (sa, sb), bias, act, residual, alpha, C, stream, split)
+
+
+def gemm_bf16_epilogue(A, B, bias=None, act: str = "none", residual=None, alpha: float = 1.0, C=None, stream=None,
+                       split: bool = True):
+    """bf16(act(A . B^T + bias[n]) + residual): A [M, K], B [N, K] bf16; the
+    rest as gemm_a8w8_epilogue."""
+    import torch
+
+    _expect(A, "A", A.shape, (torch.bfloat16,), A.device)
+    _expect(B, "B", (B.shape[0], A.shape[1]), (torch.bfloat16,), A.device)
+    return _gemm_epilogue("bf16", A, B, (), bias, act, residual, alpha, C, stream, split)
+
+
+def _gemm_epilogue(kind, A, B, scales, bias, act, residual, alpha, C, stream, split):
+    import torch
+
+    M, K = A.shape
+    N = B.shape[0]
+    if C is None:
+        C = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
+    _expect(C, "C", (M, N), (torch.bfloat16,), A.device)
+    if bias is not None:
+        _expect(bias, "bias", (N,), (torch.bfloat16,), A.device)
+    if residual is not None:
+        _expect(residual, "residual", (M, N), (torch.bfloat16,), A.device)
+    a = _activation(act)
+    with torch.cuda.device(A.device):
+        ws = _workspace(int(getattr(lib(), f"hkq_gemm_{kind}_workspace")(M, N, K)) if split else 0, A, stream)
+        call(f"hkq_gemm_{kind}_epilogue", _ptr(A), _ptr(B), *(_ptr(s) for s in scales), _opt_ptr(bias),
+             _opt_ptr(residual), _ptr(C), M, N, K, _pitch(A), _pitch(B), _pitch(residual), _pitch(C), a, alpha,
+             _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+    return C
+
+
+def gated_ffn_a8w8(X, W, sx, sw, act: str = "silu", alpha: float = 1.0, interleaved: bool = False, H=None, stream=None):
+    """Gated feed-forward projections in one kernel: H = bf16(act(g) * u), g and
+    u = X . W^T over the gate and up rows of W [2F, K] (halves, or interleaved),
+    X [M, K], both E4M3FN codes with scales sx fp32 [M], sw fp32 [2F] -> bf16
+    [M, F]."""
+    import torch
+
+    M, K = X.shape
+    F = W.shape[0] // 2
+    codes = (torch.float8_e4m3fn, torch.uint8)
+    _expect(X, "X", (M, K), codes, X.device)
+    _expect(W, "W", (2 * F, K), codes, X.device)
+    _expect(sx.view(-1), "sx", (M,), (torch.float32,), X.device)
+    _expect(sw.view(-1), "sw", (2 * F,), (torch.float32,), X.device)
+    if H is None:
+        H = torch.empty((M, F), dtype=torch.bfloat16, device=X.device)
+    _expect(H, "H", (M, F), (torch.bfloat16,), X.device)
+    a = _activation(act)
+    with torch.cuda.device(X.device):
+        call("hkq_gated_ffn_a8w8", _ptr(X), _ptr(W), _ptr(sx), _ptr(sw), _ptr(H), M, F, K, _pitch(X), _pitch(W),
+             _pitch(H), a, alpha, int(interleaved), _stream(stream))
+    return H
+
+
+def gated_ffn_bf16(X, W, act: str = "silu", alpha: float = 1.0, interleaved: bool = False, H=None, Y=None,
+                   save: bool = False, stream=None):
+    """gated_ffn_a8w8 of bf16 X [M, K], W [2F, K]: H bf16 [M, F], or with save
+    (or a Y given) (H, Y), Y bf16 [M, 2F] the projections in W's row order,
+    which gated_ffn_backward takes."""
+    import torch
+
+    M, K = X.shape
+    F = W.shape[0] // 2
+    bf16 = (torch.bfloat16,)
+    _expect(X, "X", (M, K), bf16, X.device)
+    _expect(W, "W", (2 * F, K), bf16, X.device)
+    if H is None:
+        H = torch.empty((M, F), dtype=torch.bfloat16, device=X.device)
+    if Y is None and save:
+        Y = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=X.device)
+    _expect(H, "H", (M, F), bf16, X.device)
+    if Y is not None:
+        _expect(Y, "Y", (M, 2 * F), bf16, X.device)
+    a = _activation(act)
+    with torch.cuda.device(X.device):
+        call("hkq_gated_ffn_bf16", _ptr(X), _ptr(W), _ptr(H), _opt_ptr(Y), M, F, K, _pitch(X), _pitch(W), _pitch(H),
+             _pitch(Y), a, alpha, int(interleaved), _stream(stream))
+    return H if Y is None else (H, Y)
+
+
+def gated_ffn_backward(dH, X, W, Y, act: str = "silu", alpha: float = 1.0, interleaved: bool = False, dX=None, dW=None,
+                       need_dx: bool = True, need_dw: bool = True, stream=None):
+    """Gradients (dX bf16 [M, K], dW bf16 [2F, K]) of gated_ffn_bf16 from dH bf16
+    [M, F], its inputs and the Y it kept; one that is not needed is None. Both
+    are overwritten, not accumulated."""
+    import torch
+
+    M, K = X.shape
+    F = W.shape[0] // 2
+    bf16 = (torch.bfloat16,)
+    for t, name, shape in ((X, "X", (M, K)), (W, "W", (2 * F, K)), (dH, "dH", (M, F)), (Y, "Y", (M, 2 * F))):
+        _expect(t, name, shape, bf16, X.device)
+    if need_dx and dX is None:
+        dX = torch.empty((M, K), dtype=torch.bfloat16, device=X.device)
+    if need_dw and dW is None:
+        dW = torch.empty((2 * F, K), dtype=torch.bfloat16, device=X.device)
+    dX, dW = dX if need_dx else None, dW if need_dw else None
+    for t, name, shape in ((dX, "dX", (M, K)), (dW, "dW", (2 * F, K))):
+        if t is not None:
+            _expect(t, name, shape, bf16, X.device)
+    a = _activation(act)
+    with torch.cuda.device(X.device):
+        ws = _workspace(int(lib().hkq_gated_ffn_backward_workspace(M, F, K)), X, stream)
+        call("hkq_gated_ffn_backward", _ptr(dH), _ptr(X), _ptr(W), _ptr(Y), _opt_ptr(dX), _opt_ptr(dW), M, F, K,
+             _pitch(dH), _pitch(X), _pitch(W), _pitch(Y), _pitch(dX), _pitch(dW), a, alpha, int(interleaved),
+             _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+    return dX, dW
 
 
 def moe_a8w8(X, W, hist, offs, expt_data, topk, gather=None, x_scale=None, w_scale=None, bias=None, Y=None,

@@ -109,6 +109,22 @@ int hkq_rmsnorm_quant(const void* x, const void* w, void* q, void* s, int64_t M,
 int hkq_swiglu_quant(const void* y, void* q, float* s, int64_t M, int64_t F, int64_t ldy, int64_t ldq, int64_t lds,
                      float alpha, int interleaved, int group, hkq_stream_t stream);
 
+/* Residual addition + RMSNorm + 8-bit quantization, x and res bf16 rows of D:
+ * h = bf16(x + res) (rows of ldh; res and h both NULL: h = x, not stored), then
+ * of the stored h: r = 1 / sqrt(sum(h^2) / D + eps), y = (h * r) * w, and
+ * s = max(amax / QMAX, 1e-10), q = encode(clamp(y * (1/s), +-QMAX)) per token
+ * (group 0: s[m * lds]) or per 128 columns (group 128: s[m * lds + k / 128]);
+ * kind HKQ_KIND_FP8 (E4M3FN, QMAX 448) or HKQ_KIND_INT8 (round half even,
+ * QMAX 127). The sum is fp32 in an order fixed by D; a NaN among the values of
+ * a scale makes that scale NaN. h may be x or res (same pitch). D a multiple of
+ * 8 (128 with groups) in [8, 16384]; pitches multiples of 8. No counterpart in
+ * the reference (its fused_rmsnorm_fp8_quant_fwd has no residual and 1x128
+ * scales only): what feeds the layer's first product, hkq_gemm_a8w8 /
+ * hkq_gated_ffn_a8w8 (group 0) or hkq_gemm_blockscale (group 128). */
+int hkq_add_rmsnorm_quant(const void* x, const void* res, const void* w, void* h, void* q, float* s, int64_t M,
+                          int64_t D, int64_t ldx, int64_t ldr, int64_t ldh, int64_t ldq, int64_t lds, float eps,
+                          int group, int kind, hkq_stream_t stream);
+
 /* ---- dense GEMMs (A [M, K], B [N, K], both K-contiguous; C bf16 [M, ldc]) ----
  * Row pitches: min(32, rows) rows of each operand, and of its scales, must span
  * less than 2^31 bytes; a call that no kernel can address is refused. */
@@ -234,6 +250,70 @@ int hkq_batched_gemm_bf16(const void* A, const void* B, const void* bias, void* 
                           int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int64_t batch_stride_a,
                           int64_t batch_stride_b, int64_t batch_stride_c, int64_t batch_stride_bias, void* workspace,
                           size_t workspace_bytes, hkq_stream_t stream);
+
+/* ---- products of a feed-forward layer with what follows them -------------- */
+
+/* Activations: v; max(v, 0); v / (1 + exp(-alpha v)) (the silu of
+ * hkq_swiglu_quant; alpha 1.702: the sigmoid form of GELU);
+ * v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2; v (1 + erf(v / sqrt 2)) / 2.
+ * alpha is read by HKQ_ACT_SILU only. */
+#define HKQ_ACT_NONE 0
+#define HKQ_ACT_RELU 1
+#define HKQ_ACT_SILU 2
+#define HKQ_ACT_GELU_TANH 3
+#define HKQ_ACT_GELU 4
+
+/* hkq_gemm_a8w8_ws / hkq_gemm_bf16 with a fused epilogue:
+ * C = bf16(act((A . B^T) * sa[m] * sb[n] + bias[n]) + residual[m, n]), formed in
+ * fp32 and rounded once. bias bf16 [N] and residual bf16 rows of ldr >= N
+ * elements (a multiple of 4) may be NULL; the residual may be C itself (same
+ * pitch). Shapes, strides and alignment as the plain GEMMs; the workspace is
+ * that of hkq_gemm_a8w8_workspace / hkq_gemm_bf16_workspace (NULL: no split of
+ * K over workgroups) under the rules of hkq_gemm_a8w8_ws. No counterpart in
+ * the reference beyond its block-scale multiply-add. */
+int hkq_gemm_a8w8_epilogue(const void* A, const void* B, const float* sa, const float* sb, const void* bias,
+                           const void* residual, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
+                           int64_t ldr, int64_t ldc, int act, float alpha, void* workspace, size_t workspace_bytes,
+                           hkq_stream_t stream);
+int hkq_gemm_bf16_epilogue(const void* A, const void* B, const void* bias, const void* residual, void* C, int64_t M,
+                           int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldr, int64_t ldc, int act,
+                           float alpha, void* workspace, size_t workspace_bytes, hkq_stream_t stream);
+
+/* Gated feed-forward: both projections, the activation and their product in one
+ * kernel. W [2F, ldw] holds gate and up rows, as halves (gate f at row f, up at
+ * F + f) or interleaved (rows 2f, 2f + 1), the column orders hkq_swiglu_quant
+ * takes of the unfused product:
+ *   g = (X . Wg^T) * sx[m] * swg[f],  u likewise,  H[m, f] = bf16(act(g) * u),
+ * formed from the fp32 sums. FP8: X, W E4M3FN codes, sx fp32 [M], sw fp32 [2F]
+ * in W's row order, K % 64 == 0. bf16: no scales, K % 32 == 0; Y (NULL: not
+ * kept) gets bf16(g), bf16(u) as [M, 2F] rows of ldy in W's row order, what
+ * hkq_gated_ffn_backward needs. F % 8 == 0; ldh, ldy multiples of 4; X, W, sw
+ * 16-byte, H, Y 8-byte aligned. 32 rows of W of one half (ldw, or 2 ldw
+ * interleaved, apart) and of X must span less than 2^31 bytes. No counterpart
+ * in the reference, whose gate/up product writes both halves to memory
+ * (kernels/moe-gemm/moe_op_silu_fused/kernel.cpp:1-13). */
+int hkq_gated_ffn_a8w8(const void* X, const void* W, const float* sx, const float* sw, void* H, int64_t M, int64_t F,
+                       int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int act, float alpha, int interleaved,
+                       hkq_stream_t stream);
+int hkq_gated_ffn_bf16(const void* X, const void* W, void* H, void* Y, int64_t M, int64_t F, int64_t K, int64_t ldx,
+                       int64_t ldw, int64_t ldh, int64_t ldy, int act, float alpha, int interleaved,
+                       hkq_stream_t stream);
+
+/* Gradients of the bf16 form from dH [M, F], its inputs and the kept Y:
+ *   dg = dH * u * act'(g), du = dH * act(g)  (fp32, rounded to bf16),
+ *   dX [M, K] = dg . Wg + du . Wu,  dW [2F, K] = [dg, du]^T . X in W's row order
+ * (overwritten, not accumulated; either may be NULL: not computed, and then its
+ * own other operand, W or X, may be NULL). act'(0) of ReLU is 0. F <= 2^20;
+ * lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of 4; dH, X,
+ * W, Y 16-byte, dX, dW 8-byte aligned. workspace: at least
+ * hkq_gated_ffn_backward_workspace(M, F, K) bytes, 16-byte aligned, under the
+ * rules of hkq_gemm_a8w8_ws; it holds dg and du. Three launches, no
+ * synchronisation, sums in a fixed order. */
+size_t hkq_gated_ffn_backward_workspace(int64_t M, int64_t F, int64_t K);
+int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const void* Y, void* dX, void* dW, int64_t M,
+                           int64_t F, int64_t K, int64_t lddh, int64_t ldx, int64_t ldw, int64_t ldy, int64_t lddx,
+                           int64_t lddw, int act, float alpha, int interleaved, void* workspace,
+                           size_t workspace_bytes, hkq_stream_t stream);
 
 /* ---- MoE grouped GEMM over OGS routing metadata -------------------------- */
 
