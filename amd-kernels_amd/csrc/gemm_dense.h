@@ -78,10 +78,10 @@ struct PlainOp {
     static constexpr bool FUSED = false, GATED = false, AT = false, BT = false;
 };
 
-// Activations: 0 max(v, lo) (lo -inf: none, 0: ReLU), 1 v * logistic(v (c1 + c3
-// v^2)) (SiLU with alpha: c1 = alpha; tanh GELU, whose 0.5 (1 + tanh z) is the
-// logistic function of 2z), 2 v * Phi(v), Phi the normal distribution function
-// (GELU). c1 and c3 hold a factor -log2(e).
+// Activations: 0 max(v, lo) (lo -inf: none, 0: ReLU), 1 v * logistic(c1 v) (SiLU,
+// c1 = alpha), 2 v * logistic(v (c1 + c3 v^2)) (tanh GELU, whose 0.5 (1 + tanh z)
+// is the logistic function of 2z), 3 v * Phi(v), Phi the normal distribution
+// function (GELU). c1 and c3 hold a factor -log2(e).
 struct ActParams {
     int form;
     float lo, c1, c3;
@@ -102,25 +102,33 @@ __device__ __forceinline__ float normal_cdf(float v, float* density) {
     return v < 0.0f ? tail : 1.0f - tail;
 }
 
-__device__ __forceinline__ float logistic_arg(const ActParams& a, float v) {
-    // v^2 is bounded only so that c3 = 0 never meets an infinity; the logistic
-    // function is long constant there
-    return v * __builtin_fmaf(a.c3, min_num(v * v, 1e8f), a.c1);
-}
+// 1 / (1 + 2^t)
+__device__ __forceinline__ float logistic2(float t) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)); }
 
-__device__ __forceinline__ float act1(const ActParams& a, float v) {
-    if (a.form == 0) return v < a.lo ? a.lo : v;
-    if (a.form == 1) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(logistic_arg(a, v)));
-    float d;
-    return v * normal_cdf(v, &d);
-}
-
-// The activation of four values: one uniform branch for all of them.
-__device__ __forceinline__ float4 act4(const ActParams& a, float4 v) {
+// The activation of N values: one uniform branch for all of them.
+template <int N>
+__device__ __forceinline__ void act_n(const ActParams& a, float (&v)[N]) {
     if (a.form == 0) {
-        return make_float4(v.x < a.lo ? a.lo : v.x, v.y < a.lo ? a.lo : v.y, v.z < a.lo ? a.lo : v.z, v.w < a.lo ? a.lo : v.w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] < a.lo ? a.lo : v[i];
+    } else if (a.form == 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= logistic2(a.c1 * v[i]);
+    } else if (a.form == 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= logistic2(v[i] * __builtin_fmaf(a.c3, v[i] * v[i], a.c1));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float d;
+            v[i] *= normal_cdf(v[i], &d);
+        }
     }
-    return make_float4(act1(a, v.x), act1(a, v.y), act1(a, v.z), act1(a, v.w));
+}
+__device__ __forceinline__ float4 act4(const ActParams& a, float4 v) {
+    float x[4] = {v.x, v.y, v.z, v.w};
+    act_n(a, x);
+    return make_float4(x[0], x[1], x[2], x[3]);
 }
 
 struct FusedParams : DenseParams {
@@ -176,8 +184,10 @@ constexpr int dense_ring_lds() {
     constexpr int NS = dense_ns<KTB>();
     return Whole::lds_bytes(NS) > Half::lds_bytes(NS) ? Whole::lds_bytes(NS) : Half::lds_bytes(NS);
 }
-template <int MODE, int KTB>
-constexpr int dense_lds() { return dense_ring_lds<MODE, KTB>() + (MODE == MODE_A8W8 ? 2 * DENSE_BM * 4 : 0); }
+template <class Op, int MODE, int KTB>
+constexpr int dense_lds() {
+    return dense_ring_lds<MODE, KTB>() + (MODE == MODE_A8W8 ? 2 * DENSE_BM * 4 : 0) + (Op::FUSED ? DENSE_BN * 2 : 0);
+}
 
 // K loop of one (WM*TM*32) x (WN*TN*32) block of C at (m0, n0) over K-tiles
 // [kt0, kt1): the operand sources start kt0 K-tiles into the rows, so the
@@ -411,6 +421,241 @@ __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&ac
     }
 }
 
+// Epilogue of the 256-column tiles with something to compute per element: as
+// stream_store_tile, groups of 32 rows x 64 columns through the wave's staging
+// area, but over loops instead of unrolled code. Unrolled over a wave's 256
+// accumulators the activation's instructions alone (every form of it) passed the
+// instruction cache and each tile fetched them anew: bf16 4096x28672x4096
+// without any activation 772 us against the plain GEMM's 683. A group's
+// accumulators are picked by a switch (register numbers cannot be computed), the
+// rest is one copy of the code. Stores and residual loads are buffer operations
+// that every lane issues, out of range where its row or column is: the stream
+// counts them. tile: the tile's row scales, column scales (256 fp32 each, A8W8)
+// and bias (256 bf16, FUSED) in LDS; wr / wc: the wave's first row / column of it.
+template <int N>
+__device__ __forceinline__ void read_acc(const v16f& a, float (&v)[N], int at) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[at + e]) : "a"(a[e]));
+}
+
+// A group's staged 32 rows x 64 columns (row pitch STREAM_STG_PITCH) to rows
+// [0, rows) and columns [0, cols) at `base`.
+__device__ __forceinline__ void store_group(const HKQ_LDS uint8_t* stg, int lane, uint16_t* base, int64_t ld, int rows, int cols) {
+    const auto rc = make_rsrc(base, 0x7FFFFFFFu);
+    const int sr = lane >> 3, sc = (lane & 7) * 8;
+    const bool ragged = cols < 64 && (cols & 7) != 0;
+    v4i d[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        d[q] = *reinterpret_cast<const HKQ_LDS v4i*>(stg + (q * 8 + sr) * STREAM_STG_PITCH + (lane & 7) * 16);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int m = q * 8 + sr;
+        const uint32_t at = (uint32_t)((m * ld + sc) * 2);
+        __builtin_amdgcn_raw_buffer_store_b128(d[q], rc, m < rows && sc + 8 <= cols ? at : OOB, 0, CPOL_NT);
+        if (ragged)
+            __builtin_amdgcn_raw_buffer_store_b64(v2i{d[q][0], d[q][1]}, rc, m < rows && sc + 4 == cols ? at : OOB, 0, CPOL_NT);
+    }
+}
+
+template <int MODE>
+constexpr int epi_bias_at() { return MODE == MODE_A8W8 ? 2 * DENSE_BM * 4 : 0; }  // LDS: bias after the scales
+template <class Op, int MODE>
+constexpr int epi_lds() { return epi_bias_at<MODE>() + (Op::FUSED ? DENSE_BN * 2 : 0); }
+
+// The tile's scales and bias into LDS, 64 values of each per wave (rows past M
+// and columns past N read zero); every wave issues the same loads.
+template <class Op, int MODE>
+__device__ __forceinline__ void load_tile_params(const typename Op::Params& p, HKQ_LDS uint8_t* to, int m0, int n0, int rows,
+                                                 int cols, int wave, int lane) {
+    const int c = wave * 64 + lane;
+    if constexpr (MODE == MODE_A8W8) {
+        lds_load4(static_cast<const float*>(p.sa) + m0, (uint32_t)rows * 4u, to + wave * 256, (uint32_t)c * 4u);
+        if constexpr (Op::GATED) {
+            // tile column c of wave column c / 128: a gate column where c % 128 < 64
+            const int f = n0 / 2 + gated_row<DENSE_TN>(c), up = c % (DENSE_TN * 32) >= DENSE_TN * 16;
+            lds_load4(p.sb, (uint32_t)p.F * 8u, to + DENSE_BM * 4 + wave * 256,
+                      f < p.F ? (uint32_t)(p.interleaved ? 2 * f + up : f + up * p.F) * 4u : OOB);
+        } else {
+            lds_load4(static_cast<const float*>(p.sb) + n0, (uint32_t)cols * 4u, to + DENSE_BM * 4 + wave * 256, (uint32_t)c * 4u);
+        }
+    }
+    // bias: two columns per dword, so 128 dwords (waves 2 and 3 load waves 0 and 1's again)
+    if constexpr (Op::FUSED)
+        lds_load4(p.bias + n0, p.bias ? (uint32_t)cols * 2u : 0u, to + epi_bias_at<MODE>() + (wave & 1) * 256,
+                  (uint32_t)((wave & 1) * 64 + lane) * 4u);
+}
+
+template <class Op, int MODE, int TM, int TN>
+__device__ __forceinline__ void rolled_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], const HKQ_LDS uint8_t* tile,
+                                                  HKQ_LDS uint8_t* stg, int lane, int mw, int nw, int wr, int wc) {
+    static_assert(TN == 4, "two groups of columns per wave");
+    constexpr bool A8 = MODE == MODE_A8W8;
+    int ln = lane;  // opaque copy: the lane's offsets stay out of the tile loop's prologue
+    asm volatile("" : "+v"(ln));
+    const int khalf = ln >> 5, r = ln & 31;
+    const HKQ_LDS float* rows_s = reinterpret_cast<const HKQ_LDS float*>(tile) + wr;
+    const HKQ_LDS float* cols_s = reinterpret_cast<const HKQ_LDS float*>(tile) + DENSE_BM + wc + 4 * khalf;
+    HKQ_LDS uint8_t* wr_at = stg + r * STREAM_STG_PITCH + 8 * khalf;
+    // values of n-tile i of the group's column scales: 16 per lane
+    auto scales = [&](int i, float (&s)[16]) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const v4f c = *reinterpret_cast<const HKQ_LDS v4f*>(cols_s + i * 32 + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = c[e];
+        }
+    };
+    auto put = [&](int ii, const float (&v)[16]) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<HKQ_LDS v2i*>(wr_at + (ii * 32 + 8 * g) * 2) =
+                v2i{(int)pk_bf16(v[4 * g], v[4 * g + 1]), (int)pk_bf16(v[4 * g + 2], v[4 * g + 3])};
+    };
+
+    if constexpr (Op::FUSED) {
+        const int sr = ln >> 3, sc = (ln & 7) * 8;
+        const int rows = p.M - mw, cols = p.N - nw;
+        // the residual's 32 x 64 values of a group: whole row pieces, one group ahead
+        v4i res[4];
+        auto load_res = [&](int ip, int j) {
+            const int64_t first = (int64_t)(mw + j * 32) * p.ldr + nw + ip * 64;
+            const int rr = min(rows - j * 32, 32);
+            // reads at or past the last row's end give zeros; what lies past the columns is not stored
+            const auto rs = make_rsrc(p.residual + first, rr > 0 && cols > ip * 64
+                                                              ? (uint32_t)(((rr - 1) * p.ldr + min(cols - ip * 64, 64)) * 2) : 0u);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                res[q] = __builtin_amdgcn_raw_buffer_load_b128(rs, (uint32_t)(((q * 8 + sr) * p.ldr + sc) * 2), 0, 0);
+        };
+        if (p.residual) load_res(0, 0);
+#pragma unroll 1
+        for (int ip = 0; ip < TN / 2; ++ip) {
+            float cs[2][16];
+            v2i cb[2][4];
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii) {
+                if constexpr (A8) scales(2 * ip + ii, cs[ii]);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    cb[ii][g] = *reinterpret_cast<const HKQ_LDS v2i*>(tile + epi_bias_at<MODE>() +
+                                                                      (wc + ip * 64 + ii * 32 + 8 * g + 4 * khalf) * 2);
+            }
+#pragma unroll 1
+            for (int j = 0; j < TM; ++j) {
+                if (p.residual) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<HKQ_LDS v4i*>(stg + (q * 8 + sr) * STREAM_STG_PITCH + (ln & 7) * 16) = res[q];
+                    if (j + 1 < TM) load_res(ip, j + 1);
+                    else if (ip + 1 < TN / 2) load_res(ip + 1, 0);
+                }
+                float v[32];
+                switch (ip * TM + j) {
+#define HKQ_PICK(S)                                                          \
+    case S:                                                                  \
+        if constexpr (S < TM * TN / 2) {                                     \
+            read_acc(acc[S / TM * 2][S % TM], v, 0);                         \
+            read_acc(acc[S / TM * 2 + 1][S % TM], v, 16);                    \
+        }                                                                    \
+        break;
+                    HKQ_PICK(0) HKQ_PICK(1) HKQ_PICK(2) HKQ_PICK(3) HKQ_PICK(4) HKQ_PICK(5) HKQ_PICK(6) HKQ_PICK(7)
+#undef HKQ_PICK
+                }
+                const float a = A8 ? rows_s[j * 32 + r] : 1.0f;
+#pragma unroll
+                for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t w = (uint32_t)cb[ii][g][e >> 1];
+                            const float b = bf16_to_f32(e & 1 ? w >> 16 : w & 0xFFFF);
+                            float& x = v[16 * ii + 4 * g + e];
+                            x = A8 ? x * a * cs[ii][4 * g + e] + b : x + b;
+                        }
+                act_n(p.act, v);
+                if (p.residual) {
+#pragma unroll
+                    for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const v2i rv = *reinterpret_cast<const HKQ_LDS v2i*>(wr_at + (ii * 32 + 8 * g) * 2);
+                            float* x = v + 16 * ii + 4 * g;
+                            const float4 o = add_bf16x4(make_float4(x[0], x[1], x[2], x[3]), rv);
+                            x[0] = o.x, x[1] = o.y, x[2] = o.z, x[3] = o.w;
+                        }
+                }
+                float lo[16], hi[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) lo[e] = v[e], hi[e] = v[16 + e];
+                put(0, lo);
+                put(1, hi);
+                // a wave's LDS operations complete in order: the reads see the writes
+                store_group(stg, ln, p.C + (int64_t)(mw + j * 32) * p.ldc + nw + ip * 64, p.ldc, rows - j * 32, cols - ip * 64);
+            }
+        }
+    } else {
+        const int fw = nw / 2, rows = p.M - mw, cols = p.F - fw;
+        // out 0: act(gate) * up; 1, 2: gate and up themselves (interleaved: 1, 2
+        // are the pairs of the group's first and second 32 features)
+#pragma unroll 1
+        for (int out = 0; out < (p.Y ? 3 : 1); ++out) {
+#pragma unroll 1
+            for (int j = 0; j < TM; ++j) {
+                const float a = A8 ? rows_s[j * 32 + r] : 1.0f;
+#pragma unroll 1
+                for (int ii = 0; ii < 2; ++ii) {
+                    float g[16], u[16];
+                    switch (ii * TM + j) {
+#define HKQ_PICK(S)                                            \
+    case S:                                                    \
+        if constexpr (S < TM * 2) {                            \
+            read_acc(acc[S / TM][S % TM], g, 0);               \
+            read_acc(acc[S / TM + 2][S % TM], u, 0);           \
+        }                                                      \
+        break;
+                        HKQ_PICK(0) HKQ_PICK(1) HKQ_PICK(2) HKQ_PICK(3) HKQ_PICK(4) HKQ_PICK(5) HKQ_PICK(6) HKQ_PICK(7)
+#undef HKQ_PICK
+                    }
+                    if constexpr (A8) {
+                        float cg[16], cu[16];
+                        scales(ii, cg);
+                        scales(ii + 2, cu);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) g[e] *= a * cg[e], u[e] *= a * cu[e];
+                    }
+                    if (out == 0) {
+                        act_n(p.act, g);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) g[e] *= u[e];
+                        put(ii, g);
+                    } else if (!p.interleaved) {
+                        if (out == 1) put(ii, g);
+                        else put(ii, u);
+                    } else if (ii == out - 1) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            *reinterpret_cast<HKQ_LDS v4i*>(stg + r * STREAM_STG_PITCH + (8 * q + 4 * khalf) * 4) =
+                                v4i{(int)pk_bf16(g[4 * q], u[4 * q]), (int)pk_bf16(g[4 * q + 1], u[4 * q + 1]),
+                                    (int)pk_bf16(g[4 * q + 2], u[4 * q + 2]), (int)pk_bf16(g[4 * q + 3], u[4 * q + 3])};
+                    }
+                }
+                uint16_t* base = out == 0 ? p.C : p.Y;
+                const int64_t ld = out == 0 ? p.ldc : p.ldy;
+                int col = fw, left = cols;
+                if (out != 0 && p.interleaved) {
+                    col = 2 * fw + (out - 1) * 64;
+                    left = 2 * cols - (out - 1) * 64;
+                } else if (out == 2) {
+                    col += p.F;
+                }
+                store_group(stg, ln, base + (int64_t)(mw + j * 32) * ld + col, ld, rows - j * 32, left);
+            }
+        }
+    }
+}
+
 // One (TM*64) x 256 block of C: rows [m0, m0 + TM*64) of tile (tm, tn) of the
 // 256 x 256 tile grid, starting `half` * 128 rows into the tile, on an NS-stage
 // K-tile ring (the tile's row and column scales follow the ring).
@@ -435,19 +680,7 @@ __device__ __forceinline__ void dense_block(const typename Op::Params& p, int tm
     // These loads are older than the K-tile loads, so the loop's vmcnt waits
     // cover them, and its final vmcnt(0) barrier makes them visible.
     HKQ_LDS uint8_t* scl = smem + RING;
-    if constexpr (MODE == MODE_A8W8) {
-        const float* sa = static_cast<const float*>(p.sa) + m0;
-        const float* sb = static_cast<const float*>(p.sb) + n0;
-        lds_load4(sa, (uint32_t)rows_a * 4u, scl + wave * 256, (uint32_t)(wave * 64 + lane) * 4u);
-        if constexpr (Op::GATED) {
-            // tile column c of wave column c / 128: a gate column where c % 128 < 64
-            const int c = wave * 64 + lane, f = n0 / 2 + gated_row<TN>(c), up = c % (TN * 32) >= TN * 16;
-            lds_load4(p.sb, (uint32_t)p.F * 8u, scl + DENSE_BM * 4 + wave * 256,
-                      f < p.F ? (uint32_t)(p.interleaved ? 2 * f + up : f + up * p.F) * 4u : OOB);
-        } else {
-            lds_load4(sb, (uint32_t)rows_b * 4u, scl + DENSE_BM * 4 + wave * 256, (uint32_t)(wave * 64 + lane) * 4u);
-        }
-    }
+    load_tile_params<Op, MODE>(p, scl, m0, n0, rows_a, rows_b, wave, lane);
 
     v16f acc[TN][TM];
     dense_kloop<Op, MODE, WAVES_M, WAVES_N, TM, TN, KTB, NS>(p, m0, n0, 0, p.kbytes / KTB, smem, acc);
@@ -466,10 +699,8 @@ __device__ __forceinline__ void dense_block(const typename Op::Params& p, int tm
         }
         return make_float4(1.f, 1.f, 1.f, 1.f);
     };
-    if constexpr (Op::FUSED)
-        fused_store_tile<Op, TM, TN>(p, acc, EpiResidual<Op, TM, TN>{}, smem, wave, lane, mw, nw, row_scale, col_scale4);
-    else if constexpr (Op::GATED)
-        gated_store_tile<TM, TN>(p, acc, smem, wave, lane, mw, nw / 2, row_scale, col_scale4);
+    if constexpr (Op::FUSED || Op::GATED)
+        rolled_store_tile<Op, MODE, TM, TN>(p, acc, scl, smem + wave * STREAM_STG, lane, mw, nw, wm * TM * 32, wn * TN * 32);
     else if (p.bias)
         store_tile_bf16<TM, TN>(acc, smem, wave, lane, p.C, p.ldc, p.M, p.N, mw, nw, p.c16 != 0, row_scale, col_scale4,
                                 [&](int i, int g) { return bias4(p, nw + i * 32 + 8 * g + 4 * khalf); });
@@ -523,7 +754,6 @@ __global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_g
 // and its K loop is bound by that traffic; the deeper ring gives the loads
 // two K-tiles of lead (measured on MI355X, with the staged epilogue below:
 // 4096 x 14336 x 4096 308.8K -> 293.7K cycles per workgroup, 179.4 -> 173.8 us).
-constexpr int STREAM_SCL = 2 * DENSE_BM * 4;  // one scale slot: 256 row + 256 column scales
 constexpr int HALF_NS = 3;                    // ring stages of a half tile
 
 template <int MODE>
@@ -532,22 +762,22 @@ constexpr int stream_ring_lds() {
     return 2 * Whole::STAGE + Whole::SB_BYTES;
 }
 // The staging areas follow the ring and (A8W8) the two scale slots.
-template <int MODE>
-constexpr int stream_stg_off() { return stream_ring_lds<MODE>() + (MODE == MODE_A8W8 ? 2 * STREAM_SCL : 0); }
-template <int MODE>
+template <class Op, int MODE>
+constexpr int stream_stg_off() { return stream_ring_lds<MODE>() + 2 * epi_lds<Op, MODE>(); }
+template <class Op, int MODE>
 constexpr int stream_lds() {
     using Half = DenseCfg<MODE, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM / 2, DENSE_TN, 128>;
-    constexpr int whole = stream_stg_off<MODE>() + DENSE_WAVES_M * DENSE_WAVES_N * STREAM_STG;
-    constexpr int half = Half::lds_bytes(HALF_NS) + (MODE == MODE_A8W8 ? 2 * DENSE_BM * 4 : 0);
+    constexpr int whole = stream_stg_off<Op, MODE>() + DENSE_WAVES_M * DENSE_WAVES_N * STREAM_STG;
+    constexpr int half = Half::lds_bytes(HALF_NS) + epi_lds<Op, MODE>();
     return whole > half ? whole : half;
 }
 
 // Tile k of the stream: tile id first + k * stride in tile_coords order,
 // rows [tm*256 + half*BM, +BM) of it.
-template <int BM>
+template <class Op, int BM>
 struct DenseSeq {
     static constexpr bool GATHER = false;
-    const DenseParams* p;
+    const typename Op::Params* p;
     int tiles, KT;
     uint32_t lsa, lsb;
     int first, stride, half;
@@ -566,6 +796,12 @@ struct DenseSeq {
         s.b = p->B + (int64_t)n0 * p->ldb;
         s.a_bytes = clamp_bytes((int64_t)(rows_a - 1) * p->lda + p->kbytes);
         s.b_bytes = clamp_bytes((int64_t)(rows_b - 1) * p->ldb + p->kbytes);
+        if constexpr (Op::GATED) {
+            const int f0 = n0 / 2;
+            s.b = p->B + (int64_t)f0 * p->ldb;
+            s.b2 = p->Bu + (int64_t)f0 * p->ldb;
+            s.b_bytes = clamp_bytes((int64_t)(min(p->F - f0, DENSE_BN / 2) - 1) * p->ldb + p->kbytes);
+        }
         s.as = static_cast<const uint8_t*>(p->sa) + (int64_t)m0 * p->lsa;
         s.bs = static_cast<const uint8_t*>(p->sb) + (int64_t)n0 * p->lsb;
         s.as_bytes = (uint32_t)min((int64_t)rows_a * p->lsa, (int64_t)0x7FFFFFFF);
@@ -574,28 +810,24 @@ struct DenseSeq {
     }
 };
 
-template <int MODE, int TM, int BM>
+template <class Op, int MODE, int TM, int BM>
 struct DirectEpi {
     static constexpr int TN = DENSE_TN;
     // vector-memory instructions a wave issues in end() (at least: ragged
-    // tiles add 8-byte stores) plus the next begin(); the stream's first
-    // barrier after an epilogue leaves that many in flight
-    static constexpr int VM_ISSUED = TN * TM * 2 + (MODE == MODE_A8W8 ? 2 : 0);
-    const DenseSeq<BM>* seq;
-    const DenseParams* p;
-    HKQ_LDS uint8_t* scl;  // 2 slots of STREAM_SCL bytes
+    // tiles add 8-byte stores, a residual its loads, kept projections their
+    // stores) plus the next begin(); the stream's first barrier after an
+    // epilogue leaves that many in flight
+    static constexpr int VM_ISSUED = (Op::GATED ? TM * 4 : TN * TM * 2) + (MODE == MODE_A8W8 ? 2 : 0) + (Op::FUSED ? 1 : 0);
+    const DenseSeq<Op, BM>* seq;
+    const typename Op::Params* p;
+    HKQ_LDS uint8_t* scl;  // 2 slots of epi_lds() bytes
     HKQ_LDS uint8_t* stg;  // this wave's STREAM_STG bytes of staging
     int lane, wave;
     __device__ void begin(int k) {
-        if constexpr (MODE == MODE_A8W8) {
-            int m0, n0;
-            seq->coords(k, m0, n0);
-            const int rows_a = min(p->M - m0, BM), rows_b = min(p->N - n0, DENSE_BN);
-            HKQ_LDS uint8_t* slot = scl + (k & 1) * STREAM_SCL;
-            const uint32_t off = (uint32_t)(wave * 64 + lane) * 4u;
-            lds_load4(static_cast<const float*>(p->sa) + m0, (uint32_t)rows_a * 4u, slot + wave * 256, off);
-            lds_load4(static_cast<const float*>(p->sb) + n0, (uint32_t)rows_b * 4u, slot + DENSE_BM * 4 + wave * 256, off);
-        }
+        int m0, n0;
+        seq->coords(k, m0, n0);
+        load_tile_params<Op, MODE>(*p, scl + (k & 1) * epi_lds<Op, MODE>(), m0, n0, min(p->M - m0, BM),
+                                   min(p->N - n0, DENSE_BN), wave, lane);
     }
     // Stores through the wave's staging area (stream_store_tile), with the
     // tile's row and column scales from its LDS slot.
@@ -604,41 +836,48 @@ struct DirectEpi {
         seq->coords(k, m0, n0);
         const int wm = wave / DENSE_WAVES_N, wn = wave % DENSE_WAVES_N;
         const int khalf = lane >> 5, r = lane & 31;
-        const HKQ_LDS float* sl = reinterpret_cast<const HKQ_LDS float*>(scl + (k & 1) * STREAM_SCL);
+        const HKQ_LDS uint8_t* slot = scl + (k & 1) * epi_lds<Op, MODE>();
+        const HKQ_LDS float* sl = reinterpret_cast<const HKQ_LDS float*>(slot);
         const int mw0 = m0 + wm * TM * 32, nw0 = n0 + wn * TN * 32;
-        float rs[TM];
+        if constexpr (Op::FUSED || Op::GATED) {
+            rolled_store_tile<Op, MODE, TM, TN>(*p, acc, slot, stg, lane, mw0, nw0, wm * TM * 32, wn * TN * 32);
+            return;
+        } else {
+            float rs[TM];
 #pragma unroll
-        for (int j = 0; j < TM; ++j) rs[j] = MODE == MODE_A8W8 ? sl[wm * TM * 32 + j * 32 + r] : 1.0f;
-        stream_store_tile<TM, TN>(
-            acc, stg, p->C + (int64_t)mw0 * p->ldc + nw0, p->ldc, p->M - mw0, p->N - nw0, rs,
-            [&](int i, int g) {
-                return MODE == MODE_A8W8 ? *reinterpret_cast<const HKQ_LDS v4f*>(sl + DENSE_BM + wn * TN * 32 + i * 32 +
-                                                                                 8 * g + 4 * khalf)
-                                         : v4f{1.f, 1.f, 1.f, 1.f};
-            },
-            lane);
+            for (int j = 0; j < TM; ++j) rs[j] = MODE == MODE_A8W8 ? sl[wm * TM * 32 + j * 32 + r] : 1.0f;
+            stream_store_tile<TM, TN>(
+                acc, stg, p->C + (int64_t)mw0 * p->ldc + nw0, p->ldc, p->M - mw0, p->N - nw0, rs,
+                [&](int i, int g) {
+                    return MODE == MODE_A8W8 ? *reinterpret_cast<const HKQ_LDS v4f*>(sl + DENSE_BM + wn * TN * 32 + i * 32 +
+                                                                                     8 * g + 4 * khalf)
+                                             : v4f{1.f, 1.f, 1.f, 1.f};
+                },
+                lane);
+        }
     }
 };
 
-template <int MODE, int TM>
-__device__ __forceinline__ void dense_stream(const DenseParams& p, int tiles, int first, int stride, int half,
+template <class Op, int MODE, int TM>
+__device__ __forceinline__ void dense_stream(const typename Op::Params& p, int tiles, int first, int stride, int half,
                                              HKQ_LDS uint8_t* smem) {
     constexpr int WM = DENSE_WAVES_M, WN = DENSE_WAVES_N, TN = DENSE_TN;
     using Cfg = DenseCfg<MODE, WM, WN, TM, TN, 128>;
     constexpr int BM = Cfg::BM;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    DenseSeq<BM> seq{&p, tiles, p.kbytes / 128, (uint32_t)p.lsa, (uint32_t)p.lsb, first, stride, half};
-    DirectEpi<MODE, TM, BM> epi{&seq, &p, smem + stream_ring_lds<MODE>(),
-                                smem + stream_stg_off<MODE>() + wave * STREAM_STG, lane, wave};
+    DenseSeq<Op, BM> seq{&p, tiles, p.kbytes / 128, (uint32_t)p.lsa, (uint32_t)p.lsb, first, stride, half};
+    DirectEpi<Op, MODE, TM, BM> epi{&seq, &p, smem + stream_ring_lds<MODE>(),
+                                    smem + stream_stg_off<Op, MODE>() + wave * STREAM_STG, lane, wave};
     auto a_off = dense_offs<Cfg::NW, 128, Cfg::LA>(wave, lane, p.lda);
-    const auto b_off = dense_offs<Cfg::NW, 128, Cfg::LB>(wave, lane, p.ldb);
+    const auto b_off = Op::GATED ? dense_offs_gated<Cfg::NW, 128, Cfg::LB, TN>(wave, lane, p.ldb)
+                                 : dense_offs<Cfg::NW, 128, Cfg::LB>(wave, lane, p.ldb);
     v16f acc[TN][TM];
-    gemm_stream<MODE, WM, WN, TM, TN>(seq, a_off, b_off, smem, lane, wave, acc, epi);
+    gemm_stream<MODE, WM, WN, TM, TN, false, Op::GATED>(seq, a_off, b_off, smem, lane, wave, acc, epi);
 }
 
-template <int MODE>
-__global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_stream_kernel(const DenseParams p) {
+template <class Op, int MODE>
+__global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_stream_kernel(const typename Op::Params p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
     HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
     const int b = blockIdx.x, G = gridDim.x;
@@ -653,13 +892,13 @@ __global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_s
     int tm = 0, tn = 0;
     if (has_half) tile_coords(p.n_whole + t, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
     if (half_first && has_half) {
-        dense_block<PlainOp, MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
+        dense_block<Op, MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
         // the stream's first loads overwrite the half tile's staging: every
         // wave's LDS reads are done first (its C stores may still drain)
         lds_barrier();
     }
-    if (mine > 0) dense_stream<MODE, DENSE_TM>(p, mine, b, G, 0, smem);
-    if (!half_first && has_half) dense_block<PlainOp, MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
+    if (mine > 0) dense_stream<Op, MODE, DENSE_TM>(p, mine, b, G, 0, smem);
+    if (!half_first && has_half) dense_block<Op, MODE, DENSE_TM / 2, 128, HALF_NS>(p, tm, tn, (b >> 3) & 1, smem);
 }
 
 // ---------------------------------------------------------------------------
@@ -1288,7 +1527,7 @@ static int launch_dense_tiles(typename Op::Params& p, int splits, int kt_split, 
 
 template <class Op, int MODE, int KTB>
 static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
-    constexpr int LDS = dense_lds<MODE, KTB>();
+    constexpr int LDS = dense_lds<Op, MODE, KTB>();
     static_assert(LDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
     auto kern = dense_gemm_kernel<Op, MODE, KTB>;
     static bool attr_set = false;  // per instantiation; the attribute is per-process
@@ -1310,7 +1549,7 @@ static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
     // MXFP4 stays on the one-tile kernel: its stream (the K loop below with
     // compile-time scale slots, C stored from registers since the ring and the
     // scale blocks fill the LDS) spills and measured 1.8x slower on MI355X.
-    if constexpr (KTB == 128 && MODE != MODE_MXFP4 && std::is_same<Op, PlainOp>::value) {
+    if constexpr (KTB == 128 && MODE != MODE_MXFP4 && !Op::AT && !Op::BT) {
         // the persistent streaming kernel: one workgroup per CU, whole tiles as
         // a K-tile stream (needs K-tiles per tile % 8 == 0; one 2-D GEMM without
         // bias, C's rows 16-byte aligned); HKQ_DENSE_STREAM=0 selects the
@@ -1326,11 +1565,11 @@ static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
         // the split needs 2 * roundup8(split) workgroups: grids that cannot hold
         // them within one per CU take the one-tile kernel.
         const int64_t g = std::min<int64_t>(ncu, std::max<int64_t>(p.n_whole, 2 * ((split + 7) / 8 * 8)));
-        if (stream_on && ncu > 0 && !batched && p.bias == nullptr && (p.kbytes / 128) % 8 == 0 && p.c16 &&
+        if (stream_on && ncu > 0 && !batched && (Op::FUSED || p.bias == nullptr) && (p.kbytes / 128) % 8 == 0 && p.c16 &&
             2 * ((split + 7) / 8 * 8) <= g) {
-            constexpr int SLDS = stream_lds<MODE>();
+            constexpr int SLDS = stream_lds<Op, MODE>();
             static_assert(SLDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
-            auto skern = dense_stream_kernel<MODE>;
+            auto skern = dense_stream_kernel<Op, MODE>;
             static bool sattr = false;
             if (int e = set_lds(skern, SLDS, sattr)) return e;
             skern<<<dim3((unsigned)g), 64 * DENSE_WAVES_M * DENSE_WAVES_N, SLDS, stream>>>(p);

@@ -22,8 +22,8 @@ static bool make_act(int act, float alpha, ActParams& a) {
         case HKQ_ACT_NONE: return true;
         case HKQ_ACT_RELU: a.lo = 0.f; return true;
         case HKQ_ACT_SILU: a.form = 1; a.c1 = -LOG2E * alpha; return true;
-        case HKQ_ACT_GELU_TANH: a.form = 1; a.c1 = -LOG2E * TANH_C1; a.c3 = a.c1 * 0.044715f; return true;
-        case HKQ_ACT_GELU: a.form = 2; return true;
+        case HKQ_ACT_GELU_TANH: a.form = 2; a.c1 = -LOG2E * TANH_C1; a.c3 = a.c1 * 0.044715f; return true;
+        case HKQ_ACT_GELU: a.form = 3; return true;
     }
     return false;
 }
@@ -40,9 +40,12 @@ __device__ __forceinline__ void act_grad(const ActParams& p, float v, float& f, 
     if (p.form == 0) {
         f = v < p.lo ? p.lo : v;
         df = v > p.lo ? 1.0f : 0.0f;
-    } else if (p.form == 1) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(logistic_arg(p, v)));
-        const float slope = -0.69314718056f * __builtin_fmaf(3.0f * p.c3, min_num(v * v, 1e8f), p.c1);
+    } else if (p.form <= 2) {  // SiLU: c3 = 0
+        // v^2 is bounded only so that a c3 of zero, or the logistic function's
+        // saturation, never meets an infinity
+        const float q = min_num(v * v, 1e8f);
+        const float s = logistic2(v * __builtin_fmaf(p.c3, q, p.c1));
+        const float slope = -0.69314718056f * __builtin_fmaf(3.0f * p.c3, q, p.c1);
         f = v * s;
         df = __builtin_fmaf(f * (1.0f - s), slope, s);
     } else {
@@ -168,12 +171,12 @@ static int gemm_epilogue(const void* A, const void* B, const float* sa, const fl
     HKQ_CHECK_ARG(M >= 0 && N >= 0 && K > 0, "M, N must be >= 0 and K > 0");
     HKQ_CHECK_ARG(M < (1 << 30) && N < (1 << 30) && K < (1 << 30), "dimensions must be < 2^30");
     HKQ_CHECK_ARG(N % 4 == 0, "N must be a multiple of 4");
-    HKQ_CHECK_ARG(ldc >= N && ldc % 4 == 0, "ldc must be >= N and a multiple of 4");
+    HKQ_CHECK_ARG(ldc >= N && ldc % 4 == 0 && ldc < (1 << 24), "ldc must be >= N, a multiple of 4 and < 2^24");
     HKQ_CHECK_ARG(MODE == MODE_BF16 || K % 64 == 0, "K must be a multiple of 64");
     HKQ_CHECK_ARG(MODE != MODE_BF16 || K % 32 == 0, "K must be a multiple of 32");
     HKQ_CHECK_ARG(lda >= K && ldb >= K && lda * ES % 16 == 0 && ldb * ES % 16 == 0,
                   "lda/ldb must be >= K and keep rows 16-byte aligned");
-    HKQ_CHECK_ARG(!residual || (ldr >= N && ldr % 4 == 0), "ldr must be >= N and a multiple of 4");
+    HKQ_CHECK_ARG(!residual || (ldr >= N && ldr % 4 == 0 && ldr < (1 << 24)), "ldr must be >= N, a multiple of 4 and < 2^24");
     FusedParams p{};
     if (int e = check_act(act, alpha, p.act)) return e;
     HKQ_CHECK_ARG(residual != C || ldr == ldc || !residual, "a residual in place of C must have its pitch");
@@ -213,8 +216,8 @@ static int gated_ffn(const void* X, const void* W, const float* sx, const float*
     HKQ_CHECK_ARG(MODE != MODE_BF16 || K % 32 == 0, "K must be a multiple of 32");
     HKQ_CHECK_ARG(ldx >= K && ldw >= K && ldx * ES % 16 == 0 && ldw * ES % 16 == 0,
                   "ldx/ldw must be >= K and keep rows 16-byte aligned");
-    HKQ_CHECK_ARG(ldh >= F && ldh % 4 == 0, "ldh must be >= F and a multiple of 4");
-    HKQ_CHECK_ARG(!Y || (ldy >= 2 * F && ldy % 4 == 0), "ldy must be >= 2F and a multiple of 4");
+    HKQ_CHECK_ARG(ldh >= F && ldh % 4 == 0 && ldh < (1 << 24), "ldh must be >= F, a multiple of 4 and < 2^24");
+    HKQ_CHECK_ARG(!Y || (ldy >= 2 * F && ldy % 4 == 0 && ldy < (1 << 24)), "ldy must be >= 2F, a multiple of 4 and < 2^24");
     FusedParams p{};
     if (int e = check_act(act, alpha, p.act)) return e;
     if (M == 0 || F == 0) return 0;

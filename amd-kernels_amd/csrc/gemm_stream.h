@@ -24,6 +24,7 @@ struct StreamSrc {
     const uint8_t *a, *b;    // the tile's first A / B row
     const uint8_t *as, *bs;  // MXFP4: its first e8m0 scale rows
     uint32_t a_bytes, b_bytes, as_bytes, bs_bytes;  // loads at or past these read zero
+    const uint8_t* b2 = nullptr;  // GATED: the first row of the up half (b: of the gate half)
 };
 
 // Seq: { int tiles; int KT; uint32_t lsa, lsb; __device__ StreamSrc src(int t) const;  (t < tiles)
@@ -38,8 +39,9 @@ struct StreamSrc {
 //   not touch the LDS ring. On return every wave is past a vmcnt(0) barrier.
 // BT: B tiles N-contiguous (KTileT layout, transposed fragment reads; the
 // sequence then provides b_kstep, the bytes from one K-tile of B to the next).
-template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, bool BT = false, typename AOff, typename BOff,
-          typename Seq, typename Epi>
+// GATED: B rows from the two halves of a gate/up weight (gemm_mainloop).
+template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, bool BT = false, bool GATED = false, typename AOff,
+          typename BOff, typename Seq, typename Epi>
 __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const BOff& b_off, HKQ_LDS uint8_t* smem,
                                             int lane, int wave, v16f (&acc)[TN][TM], Epi& epi) {
     constexpr int KTB = 128, NS = 2;
@@ -126,7 +128,9 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
             const int i = idx - LA;
             uint32_t kbb = kb;
             if constexpr (BT) kbb = (uint32_t)kl * seq.b_kstep;
-            lds_load16_u(ld.b + kbb, ld_live && ld.b_bytes > kbb ? ld.b_bytes - kbb : 0u,
+            const uint8_t* b = ld.b;
+            if constexpr (GATED) b = gated_up<Cfg, TN>(i) ? ld.b2 : ld.b;
+            lds_load16_u(b + kbb, ld_live && ld.b_bytes > kbb ? ld.b_bytes - kbb : 0u,
                          wave_dst(Cfg::b_stage(NS, stage) + i * NW * 1024), b_off.v[i]);
         }
     };

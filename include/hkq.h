@@ -266,8 +266,8 @@ int hkq_batched_gemm_bf16(const void* A, const void* B, const void* bias, void* 
 /* hkq_gemm_a8w8_ws / hkq_gemm_bf16 with a fused epilogue:
  * C = bf16(act((A . B^T) * sa[m] * sb[n] + bias[n]) + residual[m, n]), formed in
  * fp32 and rounded once. bias bf16 [N] and residual bf16 rows of ldr >= N
- * elements (a multiple of 4) may be NULL; the residual may be C itself (same
- * pitch). Shapes, strides and alignment as the plain GEMMs; the workspace is
+ * elements (a multiple of 4; ldr, ldc < 2^24) may be NULL; the residual may be C
+ * itself (same pitch). Shapes, strides and alignment as the plain GEMMs; the workspace is
  * that of hkq_gemm_a8w8_workspace / hkq_gemm_bf16_workspace (NULL: no split of
  * K over workgroups) under the rules of hkq_gemm_a8w8_ws. No counterpart in
  * the reference beyond its block-scale multiply-add. */
@@ -287,7 +287,7 @@ int hkq_gemm_bf16_epilogue(const void* A, const void* B, const void* bias, const
  * formed from the fp32 sums. FP8: X, W E4M3FN codes, sx fp32 [M], sw fp32 [2F]
  * in W's row order, K % 64 == 0. bf16: no scales, K % 32 == 0; Y (NULL: not
  * kept) gets bf16(g), bf16(u) as [M, 2F] rows of ldy in W's row order, what
- * hkq_gated_ffn_backward needs. F % 8 == 0; ldh, ldy multiples of 4; X, W, sw
+ * hkq_gated_ffn_backward needs. F % 8 == 0; ldh, ldy multiples of 4 below 2^24; X, W, sw
  * 16-byte, H, Y 8-byte aligned. 32 rows of W of one half (ldw, or 2 ldw
  * interleaved, apart) and of X must span less than 2^31 bytes. No counterpart
  * in the reference, whose gate/up product writes both halves to memory
