@@ -230,15 +230,11 @@ __device__ __forceinline__ void dense_kloop(const typename Op::Params& p, int m0
     }
     // rows of K across memory: columns m0 / n0 of every row from kt0 K-tiles on
     if constexpr (Op::AT) {
-        src.a = p.A + (int64_t)kt0 * 64 * p.lda + (int64_t)m0 * 2;
-        src.a_bytes = (int64_t)(p.K - kt0 * 64 - 1) * p.lda + rows_a * 2;
-        src.a_kstep = 64 * p.lda;
+        src.ta = T16Src::of(p.A + (int64_t)m0 * 2, p.lda, rows_a, kt0 * 64, p.K, kt1);
         a_off = dense_offs_t16<NW, Cfg::LA, BM>(wave, lane, p.lda);
     }
     if constexpr (Op::BT) {
-        src.b = p.B + (int64_t)kt0 * 64 * p.ldb + (int64_t)n0 * 2;
-        src.b_bytes = (int64_t)(p.K - kt0 * 64 - 1) * p.ldb + rows_b * 2;
-        src.b_kstep = 64 * p.ldb;
+        src.tb = T16Src::of(p.B + (int64_t)n0 * 2, p.ldb, rows_b, kt0 * 64, p.K, kt1);
         b_off = dense_offs_t16<NW, Cfg::LB, BN>(wave, lane, p.ldb);
     }
     gemm_mainloop<MODE, WM, WN, TM, TN, KTB, NS, Op::BT, Op::AT, Op::GATED>(src, a_off, b_off, smem, lane, wave, acc);
@@ -802,6 +798,8 @@ struct DenseSeq {
             s.b2 = p->Bu + (int64_t)f0 * p->ldb;
             s.b_bytes = clamp_bytes((int64_t)(min(p->F - f0, DENSE_BN / 2) - 1) * p->ldb + p->kbytes);
         }
+        if constexpr (Op::AT) s.ta = T16Src::of(p->A + (int64_t)m0 * 2, p->lda, rows_a, 0, p->K, KT);
+        if constexpr (Op::BT) s.tb = T16Src::of(p->B + (int64_t)n0 * 2, p->ldb, rows_b, 0, p->K, KT);
         s.as = static_cast<const uint8_t*>(p->sa) + (int64_t)m0 * p->lsa;
         s.bs = static_cast<const uint8_t*>(p->sb) + (int64_t)n0 * p->lsb;
         s.as_bytes = (uint32_t)min((int64_t)rows_a * p->lsa, (int64_t)0x7FFFFFFF);
@@ -869,11 +867,15 @@ __device__ __forceinline__ void dense_stream(const typename Op::Params& p, int t
     DenseSeq<Op, BM> seq{&p, tiles, p.kbytes / 128, (uint32_t)p.lsa, (uint32_t)p.lsb, first, stride, half};
     DirectEpi<Op, MODE, TM, BM> epi{&seq, &p, smem + stream_ring_lds<MODE>(),
                                     smem + stream_stg_off<Op, MODE>() + wave * STREAM_STG, lane, wave};
-    auto a_off = dense_offs<Cfg::NW, 128, Cfg::LA>(wave, lane, p.lda);
-    const auto b_off = Op::GATED ? dense_offs_gated<Cfg::NW, 128, Cfg::LB, TN>(wave, lane, p.ldb)
-                                 : dense_offs<Cfg::NW, 128, Cfg::LB>(wave, lane, p.ldb);
+    TableOff<Cfg::LA> a_off;
+    TableOff<Cfg::LB> b_off;
+    if constexpr (Op::AT) a_off = dense_offs_t16<Cfg::NW, Cfg::LA, BM>(wave, lane, p.lda);
+    else a_off = dense_offs<Cfg::NW, 128, Cfg::LA>(wave, lane, p.lda);
+    if constexpr (Op::GATED) b_off = dense_offs_gated<Cfg::NW, 128, Cfg::LB, TN>(wave, lane, p.ldb);
+    else if constexpr (Op::BT) b_off = dense_offs_t16<Cfg::NW, Cfg::LB, Cfg::BN>(wave, lane, p.ldb);
+    else b_off = dense_offs<Cfg::NW, 128, Cfg::LB>(wave, lane, p.ldb);
     v16f acc[TN][TM];
-    gemm_stream<MODE, WM, WN, TM, TN, false, Op::GATED>(seq, a_off, b_off, smem, lane, wave, acc, epi);
+    gemm_stream<MODE, WM, WN, TM, TN, Op::BT, Op::AT, Op::GATED>(seq, a_off, b_off, smem, lane, wave, acc, epi);
 }
 
 template <class Op, int MODE>
@@ -1348,6 +1350,20 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
             src.s_off[i] = (uint32_t)(r * (q < Cfg::PA ? p.lsa : p.lsb)) + kg_piece_half(lane);
         }
     }
+    if constexpr (Op::AT) {
+        using T = KTileT16<BM>;
+        const int r = wg * T::ROWS_PER_LOAD + lane / (T::ROW / 16);
+        src.ta = T16Src::of(p.A + (int64_t)m0 * 2, p.lda, rows_a, 0, p.K, src.KT);
+        src.a_off[0] = (uint32_t)(r * p.lda) + (uint32_t)(T::phys(r, lane % (T::ROW / 16)) << 4);
+        src.a_step = (uint32_t)(Cfg::GW * T::ROWS_PER_LOAD * p.lda);
+    }
+    if constexpr (Op::BT) {
+        using T = KTileT16<BN>;
+        const int r = wg * T::ROWS_PER_LOAD + lane / (T::ROW / 16);
+        src.tb = T16Src::of(p.B + (int64_t)n0 * 2, p.ldb, rows_b, 0, p.K, src.KT);
+        src.b_off[0] = (uint32_t)(r * p.ldb) + (uint32_t)(T::phys(r, lane % (T::ROW / 16)) << 4);
+        src.b_step = (uint32_t)(Cfg::GW * T::ROWS_PER_LOAD * p.ldb);
+    }
     const int mw = m0 + wg / Cfg::WN * TM * 32, nw = n0 + wg % Cfg::WN * TN * 32;
     EpiScales<Op, MODE, TM, TN> sc;
     sc.load(p, lane, mw, nw);
@@ -1355,7 +1371,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
     if (kg == 0) res.load(p, lane, mw, nw);
 
     v16f acc[TN][TM];
-    kgroup_kloop<Cfg, false, Op::GATED>(src, smem, lane, wg, kg, acc);
+    kgroup_kloop<Cfg, false, Op::GATED, Op::AT, Op::BT>(src, smem, lane, wg, kg, acc);
     if (kg != 0) return;
     dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wg, lane, mw, nw);
 }
@@ -1549,7 +1565,7 @@ static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
     // MXFP4 stays on the one-tile kernel: its stream (the K loop below with
     // compile-time scale slots, C stored from registers since the ring and the
     // scale blocks fill the LDS) spills and measured 1.8x slower on MI355X.
-    if constexpr (KTB == 128 && MODE != MODE_MXFP4 && !Op::AT && !Op::BT) {
+    if constexpr (KTB == 128 && MODE != MODE_MXFP4) {
         // the persistent streaming kernel: one workgroup per CU, whole tiles as
         // a K-tile stream (needs K-tiles per tile % 8 == 0; one 2-D GEMM without
         // bias, C's rows 16-byte aligned); HKQ_DENSE_STREAM=0 selects the
@@ -1594,13 +1610,13 @@ static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
 // on, 1 row from two rounds (1x9216x4096 8.5, 8.9; 4 rows 9.4, 9.0) and 4 rows
 // from three (4x12288x4096 9.6, 10.6; 4x28672x4096 19.8, 20.6; 8x28672x4096
 // 22.0, 20.6; 4x28672x2048 14.6, 12.8). Its buffer offsets are 32-bit.
-static bool use_narrow(int mode, const DenseParams& p, int64_t batch) {
+static bool use_narrow(int mode, const DenseParams& p, int64_t batch, int64_t cols) {
     const int64_t step = mode == MODE_MXFP4 ? 64 : 128, S = p.kbytes / step;
     if (p.M < 1 || p.kbytes % step != 0 || S > NARROW_MAX_STEPS) return false;
     const int64_t wide = (1ll << 31) / NARROW_ROWS;
     if (p.lda >= wide || p.ldb >= wide || p.lsa >= wide || p.lsb >= wide) return false;
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
-    const int64_t groups = (p.M + NARROW_ROWS - 1) / NARROW_ROWS, wgs = batch * ((p.N + 15) / 16);
+    const int64_t groups = (p.M + NARROW_ROWS - 1) / NARROW_ROWS, wgs = batch * ((cols + 15) / 16);
     if (groups <= 4 && groups * wgs <= ncu) return mode == MODE_A8W8 || S <= 16 || p.M <= 8;
     return mode == MODE_A8W8 && S >= 24 && p.M <= (wgs >= 3 * ncu ? 4 : wgs >= 2 * ncu ? 1 : 0);
 }
@@ -1615,8 +1631,8 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
         if (MODE == MODE_MXFP4) p.lsa = p.K / 32;
     }
     if constexpr (MODE != MODE_BF16) {
-        if (use_narrow(MODE, p, batch)) {
-            const int cols = Op::GATED ? p.N / 2 : p.N;
+        const int cols = Op::GATED ? p.N / 2 : p.N;  // gated: a workgroup's 16 columns are 16 features
+        if (use_narrow(MODE, p, batch, cols)) {
             const dim3 grid((unsigned)((cols + 15) / 16), (unsigned)batch, (unsigned)((p.M + NARROW_ROWS - 1) / NARROW_ROWS));
             narrow_gemm_kernel<Op, MODE><<<grid, 64 * NARROW_WAVES, 0, stream>>>(p);
             return hkq_launch_status();

@@ -105,29 +105,43 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restr
     }
 }
 
-// Plan of a backward product over `KT` K-tiles of 64: 256 x 256 tiles, 128 x 128
-// tiles on two workgroups per CU, or the latter with K split over workgroups
-// (partial sums in the workspace) where they fill at most half of the CUs. Costs
-// as in dense_tile_plan's bf16 table.
+// Plan of a backward product over `KT` K-tiles of 64: the least estimated time
+// over the tile sizes, rounds over the CUs * (K-tiles * us + e), or 128 x 128
+// tiles with K split over workgroups (partial sums in the workspace), one round
+// of them. us and e fitted to MI355X times of every size at 16 .. 4096 tokens of
+// two layers (K-tiles of one size cost more the more of the weight comes from
+// memory; the constants are those of a large one). Tokens x F x K, us: dX
+// 4096x14336x4096 256 x 256 672, 128 x 256 784, 128 x 128 1047; 2048x14336x4096
+// 417 (M halves), 394, 516; 1001x2816x2048 128 x 64 31, 128 x 128 36, two splits
+// 30; 64x2816x2048 21, 30, eight splits 14. dW 1001x2816x2048 256 x 256 27, 128 x
+// 256 32, 128 x 128 31; 1001x1408x2048 17, 15, 19.
 struct TransPlan {
-    int tile;  // DT_256, DT_128x128_PAIR or DT_SPLIT
+    int tile;  // a DenseTile
     int splits, kt_split;
     size_t ws_bytes;
 };
 static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT) {
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
-    auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
-    auto rounds = [](int64_t n, int64_t d) { return (float)((n + d - 1) / d); };
-    const int64_t t128 = tiles(128);
-    const float us256 = rounds(tiles(256), ncu) * ((float)KT * 0.647f + 2.1f);
-    const float us128 = t128 <= ncu ? (float)KT * 0.559f + 0.6f : rounds(t128, 2 * ncu) * ((float)KT * 0.645f + 0.9f);
-    TransPlan p{us256 <= us128 ? DT_256 : DT_128x128_PAIR, 1, (int)KT, 0};
-    if (2 * t128 <= ncu && KT >= 8) {
-        const int64_t s = std::min<int64_t>((ncu + t128 - 1) / t128, KT / 4);
-        if (s > 1) {
-            const int64_t per = (KT + s - 1) / s, n = (KT + per - 1) / per;
-            if ((float)per * 0.494f + 5.5f + 1.2f * (float)n < std::min(us256, us128))
-                p = TransPlan{DT_SPLIT, (int)n, (int)per, SPLIT_CNT_BYTES + (size_t)(n * t128) * (128 * 128 * 4)};
+    static const struct { int tile, bm, bn; TileCost c; } T[] = {
+        {DT_256, 256, 256, {1.37f, 5.7f}}, {DT_128x256, 128, 256, {0.85f, 3.2f}}, {DT_128x128, 128, 128, {0.57f, 2.2f}},
+        {DT_128x64, 128, 64, {0.40f, 2.0f}}};
+    TransPlan p{DT_256, 1, (int)KT, 0};
+    float best = 0.f;
+    for (const auto& t : T) {
+        const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn), rounds = (tiles + ncu - 1) / ncu;
+        float us = (float)rounds * ((float)KT * t.c.us + t.c.e);
+        // few tiles run as M halves (launch_dense_whole)
+        if (t.tile == DT_256 && 2 * tiles <= ncu && M > 128) us = (float)KT * 0.88f + 3.0f;
+        if (best == 0.f || us < best) p.tile = t.tile, best = us;
+    }
+    const int64_t t128 = ((M + 127) / 128) * ((N + 127) / 128);
+    const int64_t most = t128 <= SPLIT_MAX_TILES ? std::min<int64_t>(ncu / t128, KT / 4) : 0;
+    for (int64_t s = 2; s <= most; ++s) {
+        const int64_t per = (KT + s - 1) / s, n = (KT + per - 1) / per;
+        const float us = (float)per * 0.62f + 6.5f + 1.2f * (float)n;
+        if (us < best) {
+            best = us;
+            p = TransPlan{DT_SPLIT, (int)n, (int)per, SPLIT_CNT_BYTES + (size_t)(n * t128) * (128 * 128 * 4)};
         }
     }
     return p;
@@ -139,9 +153,13 @@ static int launch_trans(DenseParams& p, void* ws, hipStream_t stream) {
     using Op = TransOp<AT, true>;
     p.c16 = p.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
     const TransPlan pl = trans_plan(p.M, p.N, p.kbytes / 128);
-    if (pl.tile == DT_256) return launch_dense_whole<Op, MODE_BF16, 128>(p, stream);
-    if (pl.tile == DT_128x128_PAIR) return launch_dense_tiles<Op, MODE_BF16, 2, 2, 2, 2, 128, 2>(p, 1, p.kbytes / 128, nullptr, stream);
-    return launch_dense_tiles<Op, MODE_BF16, 2, 2, 2, 2, 128, 1, 4>(p, pl.splits, pl.kt_split, ws, stream);
+    switch (pl.tile) {
+        case DT_128x64: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 1, 2, 1, 2, 3>>(p, stream);
+        case DT_128x128: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 2, 1, 1, 2, 4>>(p, stream);
+        case DT_128x256: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 2, 4, 1, 2, 2, 3>>(p, stream);
+        case DT_SPLIT: return launch_dense_tiles<Op, MODE_BF16, 2, 2, 2, 2, 128, 1, 4>(p, pl.splits, pl.kt_split, ws, stream);
+    }
+    return launch_dense_whole<Op, MODE_BF16, 128>(p, stream);
 }
 
 // Row pitch (values) of the projections' gradients, and their place in the

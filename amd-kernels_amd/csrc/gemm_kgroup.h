@@ -84,6 +84,7 @@ struct KgSrc {
     v4i b2;  // GATED: the up half's rows; b: the gate half's (8-wave groups: each wave's own half)
     uint32_t a_off[NA], b_off[Cfg::SWP];
     uint32_t a_step, b_step;  // bytes between load i and load i + SWP (linear operands)
+    T16Src ta, tb;            // AT / BT (bf16, K across memory rows)
     uint32_t s_off[Cfg::PW > 0 ? Cfg::PW : 1], c_off[Cfg::LC > 0 ? Cfg::LC : 1];
     uint32_t bs_step;
     int sc_shift;
@@ -130,7 +131,9 @@ __device__ __forceinline__ void lds_load4_s(const v4i& desc, HKQ_LDS void* dst, 
 // GATED (see gemm_mainloop): with w = GW waves, loads idx of a wave alternate
 // between the halves every GP loads (8-wave groups: waves 4 .. 7 load the up
 // half); b_step is then the step between a half's own loads.
-template <class Cfg, bool GATHER, bool GATED = false>
+// AT / BT: A M-contiguous / B N-contiguous (bf16, KTileT16), groups of several
+// waves: one lane offset serves all of an operand's loads.
+template <class Cfg, bool GATHER, bool GATED = false, bool AT = false, bool BT = false>
 __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_LDS uint8_t* smem, int lane, int wg, int kg,
                                              v16f (&out)[Cfg::TN][Cfg::TM]) {
     using KT = typename Cfg::KT;
@@ -171,10 +174,26 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
             }
         }
     };
+    static_assert(!(AT || BT) || (Cfg::MODE == MODE_BF16 && GW > 1 && !GATHER && !GATED), "transposed operands");
+    v4i t16_a, t16_b;  // the buffers of the K-tile that is being loaded
+    T16Cursor cur_a{src.ta.base + k0 * src.ta.kstep}, cur_b{src.tb.base + k0 * src.tb.kstep};
+    auto t16_next = [&](int t) {
+        const int end = t < mine ? src.KT : 0;
+        if constexpr (AT) t16_a = cur_a.next(src.ta, k0 + t, end);
+        if constexpr (BT) t16_b = cur_b.next(src.tb, k0 + t, end);
+    };
     auto issue_piece = [&](int t, int stage, int idx) {
         const int kt = k0 + t;
         const bool live = t < mine;
         HKQ_LDS uint8_t* st = gbase + stage * STAGE;
+        if (BT && idx < LB) {
+            lds_load16_s(t16_b, st + Cfg::BM * 128 + (idx * GW + wg) * 1024, src.b_off[0], (uint32_t)idx * src.b_step);
+            return;
+        }
+        if (AT && idx >= LB && idx < LB + LA) {
+            lds_load16_s(t16_a, st + ((idx - LB) * GW + wg) * 1024, src.a_off[0], (uint32_t)(idx - LB) * src.a_step);
+            return;
+        }
         const uint32_t kb = live ? (uint32_t)kt * 128u : OOB;
         constexpr int SWP = Cfg::SWP;
         const uint32_t tail = src.half_tail && kt == src.KT - 1 ? OOB : 0u;
@@ -204,6 +223,7 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
     };
     auto issue = [&](int t, int stage) {
         issue_scales(t);
+        t16_next(t);
 #pragma unroll
         for (int i = 0; i < NLD; ++i) issue_piece(t, stage, i);
     };
@@ -216,6 +236,10 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int q = 0; q < 2; ++q) lo[ks][q] = (uint32_t)KT::swz(r, BS ? 4 * ks + 2 * khalf + q : 4 * khalf + 2 * ks + q);
+
+    const uint32_t group = (uint32_t)(uintptr_t)gbase;
+    const TBase<TN> bt = BT ? tr16_bases<TN, Cfg::BN>(group + (uint32_t)(Cfg::BM * 128), wn * TN * 32, lane) : TBase<TN>{};
+    const TBase<TM> att = AT ? tr16_bases<TM, Cfg::BM>(group, wm * TM * 32, lane) : TBase<TM>{};
 
     v16f acc[TN][TM];
 #pragma unroll
@@ -237,6 +261,16 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
         const HKQ_LDS uint8_t* st = gbase + stage * STAGE;
         const bool isb = p == 0 || p > TM;
         const int i = p == 0 ? 0 : isb ? p - TM : p - 1;
+        if ((BT && isb) || (AT && !isb)) {
+            const uint32_t at = (isb ? bt.v[isb ? i : 0] : att.v[isb ? 0 : i]) + (uint32_t)(stage * STAGE);
+            const int row = isb ? KTileT16<Cfg::BN>::ROW : KTileT16<Cfg::BM>::ROW;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    (isb ? f.b[isb ? i : 0] : f.a[isb ? 0 : i])[ks][q] = read_t16(at + (uint32_t)(8 * (2 * ks + q) * row), row);
+            return;
+        }
         const HKQ_LDS uint8_t* base = isb ? st + (Cfg::BM + (wn * TN + i) * 32) * 128 : st + (wm * TM + i) * 32 * 128;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
@@ -352,6 +386,7 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
             const int next = stage + 1 == NS ? 0 : stage + 1;
             tile_barrier<(NS - 2) * NLD>();
             issue_scales(t + NS);
+            t16_next(t + NS);
             mma(cur, [&](int s) {
 #pragma unroll
                 for (int i = s * NLD / (TN * TM); i < (s + 1) * NLD / (TN * TM); ++i) issue_piece(t + NS, stage, i);

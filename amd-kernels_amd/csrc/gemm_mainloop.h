@@ -63,6 +63,37 @@ struct DenseCfg {
     static_assert((TN * 32 * 2) % 128 == 0, "epilogue rows are whole 128-byte segments");
 };
 
+// A bf16 operand with K across memory rows: the tile's first column in row 0 of
+// K, and the bytes of a K-tile's 64 rows from one to the next, to the end of a
+// whole one's last row, and of the last one's (loads at or past these read
+// zero). The extent of the whole operand may pass 32 bits, so the base moves
+// from K-tile to K-tile (T16Cursor).
+struct T16Src {
+    const uint8_t* base = nullptr;
+    int64_t kstep = 0;
+    uint32_t whole = 0, last = 0;
+    // rows [k0, K) of an operand of rows ld bytes apart, `cols` columns from `at`
+    // on, in K-tiles up to row kt * 64
+    __device__ static T16Src of(const uint8_t* at, int64_t ld, int cols, int k0, int K, int kt) {
+        T16Src s;
+        s.base = at + (int64_t)k0 * ld;
+        s.kstep = 64 * ld;
+        s.whole = (uint32_t)(63 * ld + cols * 2);
+        const int rest = K - (kt - 1) * 64;  // rows in the last K-tile
+        s.last = rest >= 64 ? s.whole : rest > 0 ? (uint32_t)((rest - 1) * ld + cols * 2) : 0u;
+        return s;
+    }
+};
+// The buffer of the next K-tile, in K order.
+struct T16Cursor {
+    const uint8_t* at;
+    __device__ __forceinline__ v4i next(const T16Src& s, int kt, int KT) {
+        const v4i d = buffer_desc(at, kt + 1 < KT ? s.whole : kt < KT ? s.last : 0u);
+        at += s.kstep;
+        return d;
+    }
+};
+
 // Where one workgroup's K-tiles come from. `a`/`b` point at the tile's first
 // row (or at the tensor base when rows are gathered); loads at byte offsets at
 // or beyond the *_bytes bounds read zero. FP4 only: the e8m0 scale rows.
@@ -79,10 +110,10 @@ struct LoopSrc {
     // scale row is at r * lsa.
     bool sa_gathered = false;
     uint32_t sa_row[4] = {0u, 0u, 0u, 0u};
-    // N-contiguous B (BT) and M-contiguous A (AT): bytes from one K-tile to the
-    // next (FP8, FP4: 128 rows of K; bf16: 64, where the extents may pass 2^31
-    // as a whole)
-    int64_t a_kstep = 0, b_kstep = 0;
+    // N-contiguous B (BT) of FP8 and FP4: bytes from one K-tile to the next (128
+    // rows of K)
+    int64_t b_kstep = 0;
+    T16Src ta, tb;  // bf16: M-contiguous A (AT), N-contiguous B (BT)
     // GATED: first row of the up half; `b` is that of the gate half, b_bytes the
     // extent of either
     const uint8_t* b2 = nullptr;
@@ -213,6 +244,14 @@ __device__ __forceinline__ TBase<T> tr16_bases(uint32_t region, int wave_col, in
     return o;
 }
 
+// The lane's 8 values of K of its column, from two transposed reads of 4 rows
+// (`row` bytes each).
+__device__ __forceinline__ v4i read_t16(uint32_t base, int row) {
+    const v2i lo = lds_read_tr16(reinterpret_cast<const HKQ_LDS uint8_t*>((uintptr_t)base));
+    const v2i hi = lds_read_tr16(reinterpret_cast<const HKQ_LDS uint8_t*>((uintptr_t)(base + (uint32_t)(4 * row))));
+    return v4i{lo[0], lo[1], hi[0], hi[1]};
+}
+
 // Pipeline (per wave; one barrier per K-tile, NS ring stages):
 //   K-tile kt lives in stage kt % NS. Its SUB K-steps run their MFMAs with
 //   double-buffered fragments: the LDS reads of the next step are issued between
@@ -315,12 +354,13 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
     const v4i desc_a = buffer_desc(src.a, (uint32_t)(src.a_bytes < 0x7FFFFFFF ? (src.a_bytes > 0 ? src.a_bytes : 0) : 0x7FFFFFFF));
     const v4i desc_b = buffer_desc(src.b, (uint32_t)(src.b_bytes < 0x7FFFFFFF ? (src.b_bytes > 0 ? src.b_bytes : 0) : 0x7FFFFFFF));
     const v4i desc_b2 = buffer_desc(src.b2, (uint32_t)(src.b_bytes < 0x7FFFFFFF ? (src.b_bytes > 0 ? src.b_bytes : 0) : 0x7FFFFFFF));
-    // bf16 AT / BT: a K-tile's rows start kt K-tiles into the operand, whose
-    // extent may pass 32 bits, so the base moves and the extent is what is left
-    auto load_t16 = [&](const uint8_t* base, int64_t bytes, int64_t kstep, int kt, HKQ_LDS uint8_t* dst, uint32_t off) {
-        const int64_t at = (int64_t)kt * kstep;
-        const int64_t left = kt < KTN && bytes > at ? bytes - at : 0;
-        lds_load16_u(base + at, (uint32_t)(left < 0x7FFFFFFF ? left : 0x7FFFFFFF), dst, off);
+    // bf16 AT / BT: the buffers of the K-tile that is being loaded, made once
+    // before its loads
+    v4i t16_a, t16_b;
+    T16Cursor cur_a{src.ta.base}, cur_b{src.tb.base};
+    auto t16_next = [&](int kt) {
+        if constexpr (AT) t16_a = cur_a.next(src.ta, kt, KTN);
+        if constexpr (BT16) t16_b = cur_b.next(src.tb, kt, KTN);
     };
 
     // Load instruction idx of K-tile kt into `stage`: A rows, B rows, then (FP4)
@@ -342,13 +382,13 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
             }
         }
         if (AT && idx < LA) {
-            load_t16(src.a, src.a_bytes, src.a_kstep, kt, smem + Cfg::a_stage(NS, stage) + (idx * NW + wave) * 1024, a_off.v[idx]);
+            lds_load16_d(t16_a, smem + Cfg::a_stage(NS, stage) + (idx * NW + wave) * 1024, a_off.v[idx]);
         } else if (idx < LA) {
             lds_load16_d(desc_a, smem + Cfg::a_stage(NS, stage) + (idx * NW + wave) * 1024,
                          live ? a_off.v[idx] + (uint32_t)kb : 0x80000000u);
         } else if (BT16 && idx < LA + LB) {
             const int i = idx - LA;
-            load_t16(src.b, src.b_bytes, src.b_kstep, kt, smem + Cfg::b_stage(NS, stage) + (i * NW + wave) * 1024, b_off.v[i]);
+            lds_load16_d(t16_b, smem + Cfg::b_stage(NS, stage) + (i * NW + wave) * 1024, b_off.v[i]);
         } else if (idx < LA + LB) {
             const int i = idx - LA;
             if constexpr (GATED) {
@@ -401,13 +441,6 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
                               : TBase<TN>{};
     const TBase<TM> at = AT ? tr16_bases<TM, BM>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::a_stage(NS, 0), wm * TM * 32, lane)
                             : TBase<TM>{};
-    // the lane's 8 values of K 32h + 8 (2 ks + part) .. +7 of its column: two
-    // transposed reads of 4 rows each
-    auto read_t16 = [](uint32_t base, int row) {
-        const v2i lo = lds_read_tr16(reinterpret_cast<const HKQ_LDS uint8_t*>((uintptr_t)base));
-        const v2i hi = lds_read_tr16(reinterpret_cast<const HKQ_LDS uint8_t*>((uintptr_t)(base + (uint32_t)(4 * row))));
-        return v4i{lo[0], lo[1], hi[0], hi[1]};
-    };
 
     struct Frags {
         v4i a[TM][PARTS], b[TN][PARTS];
@@ -545,9 +578,11 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
         for (int i = 0; i < NLD; ++i) load_piece(1, 1, i, Q0{});
     } else {
 #pragma unroll
-        for (int t = 0; t < NS; ++t)
+        for (int t = 0; t < NS; ++t) {
+            t16_next(t);
 #pragma unroll
             for (int i = 0; i < NLD; ++i) load_piece(t, t, i, Q0{});
+        }
     }
     tile_barrier<(NS - 1) * NLD>();  // K-tile 0 (and everything issued before it) resident
 #pragma unroll
@@ -588,6 +623,7 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
         for (int c = 0; c < PRE; ++c) mfma_one(cur, LAST, S[P], c);
         __builtin_amdgcn_sched_barrier(0);
         tile_barrier<(NS - 2) * NLD>();  // K-tile kt+1 resident; stage kt % NS retired
+        t16_next(kt + NS);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < POST; ++c) {

@@ -25,6 +25,7 @@ struct StreamSrc {
     const uint8_t *as, *bs;  // MXFP4: its first e8m0 scale rows
     uint32_t a_bytes, b_bytes, as_bytes, bs_bytes;  // loads at or past these read zero
     const uint8_t* b2 = nullptr;  // GATED: the first row of the up half (b: of the gate half)
+    T16Src ta, tb;                // bf16 AT / BT
 };
 
 // Seq: { int tiles; int KT; uint32_t lsa, lsb; __device__ StreamSrc src(int t) const;  (t < tiles)
@@ -39,9 +40,9 @@ struct StreamSrc {
 //   not touch the LDS ring. On return every wave is past a vmcnt(0) barrier.
 // BT: B tiles N-contiguous (KTileT layout, transposed fragment reads; the
 // sequence then provides b_kstep, the bytes from one K-tile of B to the next).
-// GATED: B rows from the two halves of a gate/up weight (gemm_mainloop).
-template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, bool BT = false, bool GATED = false, typename AOff,
-          typename BOff, typename Seq, typename Epi>
+// GATED, AT, bf16 BT: as in gemm_mainloop.
+template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, bool BT = false, bool AT = false, bool GATED = false,
+          typename AOff, typename BOff, typename Seq, typename Epi>
 __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const BOff& b_off, HKQ_LDS uint8_t* smem,
                                             int lane, int wave, v16f (&acc)[TN][TM], Epi& epi) {
     constexpr int KTB = 128, NS = 2;
@@ -55,7 +56,9 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
     constexpr int HCH = KTB / 32;
     static_assert(SUB == 2 && !Cfg::SK, "128-byte K-tiles");
     static_assert((NS - 1) * NLD + 3 <= 63, "vmcnt budget");
-    static_assert(!BT || (Cfg::BN == KTileT::ROW && MODE == MODE_A8W8), "N-contiguous B: FP8 tiles of 256 columns");
+    constexpr bool BT16 = BT && MODE == MODE_BF16;
+    static_assert(!BT || BT16 || (Cfg::BN == KTileT::ROW && MODE == MODE_A8W8), "N-contiguous B: FP8 tiles of 256 columns");
+    static_assert(!AT || MODE == MODE_BF16, "M-contiguous A: bf16");
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
     const int KTN = seq.KT;
 
@@ -110,6 +113,14 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
                      su_off[K]);
     };
 
+    // bf16 AT / BT: the buffers of K-tile kl of `ld`, made once before its loads
+    v4i t16_a, t16_b;
+    T16Cursor cur_a{ld.ta.base}, cur_b{ld.tb.base};
+    auto t16_next = [&](int kl) {
+        if constexpr (AT) t16_a = cur_a.next(ld.ta, kl, ld_live ? KTN : 0);
+        if constexpr (BT16) t16_b = cur_b.next(ld.tb, kl, ld_live ? KTN : 0);
+    };
+
     // load instruction idx of K-tile kl of `ld` into `stage`; MXFP4: scale
     // unit kl + SB_KT - 1 of `ls` (slot KS), counted in `ls`'s own K-tiles
     // (kl + SB_KT - 1 - KTN once `ls` has switched ahead of `ld`)
@@ -121,13 +132,17 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
             }
         }
         const uint32_t kb = (uint32_t)(kl * KTB);
-        if (idx < LA) {
+        if (AT && idx < LA) {
+            lds_load16_d(t16_a, wave_dst(Cfg::a_stage(NS, stage) + idx * NW * 1024), a_off.v[idx]);
+        } else if (BT16 && idx >= LA) {
+            lds_load16_d(t16_b, wave_dst(Cfg::b_stage(NS, stage) + (idx - LA) * NW * 1024), b_off.v[idx - LA]);
+        } else if (idx < LA) {
             lds_load16_u(ld.a + kb, ld_live && ld.a_bytes > kb ? ld.a_bytes - kb : 0u,
                          wave_dst(Cfg::a_stage(NS, stage) + idx * NW * 1024), a_off.v[idx]);
         } else {
             const int i = idx - LA;
             uint32_t kbb = kb;
-            if constexpr (BT) kbb = (uint32_t)kl * seq.b_kstep;
+            if constexpr (BT && !BT16) kbb = (uint32_t)kl * seq.b_kstep;
             const uint8_t* b = ld.b;
             if constexpr (GATED) b = gated_up<Cfg, TN>(i) ? ld.b2 : ld.b;
             lds_load16_u(b + kbb, ld_live && ld.b_bytes > kbb ? ld.b_bytes - kbb : 0u,
@@ -155,14 +170,28 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
 
     // A lane's operand of one 64-byte K-step: two 16-byte parts (FP8: the two
     // halves of one MFMA operand; FP4 and BF16: one operand each).
-    const TBase<TN> bt = BT ? tr_bases<TN>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::b_stage(NS, 0), wn * TN * 32, lane)
-                            : TBase<TN>{};
+    const TBase<TN> bt = BT16 ? tr16_bases<TN, Cfg::BN>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::b_stage(NS, 0), wn * TN * 32, lane)
+                         : BT ? tr_bases<TN>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::b_stage(NS, 0), wn * TN * 32, lane)
+                              : TBase<TN>{};
+    const TBase<TM> at = AT ? tr16_bases<TM, BM>((uint32_t)(uintptr_t)smem + (uint32_t)Cfg::a_stage(NS, 0), wm * TM * 32, lane)
+                            : TBase<TM>{};
     struct Frags {
         v4i a[TM][PARTS], b[TN][PARTS];
     };
     auto read_piece = [&](int stage, int ks, Frags& f, int idx) {
         const int t = idx / (2 * PARTS), isb = (idx / PARTS) & 1, part = idx % PARTS;
         if ((isb ? TN : TM) <= t) return;
+        if (BT16 && isb) {
+            f.b[t][part] = read_t16(bt.v[t] + (uint32_t)(Cfg::b_stage(NS, stage) - Cfg::b_stage(NS, 0)) +
+                                        (uint32_t)(8 * (2 * ks + part) * KTileT16<Cfg::BN>::ROW),
+                                    KTileT16<Cfg::BN>::ROW);
+            return;
+        }
+        if (AT && !isb) {
+            f.a[t][part] = read_t16(at.v[t] + (uint32_t)Cfg::a_stage(NS, stage) + (uint32_t)(8 * (2 * ks + part) * KTileT16<BM>::ROW),
+                                    KTileT16<BM>::ROW);
+            return;
+        }
         if (BT && isb) {
             // see gemm_mainloop: two transposed reads of 8 rows of K each
             const uint32_t b = bt.v[t] + (uint32_t)(Cfg::b_stage(NS, stage) - Cfg::b_stage(NS, 0)) +
@@ -239,8 +268,10 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         load_scale_unit(1, Q1{});
         load_scale_unit(2, Q2{});
     }
+    t16_next(0);
 #pragma unroll
     for (int i = 0; i < NLD; ++i) load_piece(0, Cfg::SB_KT - 1, 0, i, Q3{});
+    t16_next(1);
 #pragma unroll
     for (int i = 0; i < NLD; ++i) load_piece(1, Cfg::SB_KT, 1, i, Q0{});
     tile_barrier<(NS - 1) * NLD>();
@@ -282,6 +313,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         }
         __builtin_amdgcn_sched_barrier(0);
         tile_barrier<VM>();  // K-tile kt+1 resident; this stage retired
+        t16_next(kl);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < NMF; ++c) {
@@ -340,6 +372,8 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         }
         ld_live = t + 1 < seq.tiles;
         ld = seq.src(min(t + 1, seq.tiles - 1));
+        cur_a.at = ld.ta.base;
+        cur_b.at = ld.tb.base;
         if constexpr (Seq::GATHER) seq.a_rows(min(t + 1, seq.tiles - 1), a_off);
         ktile(KTN - 2, Q2{}, F0{}, F0{});
         ktile(KTN - 1, Q3{}, F0{}, std::true_type{});
