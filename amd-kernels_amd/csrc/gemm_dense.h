@@ -652,22 +652,19 @@ __device__ __forceinline__ void rolled_store_tile(const FusedParams& p, v16f (&a
     }
 }
 
-// One (TM*64) x 256 block of C: rows [m0, m0 + TM*64) of tile (tm, tn) of the
-// 256 x 256 tile grid, starting `half` * 128 rows into the tile, on an NS-stage
-// K-tile ring (the tile's row and column scales follow the ring).
-template <class Op, int MODE, int TM, int KTB, int NS = dense_ns<KTB>()>
-__device__ __forceinline__ void dense_block(const typename Op::Params& p, int tm, int tn, int half, HKQ_LDS uint8_t* smem) {
+// One (TM*64) x 256 block of C at (m0, n0) on an NS-stage K-tile ring; the tile's
+// row and column scales (and bias) follow RING bytes of it.
+template <class Op, int MODE, int TM, int KTB, int NS, int RING>
+__device__ __forceinline__ void dense_rows(const typename Op::Params& p, int m0, int n0, HKQ_LDS uint8_t* smem) {
     constexpr int WAVES_M = DENSE_WAVES_M, WAVES_N = DENSE_WAVES_N, TN = DENSE_TN;
     using Cfg = DenseCfg<MODE, WAVES_M, WAVES_N, TM, TN, KTB>;
     constexpr int BM = Cfg::BM, BN = Cfg::BN;
-    constexpr int RING = NS == dense_ns<KTB>() ? dense_ring_lds<MODE, KTB>() : Cfg::lds_bytes(NS);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
     const int khalf = lane >> 5;
 
-    const int m0 = tm * DENSE_BM + half * BM, n0 = tn * BN;
     const int rows_a = min(p.M - m0, BM), rows_b = min(p.N - n0, BN);
     if (rows_a <= 0) return;  // the M half below the last row (uniform per workgroup)
 
@@ -705,6 +702,15 @@ __device__ __forceinline__ void dense_block(const typename Op::Params& p, int tm
                                 NoBias{});
 }
 
+// Rows [m0, m0 + TM*64) of tile (tm, tn) of the 256 x 256 tile grid, starting
+// `half` * 128 rows into the tile.
+template <class Op, int MODE, int TM, int KTB, int NS = dense_ns<KTB>()>
+__device__ __forceinline__ void dense_block(const typename Op::Params& p, int tm, int tn, int half, HKQ_LDS uint8_t* smem) {
+    using Cfg = DenseCfg<MODE, DENSE_WAVES_M, DENSE_WAVES_N, TM, DENSE_TN, KTB>;
+    constexpr int RING = NS == dense_ns<KTB>() ? dense_ring_lds<MODE, KTB>() : Cfg::lds_bytes(NS);
+    dense_rows<Op, MODE, TM, KTB, NS, RING>(p, tm * DENSE_BM + half * Cfg::BM, tn * DENSE_BN, smem);
+}
+
 // Workgroup u < n_whole computes tile u. When the last round of tiles would
 // leave at least half of the CUs idle, its tiles are instead computed as M
 // halves by twice as many workgroups: unit v = u - n_whole (XCD v & 7, as the
@@ -734,6 +740,23 @@ __global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_g
         tile_coords(p.n_whole + t, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
         dense_block<Op, MODE, DENSE_TM / 2, KTB>(p, tm, tn, half, smem);
     }
+}
+
+// 192 x 256 tiles (4 waves of 96 x 128), one per workgroup: where the rows fill
+// them and leave the last 256-row tile mostly empty (601 rows: 4 tiles of 192
+// on 224 of 256 CUs instead of 3 of 256 on 168).
+constexpr int MID_TM = 3, MID_BM = DENSE_WAVES_M * MID_TM * 32;
+template <class Op, int MODE>
+constexpr int mid_lds() {
+    return DenseCfg<MODE, DENSE_WAVES_M, DENSE_WAVES_N, MID_TM, DENSE_TN, 128>::lds_bytes(2) + epi_lds<Op, MODE>();
+}
+template <class Op, int MODE>
+__global__ __launch_bounds__(64 * DENSE_WAVES_M * DENSE_WAVES_N, 1) void dense_mid_kernel(const typename Op::Params p) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
+    int tm, tn;
+    tile_coords(blockIdx.x, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+    dense_rows<Op, MODE, MID_TM, 128, 2, DenseCfg<MODE, DENSE_WAVES_M, DENSE_WAVES_N, MID_TM, DENSE_TN, 128>::lds_bytes(2)>(
+        p, tm * MID_BM, tn * DENSE_BN, (HKQ_LDS uint8_t*)smem_raw);
 }
 
 // ---------------------------------------------------------------------------
@@ -1458,19 +1481,30 @@ static DensePlan dense_plan(int mode, int64_t M, int64_t N, int64_t kbytes) {
 // It is still the better one where half of the CUs' worth of tiles meets a long
 // K: 400x4096x14336 31.7 us against 34.7, 128x4096x14336 17.7 against 18.4, bf16
 // 512x4096x14336 64 against 72.
+//
+// The fused and gated products have two sizes more. 192 x 256 tiles in one round
+// of them: epilogue bf16 601x14336x4096 86 us, 256 x 256 tiles 95, 128 x 256 103;
+// 3000x4096x4096 85, 95, 110; over more rounds the streaming kernel is the better
+// one (gated bf16 601x28672x4096 165, 149). 64 x 128: gated bf16 301x5632x2048
+// 13.0, 128 x 128 15.9, 64 x 64 19.2; FP8 64x28672x4096 26.0, 28.3, 34.9; bf16
+// with up to 64 rows is bound by the weights' way from memory, where 64 x 64
+// tiles keep more of them in flight (33x28672x4096 58, 64 x 64 49).
 enum DenseTile {
     DT_32x32, DT_32x64, DT_32x128, DT_32x256, DT_64x64, DT_128x64, DT_128x128, DT_128x256,
     DT_128x128_PAIR,  // two workgroups per CU (dense_tile_kernel)
     DT_256, DT_SPLIT,
-    DT_NONE  // rows too far apart for every size
+    DT_NONE,  // rows too far apart for every size
+    // of the fused and gated products only
+    DT_64x128, DT_192x256
 };
 struct TileCost { float us, e; };
 struct TileCosts {
     TileCost tile[DT_256 + 1], alone;
     float split64_us, split64_e;           // 128 x 64 tiles: per K-tile, constant
     float split_us, split_e, split_parts;  // 128 x 128 tiles: per K-tile, constant, per split
+    TileCost t64x128, t192x256;
 };
-static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const DensePlan* split, bool gated = false) {
+static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const DensePlan* split, bool gated = false, bool fused = false) {
     const int64_t M = p.M, N = p.N, kbytes = p.kbytes;
     // Tile rows `ld` bytes apart that a 32-bit buffer offset reaches. The 256-row
     // kernels end their extents with the last live row, so only those count
@@ -1483,14 +1517,14 @@ static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const 
                      BN[] = {32, 64, 128, 256, 64, 64, 128, 256, 128, 256};
     static const TileCosts A8W8 = {{{0.082f, 1.8f}, {0.118f, 2.3f}, {0.198f, 3.4f}, {0.36f, 1.5f}, {0.145f, 3.5f},
                                     {0.245f, 2.5f}, {0.345f, 2.0f}, {0.54f, 3.0f}, {0.60f, 1.8f}, {0.716f, 4.5f}},
-                                   {0.60f, 1.8f}, 0.345f, 5.7f, 0.4f, 4.2f, 1.3f};
+                                   {0.60f, 1.8f}, 0.345f, 5.7f, 0.4f, 4.2f, 1.3f, {0.26f, 2.5f}, {0.65f, 4.0f}};
     // MXFP4's 128 x 256 tile would cost more than the 256 x 256 one
     static const TileCosts FP4 = {{{0.091f, 1.8f}, {0.125f, 1.9f}, {0.233f, 2.7f}, {0.5f, 1.1f}, {0.188f, 2.9f},
                                    {0.431f, 2.2f}, {0.478f, 2.9f}, {-1.f, 0.f}, {0.717f, 1.2f}, {0.909f, 3.9f}},
-                                  {0.611f, 0.0f}, 0.f, 0.f, 0.f, 0.f, 0.f};
+                                  {0.611f, 0.0f}, 0.f, 0.f, 0.f, 0.f, 0.f, {}, {}};
     static const TileCosts BF16 = {{{0.098f, 1.0f}, {0.132f, 1.45f}, {0.216f, 1.7f}, {0.31f, 0.85f}, {0.162f, 2.2f},
                                     {0.278f, 1.7f}, {0.347f, 0.6f}, {0.606f, 1.2f}, {0.645f, 0.9f}, {0.647f, 2.1f}},
-                                   {0.559f, 0.6f}, 0.f, 0.f, 0.494f, 5.5f, 1.2f};
+                                   {0.559f, 0.6f}, 0.f, 0.f, 0.494f, 5.5f, 1.2f, {0.29f, 2.0f}, {0.62f, 2.0f}};
     const TileCosts& T = mode == MODE_A8W8 ? A8W8 : mode == MODE_MXFP4 ? FP4 : BF16;
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     const float KT = (float)((kbytes + 64) / 128);
@@ -1508,6 +1542,17 @@ static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const 
         if (best_us == 0.f || us < best_us) {
             best = t;
             best_us = us;
+        }
+    }
+    if (gated || fused) {
+        const struct { int t, bm, bn; TileCost c; } more[] = {{DT_64x128, 64, 128, T.t64x128}, {DT_192x256, 192, 256, T.t192x256}};
+        for (const auto& o : more) {
+            if (!fits(o.bm, o.bn)) continue;
+            const int64_t tiles = batch * ((M + o.bm - 1) / o.bm) * ((N + o.bn - 1) / o.bn);
+            if (o.t == DT_192x256 && (kbytes % 128 != 0 || tiles > ncu)) continue;
+            if (o.t == DT_64x128 && mode == MODE_BF16 && M <= 64) continue;
+            const float us = (float)((tiles + ncu - 1) / ncu) * (KT * o.c.us + o.c.e);
+            if (best == DT_NONE || us < best_us) best = o.t, best_us = us;
         }
     }
     if (split != nullptr && fits(128, 128)) {
@@ -1538,6 +1583,20 @@ static int launch_dense_tiles(typename Op::Params& p, int splits, int kt_split, 
         p.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + SPLIT_CNT_BYTES);
     }
     kern<<<dim3((unsigned)(tiles * p.splits), (unsigned)std::max(1, p.batch)), 64 * WM * WN, LDS, stream>>>(p);
+    return hkq_launch_status();
+}
+
+template <class Op, int MODE>
+static int launch_dense_mid(typename Op::Params& p, hipStream_t stream) {
+    constexpr int LDS = mid_lds<Op, MODE>();
+    static_assert(LDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
+    auto kern = dense_mid_kernel<Op, MODE>;
+    static bool attr_set = false;
+    if (int e = set_lds(kern, LDS, attr_set)) return e;
+    p.tiles_m = (p.M + MID_BM - 1) / MID_BM;
+    p.tiles_n = (p.N + DENSE_BN - 1) / DENSE_BN;
+    if (p.group_m <= 0) p.group_m = 8;
+    kern<<<dim3((unsigned)((int64_t)p.tiles_m * p.tiles_n)), 64 * DENSE_WAVES_M * DENSE_WAVES_N, LDS, stream>>>(p);
     return hkq_launch_status();
 }
 
@@ -1647,7 +1706,7 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
                 ws_bytes >= pl.ws_bytes;
     }
     constexpr int M4 = MODE == MODE_MXFP4;  // the e8m0 blocks take LDS from the ring
-    switch (dense_tile_plan(MODE, p, batch, split ? &pl : nullptr, Op::GATED)) {
+    switch (dense_tile_plan(MODE, p, batch, split ? &pl : nullptr, Op::GATED, Op::FUSED)) {
         case DT_32x32:
             if constexpr (!Op::GATED) return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 1, 1, 4>>(p, stream);
             break;
@@ -1659,6 +1718,12 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
         case DT_128x128: return launch_dense_kgroup<Op, KgCfg<MODE, 4, 2, 1, 1, 2, 4>>(p, stream);
         case DT_128x256:
             if constexpr (!M4) return launch_dense_kgroup<Op, KgCfg<MODE, 2, 4, 1, 2, 2, 3>>(p, stream);
+            break;
+        case DT_64x128:
+            if constexpr (Op::FUSED || Op::GATED) return launch_dense_kgroup<Op, KgCfg<MODE, 2, 2, 2, 1, 2, 3>>(p, stream);
+            break;
+        case DT_192x256:
+            if constexpr (Op::FUSED || Op::GATED) return launch_dense_mid<Op, MODE>(p, stream);
             break;
         case DT_128x128_PAIR:
             return launch_dense_tiles<Op, MODE, 2, 2, 2, 2, 128, 2>(p, 1, p.kbytes / 128, nullptr, stream);
