@@ -103,6 +103,35 @@ inline Workspace workspace(size_t bytes, py::object like) {
     return w;
 }
 
+// The tensors of a call (None: skipped) are on one device, which is torch's
+// current one while this object lives, so that the stream and the workspace
+// taken meanwhile are that device's.
+struct OnDevice {
+    py::object guard;
+    explicit OnDevice(std::initializer_list<py::object> tensors) {
+        py::object dev;
+        for (const auto& t : tensors) {
+            if (t.is_none() || !py::hasattr(t, "device")) continue;
+            if (!dev) dev = t.attr("device");
+            else if (!dev.equal(t.attr("device"))) throw py::value_error("the tensors are on different devices");
+        }
+        py::dict mods = py::module_::import("sys").attr("modules");
+        if (!dev || !mods.contains("torch") || py::str(dev.attr("type")).cast<std::string>() != "cuda") return;
+        guard = py::module_::import("torch").attr("cuda").attr("device")(dev);
+        guard.attr("__enter__")();
+    }
+    ~OnDevice() {
+        if (!guard) return;
+        try {
+            guard.attr("__exit__")(py::none(), py::none(), py::none());
+        } catch (py::error_already_set& e) {
+            e.discard_as_unraisable("OnDevice");
+        }
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
 // HKQ_ACT_* of an activation's name.
 inline int activation(const std::string& act) {
     if (act == "none") return HKQ_ACT_NONE;

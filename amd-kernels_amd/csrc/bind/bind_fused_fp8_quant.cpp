@@ -33,6 +33,7 @@ void fused_rmsnorm_fp8_quant_fwd(py::object input, py::object weight, py::object
 // bf16(input + residual); it may be either of them.
 void fused_add_rmsnorm_quant_fwd(py::object input, py::object residual, py::object weight, py::object hidden,
                                  py::object output, py::object scales, float eps, int64_t group_size) {
+    const OnDevice on({input, residual, weight, hidden, output, scales});
     auto x = view(input, "input"), w = view(weight, "weight"), q = view(output, "output"), s = view(scales, "scales");
     expect_dtype(x, "input", {kBF16});
     expect_dtype(w, "weight", {kBF16});

@@ -21,6 +21,7 @@ TensorView matrix(py::object t, const char* name, int64_t rows, int64_t cols, in
 
 void gated_ffn_a8w8(py::object X, py::object W, py::object x_scale, py::object w_scale, py::object H,
                     const std::string& act, float alpha, bool interleaved) {
+    const OnDevice on({X, W, x_scale, w_scale, H});
     auto x = view(X, "X"), w = view(W, "W"), sx = view(x_scale, "x_scale"), sw = view(w_scale, "w_scale");
     expect_dtype(x, "X", {kFP8, kU8});
     expect_dtype(w, "W", {kFP8, kU8});
@@ -41,6 +42,7 @@ void gated_ffn_a8w8(py::object X, py::object W, py::object x_scale, py::object w
 
 void gated_ffn_bf16(py::object X, py::object W, py::object H, py::object Y, const std::string& act, float alpha,
                     bool interleaved) {
+    const OnDevice on({X, W, H, Y});
     auto x = view(X, "X"), w = view(W, "W");
     expect_dtype(x, "X", {kBF16});
     expect_dtype(w, "W", {kBF16});
@@ -58,6 +60,7 @@ void gated_ffn_bf16(py::object X, py::object W, py::object H, py::object Y, cons
 
 void gated_ffn_backward(py::object dH, py::object X, py::object W, py::object Y, py::object dX, py::object dW,
                         const std::string& act, float alpha, bool interleaved) {
+    const OnDevice on({dH, X, W, Y, dX, dW});
     auto x = view(X, "X"), w = view(W, "W");
     expect_dtype(x, "X", {kBF16});
     expect_dtype(w, "W", {kBF16});

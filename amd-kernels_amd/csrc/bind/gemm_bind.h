@@ -97,6 +97,7 @@ inline void gemm_bf16(py::object A, py::object B, py::object C, const char* what
 // a_scale / b_scale as gemm_a8w8 (FP8) or null objects (bf16).
 inline void gemm_epilogue(bool fp8, py::object A, py::object B, py::object a_scale, py::object b_scale, py::object C,
                           py::object bias, py::object residual, const std::string& act, float alpha, const char* what) {
+    const OnDevice on({A, B, a_scale, b_scale, C, bias, residual});
     auto a = view(A, "A"), b = view(B, "B"), c = view(C, "C");
     if (fp8) {
         expect_dtype(a, "A", {kFP8, kU8});

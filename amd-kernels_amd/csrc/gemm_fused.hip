@@ -162,6 +162,19 @@ static int launch_trans(DenseParams& p, void* ws, hipStream_t stream) {
     return launch_dense_whole<Op, MODE_BF16, 128>(p, stream);
 }
 
+// rows x cols zeros (cols a multiple of 4) in rows ld apart: a gradient without
+// tokens or features.
+__global__ __launch_bounds__(256) void zero_rows_kernel(uint16_t* out, int64_t rows, int64_t cols, int64_t ld) {
+    const int64_t quads = cols / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads; i += (int64_t)gridDim.x * 256)
+        *reinterpret_cast<v2i*>(out + i / quads * ld + i % quads * 4) = v2i{0, 0};
+}
+static int launch_zero_rows(void* out, int64_t rows, int64_t cols, int64_t ld, hipStream_t stream) {
+    const int64_t blocks = (rows * (cols / 4) + 255) / 256;
+    zero_rows_kernel<<<(unsigned)std::min<int64_t>(blocks, 1 << 16), 256, 0, stream>>>(static_cast<uint16_t*>(out), rows, cols, ld);
+    return hkq_launch_status();
+}
+
 // Row pitch (values) of the projections' gradients, and their place in the
 // backward's workspace after the split counters and partial sums of either
 // product.
@@ -177,7 +190,7 @@ using namespace hkq;
 
 static int check_act(int act, float alpha, ActParams& a) {
     HKQ_CHECK_ARG(make_act(act, alpha, a), "act must be one of HKQ_ACT_NONE, _RELU, _SILU, _GELU_TANH, _GELU");
-    HKQ_CHECK_ARG(act != HKQ_ACT_SILU || (alpha == alpha && alpha - alpha == 0.0f), "alpha must be finite");
+    HKQ_CHECK_ARG(act != HKQ_ACT_SILU || (alpha >= -1e30f && alpha <= 1e30f), "alpha must be a number in [-1e30, 1e30]");
     return 0;
 }
 
@@ -228,7 +241,7 @@ static int gated_ffn(const void* X, const void* W, const float* sx, const float*
                      hipStream_t stream) {
     constexpr int ES = MODE == MODE_BF16 ? 2 : 1;
     HKQ_CHECK_ARG(M >= 0 && F >= 0 && K > 0, "M, F must be >= 0 and K > 0");
-    HKQ_CHECK_ARG(M < (1 << 30) && F < (1 << 29) && K < (1 << 30), "M and K must be < 2^30, F < 2^29");
+    HKQ_CHECK_ARG(M < (1 << 30) && F < (1 << 28) && K < (1 << 30), "M and K must be < 2^30, F < 2^28");
     HKQ_CHECK_ARG(F % 8 == 0, "F must be a multiple of 8");
     HKQ_CHECK_ARG(MODE == MODE_BF16 || K % 64 == 0, "K must be a multiple of 64");
     HKQ_CHECK_ARG(MODE != MODE_BF16 || K % 32 == 0, "K must be a multiple of 32");
@@ -306,8 +319,8 @@ int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const v
     HKQ_CHECK_ARG(ldy >= 2 * F && ldy % 8 == 0, "ldy must be >= 2F and a multiple of 8");
     HKQ_CHECK_ARG(!dW || (ldx >= K && ldx % 8 == 0 && ldx < (1 << 24)), "ldx must be >= K, a multiple of 8 and < 2^24");
     HKQ_CHECK_ARG(!dX || (ldw >= K && ldw % 8 == 0 && ldw < (1 << 24)), "ldw must be >= K, a multiple of 8 and < 2^24");
-    HKQ_CHECK_ARG(!dX || (lddx >= K && lddx % 4 == 0), "lddx must be >= K and a multiple of 4");
-    HKQ_CHECK_ARG(!dW || (lddw >= K && lddw % 4 == 0), "lddw must be >= K and a multiple of 4");
+    HKQ_CHECK_ARG(!dX || (lddx >= K && lddx % 4 == 0 && lddx < (1 << 23)), "lddx must be >= K, a multiple of 4 and < 2^23");
+    HKQ_CHECK_ARG(!dW || (lddw >= K && lddw % 4 == 0 && lddw < (1 << 23)), "lddw must be >= K, a multiple of 4 and < 2^23");
     ActParams a;
     if (int e = check_act(act, alpha, a)) return e;
     if (F == 0 && (M == 0 || !dX)) return 0;
@@ -322,25 +335,24 @@ int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const v
     HKQ_CHECK_ALIGN(dX, 8);
     HKQ_CHECK_ALIGN(dW, 8);
     HKQ_CHECK_ALIGN(workspace, 16);
+    if (M == 0) return dW ? launch_zero_rows(dW, 2 * F, K, lddw, stream) : 0;
+    if (F == 0) return launch_zero_rows(dX, M, K, lddx, stream);
     const int64_t P = grad_pitch(F);
-    const uint8_t* dy = static_cast<const uint8_t*>(workspace);
-    if (M > 0 && F > 0) {
-        uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + grad_offset(M, F, K));
-        dy = reinterpret_cast<const uint8_t*>(out);
-        const int segs = (int)((F / 8 + 255) / 256);
-        gated_grad_kernel<<<(unsigned)std::min<int64_t>(M * segs, 1 << 20), 256, 0, stream>>>(
-            static_cast<const uint16_t*>(dH), static_cast<const uint16_t*>(Y), out, M, (int)F, lddh, ldy, P, segs,
-            interleaved != 0, a);
-        if (int e = hkq_launch_status()) return e;
-    }
-    if (dX && M > 0) {  // [M, K] = dY [M, 2F] . W [2F, K]
+    uint16_t* dy_rows = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + grad_offset(M, F, K));
+    const uint8_t* dy = reinterpret_cast<const uint8_t*>(dy_rows);
+    const int segs = (int)((F / 8 + 255) / 256);
+    gated_grad_kernel<<<(unsigned)std::min<int64_t>(M * segs, 1 << 20), 256, 0, stream>>>(
+        static_cast<const uint16_t*>(dH), static_cast<const uint16_t*>(Y), dy_rows, M, (int)F, lddh, ldy, P, segs,
+        interleaved != 0, a);
+    if (int e = hkq_launch_status()) return e;
+    if (dX) {  // [M, K] = dY [M, 2F] . W [2F, K]
         DenseParams p{};
         p.A = dy; p.B = static_cast<const uint8_t*>(W); p.C = static_cast<uint16_t*>(dX);
         p.M = (int)M; p.N = (int)K; p.K = (int)(2 * F); p.kbytes = (int)(2 * P);
         p.lda = 2 * P; p.ldb = 2 * ldw; p.ldc = lddx;
         if (int e = launch_trans<false>(p, workspace, stream)) return e;
     }
-    if (dW && F > 0) {  // [2F, K] = dY^T . X [M, K]; without tokens zeros
+    if (dW) {  // [2F, K] = dY^T . X [M, K]
         DenseParams p{};
         p.A = dy; p.B = static_cast<const uint8_t*>(X); p.C = static_cast<uint16_t*>(dW);
         p.M = (int)(2 * F); p.N = (int)K; p.K = (int)M; p.kbytes = (int)((M + 63) / 64 * 128);

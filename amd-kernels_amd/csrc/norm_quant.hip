@@ -489,6 +489,7 @@ extern "C" int hkq_add_rmsnorm_quant(const void* x, const void* res, const void*
     HKQ_CHECK_ARG(lds >= (group ? D / 128 : 1), "lds must hold a row of scales");
     HKQ_CHECK_ARG(eps >= 0.0f, "eps must be non-negative");
     HKQ_CHECK_ARG((res != nullptr) == (h != nullptr), "res and h go together: both or neither");
+    HKQ_CHECK_ARG(!h || ((h != x || ldh == ldx) && (h != res || ldh == ldr)), "h in place of x or res must have its pitch");
     if (M == 0) return 0;
     HKQ_CHECK_ARG(x && w && q && s, "x, w, q and s are required");
     HKQ_CHECK_ALIGN(x, 16);

@@ -7,6 +7,7 @@ is no fallback path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -226,20 +227,20 @@ def add_rmsnorm_quant(x, w, residual=None, eps: float = 1e-6, kind: int = KIND_F
 
     M, D = x.shape
     bf16, codes = (torch.bfloat16,), (torch.int8,) if kind == KIND_INT8 else (torch.float8_e4m3fn, torch.uint8)
-    if residual is not None and h is None:
-        h = torch.empty((M, D), dtype=torch.bfloat16, device=x.device)
+    scales = (M,) if group == 0 else (M, D // 128)
     if residual is None and h is not None:
         raise ValueError("h is written with a residual only")
-    if q is None:
-        q = torch.empty((M, D), dtype=codes[0], device=x.device)
-    if s is None:
-        s = torch.empty((M,) if group == 0 else (M, D // 128), dtype=torch.float32, device=x.device)
     for t, name, shape, types in ((x, "x", (M, D), bf16), (w, "w", (D,), bf16), (residual, "residual", (M, D), bf16),
-                                  (h, "h", (M, D), bf16), (q, "q", (M, D), codes),
-                                  (s, "s", (M,) if group == 0 else (M, D // 128), (torch.float32,))):
+                                  (h, "h", (M, D), bf16), (q, "q", (M, D), codes), (s, "s", scales, (torch.float32,))):
         if t is not None:
             _expect(t, name, shape, types, x.device)
-    with torch.cuda.device(x.device):
+    with _on(x.device, stream):
+        if residual is not None and h is None:
+            h = torch.empty((M, D), dtype=torch.bfloat16, device=x.device)
+        if q is None:
+            q = torch.empty((M, D), dtype=codes[0], device=x.device)
+        if s is None:
+            s = torch.empty(scales, dtype=torch.float32, device=x.device)
         call("hkq_add_rmsnorm_quant", _ptr(x), _opt_ptr(residual), _ptr(w), _opt_ptr(h), _ptr(q), _ptr(s), M, D, _pitch(x),
              _pitch(residual), _pitch(h), _pitch(q), _pitch(s) if group else 1, eps, group, kind, _stream(stream))
     return q, s, h
@@ -285,13 +286,22 @@ def _expect(t, name: str, shape, dtypes, device) -> None:
         raise ValueError(f"{name} must have a contiguous last dimension")
 
 
-def _workspace(nbytes: int, like, stream=None):
-    """Scratch memory of `stream` (the current one): handed out again in that stream's order."""
+@contextlib.contextmanager
+def _on(device, stream):
+    """The operands' device, and `stream` if one is given, as the current ones:
+    memory allocated inside belongs to the stream that the launch uses, and is
+    handed out again in that stream's order."""
     import torch
 
-    if stream is not None and nbytes:
-        with torch.cuda.stream(stream):
-            return _workspace(nbytes, like)
+    if stream is not None and stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the operands on {device}")
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        yield
+
+
+def _workspace(nbytes: int, like):
+    import torch
+
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
@@ -434,19 +444,20 @@ def _gemm_epilogue(kind, A, B, scales, bias, act, residual, alpha, C, stream, sp
 
     M, K = A.shape
     N = B.shape[0]
-    if C is None:
-        C = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
-    _expect(C, "C", (M, N), (torch.bfloat16,), A.device)
+    if C is not None:
+        _expect(C, "C", (M, N), (torch.bfloat16,), A.device)
     if bias is not None:
         _expect(bias, "bias", (N,), (torch.bfloat16,), A.device)
     if residual is not None:
         _expect(residual, "residual", (M, N), (torch.bfloat16,), A.device)
     a = _activation(act)
-    with torch.cuda.device(A.device):
-        ws = _workspace(int(getattr(lib(), f"hkq_gemm_{kind}_workspace")(M, N, K)) if split else 0, A, stream)
+    with _on(A.device, stream):
+        if C is None:
+            C = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
+        ws = _workspace(int(getattr(lib(), f"hkq_gemm_{kind}_workspace")(M, N, K)) if split else 0, A)
         call(f"hkq_gemm_{kind}_epilogue", _ptr(A), _ptr(B), *(_ptr(s) for s in scales), _opt_ptr(bias),
              _opt_ptr(residual), _ptr(C), M, N, K, _pitch(A), _pitch(B), _pitch(residual), _pitch(C), a, alpha,
-             _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+             _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream())
     return C
 
 
@@ -464,11 +475,12 @@ def gated_ffn_a8w8(X, W, sx, sw, act: str = "silu", alpha: float = 1.0, interlea
     _expect(W, "W", (2 * F, K), codes, X.device)
     _expect(sx.view(-1), "sx", (M,), (torch.float32,), X.device)
     _expect(sw.view(-1), "sw", (2 * F,), (torch.float32,), X.device)
-    if H is None:
-        H = torch.empty((M, F), dtype=torch.bfloat16, device=X.device)
-    _expect(H, "H", (M, F), (torch.bfloat16,), X.device)
+    if H is not None:
+        _expect(H, "H", (M, F), (torch.bfloat16,), X.device)
     a = _activation(act)
-    with torch.cuda.device(X.device):
+    with _on(X.device, stream):
+        if H is None:
+            H = torch.empty((M, F), dtype=torch.bfloat16, device=X.device)
         call("hkq_gated_ffn_a8w8", _ptr(X), _ptr(W), _ptr(sx), _ptr(sw), _ptr(H), M, F, K, _pitch(X), _pitch(W),
              _pitch(H), a, alpha, int(interleaved), _stream(stream))
     return H
@@ -486,15 +498,15 @@ def gated_ffn_bf16(X, W, act: str = "silu", alpha: float = 1.0, interleaved: boo
     bf16 = (torch.bfloat16,)
     _expect(X, "X", (M, K), bf16, X.device)
     _expect(W, "W", (2 * F, K), bf16, X.device)
-    if H is None:
-        H = torch.empty((M, F), dtype=torch.bfloat16, device=X.device)
-    if Y is None and save:
-        Y = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=X.device)
-    _expect(H, "H", (M, F), bf16, X.device)
-    if Y is not None:
-        _expect(Y, "Y", (M, 2 * F), bf16, X.device)
+    for t, name, shape in ((H, "H", (M, F)), (Y, "Y", (M, 2 * F))):
+        if t is not None:
+            _expect(t, name, shape, bf16, X.device)
     a = _activation(act)
-    with torch.cuda.device(X.device):
+    with _on(X.device, stream):
+        if H is None:
+            H = torch.empty((M, F), dtype=torch.bfloat16, device=X.device)
+        if Y is None and save:
+            Y = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=X.device)
         call("hkq_gated_ffn_bf16", _ptr(X), _ptr(W), _ptr(H), _opt_ptr(Y), M, F, K, _pitch(X), _pitch(W), _pitch(H),
              _pitch(Y), a, alpha, int(interleaved), _stream(stream))
     return H if Y is None else (H, Y)
@@ -512,17 +524,17 @@ def gated_ffn_backward(dH, X, W, Y, act: str = "silu", alpha: float = 1.0, inter
     bf16 = (torch.bfloat16,)
     for t, name, shape in ((X, "X", (M, K)), (W, "W", (2 * F, K)), (dH, "dH", (M, F)), (Y, "Y", (M, 2 * F))):
         _expect(t, name, shape, bf16, X.device)
-    if need_dx and dX is None:
-        dX = torch.empty((M, K), dtype=torch.bfloat16, device=X.device)
-    if need_dw and dW is None:
-        dW = torch.empty((2 * F, K), dtype=torch.bfloat16, device=X.device)
     dX, dW = dX if need_dx else None, dW if need_dw else None
     for t, name, shape in ((dX, "dX", (M, K)), (dW, "dW", (2 * F, K))):
         if t is not None:
             _expect(t, name, shape, bf16, X.device)
     a = _activation(act)
-    with torch.cuda.device(X.device):
-        ws = _workspace(int(lib().hkq_gated_ffn_backward_workspace(M, F, K)), X, stream)
+    with _on(X.device, stream):
+        if need_dx and dX is None:
+            dX = torch.empty((M, K), dtype=torch.bfloat16, device=X.device)
+        if need_dw and dW is None:
+            dW = torch.empty((2 * F, K), dtype=torch.bfloat16, device=X.device)
+        ws = _workspace(int(lib().hkq_gated_ffn_backward_workspace(M, F, K)), X)
         call("hkq_gated_ffn_backward", _ptr(dH), _ptr(X), _ptr(W), _ptr(Y), _opt_ptr(dX), _opt_ptr(dW), M, F, K,
              _pitch(dH), _pitch(X), _pitch(W), _pitch(Y), _pitch(dX), _pitch(dW), a, alpha, int(interleaved),
              _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))

@@ -256,7 +256,7 @@ int hkq_batched_gemm_bf16(const void* A, const void* B, const void* bias, void* 
 /* Activations: v; max(v, 0); v / (1 + exp(-alpha v)) (the silu of
  * hkq_swiglu_quant; alpha 1.702: the sigmoid form of GELU);
  * v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) / 2; v (1 + erf(v / sqrt 2)) / 2.
- * alpha is read by HKQ_ACT_SILU only. */
+ * alpha (within +-1e30) is read by HKQ_ACT_SILU only. */
 #define HKQ_ACT_NONE 0
 #define HKQ_ACT_RELU 1
 #define HKQ_ACT_SILU 2
@@ -304,10 +304,10 @@ int hkq_gated_ffn_bf16(const void* X, const void* W, void* H, void* Y, int64_t M
  *   dX [M, K] = dg . Wg + du . Wu,  dW [2F, K] = [dg, du]^T . X in W's row order
  * (overwritten, not accumulated; either may be NULL: not computed, and then its
  * own other operand, W or X, may be NULL). act'(0) of ReLU is 0. F <= 2^20;
- * lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of 4; dH, X,
+ * lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of 4 (< 2^23); dH, X,
  * W, Y 16-byte, dX, dW 8-byte aligned. workspace: at least
  * hkq_gated_ffn_backward_workspace(M, F, K) bytes, 16-byte aligned, under the
- * rules of hkq_gemm_a8w8_ws; it holds dg and du. Three launches, no
+ * rules of hkq_gemm_a8w8_ws; it holds dg and du. At most three launches, no
  * synchronisation, sums in a fixed order. */
 size_t hkq_gated_ffn_backward_workspace(int64_t M, int64_t F, int64_t K);
 int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const void* Y, void* dX, void* dW, int64_t M,

@@ -28,7 +28,7 @@ def norm(**kw):
     (dict(D=260, ldx=264), "multiple of 8"), (dict(D=4, group=0), "multiple of 8"), (dict(D=16392, group=0), "16384"),
     (dict(D=200), "128 with groups"), (dict(ldx=248), "ldx"), (dict(ldx=260), "ldx"), (dict(ldr=100), "ldr"),
     (dict(ldh=252), "ldh"), (dict(ldq=260), "ldq"), (dict(lds=1), "lds"), (dict(eps=-1.0), "eps"),
-    (dict(h=None), "both or neither"), (dict(res=None), "both or neither"), (dict(w=None), "required"),
+    (dict(h=P, res=2 * P, ldh=264), "pitch"), (dict(x=2 * P, h=P, ldh=264), "pitch"), (dict(h=None), "both or neither"), (dict(res=None), "both or neither"), (dict(w=None), "required"),
     (dict(x=P + 8), "aligned"), (dict(res=P + 8), "aligned"), (dict(h=P + 2), "aligned"), (dict(q=P + 4), "aligned")])
 def test_norm_refusals(kw, match):
     refused(*norm(**kw), match=match)
@@ -47,7 +47,8 @@ def epilogue(kind, **kw):
     (dict(M=-1), "M, N must"), (dict(N=62), "N must be a multiple of 4"), (dict(K=0), "K > 0"), (dict(K=40, lda=48, ldb=48), "K must be"),
     (dict(M=1 << 30), "2\\^30"), (dict(lda=64), "lda"), (dict(ldb=132), "ldb"), (dict(ldc=60), "ldc"), (dict(ldc=66), "ldc"),
     (dict(ldr=60), "ldr"), (dict(ldr=66), "ldr"), (dict(act=5), "act"), (dict(act=-1), "act"),
-    (dict(alpha=float("nan")), "alpha"), (dict(alpha=float("inf")), "alpha"), (dict(res=2 * P, ldr=128), "pitch"),
+    (dict(alpha=float("nan")), "alpha"), (dict(alpha=float("inf")), "alpha"), (dict(alpha=2e30), "alpha"), (dict(res=2 * P, ldr=128), "pitch"),
+    (dict(ldc=1 << 24), "ldc"), (dict(ldr=1 << 24), "ldr"),
     (dict(A=None), "required"), (dict(C=None), "required"), (dict(A=P + 8), "aligned"), (dict(B=P + 4), "aligned"),
     (dict(C=2 * P + 4), "aligned"), (dict(bias=P + 4), "aligned"), (dict(res=P + 2), "aligned"), (dict(ws=P + 4, n=64), "aligned"),
     (dict(lda=1 << 27, ldb=1 << 27), "row pitches too large")])
@@ -65,8 +66,8 @@ def gated(kind, **kw):
 
 @pytest.mark.parametrize("kind", ["a8w8", "bf16"])
 @pytest.mark.parametrize("kw,match", [
-    (dict(M=-1), "M, F must"), (dict(F=60), "multiple of 8"), (dict(F=1 << 29), "2\\^29"), (dict(K=40, ldx=48, ldw=48), "K must be"),
-    (dict(ldx=64), "ldx"), (dict(ldw=132), "ldw"), (dict(ldh=60), "ldh"), (dict(act=9), "act"), (dict(alpha=float("inf")), "alpha"),
+    (dict(M=-1), "M, F must"), (dict(F=60), "multiple of 8"), (dict(F=1 << 28), "2\\^28"), (dict(K=40, ldx=48, ldw=48), "K must be"),
+    (dict(ldx=64), "ldx"), (dict(ldw=132), "ldw"), (dict(ldh=60), "ldh"), (dict(ldh=1 << 24), "ldh"), (dict(act=9), "act"), (dict(alpha=float("inf")), "alpha"),
     (dict(W=None), "required"), (dict(X=P + 8), "aligned"), (dict(H=P + 4), "aligned"),
     (dict(ldw=1 << 27), "row pitches too large"), (dict(ldw=1 << 26, inter=1), "row pitches too large")])
 def test_gated_refusals(kind, kw, match):
@@ -89,7 +90,7 @@ def backward(**kw):
 @pytest.mark.parametrize("kw,match", [
     (dict(M=-1), "M, F must"), (dict(F=60), "multiple of 8"), (dict(F=(1 << 20) + 8), "2\\^20"), (dict(K=48), "multiple of 32"),
     (dict(lddh=60), "lddh"), (dict(ldx=100), "ldx"), (dict(ldw=132), "ldw"), (dict(ldx=1 << 24), "ldx"), (dict(ldy=132), "ldy"),
-    (dict(lddx=100), "lddx"), (dict(lddw=130), "lddw"), (dict(act=5), "act"), (dict(alpha=float("nan")), "alpha"),
+    (dict(lddx=100), "lddx"), (dict(lddw=130), "lddw"), (dict(lddx=1 << 23), "lddx"), (dict(lddw=1 << 23), "lddw"), (dict(act=5), "act"), (dict(alpha=float("nan")), "alpha"),
     (dict(dH=None), "required"), (dict(X=None), "required"), (dict(W=None), "required"), (dict(n=0), "workspace"),
     (dict(ws=None), "workspace"), (dict(ws=P + 8), "aligned"), (dict(Y=P + 8), "aligned"), (dict(dX=P + 4), "aligned")])
 def test_backward_refusals(kw, match):

@@ -67,7 +67,7 @@ def act64(v, name, alpha=1.0):
 
 
 def close(got, ref, tol, what, roundings=1):
-    got = got.detach().double().cpu()
+    got = got.detach().double().to(ref.device)
     assert got.shape == ref.shape, f"{what}: {got.shape} vs {ref.shape}"
     if roundings and ref.numel() >= 1024:  # enough values for a norm to say something
         off = float(torch.linalg.norm(got - ref) / torch.linalg.norm(ref))
@@ -326,6 +326,31 @@ def test_epilogue_split_k_repeats(kind):
     close(epilogue(kind, *cu, split=False, **kw), *want, "unsplit")
 
 
+# grids of the streaming kernel (whole tiles over several rounds and a last round
+# in halves; its K-tiles come in eights: K a multiple of 512 bf16 or 1024 FP8
+# values) and of 192-row tiles, ragged in both directions, rows of C pitched
+LARGE = {"a8w8": [(2300, 14340, 1024), (601, 14340, 2048), (1100, 6152, 1088)],
+         "bf16": [(2300, 14340, 512), (601, 14340, 1024), (1100, 6152, 544)]}
+
+
+@pytest.mark.parametrize("kind", ["a8w8", "bf16"])
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("act,bias,residual", [("gelu", True, True), ("silu", True, False), ("none", False, True)])
+def test_epilogue_large_tiles(kind, which, act, bias, residual):
+    """The reference in 64 bits on the GPU."""
+    require_gpu()
+    M, N, K = LARGE[kind][which]
+    A, B, sa, sb = (t if t is None else t.cuda() for t in operands(kind, M, N, K, M + which))
+    b = bf16((N,), 3).cuda() if bias else None
+    rbuf = bf16((M, N + 4), 4, 2.0).cuda()  # rows 8-, not 16-byte aligned
+    r = rbuf[:, :N] if residual else None
+    buf, C = guarded(M, N, N + 4 if which != 1 else N + 12)
+    epilogue(kind, A, B, sa, sb, bias=b, act=act, residual=r, C=C)
+    v, err = sums(kind, A, B, sa, sb)
+    close(C, *epilogue_ref(v, err, b, act, 1.0, r), f"{kind} {M}x{N}x{K} {act}")
+    untouched(buf, M, N)
+
+
 def test_epilogue_special_values():
     """Saturated activations, infinities and NaN as in the formulas."""
     require_gpu()
@@ -405,6 +430,28 @@ def test_gated_shapes(kind, interleaved, M, F, K):
         untouched(ybuf, M, 2 * F)
 
 
+@pytest.mark.parametrize("kind", ["a8w8", "bf16", "bf16_save"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("which,act", [(0, "silu"), (1, "gelu_tanh"), (2, "gelu")])
+def test_gated_large_tiles(kind, interleaved, which, act):
+    require_gpu()
+    save, kind = kind.endswith("save"), kind[:4]
+    M, N, K = LARGE[kind][which]
+    F = N // 16 * 8
+    A, W, sa, sw = (t if t is None else t.cuda() for t in operands(kind, M, 2 * F, K, M + which))
+    hbuf, H = guarded(M, F, F + 8)
+    kw = {}
+    if save:
+        ybuf, kw["Y"] = guarded(M, 2 * F, 2 * F + 4)
+    gated(kind, A, W, sa, sw, act=act, interleaved=interleaved, H=H, **kw)
+    y, err = sums(kind, A, W, sa, sw)
+    close(H, *gated_ref(y, err, act, 1.0, interleaved), f"{kind} {M}x{F}x{K} {act}")
+    untouched(hbuf, M, F)
+    if save:
+        close(kw["Y"], y, err + U * y.abs(), "kept projections")
+        untouched(ybuf, M, 2 * F)
+
+
 @pytest.mark.parametrize("kind", ["a8w8", "bf16"])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M", [2, 40, 600])
@@ -463,6 +510,25 @@ def test_backward_shapes(interleaved, M, F, K):
     wb, dW = guarded(2 * F, K, K + 4)
     hkq.gated_ffn_backward(dH.cuda(), X.cuda(), W.cuda(), Y.cuda(), act=act, interleaved=interleaved, dX=dX, dW=dW)
     torch.cuda.synchronize()
+    rx, rw = backward_ref(dH, X, W, Y, act, 1.0, interleaved)
+    close(dX, *rx, f"dX {M}x{F}x{K} {act}", 2)
+    close(dW, *rw, f"dW {M}x{F}x{K} {act}", 2)
+    untouched(xb, M, K)
+    untouched(wb, 2 * F, K)
+
+
+# the streaming kernel over several rounds (K-tiles in eights), 128 x 256 tiles,
+# an odd count of tokens whose last K-tile holds one row
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("M,F,K,act", [(2048, 2048, 4096, "silu"), (4096, 4352, 2080, "gelu_tanh"), (1025, 4352, 4096, "gelu"),
+                                       (2300, 2056, 2048, "relu")])
+def test_backward_large_tiles(interleaved, M, F, K, act):
+    """The reference in 64 bits on the GPU."""
+    require_gpu()
+    X, W, Y, dH = bf16((M, K), 1).cuda(), bf16((2 * F, K), 2, 0.05).cuda(), bf16((M, 2 * F), 3, 1.5).cuda(), bf16((M, F), 4, 0.3).cuda()
+    xb, dX = guarded(M, K, K + 8)
+    wb, dW = guarded(2 * F, K, K + 8)
+    hkq.gated_ffn_backward(dH, X, W, Y, act=act, interleaved=interleaved, dX=dX, dW=dW)
     rx, rw = backward_ref(dH, X, W, Y, act, 1.0, interleaved)
     close(dX, *rx, f"dX {M}x{F}x{K} {act}", 2)
     close(dW, *rw, f"dW {M}x{F}x{K} {act}", 2)
@@ -533,12 +599,42 @@ def test_backward_without_tokens_or_features():
     X, W = bf16((0, 64), 1).cuda(), bf16((32, 64), 2).cuda()
     dX, dW = hkq.gated_ffn_backward(bf16((0, 16), 3).cuda(), X, W, bf16((0, 32), 4).cuda())
     assert dX.shape == (0, 64) and dW.shape == (32, 64) and not dW.any()
+    X, W = bf16((0, 2048), 1).cuda(), bf16((16384, 2048), 2).cuda()  # as many tiles as a large layer has
+    wb, dW = guarded(16384, 2048, 2056)
+    hkq.gated_ffn_backward(bf16((0, 8192), 3).cuda(), X, W, bf16((0, 16384), 4).cuda(), dW=dW)
+    assert not dW.any()
+    untouched(wb, 16384, 2048)
     X, W = bf16((5, 64), 1).cuda(), bf16((0, 64), 2).cuda()
     dX, dW = hkq.gated_ffn_backward(bf16((5, 0), 3).cuda(), X, W, bf16((5, 0), 4).cuda())
     assert dX.shape == (5, 64) and not dX.any() and dW.shape == (0, 64)
 
 
 # -------------------------------------------------------------- together, streams, graphs
+
+def test_outputs_belong_to_the_stream_of_the_call():
+    """Outputs and workspaces of a call on another stream are that stream's memory:
+    they are not a block that work pending on the current stream still uses."""
+    require_gpu()
+    M, K, F = 256, 512, 1024
+    x, w = bf16((M, K), 1).cuda(), bf16((2 * F, K), 2, 0.05).cuda()
+    dh = bf16((M, F), 3).cuda()
+    want = hkq.gated_ffn_bf16(x, w, save=True)
+    want += hkq.gated_ffn_backward(dh, x, w, want[1])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        # blocks of the outputs' sizes, freed here while the current stream is still to write them
+        busy = torch.randn(4096, 4096, device="cuda")
+        for _ in range(4):
+            busy = busy @ busy * 1e-4
+        junk = [torch.full_like(t, 3.0) for t in want]
+        del junk
+        H, Y = hkq.gated_ffn_bf16(x, w, save=True, stream=side)
+        got = (H, Y) + hkq.gated_ffn_backward(dh, x, w, Y, stream=side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 
 def layer_fp8(x, res, w, w1, s1, w2, s2, stream=None):
     """A serving step's dense feed-forward layer: the new stream and the layer's own output."""
