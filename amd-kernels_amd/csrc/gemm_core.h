@@ -127,14 +127,14 @@ __device__ __forceinline__ v2i lds_read_tr8(const HKQ_LDS uint8_t* p) {
 // bf16 operands that lie with their rows (or columns) contiguous and K across
 // memory rows: a K-tile is 64 rows of K, each holding the tile's COLS rows of
 // the operand (COLS * 2 bytes). Logical 16-byte chunk c of row r lives at
-// physical chunk c ^ (4 * (r & 3)), rows of 64 columns c ^ (4 * (r / 2 & 1)):
-// 32 lanes of a transposed read touch 4 consecutive rows at 64 aligned bytes
+// physical chunk c ^ (4 * (r & 3)), where a row is an odd multiple of 128 bytes
+// (64, 192 columns) c ^ (4 * (r / 2 & 1)): 32 lanes of a transposed read touch 4 consecutive rows at 64 aligned bytes
 // each, which then fall on the 4 quarters of the 64 banks.
 template <int COLS>
 struct KTileT16 {
-    static constexpr int ROW = COLS * 2, ROWS = 64;
+    static constexpr int ROW = COLS * 2, ROWS = 64, CHUNKS = ROW / 16;
     static constexpr int ROWS_PER_LOAD = 1024 / ROW;  // rows written by one wave-wide 16-byte LDS-direct load
-    __device__ static __forceinline__ int phys(int r, int c) { return c ^ (4 * (COLS == 64 ? r >> 1 & 1 : r & 3)); }
+    __device__ static __forceinline__ int phys(int r, int c) { return c ^ (4 * (COLS % 128 ? r >> 1 & 1 : r & 3)); }
 };
 
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane j receives 16-bit word

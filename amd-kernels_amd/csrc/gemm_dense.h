@@ -1039,39 +1039,15 @@ __device__ __forceinline__ int split_ticket(uint64_t* cnt, int splits) {
     }
 }
 
-template <class Op, int MODE, int WM, int WN, int TM, int TN, int KTB, int MINB, int NS>
-__global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const typename Op::Params pb) {
-    using Cfg = DenseCfg<MODE, WM, WN, TM, TN, KTB>;
-    constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW;
+// The partial sums of a split tile: this workgroup's go to the workspace, and the
+// split that arrives last returns true with all of them added in `sum`
+// (`summing` runs in it before the partial sums are read). WIDE: registers for
+// three splits' float4 at a time. last_split: LDS past the epilogue's staging, in
+// the (idle) K-tile ring.
+template <int TM, int TN, int NW, bool WIDE, typename Summing>
+__device__ __forceinline__ bool split_sum(const DenseParams& p, v16f (&acc)[TN][TM], v16f (&sum)[TN][TM], int split, int tile,
+                                          int tiles, int wave, int lane, HKQ_LDS int& last_split, Summing summing) {
     constexpr int NQ = TN * TM * 4;  // float4 of accumulators per lane
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
-    HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
-    const typename Op::Params p = batch_slice(pb);
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-    int tm, tn;
-    tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    const int KT = p.kbytes / KTB;
-    const int kt0 = split * p.kt_split, kt1 = min(KT, kt0 + p.kt_split);
-    const int wm = wave / WN, wn = wave % WN;
-    const int mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
-
-    // older than the K-tile loads: the loop's vmcnt waits cover them
-    EpiScales<Op, MODE, TM, TN> sc;
-    sc.load(p, lane, mw, nw);
-    EpiResidual<Op, TM, TN> res;
-    if (p.splits == 1) res.load(p, lane, mw, nw);
-
-    v16f acc[TN][TM];
-    dense_kloop<Op, MODE, WM, WN, TM, TN, KTB, NS>(p, m0, n0, kt0, kt1, smem, acc);
-
-    if (p.splits == 1) {
-        dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wave, lane, mw, nw);
-        return;
-    }
     // this split's partial: float4 q of lane l of wave w at
     // ((s * tiles + tile) * NW + w) * NQ * 64 + q * 64 + l
     const uint32_t wave_slot = (uint32_t)(((int64_t)tile * NW + wave) * NQ * 64 + lane) * 16u;
@@ -1091,10 +1067,7 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
                                                        0, CPOL_SC1);
             }
     __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
-    // count this split in (one thread per workgroup); the flag lies past the
-    // epilogue's staging, in the (idle) K-tile ring
-    static_assert(Cfg::EP_BYTES + 16 <= Cfg::lds_bytes(NS), "room for the split flag");
-    HKQ_LDS int& last_split = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::lds_bytes(NS) - 16);
+    // count this split in (one thread per workgroup)
     __syncthreads();
     if (threadIdx.x == 0) {
         const bool last = split_ticket(p.split_cnt + tile, p.splits) == p.splits - 1;
@@ -1102,14 +1075,13 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
         last_split = last;
     }
     __syncthreads();
-    if (!last_split) return;
-    res.load(p, lane, mw, nw);  // by the one split that adds it, under the partial sums' loads
+    if (!last_split) return false;
+    summing();
     // sum in split order; the other splits' float4 come in chunks of RCH
     // splits, all loads of a chunk in flight together (three splits' worth of
     // registers where the budget allows: 8 float4 per lane, or one workgroup
     // per CU)
-    constexpr int RCH = (NQ <= 8 || MINB == 1) ? 3 : 1;
-    v16f sum[TN][TM];
+    constexpr int RCH = (NQ <= 8 || WIDE) ? 3 : 1;
     for (int s0 = 0; s0 < p.splits; s0 += RCH) {
         v4f part[RCH][NQ] = {};
 #pragma unroll
@@ -1143,6 +1115,45 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
                     }
         }
     }
+    return true;
+}
+
+template <class Op, int MODE, int WM, int WN, int TM, int TN, int KTB, int MINB, int NS>
+__global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const typename Op::Params pb) {
+    using Cfg = DenseCfg<MODE, WM, WN, TM, TN, KTB>;
+    constexpr int BM = Cfg::BM, BN = Cfg::BN, NW = Cfg::NW;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
+    HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
+    const typename Op::Params p = batch_slice(pb);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = p.tiles_m * p.tiles_n;
+    const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+    int tm, tn;
+    tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int KT = p.kbytes / KTB;
+    const int kt0 = split * p.kt_split, kt1 = min(KT, kt0 + p.kt_split);
+    const int wm = wave / WN, wn = wave % WN;
+    const int mw = m0 + wm * TM * 32, nw = n0 + wn * TN * 32;
+
+    // older than the K-tile loads: the loop's vmcnt waits cover them
+    EpiScales<Op, MODE, TM, TN> sc;
+    sc.load(p, lane, mw, nw);
+    EpiResidual<Op, TM, TN> res;
+    if (p.splits == 1) res.load(p, lane, mw, nw);
+
+    v16f acc[TN][TM];
+    dense_kloop<Op, MODE, WM, WN, TM, TN, KTB, NS>(p, m0, n0, kt0, kt1, smem, acc);
+
+    if (p.splits == 1) {
+        dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wave, lane, mw, nw);
+        return;
+    }
+    v16f sum[TN][TM];
+    static_assert(Cfg::EP_BYTES + 16 <= Cfg::lds_bytes(NS), "room for the split flag");
+    HKQ_LDS int& flag = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::lds_bytes(NS) - 16);
+    if (!split_sum<TM, TN, NW, MINB == 1>(p, acc, sum, split, tile, tiles, wave, lane, flag, [&] { res.load(p, lane, mw, nw); })) return;
     dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, smem, wave, lane, mw, nw);
 }
 
@@ -1331,14 +1342,26 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wg = wave % Cfg::GW, kg = wave / Cfg::GW;
     int tm, tn;
-    tile_coords(blockIdx.x, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+    // BT, eight waves of one sub-tile row: K may be split over workgroups (this
+    // one takes K-tiles [kt0, kt1) of its tile)
+    constexpr bool SPLITS = Op::BT && Cfg::KG == 1 && TM * TN <= 2;
+    int tile = blockIdx.x, split = 0, kt0 = 0, kt1 = (p.kbytes + 64) / 128;
+    if constexpr (SPLITS)
+        if (p.splits > 1) {
+            const int tiles = p.tiles_m * p.tiles_n;
+            split = tile / tiles;
+            tile -= split * tiles;
+            kt0 = split * p.kt_split;
+            kt1 = min(kt1, kt0 + p.kt_split);
+        }
+    tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int rows_a = min(p.M - m0, BM), rows_b = min(p.N - n0, BN);
 
     KgSrc<Cfg> src;
-    src.KT = (p.kbytes + 64) / 128;
+    src.KT = kt1 - kt0;
     src.half_tail = p.kbytes % 128 != 0;
-    src.a = buffer_desc(p.A + (int64_t)m0 * p.lda, clamp_bytes((int64_t)rows_a * p.lda));
+    src.a = buffer_desc(p.A + (int64_t)m0 * p.lda + kt0 * 128, clamp_bytes((int64_t)rows_a * p.lda - kt0 * 128));
     src.b = buffer_desc(p.B + (int64_t)n0 * p.ldb, clamp_bytes((int64_t)rows_b * p.ldb));
 #pragma unroll
     for (int i = 0; i < Cfg::SWP; ++i) {
@@ -1376,14 +1399,14 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
     if constexpr (Op::AT) {
         using T = KTileT16<BM>;
         const int r = wg * T::ROWS_PER_LOAD + lane / (T::ROW / 16);
-        src.ta = T16Src::of(p.A + (int64_t)m0 * 2, p.lda, rows_a, 0, p.K, src.KT);
+        src.ta = T16Src::of(p.A + (int64_t)m0 * 2, p.lda, rows_a, kt0 * 64, p.K, kt1);
         src.a_off[0] = (uint32_t)(r * p.lda) + (uint32_t)(T::phys(r, lane % (T::ROW / 16)) << 4);
         src.a_step = (uint32_t)(Cfg::GW * T::ROWS_PER_LOAD * p.lda);
     }
     if constexpr (Op::BT) {
         using T = KTileT16<BN>;
         const int r = wg * T::ROWS_PER_LOAD + lane / (T::ROW / 16);
-        src.tb = T16Src::of(p.B + (int64_t)n0 * 2, p.ldb, rows_b, 0, p.K, src.KT);
+        src.tb = T16Src::of(p.B + (int64_t)n0 * 2, p.ldb, rows_b, kt0 * 64, p.K, kt1);
         src.b_off[0] = (uint32_t)(r * p.ldb) + (uint32_t)(T::phys(r, lane % (T::ROW / 16)) << 4);
         src.b_step = (uint32_t)(Cfg::GW * T::ROWS_PER_LOAD * p.ldb);
     }
@@ -1395,19 +1418,35 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
 
     v16f acc[TN][TM];
     kgroup_kloop<Cfg, false, Op::GATED, Op::AT, Op::BT>(src, smem, lane, wg, kg, acc);
+    if constexpr (SPLITS)
+        if (p.splits > 1) {
+            v16f sum[TN][TM];
+            static_assert(Cfg::EP + 16 <= Cfg::LDS, "room for the split flag");
+            HKQ_LDS int& flag = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::LDS - 16);
+            if (split_sum<TM, TN, Cfg::GW, true>(p, acc, sum, split, tile, p.tiles_m * p.tiles_n, wg, lane, flag, [] {}))
+                dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, smem, wg, lane, mw, nw);
+            return;
+        }
     if (kg != 0) return;
     dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wg, lane, mw, nw);
 }
 
 template <class Op, class Cfg>
-static int launch_dense_kgroup(typename Op::Params& p, hipStream_t stream) {
+static int launch_dense_kgroup(typename Op::Params& p, hipStream_t stream, int splits = 1, int kt_split = 0, void* ws = nullptr) {
     auto kern = dense_kgroup_kernel<Op, Cfg>;
     static bool attr_set = false;
     if (int e = set_lds(kern, Cfg::LDS, attr_set)) return e;
     p.tiles_m = (p.M + Cfg::BM - 1) / Cfg::BM;
     p.tiles_n = (p.N + Cfg::BN - 1) / Cfg::BN;
     if (p.group_m <= 0) p.group_m = 8;
-    kern<<<dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)std::max(1, p.batch)), Cfg::THREADS, Cfg::LDS, stream>>>(p);
+    p.splits = splits;
+    if (splits > 1) {  // the arrival counters, then the partial sums (one K group, BT)
+        p.kt_split = kt_split;
+        p.split_cnt = static_cast<uint64_t*>(ws);
+        p.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + SPLIT_CNT_BYTES);
+    }
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    kern<<<dim3((unsigned)(tiles * splits), (unsigned)std::max(1, p.batch)), Cfg::THREADS, Cfg::LDS, stream>>>(p);
     return hkq_launch_status();
 }
 

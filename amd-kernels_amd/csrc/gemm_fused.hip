@@ -113,8 +113,9 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restr
 // memory; the constants are those of a large one). Tokens x F x K, us: dX
 // 4096x14336x4096 256 x 256 672, 128 x 256 784, 128 x 128 1047; 2048x14336x4096
 // 417 (M halves), 394, 516; 1001x2816x2048 128 x 64 31, 128 x 128 36, two splits
-// 30; 64x2816x2048 21, 30, eight splits 14. dW 1001x2816x2048 256 x 256 27, 128 x
-// 256 32, 128 x 128 31; 1001x1408x2048 17, 15, 19.
+// 30; 64x2816x2048 21, 33, six splits 12.5. dW 1001x2816x2048 192 x 256 (one
+// round only) 26, 256 x 256 29, 128 x 256 34, 128 x 128 34; 1001x1408x2048 21, 21,
+// 18.5, 23.
 struct TransPlan {
     int tile;  // a DenseTile
     int splits, kt_split;
@@ -124,11 +125,12 @@ static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT) {
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     static const struct { int tile, bm, bn; TileCost c; } T[] = {
         {DT_256, 256, 256, {1.37f, 5.7f}}, {DT_128x256, 128, 256, {0.85f, 3.2f}}, {DT_128x128, 128, 128, {0.57f, 2.2f}},
-        {DT_128x64, 128, 64, {0.40f, 2.0f}}};
+        {DT_128x64, 128, 64, {0.40f, 2.0f}}, {DT_192x256, 192, 256, {1.06f, 5.0f}}};
     TransPlan p{DT_256, 1, (int)KT, 0};
     float best = 0.f;
     for (const auto& t : T) {
         const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn), rounds = (tiles + ncu - 1) / ncu;
+        if (t.tile == DT_192x256 && rounds > 1) continue;
         float us = (float)rounds * ((float)KT * t.c.us + t.c.e);
         // few tiles run as M halves (launch_dense_whole)
         if (t.tile == DT_256 && 2 * tiles <= ncu && M > 128) us = (float)KT * 0.88f + 3.0f;
@@ -157,7 +159,8 @@ static int launch_trans(DenseParams& p, void* ws, hipStream_t stream) {
         case DT_128x64: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 1, 2, 1, 2, 3>>(p, stream);
         case DT_128x128: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 2, 1, 1, 2, 4>>(p, stream);
         case DT_128x256: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 2, 4, 1, 2, 2, 3>>(p, stream);
-        case DT_SPLIT: return launch_dense_tiles<Op, MODE_BF16, 2, 2, 2, 2, 128, 1, 4>(p, pl.splits, pl.kt_split, ws, stream);
+        case DT_192x256: return launch_dense_mid<Op, MODE_BF16>(p, stream);
+        case DT_SPLIT: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 2, 1, 1, 2, 4>>(p, stream, pl.splits, pl.kt_split, ws);
     }
     return launch_dense_whole<Op, MODE_BF16, 128>(p, stream);
 }

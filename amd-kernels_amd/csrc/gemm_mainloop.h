@@ -178,12 +178,11 @@ __device__ __forceinline__ TableOff<N> dense_offs_t(int wave, int lane, int64_t 
 template <int NW, int N, int COLS>
 __device__ __forceinline__ TableOff<N> dense_offs_t16(int wave, int lane, int64_t ld) {
     using T = KTileT16<COLS>;
-    constexpr int CHUNKS = T::ROW / 16;
     TableOff<N> o;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int r = (i * NW + wave) * T::ROWS_PER_LOAD + lane / CHUNKS;
-        o.v[i] = (uint32_t)(r * ld) + (uint32_t)(T::phys(r, lane % CHUNKS) << 4);
+        const int c = (i * NW + wave) * 64 + lane, r = c / T::CHUNKS;  // rows of 192 columns: a load ends inside one
+        o.v[i] = (uint32_t)(r * ld) + (uint32_t)(T::phys(r, c % T::CHUNKS) << 4);
     }
     return o;
 }
