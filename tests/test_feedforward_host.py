@@ -24,7 +24,8 @@ def norm(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(kind=2), "kind"), (dict(group=64), "group"), (dict(M=-1), "M must"), (dict(M=1 << 31), "M must"),
+    (dict(kind=2), "kind"), (dict(group=64), "group"), (dict(M=-1), "M must"), (dict(M=1 << 31), "M must"), (dict(M=1 << 26), "M must"),
+    (dict(M=1 << 24, D=2176, ldx=2176, ldr=2176, ldh=2176, ldq=2176, lds=17), "M must"),
     (dict(D=260, ldx=264), "multiple of 8"), (dict(D=4, group=0), "multiple of 8"), (dict(D=16392, group=0), "16384"),
     (dict(D=200), "128 with groups"), (dict(ldx=248), "ldx"), (dict(ldx=260), "ldx"), (dict(ldr=100), "ldr"),
     (dict(ldh=252), "ldh"), (dict(ldq=260), "ldq"), (dict(lds=1), "lds"), (dict(eps=-1.0), "eps"),
