@@ -128,8 +128,9 @@ __device__ __forceinline__ v2i lds_read_tr8(const HKQ_LDS uint8_t* p) {
 // memory rows: a K-tile is 64 rows of K, each holding the tile's COLS rows of
 // the operand (COLS * 2 bytes). Logical 16-byte chunk c of row r lives at
 // physical chunk c ^ (4 * (r & 3)), where a row is an odd multiple of 128 bytes
-// (64, 192 columns) c ^ (4 * (r / 2 & 1)): 32 lanes of a transposed read touch 4 consecutive rows at 64 aligned bytes
-// each, which then fall on the 4 quarters of the 64 banks.
+// (64, 192 columns) c ^ (4 * (r / 2 & 1)): 32 lanes of a transposed read touch 4
+// consecutive rows at 64 aligned bytes each, which then fall on the 4 quarters
+// of the 64 banks.
 template <int COLS>
 struct KTileT16 {
     static constexpr int ROW = COLS * 2, ROWS = 64, CHUNKS = ROW / 16;

@@ -39,7 +39,7 @@ static bool make_act(int act, float alpha, ActParams& a) {
 __device__ __forceinline__ void act_grad(const ActParams& p, float v, float& f, float& df) {
     if (p.form == 0) {
         f = v < p.lo ? p.lo : v;
-        df = v > p.lo ? 1.0f : 0.0f;
+        df = p.lo == 0.0f && v <= 0.0f ? 0.0f : 1.0f;
     } else if (p.form <= 2) {  // SiLU: c3 = 0
         // v^2 is bounded only so that a c3 of zero, or the logistic function's
         // saturation, never meets an infinity
@@ -315,7 +315,8 @@ int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const v
                            int64_t lddw, int act, float alpha, int interleaved, void* workspace, size_t workspace_bytes,
                            hipStream_t stream) {
     HKQ_CHECK_ARG(M >= 0 && F >= 0 && K > 0, "M, F must be >= 0 and K > 0");
-    HKQ_CHECK_ARG(M < (1 << 30) && F <= (1 << 20) && K < (1 << 30), "M and K must be < 2^30, F <= 2^20");
+    // tokens are dW's K: their bytes count in 32 bits
+    HKQ_CHECK_ARG(M < (1 << 29) && F <= (1 << 20) && K < (1 << 30), "M must be < 2^29, K < 2^30, F <= 2^20");
     HKQ_CHECK_ARG(F % 8 == 0, "F must be a multiple of 8");
     HKQ_CHECK_ARG(K % 32 == 0, "K must be a multiple of 32");
     HKQ_CHECK_ARG(lddh >= F && lddh % 8 == 0, "lddh must be >= F and a multiple of 8");

@@ -267,10 +267,10 @@ int hkq_batched_gemm_bf16(const void* A, const void* B, const void* bias, void* 
  * C = bf16(act((A . B^T) * sa[m] * sb[n] + bias[n]) + residual[m, n]), formed in
  * fp32 and rounded once. bias bf16 [N] and residual bf16 rows of ldr >= N
  * elements (a multiple of 4; ldr, ldc < 2^24) may be NULL; the residual may be C
- * itself (same pitch). Shapes, strides and alignment as the plain GEMMs; the workspace is
- * that of hkq_gemm_a8w8_workspace / hkq_gemm_bf16_workspace (NULL: no split of
- * K over workgroups) under the rules of hkq_gemm_a8w8_ws. No counterpart in
- * the reference beyond its block-scale multiply-add. */
+ * itself (same pitch). Shapes, strides and alignment as the plain GEMMs; the
+ * workspace is that of hkq_gemm_a8w8_workspace / hkq_gemm_bf16_workspace (NULL:
+ * no split of K over workgroups) under the rules of hkq_gemm_a8w8_ws. No
+ * counterpart in the reference beyond its block-scale multiply-add. */
 int hkq_gemm_a8w8_epilogue(const void* A, const void* B, const float* sa, const float* sb, const void* bias,
                            const void* residual, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
                            int64_t ldr, int64_t ldc, int act, float alpha, void* workspace, size_t workspace_bytes,
@@ -287,8 +287,8 @@ int hkq_gemm_bf16_epilogue(const void* A, const void* B, const void* bias, const
  * formed from the fp32 sums. FP8: X, W E4M3FN codes, sx fp32 [M], sw fp32 [2F]
  * in W's row order, K % 64 == 0. bf16: no scales, K % 32 == 0; Y (NULL: not
  * kept) gets bf16(g), bf16(u) as [M, 2F] rows of ldy in W's row order, what
- * hkq_gated_ffn_backward needs. F % 8 == 0; ldh, ldy multiples of 4 below 2^24; X, W, sw
- * 16-byte, H, Y 8-byte aligned. 32 rows of W of one half (ldw, or 2 ldw
+ * hkq_gated_ffn_backward needs. F % 8 == 0; ldh, ldy multiples of 4 below 2^24;
+ * X, W, sw 16-byte, H, Y 8-byte aligned. 32 rows of W of one half (ldw, or 2 ldw
  * interleaved, apart) and of X must span less than 2^31 bytes. No counterpart
  * in the reference, whose gate/up product writes both halves to memory
  * (kernels/moe-gemm/moe_op_silu_fused/kernel.cpp:1-13). */
@@ -303,9 +303,9 @@ int hkq_gated_ffn_bf16(const void* X, const void* W, void* H, void* Y, int64_t M
  *   dg = dH * u * act'(g), du = dH * act(g)  (fp32, rounded to bf16),
  *   dX [M, K] = dg . Wg + du . Wu,  dW [2F, K] = [dg, du]^T . X in W's row order
  * (overwritten, not accumulated; either may be NULL: not computed, and then its
- * own other operand, W or X, may be NULL). act'(0) of ReLU is 0. F <= 2^20;
- * lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of 4 (< 2^23); dH, X,
- * W, Y 16-byte, dX, dW 8-byte aligned. workspace: at least
+ * own other operand, W or X, may be NULL). act'(0) of ReLU is 0. M < 2^29,
+ * F <= 2^20; lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of
+ * 4 (< 2^23); dH, X, W, Y 16-byte, dX, dW 8-byte aligned. workspace: at least
  * hkq_gated_ffn_backward_workspace(M, F, K) bytes, 16-byte aligned, under the
  * rules of hkq_gemm_a8w8_ws; it holds dg and du. At most three launches, no
  * synchronisation, sums in a fixed order. */

@@ -89,7 +89,7 @@ def backward(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(M=-1), "M, F must"), (dict(F=60), "multiple of 8"), (dict(F=(1 << 20) + 8), "2\\^20"), (dict(K=48), "multiple of 32"),
+    (dict(M=-1), "M, F must"), (dict(M=1 << 29), "2\\^29"), (dict(F=60), "multiple of 8"), (dict(F=(1 << 20) + 8), "2\\^20"), (dict(K=48), "multiple of 32"),
     (dict(lddh=60), "lddh"), (dict(ldx=100), "ldx"), (dict(ldw=132), "ldw"), (dict(ldx=1 << 24), "ldx"), (dict(ldy=132), "ldy"),
     (dict(lddx=100), "lddx"), (dict(lddw=130), "lddw"), (dict(lddx=1 << 23), "lddx"), (dict(lddw=1 << 23), "lddw"), (dict(act=5), "act"), (dict(alpha=float("nan")), "alpha"),
     (dict(dH=None), "required"), (dict(X=None), "required"), (dict(W=None), "required"), (dict(n=0), "workspace"),

@@ -594,6 +594,30 @@ def test_backward_against_differences(act):
     assert abs(got - num) <= 0.05 * tol + 1e-5 * abs(num), (got, num, tol)
 
 
+@pytest.mark.parametrize("act", ACTS)
+def test_backward_slopes_at_the_ends(act):
+    """Activations that saturate have slopes 1 and 0 far out; "none" and ReLU
+    also at infinities and NaN (ReLU passes a NaN's gradient on). One token with
+    X of ones: row f of dW is the projection's gradient itself, exactly."""
+    require_gpu()
+    inf, nan, big = float("inf"), float("nan"), 2.0 ** 127
+    g = torch.tensor([big, -big, 0.0, -0.0, 1e4, -1e4, 2.0 ** 60, -2.0 ** 60])
+    if act in ("none", "relu"):
+        g = torch.cat((g, torch.tensor([inf, -inf, nan, 1.0, -1.0, 2.0, -2.0, 0.5])))
+    F, K = len(g), 32
+    u, dh = torch.full((1, F), 2.0), torch.full((1, F), 0.25)
+    Y = torch.cat((g.to(BF16)[None], u.to(BF16)), 1).cuda()
+    _, dW = hkq.gated_ffn_backward(dh.to(BF16).cuda(), torch.ones(1, K, dtype=BF16).cuda(),
+                                   torch.zeros(2 * F, K, dtype=BF16).cuda(), Y, act=act, need_dx=False)
+    g = g.to(BF16).double()
+    slope = torch.ones(F).double() if act == "none" else (~(g <= 0)).double()
+    if act not in ("none", "relu"):
+        slope[g == 0] = 0.5
+    value = g if act == "none" else torch.where(g <= 0, torch.zeros_like(g), g)
+    want = torch.cat((0.5 * slope, 0.25 * value))[:, None].expand(2 * F, K)
+    assert torch.equal(torch.nan_to_num(dW.cpu().double(), nan=7.0), torch.nan_to_num(want, nan=7.0))
+
+
 def test_backward_without_tokens_or_features():
     require_gpu()
     X, W = bf16((0, 64), 1).cuda(), bf16((32, 64), 2).cuda()
