@@ -2,8 +2,10 @@
 // operation `Op` that says what a workgroup does around the K loop:
 //   PlainOp  C = bf16(sums x scales (+ bias)), one or a batch of GEMMs
 //            (gemm.hip);
-//   FusedOp  bias, activation and residual in the epilogue, and GatedOp, the
-//            gate and up rows of one weight in one tile (gemm_fused.hip).
+//   FusedOp  bias, activation and residual in the epilogue;
+//   GatedOp  gate and up rows of one weight in one tile;
+//   TransOp  bf16 operands with K across memory rows (these three:
+//            gemm_fused.hip).
 #pragma once
 #include <algorithm>
 #include <cstdlib>

@@ -9,6 +9,21 @@
 // The K loops, tile sizes and their choice are the dense GEMMs' (gemm_dense.h);
 // this file adds the epilogues, the pairing of gate and up columns in a tile,
 // and for the backward products bf16 operands whose K runs across memory rows.
+//
+// Few rows are bound by the weights' way from memory, many by the matrix cores;
+// what a fused epilogue saves is the passes after the product (an activation of
+// [M, 2F] alone reads 4 and writes 2 bytes per feature). us on MI355X, M x N x K
+// (gated: M x F x K), inputs that rotate:
+//   FP8 + residual      16x4096x14336 12.7 (the weights at 4.6 TB/s), 4096x4096x14336
+//                       185 (2.60 PFLOP/s);
+//   bf16, bias, GELU    601x14336x4096 88 (0.80 PFLOP/s: a fifth of the 192-row
+//                       tiles' rows is padding, 224 of them on 256 CUs);
+//   gated FP8           24x14336x4096 25.9 (4.5 TB/s), 4096x14336x4096 363 (2.65
+//                       PFLOP/s);
+//   gated bf16          301x2816x2048 13.1, 4096x14336x4096 with the projections
+//                       kept 742 (1.30 PFLOP/s, and 352 MB written);
+//   gated backward      1001x2816x2048 63.5, 4096x14336x4096 1510 (1.27 PFLOP/s
+//                       and the gradients' pass over memory).
 #include <limits>
 
 #include "gemm_dense.h"
@@ -34,7 +49,10 @@ static bool make_act(int act, float alpha, ActParams& a) {
 // in fp32, rounded to bf16 (they are operands of bf16 matrix products) into
 // rows of P values in Y's column order; values 2F .. P - 1 are zeros, so that
 // the products take whole K-tiles. HBM-bound: 6 bytes read and 4 written per
-// feature; a thread owns 8 features.
+// feature; a thread owns 8 features. 4096x14336 91 us (6.4 TB/s), 1001x2816 8.0.
+// A pass of its own, not the products' operand load: both products read dY, each
+// of its values once per column of tiles, and the activation would be formed
+// anew every time (16 times in either at 4096x14336x4096).
 // --------------------------------------------------------------------------
 __device__ __forceinline__ void act_grad(const ActParams& p, float v, float& f, float& df) {
     if (p.form == 0) {
@@ -150,6 +168,10 @@ static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT) {
 }
 
 // C [M, N] = A . B^T over K rows of memory (B, and A with AT), K-tiles of 64.
+// Weights and activations stay as the forward has them: a transposed copy of W
+// alone would read and write 235 MB each at 14336x4096 features, 90 us; the
+// transposed LDS reads cost nothing against the plain product's (dX 693 us, dW
+// 702, the forward's gate and up 735; 1.39 PFLOP/s).
 template <bool AT>
 static int launch_trans(DenseParams& p, void* ws, hipStream_t stream) {
     using Op = TransOp<AT, true>;
