@@ -111,8 +111,9 @@ __device__ __forceinline__ float logistic2(float t) { return __builtin_amdgcn_rc
 template <int N>
 __device__ __forceinline__ void act_n(const ActParams& a, float (&v)[N]) {
     if (a.form == 0) {
+        if (a.lo != 0.0f) return;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] < a.lo ? a.lo : v[i];
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
     } else if (a.form == 1) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] *= logistic2(a.c1 * v[i]);
@@ -131,6 +132,17 @@ __device__ __forceinline__ float4 act4(const ActParams& a, float4 v) {
     float x[4] = {v.x, v.y, v.z, v.w};
     act_n(a, x);
     return make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// The activation of a wave's sub-tile.
+template <int TN, int TM>
+__device__ __forceinline__ void act_tile(const ActParams& a, v16f (&v)[TN][TM]) {
+    float x[TN * TM * 16];
+#pragma unroll
+    for (int i = 0; i < TN * TM * 16; ++i) x[i] = v[i / 16 / TM][i / 16 % TM][i % 16];
+    act_n(a, x);
+#pragma unroll
+    for (int i = 0; i < TN * TM * 16; ++i) v[i / 16 / TM][i / 16 % TM][i % 16] = x[i];
 }
 
 struct FusedParams : DenseParams {
@@ -275,6 +287,8 @@ struct EpiResidual {
     v2i v[HELD ? TN : 1][4][HELD ? TM : 1];
     __device__ __forceinline__ void load(const typename Op::Params& p, int lane, int mw, int nw) {
         if constexpr (HELD) {
+            // no residual: an empty buffer, whose loads give zeros
+            const auto rc = make_rsrc(p.residual + (int64_t)mw * p.ldr + nw, p.residual ? 0x7FFFFFFFu : 0u);
             const int khalf = lane >> 5;
 #pragma unroll
             for (int i = 0; i < TN; ++i)
@@ -282,11 +296,25 @@ struct EpiResidual {
                 for (int g = 0; g < 4; ++g)
 #pragma unroll
                     for (int j = 0; j < TM; ++j) {
-                        const int m = mw + j * 32 + (lane & 31), n = nw + i * 32 + 8 * g + 4 * khalf;
-                        v[i][g][j] = v2i{0, 0};
-                        if (p.residual && m < p.M && n < p.N)
-                            v[i][g][j] = *reinterpret_cast<const v2i*>(p.residual + (int64_t)m * p.ldr + n);
+                        const int m = j * 32 + (lane & 31), n = i * 32 + 8 * g + 4 * khalf;
+                        v[i][g][j] = __builtin_amdgcn_raw_buffer_load_b64(
+                            rc, mw + m < p.M && nw + n < p.N ? (uint32_t)((m * p.ldr + n) * 2) : OOB, 0, 0);
                     }
+        }
+    }
+};
+// Bias of a wave's columns, loaded before the K loop likewise.
+template <class Op, int TN>
+struct EpiBias {
+    v2i v[Op::FUSED ? TN : 1][4];
+    __device__ __forceinline__ void load(const typename Op::Params& p, int lane, int nw) {
+        if constexpr (Op::FUSED) {
+            const auto rc = make_rsrc(p.bias + nw, p.bias && nw < p.N ? (uint32_t)(p.N - nw) * 2u : 0u);
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    v[i][g] = __builtin_amdgcn_raw_buffer_load_b64(rc, (uint32_t)(i * 32 + 8 * g + 4 * (lane >> 5)) * 2u, 0, 0);
         }
     }
 };
@@ -301,10 +329,13 @@ __device__ __forceinline__ float4 add_bf16x4(float4 v, const v2i& r) {
 // through the staging area: whole row pieces (16 bytes per lane, full lines)
 // are put where the results will go, and each lane replaces its own values.
 // Read straight in the accumulators' layout, 32 rows x 8 bytes per load, they
-// would cost a line request per row and load.
+// would cost a line request per row and load. One branch on the activation for
+// the whole sub-tile: one per four columns jumped over the other forms' code
+// 8 to 16 times, each a fetch of instructions from L2 (FP8 1024x1024x1024 with
+// no activation at all 8.5 us, the plain GEMM 7.0).
 template <class Op, int TM, int TN, typename RowScale, typename ColScale4>
 __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], const EpiResidual<Op, TM, TN>& res,
-                                                 HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw,
+                                                 const EpiBias<Op, TN>& bias, HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw,
                                                  RowScale row_scale, ColScale4 col_scale4) {
     constexpr int PITCH = TN * 32 * 2 + 16;
     constexpr bool HELD = EpiResidual<Op, TM, TN>::HELD;
@@ -348,13 +379,26 @@ __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&ac
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int nl = i * 32 + 8 * g + 4 * khalf;
-            const float4 cs = col_scale4(i, g), cb = bias4(p, nw + nl);
+            const float4 cs = col_scale4(i, g), cb = add_bf16x4(make_float4(0.f, 0.f, 0.f, 0.f), bias.v[i][g]);
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
                 const float a = rs[j];
-                float4 v = act4(p.act, make_float4(acc[i][j][4 * g + 0] * a * cs.x + cb.x, acc[i][j][4 * g + 1] * a * cs.y + cb.y,
-                                                   acc[i][j][4 * g + 2] * a * cs.z + cb.z, acc[i][j][4 * g + 3] * a * cs.w + cb.w));
+                v16f& v = acc[i][j];
+                v[4 * g + 0] = v[4 * g + 0] * a * cs.x + cb.x;
+                v[4 * g + 1] = v[4 * g + 1] * a * cs.y + cb.y;
+                v[4 * g + 2] = v[4 * g + 2] * a * cs.z + cb.z;
+                v[4 * g + 3] = v[4 * g + 3] * a * cs.w + cb.w;
+            }
+        }
+    act_tile(p.act, acc);
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int nl = i * 32 + 8 * g + 4 * khalf;
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                float4 v = make_float4(acc[i][j][4 * g + 0], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
                 HKQ_LDS v2i* at = reinterpret_cast<HKQ_LDS v2i*>(ep + (j * 32 + (lane & 31)) * PITCH + nl * 2);
                 if constexpr (HELD) {
                     if (p.residual) v = add_bf16x4(v, res.v[i][g][j]);
@@ -394,8 +438,15 @@ __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&ac
 #pragma unroll
                 for (int j = 0; j < TM; ++j) put(i, g, j, j * 32 + (lane & 31), i * 32 + 8 * g + 4 * khalf);
     };
+    v16f gate[HN][TM];
+    each([&](int i, int g, int j, int, int) {
+        const float4 v = value(i, j, g);
+        gate[i][j][4 * g + 0] = v.x, gate[i][j][4 * g + 1] = v.y, gate[i][j][4 * g + 2] = v.z, gate[i][j][4 * g + 3] = v.w;
+    });
+    act_tile(p.act, gate);
     each([&](int i, int g, int j, int r, int n) {
-        const float4 u = value(i + HN, j, g), a = act4(p.act, value(i, j, g));
+        const v16f& v = gate[i][j];
+        const float4 u = value(i + HN, j, g), a = make_float4(v[4 * g + 0], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) = v2i{(int)pk_bf16(a.x * u.x, a.y * u.y), (int)pk_bf16(a.z * u.z, a.w * u.w)};
     });
     store_staged<TM, HN * 32, PITCH>(ep, lane, p.C, p.ldc, p.M, p.F, mw, fw, p.c16 != 0);
@@ -567,11 +618,16 @@ __device__ __forceinline__ void rolled_store_tile(const FusedParams& p, v16f (&a
                     for (int g = 0; g < 4; ++g)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t w = (uint32_t)cb[ii][g][e >> 1];
-                            const float b = bf16_to_f32(e & 1 ? w >> 16 : w & 0xFFFF);
                             float& x = v[16 * ii + 4 * g + e];
-                            x = A8 ? x * a * cs[ii][4 * g + e] + b : x + b;
+                            if constexpr (A8) x = x * a * cs[ii][4 * g + e];
                         }
+                if (p.bias) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const uint32_t w = (uint32_t)cb[e / 16][e / 4 % 4][e % 4 >> 1];
+                        v[e] += bf16_to_f32(e & 1 ? w >> 16 : w & 0xFFFF);
+                    }
+                }
                 act_n(p.act, v);
                 if (p.residual) {
 #pragma unroll
@@ -984,13 +1040,13 @@ struct EpiScales {
 template <class Op, int MODE, int TM, int TN>
 __device__ __forceinline__ void dense_epilogue_global(const typename Op::Params& p, v16f (&acc)[TN][TM],
                                                       const EpiScales<Op, MODE, TM, TN>& sc,
-                                                      const EpiResidual<Op, TM, TN>& res, HKQ_LDS uint8_t* smem, int wave,
-                                                      int lane, int mw, int nw) {
+                                                      const EpiResidual<Op, TM, TN>& res, const EpiBias<Op, TN>& bias,
+                                                      HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw) {
     const int khalf = lane >> 5;
     auto row_scale = [&](int j) { return sc.r[j]; };
     auto col_scale4 = [&](int i, int g) { return sc.c[i][g]; };
     if constexpr (Op::FUSED)
-        fused_store_tile<Op, TM, TN>(p, acc, res, smem, wave, lane, mw, nw, row_scale, col_scale4);
+        fused_store_tile<Op, TM, TN>(p, acc, res, bias, smem, wave, lane, mw, nw, row_scale, col_scale4);
     else if constexpr (Op::GATED)
         gated_store_tile<TM, TN>(p, acc, smem, wave, lane, mw, nw / 2, row_scale, col_scale4);
     else if (p.bias)
@@ -1144,19 +1200,21 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
     sc.load(p, lane, mw, nw);
     EpiResidual<Op, TM, TN> res;
     if (p.splits == 1) res.load(p, lane, mw, nw);
+    EpiBias<Op, TN> bias;
+    bias.load(p, lane, nw);
 
     v16f acc[TN][TM];
     dense_kloop<Op, MODE, WM, WN, TM, TN, KTB, NS>(p, m0, n0, kt0, kt1, smem, acc);
 
     if (p.splits == 1) {
-        dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wave, lane, mw, nw);
+        dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, bias, smem, wave, lane, mw, nw);
         return;
     }
     v16f sum[TN][TM];
     static_assert(Cfg::EP_BYTES + 16 <= Cfg::lds_bytes(NS), "room for the split flag");
     HKQ_LDS int& flag = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::lds_bytes(NS) - 16);
     if (!split_sum<TM, TN, NW, MINB == 1>(p, acc, sum, split, tile, tiles, wave, lane, flag, [&] { res.load(p, lane, mw, nw); })) return;
-    dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, smem, wave, lane, mw, nw);
+    dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, bias, smem, wave, lane, mw, nw);
 }
 
 // ---------------------------------------------------------------------------
@@ -1417,6 +1475,8 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
     sc.load(p, lane, mw, nw);
     EpiResidual<Op, TM, TN> res;
     if (kg == 0) res.load(p, lane, mw, nw);
+    EpiBias<Op, TN> bias;
+    bias.load(p, lane, nw);
 
     v16f acc[TN][TM];
     kgroup_kloop<Cfg, false, Op::GATED, Op::AT, Op::BT>(src, smem, lane, wg, kg, acc);
@@ -1426,11 +1486,11 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
             static_assert(Cfg::EP + 16 <= Cfg::LDS, "room for the split flag");
             HKQ_LDS int& flag = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::LDS - 16);
             if (split_sum<TM, TN, Cfg::GW, true>(p, acc, sum, split, tile, p.tiles_m * p.tiles_n, wg, lane, flag, [] {}))
-                dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, smem, wg, lane, mw, nw);
+                dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, bias, smem, wg, lane, mw, nw);
             return;
         }
     if (kg != 0) return;
-    dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, smem, wg, lane, mw, nw);
+    dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, bias, smem, wg, lane, mw, nw);
 }
 
 template <class Op, class Cfg>
