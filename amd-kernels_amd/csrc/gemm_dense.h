@@ -147,11 +147,9 @@ __device__ __forceinline__ void act_tile(const ActParams& a, v16f (&v)[TN][TM]) 
 
 struct FusedParams : DenseParams {
     ActParams act;
-    // FUSED: residual bf16 [M, N] (nullptr: none), rows ldr elements apart; r16:
-    // they are 16-byte aligned
+    // FUSED: residual bf16 [M, N] (nullptr: none), rows ldr elements apart
     const uint16_t* residual;
     int64_t ldr;
-    int r16;
     // GATED: B holds F gate and F up rows, the up rows from Bu, both p.ldb bytes
     // apart; N = 2F. C is [M, F]. Column scales (A8W8) in the weight's row order:
     // feature f's at f and F + f, or (interleaved) 2f and 2f + 1. Y: nullptr, or
@@ -278,16 +276,22 @@ __device__ __forceinline__ void store_staged(const HKQ_LDS uint8_t* ep, int lane
     }
 }
 
-// Residual of a wave's sub-tile in the accumulators' layout, for tiles small
-// enough to hold it in registers from before the K loop (nothing waits on it
-// after the sums).
+// Residual of a wave's sub-tile, in registers from before the K loop, so that
+// nothing waits on it after the sums (no residual: an empty buffer, whose loads
+// give zeros). Tiles of one or two accumulator blocks HOLD it in the
+// accumulators' layout; larger ones as whole row pieces (16 bytes per lane, full
+// lines), which reach that layout through the staging area: read straight, 32 rows
+// x 8 bytes per load, they would cost a line request per row and load. FP8
+// 128x5632x2048 with a residual 10.2 us, 10.6 with the pieces fetched after the
+// sums.
 template <class Op, int TM, int TN>
 struct EpiResidual {
     static constexpr bool HELD = Op::FUSED && (TM == 1 || TM * TN <= 2);
+    static constexpr int SEGS = TN * 4, ROWS_PER_PASS = 64 / SEGS, PASSES = TM * 32 / ROWS_PER_PASS;
     v2i v[HELD ? TN : 1][4][HELD ? TM : 1];
+    v4i piece[Op::FUSED && !HELD ? PASSES : 1];
     __device__ __forceinline__ void load(const typename Op::Params& p, int lane, int mw, int nw) {
         if constexpr (HELD) {
-            // no residual: an empty buffer, whose loads give zeros
             const auto rc = make_rsrc(p.residual + (int64_t)mw * p.ldr + nw, p.residual ? 0x7FFFFFFFu : 0u);
             const int khalf = lane >> 5;
 #pragma unroll
@@ -300,6 +304,15 @@ struct EpiResidual {
                         v[i][g][j] = __builtin_amdgcn_raw_buffer_load_b64(
                             rc, mw + m < p.M && nw + n < p.N ? (uint32_t)((m * p.ldr + n) * 2) : OOB, 0, 0);
                     }
+        } else if constexpr (Op::FUSED) {
+            // reads at or past the last row's end give zeros; what lies past the columns is not stored
+            const int rows = min(p.M - mw, TM * 32), cols = min(p.N - nw, TN * 32);
+            const auto rc = make_rsrc(p.residual + (int64_t)mw * p.ldr + nw,
+                                      p.residual && rows > 0 && cols > 0 ? (uint32_t)(((rows - 1) * p.ldr + cols) * 2) : 0u);
+#pragma unroll
+            for (int k = 0; k < PASSES; ++k)
+                piece[k] = __builtin_amdgcn_raw_buffer_load_b128(
+                    rc, (uint32_t)(((k * ROWS_PER_PASS + lane / SEGS) * p.ldr + lane % SEGS * 8) * 2), 0, 0);
         }
     }
 };
@@ -325,14 +338,11 @@ __device__ __forceinline__ float4 add_bf16x4(float4 v, const v2i& r) {
 }
 
 // FUSED epilogue: act(sums * scales + bias) + residual in fp32, one rounding,
-// staged and stored as store_tile_bf16 does. A large tile's residual comes
-// through the staging area: whole row pieces (16 bytes per lane, full lines)
-// are put where the results will go, and each lane replaces its own values.
-// Read straight in the accumulators' layout, 32 rows x 8 bytes per load, they
-// would cost a line request per row and load. One branch on the activation for
-// the whole sub-tile: one per four columns jumped over the other forms' code
-// 8 to 16 times, each a fetch of instructions from L2 (FP8 1024x1024x1024 with
-// no activation at all 8.5 us, the plain GEMM 7.0).
+// staged and stored as store_tile_bf16 does. A residual in row pieces is put where
+// the results will go, and each lane replaces its own values. One branch on the activation for
+// the whole sub-tile: one per four columns jumped over the other forms' code 8 to
+// 16 times, each a fetch of instructions from L2 (FP8 1024x1024x1024 with bias 9.0
+// us, with one branch 8.0, the plain GEMM 7.0).
 template <class Op, int TM, int TN, typename RowScale, typename ColScale4>
 __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], const EpiResidual<Op, TM, TN>& res,
                                                  const EpiBias<Op, TN>& bias, HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw,
@@ -343,34 +353,13 @@ __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&ac
     const int khalf = lane >> 5;
     const bool staged = !HELD && p.residual != nullptr;
     if (staged) {
-        constexpr int SEGS = TN * 4, ROWS_PER_PASS = 64 / SEGS, PASSES = TM * 32 / ROWS_PER_PASS;
-        constexpr int BATCH = PASSES < 16 ? PASSES : 16;
+        using R = EpiResidual<Op, TM, TN>;
         int ln = lane;
         asm volatile("" : "+v"(ln));
-        const int rl = ln / SEGS, seg = ln % SEGS, left = p.N - nw - seg * 8;
-        const uint16_t* src = p.residual + (int64_t)(mw + rl) * p.ldr + nw + seg * 8;
+        const int rl = ln / R::SEGS, seg = ln % R::SEGS;
 #pragma unroll
-        for (int b = 0; b < PASSES; b += BATCH) {
-            v4i v[BATCH];
-#pragma unroll
-            for (int k = 0; k < BATCH; ++k) {
-                const int r = (b + k) * ROWS_PER_PASS;
-                const uint16_t* at = src + (int64_t)r * p.ldr;
-                v[k] = v4i{0, 0, 0, 0};
-                if (mw + r + rl < p.M) {
-                    if (left >= 8 && p.r16) {
-                        v[k] = *reinterpret_cast<const v4i*>(at);
-                    } else if (left > 0) {
-                        const v2i lo = *reinterpret_cast<const v2i*>(at);
-                        const v2i hi = left >= 8 ? *reinterpret_cast<const v2i*>(at + 4) : v2i{0, 0};
-                        v[k] = v4i{lo[0], lo[1], hi[0], hi[1]};
-                    }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < BATCH; ++k)
-                *reinterpret_cast<HKQ_LDS v4i*>(ep + ((b + k) * ROWS_PER_PASS + rl) * PITCH + seg * 16) = v[k];
-        }
+        for (int k = 0; k < (HELD ? 0 : R::PASSES); ++k)
+            *reinterpret_cast<HKQ_LDS v4i*>(ep + (k * R::ROWS_PER_PASS + rl) * PITCH + seg * 16) = res.piece[k];
     }
     float rs[TM];
 #pragma unroll
@@ -418,7 +407,10 @@ __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&ac
 template <int TM, int TN, typename RowScale, typename ColScale4>
 __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], HKQ_LDS uint8_t* smem, int wave,
                                                  int lane, int mw, int fw, RowScale row_scale, ColScale4 col_scale4) {
-    constexpr int HN = TN / 2, PITCH = HN * 64 + 16, PITCH_Y = TN * 64 + 16;
+    // one n-tile: its rows 0 .. 15 are the gate's, 16 .. 31 the up's, so groups g
+    // and g + 2 of a lane's registers belong together
+    constexpr int HN = TN == 1 ? 1 : TN / 2, HG = TN == 1 ? 2 : 4, UN = TN / 2, UG = 4 - HG;
+    constexpr int PITCH = TN * 32 + 16, PITCH_Y = TN * 64 + 16;
     HKQ_LDS uint8_t* ep = smem + wave * (TM * 32) * PITCH_Y;
     const int khalf = lane >> 5;
     float rs[TM];
@@ -434,11 +426,11 @@ __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&ac
 #pragma unroll
         for (int i = 0; i < HN; ++i)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int g = 0; g < HG; ++g)
 #pragma unroll
                 for (int j = 0; j < TM; ++j) put(i, g, j, j * 32 + (lane & 31), i * 32 + 8 * g + 4 * khalf);
     };
-    v16f gate[HN][TM];
+    v16f gate[HN][TM] = {};
     each([&](int i, int g, int j, int, int) {
         const float4 v = value(i, j, g);
         gate[i][j][4 * g + 0] = v.x, gate[i][j][4 * g + 1] = v.y, gate[i][j][4 * g + 2] = v.z, gate[i][j][4 * g + 3] = v.w;
@@ -446,14 +438,14 @@ __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&ac
     act_tile(p.act, gate);
     each([&](int i, int g, int j, int r, int n) {
         const v16f& v = gate[i][j];
-        const float4 u = value(i + HN, j, g), a = make_float4(v[4 * g + 0], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        const float4 u = value(i + UN, j, g + UG), a = make_float4(v[4 * g + 0], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) = v2i{(int)pk_bf16(a.x * u.x, a.y * u.y), (int)pk_bf16(a.z * u.z, a.w * u.w)};
     });
-    store_staged<TM, HN * 32, PITCH>(ep, lane, p.C, p.ldc, p.M, p.F, mw, fw, p.c16 != 0);
+    store_staged<TM, TN * 16, PITCH>(ep, lane, p.C, p.ldc, p.M, p.F, mw, fw, p.c16 != 0);
     if (!p.Y) return;
     if (p.interleaved) {
         each([&](int i, int g, int j, int r, int n) {
-            const float4 a = value(i, j, g), u = value(i + HN, j, g);
+            const float4 a = value(i, j, g), u = value(i + UN, j, g + UG);
             *reinterpret_cast<HKQ_LDS v4i*>(ep + r * PITCH_Y + n * 4) =
                 v4i{(int)pk_bf16(a.x, u.x), (int)pk_bf16(a.y, u.y), (int)pk_bf16(a.z, u.z), (int)pk_bf16(a.w, u.w)};
         });
@@ -463,10 +455,10 @@ __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&ac
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         each([&](int i, int g, int j, int r, int n) {
-            const float4 v = value(i + half * HN, j, g);
+            const float4 v = value(i + half * UN, j, g + half * UG);
             *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) = v2i{(int)pk_bf16(v.x, v.y), (int)pk_bf16(v.z, v.w)};
         });
-        store_staged<TM, HN * 32, PITCH>(ep, lane, p.Y + (half ? p.F : 0), p.ldy, p.M, p.F, mw, fw, p.y16 != 0);
+        store_staged<TM, TN * 16, PITCH>(ep, lane, p.Y + (half ? p.F : 0), p.ldy, p.M, p.F, mw, fw, p.y16 != 0);
     }
 }
 
@@ -1017,8 +1009,8 @@ struct EpiScales {
             for (int g = 0; g < 4; ++g) {
                 if constexpr (Op::GATED) {
                     c[i][g] = make_float4(1.f, 1.f, 1.f, 1.f);
-                    const int f = nw / 2 + i % (TN / 2) * 32 + 8 * g + 4 * khalf;
-                    const bool up = i >= TN / 2;
+                    const int f = nw / 2 + (TN == 1 ? 8 * (g & 1) : i % (TN / 2) * 32 + 8 * g) + 4 * khalf;
+                    const bool up = TN == 1 ? g >= 2 : i >= TN / 2;
                     if (MODE == MODE_A8W8 && f < p.F) {
                         const float* s = static_cast<const float*>(p.sb) + (p.interleaved ? 2 * f : up ? p.F + f : f);
                         c[i][g] = *reinterpret_cast<const float4*>(s);
@@ -1199,7 +1191,8 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
     EpiScales<Op, MODE, TM, TN> sc;
     sc.load(p, lane, mw, nw);
     EpiResidual<Op, TM, TN> res;
-    if (p.splits == 1) res.load(p, lane, mw, nw);
+    constexpr bool EARLY = MINB == 1;  // two workgroups per CU: no registers for it (57 spilled)
+    if (EARLY && p.splits == 1) res.load(p, lane, mw, nw);
     EpiBias<Op, TN> bias;
     bias.load(p, lane, nw);
 
@@ -1207,13 +1200,15 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
     dense_kloop<Op, MODE, WM, WN, TM, TN, KTB, NS>(p, m0, n0, kt0, kt1, smem, acc);
 
     if (p.splits == 1) {
+        if (!EARLY) res.load(p, lane, mw, nw);
         dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, bias, smem, wave, lane, mw, nw);
         return;
     }
     v16f sum[TN][TM];
     static_assert(Cfg::EP_BYTES + 16 <= Cfg::lds_bytes(NS), "room for the split flag");
     HKQ_LDS int& flag = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::lds_bytes(NS) - 16);
-    if (!split_sum<TM, TN, NW, MINB == 1>(p, acc, sum, split, tile, tiles, wave, lane, flag, [&] { res.load(p, lane, mw, nw); })) return;
+    if (!split_sum<TM, TN, NW, MINB == 1>(p, acc, sum, split, tile, tiles, wave, lane, flag, [&] { if (EARLY) res.load(p, lane, mw, nw); })) return;
+    if (!EARLY) res.load(p, lane, mw, nw);
     dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, bias, smem, wave, lane, mw, nw);
 }
 
@@ -1243,7 +1238,12 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
 // read nothing and whose scales were fetched after the sums.
 constexpr int NARROW_WAVES = 4, NARROW_ROWS = 16, NARROW_MAX_STEPS = 32;
 
-template <class Op, int MODE>
+// GATED: 16 features per workgroup, a gate and an up row of the weight per lane
+// and step; PAIR: 8 features, rows 0 .. 7 of the operand the gate's and 8 .. 15
+// the up's, as many workgroups as the plain product has and no more loads in
+// each; a feature's sums then lie in lanes l and l + 32. One row of 4096x4096
+// (F 2048): PAIR 5.4 us, 16 features 7.3, the plain product 5.3.
+template <class Op, int MODE, bool PAIR = false>
 __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const typename Op::Params pb) {
     constexpr bool FP4 = MODE == MODE_MXFP4;
     constexpr int SB = FP4 ? 64 : 128;                      // bytes of a row per K-step
@@ -1253,25 +1253,28 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const ty
         uint32_t sb, sa;     // FP4: e8m0 scales of the step's 4 blocks (byte q is the lane's)
         v4i u0, u1;          // GATED (FP8): the up row
     };
-    constexpr bool GATED = Op::GATED;
-    static_assert(!GATED || !FP4, "gated: FP8");
+    constexpr bool GATED = Op::GATED && !PAIR;
+    constexpr int COLS = PAIR ? 8 : 16;
+    static_assert(!Op::GATED || !FP4, "gated: FP8");
     __shared__ v4f red[GATED ? 2 : 1][NARROW_WAVES][64];
     const typename Op::Params p = batch_slice(pb);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.z * NARROW_ROWS;
+    const int n0 = blockIdx.x * COLS, m0 = blockIdx.z * NARROW_ROWS;
     const int S = p.kbytes / SB;
     const int s0 = wave * S / NARROW_WAVES, s1 = (wave + 1) * S / NARROW_WAVES;
     int cols = p.N;  // GATED: n counts features
-    if constexpr (GATED) cols = p.F;
-    const int rows_a = min(NARROW_ROWS, p.M - m0), rows_b = min(16, cols - n0);
-    const auto rb = make_rsrc(p.B + (int64_t)n0 * p.ldb, (uint32_t)(rows_b * p.ldb));
+    if constexpr (Op::GATED) cols = p.F;
+    const int rows_a = min(NARROW_ROWS, p.M - m0), rows_b = min(COLS, cols - n0);
+    uint32_t to_up = 0;  // PAIR (F % 8 == 0: all 8 features): from a gate row to its up row
+    if constexpr (PAIR) to_up = (uint32_t)(p.Bu - p.B);
+    const auto rb = make_rsrc(p.B + (int64_t)n0 * p.ldb, to_up + (uint32_t)(rows_b * p.ldb));
     const uint8_t* up = p.B;
     if constexpr (GATED) up = p.Bu;
     const auto ru = make_rsrc(up + (int64_t)n0 * p.ldb, (uint32_t)(rows_b * p.ldb));
     const auto ra = make_rsrc(p.A + (int64_t)m0 * p.lda, (uint32_t)(rows_a * p.lda));
-    const uint32_t b_off = (uint32_t)(r * p.ldb + 16 * q), a_off = (uint32_t)(r * p.lda + 16 * q);
+    const uint32_t b_off = PAIR ? (uint32_t)((r & 7) * p.ldb + 16 * q) + (r >= 8 ? to_up : 0u) : (uint32_t)(r * p.ldb + 16 * q), a_off = (uint32_t)(r * p.lda + 16 * q);
     const auto rsb = make_rsrc(FP4 ? static_cast<const uint8_t*>(p.sb) + (int64_t)n0 * p.lsb : p.B,
                                FP4 ? (uint32_t)((rows_b - 1) * p.lsb + 4 * S) : 0u);
     const auto rsa = make_rsrc(FP4 ? static_cast<const uint8_t*>(p.sa) + (int64_t)m0 * p.lsa : p.A,
@@ -1314,14 +1317,14 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const ty
     // the epilogue's scales go out before the operands: no memory latency
     // follows the K loop
     const int n = n0 + 4 * q, m = m0 + r;
-    const bool in = n < cols && m < p.M;  // N % 4 == 0: n .. n+3 all in or all out
+    const bool in = n < cols && m < p.M && (!PAIR || q < 2);  // N % 4 == 0: n .. n+3 all in or all out
     float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), cu = cs;
     float a = 1.f;
     v2i res = v2i{0, 0};
     if (!FP4 && in) {
         const float* sb = static_cast<const float*>(p.sb);
         a = static_cast<const float*>(p.sa)[m];
-        if constexpr (GATED) {
+        if constexpr (Op::GATED) {
             cs = *reinterpret_cast<const float4*>(sb + (p.interleaved ? 2 * n : n));
             cu = *reinterpret_cast<const float4*>(sb + (p.interleaved ? 2 * n + 4 : p.F + n));
             if (p.interleaved) {
@@ -1335,7 +1338,8 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const ty
         if constexpr (Op::FUSED)
             if (p.residual) res = *reinterpret_cast<const v2i*>(p.residual + (int64_t)m * p.ldr + n);
     }
-    const float4 c = bias4(p, n);
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (!Op::GATED) c = bias4(p, n);
     Frag f[DEPTH];
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) load(s0 + d, f[d]);
@@ -1348,10 +1352,11 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const ty
     v4f v = red[0][0][lane];
 #pragma unroll
     for (int w = 1; w < NARROW_WAVES; ++w) v += red[0][w][lane];
-    if constexpr (GATED) {
-        v4f u = red[1][0][lane];
+    if constexpr (Op::GATED) {
+        const int at = PAIR ? lane + 32 : lane, h = PAIR ? 0 : 1;
+        v4f u = red[h][0][at];
 #pragma unroll
-        for (int w = 1; w < NARROW_WAVES; ++w) u += red[1][w][lane];
+        for (int w = 1; w < NARROW_WAVES; ++w) u += red[h][w][at];
         const float4 g = act4(p.act, make_float4(v[0] * a * cs.x, v[1] * a * cs.y, v[2] * a * cs.z, v[3] * a * cs.w));
         *reinterpret_cast<v2i*>(p.C + (int64_t)m * p.ldc + n) =
             v2i{(int)pk_bf16(g.x * (u[0] * a * cu.x), g.y * (u[1] * a * cu.y)),
@@ -1474,7 +1479,8 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
     EpiScales<Op, MODE, TM, TN> sc;
     sc.load(p, lane, mw, nw);
     EpiResidual<Op, TM, TN> res;
-    if (kg == 0) res.load(p, lane, mw, nw);
+    constexpr bool EARLY = !(MODE == MODE_A8W8 && Cfg::GW == 8 && TM * TN == 4);  // no registers for it (48 spilled)
+    if (EARLY && kg == 0) res.load(p, lane, mw, nw);
     EpiBias<Op, TN> bias;
     bias.load(p, lane, nw);
 
@@ -1490,6 +1496,7 @@ __global__ __launch_bounds__(Cfg::THREADS, 1) void dense_kgroup_kernel(const typ
             return;
         }
     if (kg != 0) return;
+    if (!EARLY) res.load(p, lane, mw, nw);
     dense_epilogue_global<Op, MODE, TM, TN>(p, acc, sc, res, bias, smem, wg, lane, mw, nw);
 }
 
@@ -1632,8 +1639,7 @@ static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const 
     int best = DT_NONE;
     float best_us = 0.f;
     for (int t = DT_256; t >= 0; --t) {
-        if (T.tile[t].us < 0.f || (t == DT_128x128_PAIR && kbytes % 128 != 0) || (t == DT_32x256 && (M > 32 || KT > 8)) ||
-            (gated && t == DT_32x32))  // one n-tile per wave: no pair of them
+        if (T.tile[t].us < 0.f || (t == DT_128x128_PAIR && kbytes % 128 != 0) || (t == DT_32x256 && (M > 32 || KT > 8)))
             continue;
         if (!(t == DT_256 ? fits(std::min<int64_t>(M, 256), std::min<int64_t>(N, 256)) : fits(BM[t], BN[t]))) continue;
         const int64_t tiles = batch * ((M + BM[t] - 1) / BM[t]) * ((N + BN[t] - 1) / BN[t]);
@@ -1770,7 +1776,7 @@ static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
 // on, 1 row from two rounds (1x9216x4096 8.5, 8.9; 4 rows 9.4, 9.0) and 4 rows
 // from three (4x12288x4096 9.6, 10.6; 4x28672x4096 19.8, 20.6; 8x28672x4096
 // 22.0, 20.6; 4x28672x2048 14.6, 12.8). Its buffer offsets are 32-bit.
-static bool use_narrow(int mode, const DenseParams& p, int64_t batch, int64_t cols) {
+static bool use_narrow(int mode, const DenseParams& p, int64_t batch, int64_t cols, bool one_round = false) {
     const int64_t step = mode == MODE_MXFP4 ? 64 : 128, S = p.kbytes / step;
     if (p.M < 1 || p.kbytes % step != 0 || S > NARROW_MAX_STEPS) return false;
     const int64_t wide = (1ll << 31) / NARROW_ROWS;
@@ -1778,7 +1784,7 @@ static bool use_narrow(int mode, const DenseParams& p, int64_t batch, int64_t co
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     const int64_t groups = (p.M + NARROW_ROWS - 1) / NARROW_ROWS, wgs = batch * ((cols + 15) / 16);
     if (groups <= 4 && groups * wgs <= ncu) return mode == MODE_A8W8 || S <= 16 || p.M <= 8;
-    return mode == MODE_A8W8 && S >= 24 && p.M <= (wgs >= 3 * ncu ? 4 : wgs >= 2 * ncu ? 1 : 0);
+    return !one_round && mode == MODE_A8W8 && S >= 24 && p.M <= (wgs >= 3 * ncu ? 4 : wgs >= 2 * ncu ? 1 : 0);
 }
 
 template <class Op, int MODE>
@@ -1791,8 +1797,18 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
         if (MODE == MODE_MXFP4) p.lsa = p.K / 32;
     }
     if constexpr (MODE != MODE_BF16) {
-        const int cols = Op::GATED ? p.N / 2 : p.N;  // gated: a workgroup's 16 columns are 16 features
-        if (use_narrow(MODE, p, batch, cols)) {
+        if constexpr (Op::GATED) {  // 8 features per workgroup where that is one round, buffer offsets in 32 bits
+            const int64_t span = (p.Bu - p.B) + 8 * p.ldb;
+            if (span < (1ll << 31) && use_narrow(MODE, p, batch, p.N, true)) {
+                const dim3 grid((unsigned)(p.F / 8), 1, (unsigned)((p.M + NARROW_ROWS - 1) / NARROW_ROWS));
+                narrow_gemm_kernel<Op, MODE, true><<<grid, 64 * NARROW_WAVES, 0, stream>>>(p);
+                return hkq_launch_status();
+            }
+        }
+        // gated: a workgroup's 16 columns are 16 features, for up to 8 rows: us against small
+        // tiles 8x5632x2048 (F 2816) 6.0, 6.0, 16 rows 6.3, 6.0; 24x4096x4096 8.6, 7.9
+        const int cols = Op::GATED ? p.N / 2 : p.N;
+        if ((!Op::GATED || p.M <= 8) && use_narrow(MODE, p, batch, cols)) {
             const dim3 grid((unsigned)((cols + 15) / 16), (unsigned)batch, (unsigned)((p.M + NARROW_ROWS - 1) / NARROW_ROWS));
             narrow_gemm_kernel<Op, MODE><<<grid, 64 * NARROW_WAVES, 0, stream>>>(p);
             return hkq_launch_status();
@@ -1808,9 +1824,7 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
     }
     constexpr int M4 = MODE == MODE_MXFP4;  // the e8m0 blocks take LDS from the ring
     switch (dense_tile_plan(MODE, p, batch, split ? &pl : nullptr, Op::GATED, Op::FUSED)) {
-        case DT_32x32:
-            if constexpr (!Op::GATED) return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 1, 1, 4>>(p, stream);
-            break;
+        case DT_32x32: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 1, 1, 4>>(p, stream);
         case DT_32x64: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4, 1, 2, 3 - M4>>(p, stream);
         case DT_32x128: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 1, 4 - M4, 1, 4, 2>>(p, stream);
         case DT_32x256: return launch_dense_kgroup<Op, KgCfg<MODE, 1, 4, 1, 1, 2, 3>>(p, stream);

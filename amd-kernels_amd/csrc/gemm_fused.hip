@@ -256,7 +256,6 @@ static int gemm_epilogue(const void* A, const void* B, const float* sa, const fl
     p.lda = lda * ES; p.ldb = ldb * ES; p.ldc = ldc;
     p.residual = static_cast<const uint16_t*>(residual);
     p.ldr = ldr;
-    p.r16 = ldr % 8 == 0 && reinterpret_cast<uintptr_t>(residual) % 16 == 0;
     return launch_dense<FusedOp, MODE>(p, workspace, workspace_bytes, stream);
 }
 

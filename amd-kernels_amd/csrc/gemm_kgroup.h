@@ -198,8 +198,8 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
         constexpr int SWP = Cfg::SWP;
         const uint32_t tail = src.half_tail && kt == src.KT - 1 ? OOB : 0u;
         if (GATED && idx < LB) {
-            static_assert(!GATED || (!GATHER && !FP4 && !BS && TN % 2 == 0 && (GW <= 4 || (GW == 8 && TN == 2))), "gated tiles");
-            constexpr int GP = GW <= 4 && GATED ? TN / 2 * 4 / GW : 1;
+            static_assert(!GATED || (!GATHER && !FP4 && !BS && (TN % 2 == 0 || (TN == 1 && GW == 1)) && (GW <= 4 || (GW == 8 && TN == 2))), "gated tiles");
+            constexpr int GP = GW <= 4 && GATED ? TN * 2 / GW : 1;
             const bool up = GW <= 4 && (idx / GP) % 2 != 0;
             const int fi = GW <= 4 ? idx / (2 * GP) * GP + idx % GP : idx;
             lds_load16_s(up ? src.b2 : src.b, st + Cfg::BM * 128 + (idx * GW + wg) * 1024,
