@@ -1603,7 +1603,8 @@ enum DenseTile {
     DT_256, DT_SPLIT,
     DT_NONE,  // rows too far apart for every size
     // of the fused and gated products only
-    DT_64x128, DT_192x256
+    DT_64x128, DT_192x256,
+    DT_PART  // 256 x 256 tiles, K split over workgroups, the sums in a second launch (gemm_fused.hip)
 };
 struct TileCost { float us, e; };
 struct TileCosts {

@@ -123,23 +123,112 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restr
     }
 }
 
+// --------------------------------------------------------------------------
+// dX of few tokens and a wide layer: 256 x 256 tiles whose K is split over
+// workgroups, each writing its fp32 sums to the workspace in register order (per
+// wave, float4 q of lane l at (q * 64 + l) * 16 bytes), and a second launch that
+// adds a value's partial sums in split order. The tile that feeds the matrix
+// cores best thus serves products of a quarter of the tiles that the CUs want;
+// 128 x 128 tiles, which fill the CUs without a split, are bound by their LDS
+// reads. A wave's 256 accumulators leave no room for a sum in the same launch.
+// --------------------------------------------------------------------------
+template <class Op>
+__global__ __launch_bounds__(256, 1) void part_gemm_kernel(const DenseParams p) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = p.tiles_m * p.tiles_n;
+    const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+    int tm, tn;
+    tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+    const int m0 = tm * DENSE_BM, n0 = tn * DENSE_BN;
+    const int kt0 = split * p.kt_split, kt1 = min(p.kbytes / 128, kt0 + p.kt_split);
+    v16f acc[DENSE_TN][DENSE_TM];
+    dense_kloop<Op, MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM, DENSE_TN, 128>(p, m0, n0, kt0, kt1,
+                                                                                      (HKQ_LDS uint8_t*)smem_raw, acc);
+    const int rows = p.M - m0 - wave / DENSE_WAVES_N * 128;
+    float4* out = reinterpret_cast<float4*>(p.ws) + ((int64_t)(split * tiles + tile) * 4 + wave) * (64 * 64) + lane;
+#pragma unroll
+    for (int j = 0; j < DENSE_TM; ++j) {
+        if (j * 32 >= rows) continue;  // (uniform) rows past the last
+#pragma unroll
+        for (int i = 0; i < DENSE_TN; ++i) {
+            float v[16];
+            read_acc(acc[i][j], v, 0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                out[((i * DENSE_TM + j) * 4 + g) * 64] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        }
+    }
+}
+// A wave per 32 x 32 values.
+__global__ __launch_bounds__(256) void part_sum_kernel(const DenseParams p) {
+    const int lane = threadIdx.x & 63;
+    const int block = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int tiles = p.tiles_m * p.tiles_n, tile = block >> 6, w = block >> 4 & 3, i = block >> 2 & 3, j = block & 3;
+    int tm, tn;
+    tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+    const int m = tm * DENSE_BM + w / DENSE_WAVES_N * 128 + j * 32, n = tn * DENSE_BN + w % DENSE_WAVES_N * 128 + i * 32;
+    if (m >= p.M || n >= p.N) return;
+    const float4* in = reinterpret_cast<const float4*>(p.ws) + ((int64_t)tile * 4 + w) * (64 * 64) + (i * DENSE_TM + j) * 256 + lane;
+    const int64_t stride = (int64_t)tiles * 4 * (64 * 64);
+    float4 sum[4] = {in[0], in[64], in[128], in[192]};
+#pragma unroll 3
+    for (int s = 1; s < p.splits; ++s) {
+        in += stride;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 v = in[g * 64];
+            sum[g].x += v.x, sum[g].y += v.y, sum[g].z += v.z, sum[g].w += v.w;
+        }
+    }
+    const int row = m + (lane & 31);
+    if (row >= p.M) return;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int col = n + 8 * g + 4 * (lane >> 5);
+        if (col < p.N)
+            *reinterpret_cast<v2i*>(p.C + (int64_t)row * p.ldc + col) = v2i{(int)pk_bf16(sum[g].x, sum[g].y), (int)pk_bf16(sum[g].z, sum[g].w)};
+    }
+}
+template <class Op>
+static int launch_part(DenseParams& p, int splits, int kt_split, void* ws, hipStream_t stream) {
+    constexpr int LDS = dense_ring_lds<MODE_BF16, 128>();
+    auto kern = part_gemm_kernel<Op>;
+    static bool attr_set = false;
+    if (int e = set_lds(kern, LDS, attr_set)) return e;
+    p.tiles_m = (p.M + DENSE_BM - 1) / DENSE_BM;
+    p.tiles_n = (p.N + DENSE_BN - 1) / DENSE_BN;
+    if (p.group_m <= 0) p.group_m = 8;
+    p.splits = splits;
+    p.kt_split = kt_split;
+    p.ws = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + SPLIT_CNT_BYTES);
+    const unsigned tiles = (unsigned)(p.tiles_m * p.tiles_n);
+    kern<<<tiles * splits, 256, LDS, stream>>>(p);
+    if (int e = hkq_launch_status()) return e;
+    part_sum_kernel<<<tiles * 16, 256, 0, stream>>>(p);
+    return hkq_launch_status();
+}
+
 // Plan of a backward product over `KT` K-tiles of 64: the least estimated time
-// over the tile sizes, rounds over the CUs * (K-tiles * us + e), or 128 x 128
-// tiles with K split over workgroups (partial sums in the workspace), one round
-// of them. us and e fitted to MI355X times of every size at 16 .. 4096 tokens of
-// two layers (K-tiles of one size cost more the more of the weight comes from
-// memory; the constants are those of a large one). Tokens x F x K, us: dX
-// 4096x14336x4096 256 x 256 672, 128 x 256 784, 128 x 128 1047; 2048x14336x4096
-// 417 (M halves), 394, 516; 1001x2816x2048 128 x 64 31, 128 x 128 36, two splits
-// 30; 64x2816x2048 21, 33, six splits 12.5. dW 1001x2816x2048 192 x 256 (one
-// round only) 26, 256 x 256 29, 128 x 256 34, 128 x 128 34; 1001x1408x2048 21, 21,
-// 18.5, 23.
+// over the tile sizes, rounds over the CUs * (K-tiles * us + e), or K split over
+// workgroups in one round of them, on 128 x 128 tiles (summed by the last one) or
+// (`part`, dX) on 256 x 256 tiles with a second launch. us and e fitted to MI355X
+// times of every size at 16 .. 4096 tokens of six layers (K-tiles of one size cost
+// more the more of the weight comes from memory; the constants are those of a
+// large one). Tokens x F x K, us: dX 4096x14336x4096 256 x 256 672, 128 x 256 784,
+// 128 x 128 1047; 1024x14336x4096 256 x 256 in four parts 209, 128 x 128 280;
+// 512x14336x4096 eight parts 121, 128 x 128 in two splits 155; 256x14336x4096
+// twelve parts 86, four splits 83; 1001x2816x2048 128 x 64 31, 128 x 128 36, two
+// splits 30, six parts 41; 64x2816x2048 21, 33, six splits 12.5. dW 1001x2816x2048
+// 192 x 256 (one round only) 26, 256 x 256 29, 128 x 256 34, 128 x 128 34;
+// 1001x1408x2048 21, 21, 18.5, 23.
 struct TransPlan {
     int tile;  // a DenseTile
     int splits, kt_split;
     size_t ws_bytes;
 };
-static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT) {
+static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT, bool part) {
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     static const struct { int tile, bm, bn; TileCost c; } T[] = {
         {DT_256, 256, 256, {1.37f, 5.7f}}, {DT_128x256, 128, 256, {0.85f, 3.2f}}, {DT_128x128, 128, 128, {0.57f, 2.2f}},
@@ -164,6 +253,19 @@ static TransPlan trans_plan(int64_t M, int64_t N, int64_t KT) {
             p = TransPlan{DT_SPLIT, (int)n, (int)per, SPLIT_CNT_BYTES + (size_t)(n * t128) * (128 * 128 * 4)};
         }
     }
+    // the parts take 12 % less than the rest or stay out: the estimates are those of
+    // a weight that comes from memory (1500x5632x2048, whose weight the caches hold,
+    // estimated 97 and 102, measured 81 and 73)
+    const int64_t t256 = ((M + 255) / 256) * ((N + 255) / 256);
+    best *= 0.88f;
+    for (int64_t s = 2; part && s <= std::min<int64_t>(ncu / t256, KT / 8); ++s) {
+        const int64_t per = (KT + s - 1) / s, n = (KT + per - 1) / per;
+        const float us = (float)per * 1.30f + 4.6f + (float)(n * t256) * 0.19f;
+        if (us < best) {
+            best = us;
+            p = TransPlan{DT_PART, (int)n, (int)per, SPLIT_CNT_BYTES + (size_t)(n * t256) * (256 * 256 * 4)};
+        }
+    }
     return p;
 }
 
@@ -176,12 +278,15 @@ template <bool AT>
 static int launch_trans(DenseParams& p, void* ws, hipStream_t stream) {
     using Op = TransOp<AT, true>;
     p.c16 = p.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
-    const TransPlan pl = trans_plan(p.M, p.N, p.kbytes / 128);
+    const TransPlan pl = trans_plan(p.M, p.N, p.kbytes / 128, !AT);
     switch (pl.tile) {
         case DT_128x64: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 1, 2, 1, 2, 3>>(p, stream);
         case DT_128x128: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 2, 1, 1, 2, 4>>(p, stream);
         case DT_128x256: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 2, 4, 1, 2, 2, 3>>(p, stream);
         case DT_192x256: return launch_dense_mid<Op, MODE_BF16>(p, stream);
+        case DT_PART:
+            if constexpr (!AT) return launch_part<Op>(p, pl.splits, pl.kt_split, ws, stream);
+            break;
         case DT_SPLIT: return launch_dense_kgroup<Op, KgCfg<MODE_BF16, 4, 2, 1, 1, 2, 4>>(p, stream, pl.splits, pl.kt_split, ws);
     }
     return launch_dense_whole<Op, MODE_BF16, 128>(p, stream);
@@ -205,7 +310,8 @@ static int launch_zero_rows(void* out, int64_t rows, int64_t cols, int64_t ld, h
 // product.
 static int64_t grad_pitch(int64_t F) { return (2 * F + 63) / 64 * 64; }
 static size_t grad_offset(int64_t M, int64_t F, int64_t K) {
-    const size_t dx = trans_plan(M, K, grad_pitch(F) / 64).ws_bytes, dw = trans_plan(2 * F, K, (M + 63) / 64).ws_bytes;
+    const size_t dx = trans_plan(M, K, grad_pitch(F) / 64, true).ws_bytes,
+                 dw = trans_plan(2 * F, K, (M + 63) / 64, false).ws_bytes;
     return ((dx > dw ? dx : dw) + 255) / 256 * 256;
 }
 

@@ -105,6 +105,8 @@ def test_backward_workspace_query():
     assert q(4096, 14336, 4096) == 4096 * 28672 * 2          # many tiles each: no split
     assert q(10, 40, 64) == 10 * 128 * 2                     # rows of whole 64-value K-tiles
     assert q(16, 14336, 512) > 16 * 28672 * 2                # 4 tiles over 448 K-tiles
+    # dX's 64 tiles of 256 x 256 in four parts
+    assert q(1024, 14336, 4096) == 4096 + 4 * 64 * 256 * 256 * 4 + 1024 * 28672 * 2
 
 
 def test_tensor_layer_refusals():

@@ -536,6 +536,29 @@ def test_backward_large_tiles(interleaved, M, F, K, act):
     untouched(wb, 2 * F, K)
 
 
+# few tokens of a wide layer: dX's K split over 256 x 256 tiles; rows and columns
+# that end inside a tile, a last part shorter than the others
+@pytest.mark.parametrize("M,F,K,interleaved", [(600, 8200, 3328, False), (1300, 8200, 3232, True), (513, 8192, 3296, False)])
+def test_backward_parts(M, F, K, interleaved):
+    """The reference in 64 bits on the GPU; the same bits again from a workspace that held NaN."""
+    require_gpu()
+    X, W, Y, dH = bf16((M, K), 1).cuda(), bf16((2 * F, K), 2, 0.05).cuda(), bf16((M, 2 * F), 3, 1.5).cuda(), bf16((M, F), 4, 0.3).cuda()
+    xb, dX = guarded(M, K, K + 8)
+    hkq.gated_ffn_backward(dH, X, W, Y, interleaved=interleaved, dX=dX, need_dw=False)
+    n = hkq.lib().hkq_gated_ffn_backward_workspace(M, F, K)
+    assert n >= M * 4 * F + 2 * 4 * (M // 256 + 1) * 256 * K  # two parts at least
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
+    again = torch.empty((M, K), dtype=BF16, device="cuda")
+    hkq.call("hkq_gated_ffn_backward", dH.data_ptr(), None, W.data_ptr(), Y.data_ptr(), again.data_ptr(), None, M, F, K,
+             F, K, K, 2 * F, K, K, hkq.ACTIVATIONS["silu"], 1.0, int(interleaved), ws.data_ptr(), n,
+             torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(again, dX)
+    rx, _ = backward_ref(dH, X[:, :32], W, Y, "silu", 1.0, interleaved)
+    close(dX, *rx, f"dX {M}x{F}x{K}", 2)
+    untouched(xb, M, K)
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_backward_activations_pitches_and_one_gradient(act):
     """NaN between the operands' rows reaches nothing; either gradient alone gives the same bits."""
