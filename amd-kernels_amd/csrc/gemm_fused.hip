@@ -14,15 +14,15 @@
 // what a fused epilogue saves is the passes after the product (an activation of
 // [M, 2F] alone reads 4 and writes 2 bytes per feature). us on MI355X, M x N x K
 // (gated: M x F x K), inputs that rotate:
-//   FP8 + residual      16x4096x14336 12.7 (the weights at 4.6 TB/s), 4096x4096x14336
-//                       185 (2.60 PFLOP/s);
-//   bf16, bias, GELU    601x14336x4096 88 (0.80 PFLOP/s: a fifth of the 192-row
+//   FP8 + residual      16x4096x14336 12.4 (the weights at 4.7 TB/s), 4096x4096x14336
+//                       184 (2.61 PFLOP/s);
+//   bf16, bias, GELU    601x14336x4096 87 (0.81 PFLOP/s: a fifth of the 192-row
 //                       tiles' rows is padding, 224 of them on 256 CUs);
-//   gated FP8           24x14336x4096 25.9 (4.5 TB/s), 4096x14336x4096 363 (2.65
+//   gated FP8           24x14336x4096 25.3 (4.6 TB/s), 4096x14336x4096 359 (2.68
 //                       PFLOP/s);
-//   gated bf16          301x2816x2048 13.1, 4096x14336x4096 with the projections
-//                       kept 742 (1.30 PFLOP/s, and 352 MB written);
-//   gated backward      1001x2816x2048 63.5, 4096x14336x4096 1510 (1.27 PFLOP/s
+//   gated bf16          301x2816x2048 12.7, 4096x14336x4096 with the projections
+//                       kept 737 (1.30 PFLOP/s, and 352 MB written);
+//   gated backward      1001x2816x2048 62.9, 4096x14336x4096 1484 (1.30 PFLOP/s
 //                       and the gradients' pass over memory).
 #include <limits>
 
