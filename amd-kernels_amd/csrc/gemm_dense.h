@@ -1770,8 +1770,8 @@ static int launch_dense_whole(typename Op::Params& p, hipStream_t stream) {
 // cheaper ones, takes more than 16 steps to 8 rows only. Measured on MI355X
 // against the small tiles, us: A8W8 1x4096x4096 4.0 and 5.3, 16x4096x4096 5.4
 // both, 32x1000x256 3.7 and 4.1, 64x1000x4096 5.6 and 5.7; MXFP4 1x1000x256 3.7
-// and 3.9, 32x1000x1024 3.7 and 4.2, 8x2048x4096 4.6 and 4.7, 16x2048x3072 4.8
-// and 4.5. More workgroups start one after another, 0.9 us per round of them
+// and 3.9, 32x1000x1024 3.7 and 4.2, 8x2048x4096 4.6 and 4.7, 16 rows of
+// 24 steps 4.8 and 4.5. More workgroups start one after another, 0.9 us per round of them
 // whatever K is (A8W8 1x28672x128 8.3 us, 4.0 on small tiles; 1x6144x4096 6.2,
 // 5.4), which only a stream that is long by itself hides: A8W8 from 24 K-steps
 // on, 1 row from two rounds (1x9216x4096 8.5, 8.9; 4 rows 9.4, 9.0) and 4 rows
