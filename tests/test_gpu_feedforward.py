@@ -430,6 +430,29 @@ def test_gated_shapes(kind, interleaved, M, F, K):
         untouched(ybuf, M, 2 * F)
 
 
+# workgroups of 8 features and of 16, one and several groups of rows, 32 x 32 tiles
+# over a long K and with a half K-tile at its end
+@pytest.mark.parametrize("kind", ["a8w8", "bf16_save"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("M,F,K", [(1, 2048, 4096), (4, 1000, 2048), (8, 4000, 512), (2, 14336, 4096), (16, 2048, 128),
+                                   (24, 2040, 8192), (33, 504, 1088), (63, 1024, 2816), (64, 512, 4096)])
+def test_gated_few_rows(kind, interleaved, M, F, K):
+    require_gpu()
+    save, kind = kind.endswith("save"), kind[:4]
+    A, W, sa, sw = (t if t is None else t.cuda() for t in operands(kind, M, 2 * F, K, M + F + K))
+    hbuf, H = guarded(M, F, F + 8)
+    kw = {}
+    if save:
+        ybuf, kw["Y"] = guarded(M, 2 * F, 2 * F + 8)
+    gated(kind, A, W, sa, sw, act="gelu_tanh", interleaved=interleaved, H=H, **kw)
+    y, err = sums(kind, A, W, sa, sw)
+    close(H, *gated_ref(y, err, "gelu_tanh", 1.0, interleaved), f"{kind} {M}x{F}x{K}")
+    untouched(hbuf, M, F)
+    if save:
+        close(kw["Y"], y, err + U * y.abs(), "kept projections")
+        untouched(ybuf, M, 2 * F)
+
+
 @pytest.mark.parametrize("kind", ["a8w8", "bf16", "bf16_save"])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("which,act", [(0, "silu"), (1, "gelu_tanh"), (2, "gelu")])
