@@ -326,6 +326,25 @@ def test_epilogue_split_k_repeats(kind):
     close(epilogue(kind, *cu, split=False, **kw), *want, "unsplit")
 
 
+@pytest.mark.parametrize("kind", ["a8w8", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(3, 1000, 512), (40, 4100, 1024), (100, 5632, 2048), (300, 1036, 1024), (300, 14340, 512),
+                                   (1024, 1024, 1024), (1100, 7172, 512), (500, 4096, 14336)])
+def test_epilogue_residual_in_place(kind, M, N, K):
+    """The residual as C gives the bits of a residual of its own, in every tile size."""
+    require_gpu()
+    A, B, sa, sb = (t if t is None else t.cuda() for t in operands(kind, M, N, K, M + N))
+    res, bias = bf16((M, N), 7).cuda(), bf16((N,), 8).cuda()
+    call = (lambda **kw: hkq.gemm_a8w8_epilogue(A, B, sa, sb, **kw)) if kind == "a8w8" else \
+        (lambda **kw: hkq.gemm_bf16_epilogue(A, B, **kw))
+    want = call(bias=bias, act="silu", residual=res)
+    buf, C = guarded(M, N, N + 4)
+    C.copy_(res)
+    call(bias=bias, act="silu", residual=C, C=C)
+    torch.cuda.synchronize()
+    assert torch.equal(C, want)
+    untouched(buf, M, N)
+
+
 # grids of the streaming kernel (whole tiles over several rounds and a last round
 # in halves; its K-tiles come in eights: K a multiple of 512 bf16 or 1024 FP8
 # values) and of 192-row tiles, ragged in both directions, rows of C pitched
