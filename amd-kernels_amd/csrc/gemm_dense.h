@@ -339,10 +339,10 @@ __device__ __forceinline__ float4 add_bf16x4(float4 v, const v2i& r) {
 
 // FUSED epilogue: act(sums * scales + bias) + residual in fp32, one rounding,
 // staged and stored as store_tile_bf16 does. A residual in row pieces is put where
-// the results will go, and each lane replaces its own values. One branch on the activation for
-// the whole sub-tile: one per four columns jumped over the other forms' code 8 to
-// 16 times, each a fetch of instructions from L2 (FP8 1024x1024x1024 with bias 9.0
-// us, with one branch 8.0, the plain GEMM 7.0).
+// the results will go, and each lane replaces its own values. One branch on the
+// activation for the whole sub-tile: one per four columns jumped over the other
+// forms' code 8 to 16 times, each a fetch of instructions from L2 (FP8
+// 1024x1024x1024 with bias 9.0 us, with one branch 8.0, the plain GEMM 7.0).
 template <class Op, int TM, int TN, typename RowScale, typename ColScale4>
 __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], const EpiResidual<Op, TM, TN>& res,
                                                  const EpiBias<Op, TN>& bias, HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw,
