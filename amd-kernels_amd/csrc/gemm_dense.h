@@ -345,8 +345,8 @@ __device__ __forceinline__ float4 add_bf16x4(float4 v, const v2i& r) {
 // 1024x1024x1024 with bias 9.0 us, with one branch 8.0, the plain GEMM 7.0).
 template <class Op, int TM, int TN, typename RowScale, typename ColScale4>
 __device__ __forceinline__ void fused_store_tile(const FusedParams& p, v16f (&acc)[TN][TM], const EpiResidual<Op, TM, TN>& res,
-                                                 const EpiBias<Op, TN>& bias, HKQ_LDS uint8_t* smem, int wave, int lane, int mw, int nw,
-                                                 RowScale row_scale, ColScale4 col_scale4) {
+                                                 const EpiBias<Op, TN>& bias, HKQ_LDS uint8_t* smem, int wave,
+                                                 int lane, int mw, int nw, RowScale row_scale, ColScale4 col_scale4) {
     constexpr int PITCH = TN * 32 * 2 + 16;
     constexpr bool HELD = EpiResidual<Op, TM, TN>::HELD;
     HKQ_LDS uint8_t* ep = smem + wave * (TM * 32) * PITCH;
@@ -439,7 +439,8 @@ __device__ __forceinline__ void gated_store_tile(const FusedParams& p, v16f (&ac
     each([&](int i, int g, int j, int r, int n) {
         const v16f& v = gate[i][j];
         const float4 u = value(i + UN, j, g + UG), a = make_float4(v[4 * g + 0], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-        *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) = v2i{(int)pk_bf16(a.x * u.x, a.y * u.y), (int)pk_bf16(a.z * u.z, a.w * u.w)};
+        *reinterpret_cast<HKQ_LDS v2i*>(ep + r * PITCH + n * 2) =
+            v2i{(int)pk_bf16(a.x * u.x, a.y * u.y), (int)pk_bf16(a.z * u.z, a.w * u.w)};
     });
     store_staged<TM, TN * 16, PITCH>(ep, lane, p.C, p.ldc, p.M, p.F, mw, fw, p.c16 != 0);
     if (!p.Y) return;
@@ -1016,7 +1017,8 @@ struct EpiScales {
                         c[i][g] = *reinterpret_cast<const float4*>(s);
                         if (p.interleaved) {
                             const float4 d = *reinterpret_cast<const float4*>(s + 4);
-                            c[i][g] = up ? make_float4(c[i][g].y, c[i][g].w, d.y, d.w) : make_float4(c[i][g].x, c[i][g].z, d.x, d.z);
+                            c[i][g] = up ? make_float4(c[i][g].y, c[i][g].w, d.y, d.w)
+                                         : make_float4(c[i][g].x, c[i][g].z, d.x, d.z);
                         }
                     }
                     continue;
@@ -1207,7 +1209,10 @@ __global__ __launch_bounds__(64 * WM * WN, MINB) void dense_tile_kernel(const ty
     v16f sum[TN][TM];
     static_assert(Cfg::EP_BYTES + 16 <= Cfg::lds_bytes(NS), "room for the split flag");
     HKQ_LDS int& flag = *reinterpret_cast<HKQ_LDS int*>(smem + Cfg::lds_bytes(NS) - 16);
-    if (!split_sum<TM, TN, NW, MINB == 1>(p, acc, sum, split, tile, tiles, wave, lane, flag, [&] { if (EARLY) res.load(p, lane, mw, nw); })) return;
+    auto summing = [&] {
+        if (EARLY) res.load(p, lane, mw, nw);
+    };
+    if (!split_sum<TM, TN, NW, MINB == 1>(p, acc, sum, split, tile, tiles, wave, lane, flag, summing)) return;
     if (!EARLY) res.load(p, lane, mw, nw);
     dense_epilogue_global<Op, MODE, TM, TN>(p, sum, sc, res, bias, smem, wave, lane, mw, nw);
 }
@@ -1274,7 +1279,8 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const ty
     if constexpr (GATED) up = p.Bu;
     const auto ru = make_rsrc(up + (int64_t)n0 * p.ldb, (uint32_t)(rows_b * p.ldb));
     const auto ra = make_rsrc(p.A + (int64_t)m0 * p.lda, (uint32_t)(rows_a * p.lda));
-    const uint32_t b_off = PAIR ? (uint32_t)((r & 7) * p.ldb + 16 * q) + (r >= 8 ? to_up : 0u) : (uint32_t)(r * p.ldb + 16 * q), a_off = (uint32_t)(r * p.lda + 16 * q);
+    const uint32_t b_off = (uint32_t)((PAIR ? r & 7 : r) * p.ldb + 16 * q) + (PAIR && r >= 8 ? to_up : 0u);
+    const uint32_t a_off = (uint32_t)(r * p.lda + 16 * q);
     const auto rsb = make_rsrc(FP4 ? static_cast<const uint8_t*>(p.sb) + (int64_t)n0 * p.lsb : p.B,
                                FP4 ? (uint32_t)((rows_b - 1) * p.lsb + 4 * S) : 0u);
     const auto rsa = make_rsrc(FP4 ? static_cast<const uint8_t*>(p.sa) + (int64_t)m0 * p.lsa : p.A,
@@ -1364,7 +1370,8 @@ __global__ __launch_bounds__(64 * NARROW_WAVES) void narrow_gemm_kernel(const ty
         return;
     }
     if constexpr (Op::FUSED) {
-        float4 o = act4(p.act, make_float4(v[0] * a * cs.x + c.x, v[1] * a * cs.y + c.y, v[2] * a * cs.z + c.z, v[3] * a * cs.w + c.w));
+        float4 o = act4(p.act, make_float4(v[0] * a * cs.x + c.x, v[1] * a * cs.y + c.y, v[2] * a * cs.z + c.z,
+                                           v[3] * a * cs.w + c.w));
         if (p.residual) o = add_bf16x4(o, res);
         *reinterpret_cast<v2i*>(p.C + (int64_t)m * p.ldc + n) = v2i{(int)pk_bf16(o.x, o.y), (int)pk_bf16(o.z, o.w)};
         return;
@@ -1613,7 +1620,8 @@ struct TileCosts {
     float split_us, split_e, split_parts;  // 128 x 128 tiles: per K-tile, constant, per split
     TileCost t64x128, t192x256;
 };
-static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const DensePlan* split, bool gated = false, bool fused = false) {
+static int dense_tile_plan(int mode, const DenseParams& p, int64_t batch, const DensePlan* split, bool gated = false,
+                           bool fused = false) {
     const int64_t M = p.M, N = p.N, kbytes = p.kbytes;
     // Tile rows `ld` bytes apart that a 32-bit buffer offset reaches. The 256-row
     // kernels end their extents with the last live row, so only those count
@@ -1820,8 +1828,8 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
     bool split = false;
     if constexpr (MODE != MODE_MXFP4) {
         pl = dense_plan(MODE, p.M, p.N, p.kbytes);
-        split = !Op::GATED && p.batch <= 1 && (Op::FUSED || p.bias == nullptr) && pl.geo != GEO_SKINNY && pl.splits > 1 && ws != nullptr &&
-                ws_bytes >= pl.ws_bytes;
+        split = !Op::GATED && p.batch <= 1 && (Op::FUSED || p.bias == nullptr) && pl.geo != GEO_SKINNY && pl.splits > 1 &&
+                ws != nullptr && ws_bytes >= pl.ws_bytes;
     }
     constexpr int M4 = MODE == MODE_MXFP4;  // the e8m0 blocks take LDS from the ring
     switch (dense_tile_plan(MODE, p, batch, split ? &pl : nullptr, Op::GATED, Op::FUSED)) {

@@ -170,7 +170,8 @@ __global__ __launch_bounds__(256) void part_sum_kernel(const DenseParams p) {
     tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
     const int m = tm * DENSE_BM + w / DENSE_WAVES_N * 128 + j * 32, n = tn * DENSE_BN + w % DENSE_WAVES_N * 128 + i * 32;
     if (m >= p.M || n >= p.N) return;
-    const float4* in = reinterpret_cast<const float4*>(p.ws) + ((int64_t)tile * 4 + w) * (64 * 64) + (i * DENSE_TM + j) * 256 + lane;
+    const float4* in = reinterpret_cast<const float4*>(p.ws) + ((int64_t)tile * 4 + w) * (64 * 64) +
+                       (i * DENSE_TM + j) * 256 + lane;
     const int64_t stride = (int64_t)tiles * 4 * (64 * 64);
     float4 sum[4] = {in[0], in[64], in[128], in[192]};
 #pragma unroll 3
@@ -188,7 +189,8 @@ __global__ __launch_bounds__(256) void part_sum_kernel(const DenseParams p) {
     for (int g = 0; g < 4; ++g) {
         const int col = n + 8 * g + 4 * (lane >> 5);
         if (col < p.N)
-            *reinterpret_cast<v2i*>(p.C + (int64_t)row * p.ldc + col) = v2i{(int)pk_bf16(sum[g].x, sum[g].y), (int)pk_bf16(sum[g].z, sum[g].w)};
+            *reinterpret_cast<v2i*>(p.C + (int64_t)row * p.ldc + col) =
+                v2i{(int)pk_bf16(sum[g].x, sum[g].y), (int)pk_bf16(sum[g].z, sum[g].w)};
     }
 }
 template <class Op>
