@@ -486,8 +486,9 @@ extern "C" int hkq_add_rmsnorm_quant(const void* x, const void* res, const void*
                                      int group, int kind, hkq_stream_t stream) {
     HKQ_CHECK_ARG(kind == HKQ_KIND_FP8 || kind == HKQ_KIND_INT8, "kind must be HKQ_KIND_FP8 or HKQ_KIND_INT8");
     HKQ_CHECK_ARG(group == 0 || group == 128, "group must be 0 (per token) or 128");
-    // one launch: fewer than 2^32 threads
-    HKQ_CHECK_ARG(M >= 0 && M < (D <= 1024 ? 1 << 26 : 1 << 24), "M must be in [0, 2^24), below 2^26 for D <= 1024");
+    // one launch: fewer than 2^32 threads, 256 per row or (D <= 1024) per four rows, the last four counted whole
+    HKQ_CHECK_ARG(M >= 0 && M <= (D <= 1024 ? (1 << 26) - 4 : (1 << 24) - 1),
+                  "M must be in [0, 2^24), for D <= 1024 in [0, 2^26 - 4]");
     HKQ_CHECK_ARG(D >= 8 && D <= 16384 && D % (group ? 128 : 8) == 0,
                   "D must be a multiple of 8 (128 with groups) in [8, 16384]");
     HKQ_CHECK_ARG(ldx >= D && ldx % 8 == 0, "ldx must be >= D and a multiple of 8");

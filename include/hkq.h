@@ -117,10 +117,11 @@ int hkq_swiglu_quant(const void* y, void* q, float* s, int64_t M, int64_t F, int
  * kind HKQ_KIND_FP8 (E4M3FN, QMAX 448) or HKQ_KIND_INT8 (round half even,
  * QMAX 127). The sum is fp32 in an order fixed by D; a NaN among the values of
  * a scale makes that scale NaN. h may be x or res (same pitch). D a multiple of
- * 8 (128 with groups) in [8, 16384]; pitches multiples of 8; M < 2^24 (2^26 for
- * D <= 1024). No counterpart in the reference (its fused_rmsnorm_fp8_quant_fwd
- * has no residual and 1x128 scales only): what feeds the layer's first product,
- * hkq_gemm_a8w8 / hkq_gated_ffn_a8w8 (group 0) or hkq_gemm_blockscale (group 128). */
+ * 8 (128 with groups) in [8, 16384]; pitches multiples of 8; M < 2^24 (up to
+ * 2^26 - 4 for D <= 1024). No counterpart in the reference (its
+ * fused_rmsnorm_fp8_quant_fwd has no residual and 1x128 scales only): what feeds
+ * the layer's first product, hkq_gemm_a8w8 / hkq_gated_ffn_a8w8 (group 0) or
+ * hkq_gemm_blockscale (group 128). */
 int hkq_add_rmsnorm_quant(const void* x, const void* res, const void* w, void* h, void* q, float* s, int64_t M,
                           int64_t D, int64_t ldx, int64_t ldr, int64_t ldh, int64_t ldq, int64_t lds, float eps,
                           int group, int kind, hkq_stream_t stream);

@@ -154,3 +154,9 @@ def test_modules_offer_the_operators():
         hk.ffn.gated.gated_ffn_bf16(x, x, x)
     with pytest.raises(ValueError, match="GPU tensor"):
         hk.fused_add_rmsnorm_quant_fwd(x, None, x, None, x, x, 1e-6)
+
+
+@pytest.mark.parametrize("M", [(1 << 26) - 3, (1 << 26) - 1])
+def test_norm_rows_of_one_launch(M):
+    """Four rows per workgroup of 256 threads: 2^26 - 3 rows round up to 2^24 workgroups, 2^32 threads."""
+    refused(*norm(M=M, D=8, ldx=8, ldr=8, ldh=8, ldq=8, lds=1, group=0), match="M must")
