@@ -468,6 +468,19 @@ int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const v
     HKQ_CHECK_ALIGN(dX, 8);
     HKQ_CHECK_ALIGN(dW, 8);
     HKQ_CHECK_ALIGN(workspace, 16);
+    // The outputs over the operands of the products: dX = dY . W and dW = dY^T . X
+    // run one after the other, dW first where dX takes X's memory.
+    const MemRows mx{X, M, 2 * K, 2 * ldx}, mw{W, 2 * F, 2 * K, 2 * ldw}, mdx{dX, M, 2 * K, 2 * lddx},
+        mdw{dW, 2 * F, 2 * K, 2 * lddw}, mws{workspace, 1, (int64_t)hkq_gated_ffn_backward_workspace(M, F, K), 0};
+    HKQ_CHECK_ARG(!overlap(mdx, mw), "dX must not overlap W");
+    HKQ_CHECK_ARG(!overlap(mdw, mx), "dW must not overlap X");
+    HKQ_CHECK_ARG(!overlap(mdx, mdw), "dX and dW must not overlap");
+    const bool dw_first = dW && overlap(mdx, mx);
+    HKQ_CHECK_ARG(!dw_first || !overlap(mdw, mw), "dX over X and dW over W: one of the two at most");
+    const MemRows mdh{dH, M, 2 * F, 2 * lddh}, my{Y, M, 4 * F, 2 * ldy};
+    HKQ_CHECK_ARG(!overlap(mws, mdh) && !overlap(mws, my) && !(dW && overlap(mws, mx)) && !(dX && overlap(mws, mw)) &&
+                      !overlap(mws, mdx) && !overlap(mws, mdw),
+                  "the workspace must not overlap an operand");
     if (M == 0) return dW ? launch_zero_rows(dW, 2 * F, K, lddw, stream) : 0;
     if (F == 0) return launch_zero_rows(dX, M, K, lddx, stream);
     const int64_t P = grad_pitch(F);
@@ -478,20 +491,26 @@ int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const v
         static_cast<const uint16_t*>(dH), static_cast<const uint16_t*>(Y), dy_rows, M, (int)F, lddh, ldy, P, segs,
         interleaved != 0, a);
     if (int e = hkq_launch_status()) return e;
-    if (dX) {  // [M, K] = dY [M, 2F] . W [2F, K]
+    auto product_dx = [&]() -> int {  // [M, K] = dY [M, 2F] . W [2F, K]
         DenseParams p{};
         p.A = dy; p.B = static_cast<const uint8_t*>(W); p.C = static_cast<uint16_t*>(dX);
         p.M = (int)M; p.N = (int)K; p.K = (int)(2 * F); p.kbytes = (int)(2 * P);
         p.lda = 2 * P; p.ldb = 2 * ldw; p.ldc = lddx;
-        if (int e = launch_trans<false>(p, workspace, stream)) return e;
-    }
-    if (dW) {  // [2F, K] = dY^T . X [M, K]
+        return launch_trans<false>(p, workspace, stream);
+    };
+    auto product_dw = [&]() -> int {  // [2F, K] = dY^T . X [M, K]
         DenseParams p{};
         p.A = dy; p.B = static_cast<const uint8_t*>(X); p.C = static_cast<uint16_t*>(dW);
         p.M = (int)(2 * F); p.N = (int)K; p.K = (int)M; p.kbytes = (int)((M + 63) / 64 * 128);
         p.lda = 2 * P; p.ldb = 2 * ldx; p.ldc = lddw;
-        if (int e = launch_trans<true>(p, workspace, stream)) return e;
-    }
+        return launch_trans<true>(p, workspace, stream);
+    };
+    if (dw_first)
+        if (int e = product_dw()) return e;
+    if (dX)
+        if (int e = product_dx()) return e;
+    if (dW && !dw_first)
+        if (int e = product_dw()) return e;
     return 0;
 }
 

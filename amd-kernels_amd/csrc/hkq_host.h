@@ -11,6 +11,25 @@ namespace hkq {
 void set_error(const char* fmt, ...);
 int fail_arg(const char* file, int line, const char* msg);
 int cu_count();
+
+// An operand's memory: `rows` rows of `width` bytes, `pitch` bytes apart (p null: none).
+struct MemRows {
+    const void* p;
+    int64_t rows, width, pitch;
+};
+// Whether two operands share a byte. Exact for one pitch (columns side by side
+// in the rows of one buffer do not); rows of two pitches that lie in each other's
+// range count as shared.
+inline bool overlap(const MemRows& a, const MemRows& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+    if (d >= (a.rows - 1) * a.pitch + a.width || -d >= (b.rows - 1) * b.pitch + b.width) return false;
+    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    if (b.rows > 1 && b.pitch != pitch) return true;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const int64_t col = (d % pitch + pitch) % pitch;  // b's first byte in a's rows
+    return col < a.width || col + b.width > pitch;
+}
 }  // namespace hkq
 
 #define HKQ_CHECK_ARG(cond, msg)                                     \

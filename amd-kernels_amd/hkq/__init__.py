@@ -516,7 +516,7 @@ def gated_ffn_backward(dH, X, W, Y, act: str = "silu", alpha: float = 1.0, inter
                        need_dx: bool = True, need_dw: bool = True, stream=None):
     """Gradients (dX bf16 [M, K], dW bf16 [2F, K]) of gated_ffn_bf16 from dH bf16
     [M, F], its inputs and the Y it kept; one that is not needed is None. Both
-    are overwritten, not accumulated."""
+    are overwritten, not accumulated; dX may be X, or dW W."""
     import torch
 
     M, K = X.shape

@@ -306,9 +306,11 @@ int hkq_gated_ffn_bf16(const void* X, const void* W, void* H, void* Y, int64_t M
  * (overwritten, not accumulated; either may be NULL: not computed, and then its
  * own other operand, W or X, may be NULL). act'(0) of ReLU is 0. M < 2^29,
  * F <= 2^20; lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of
- * 4 (< 2^23); dH, X, W, Y 16-byte, dX, dW 8-byte aligned. workspace: at least
- * hkq_gated_ffn_backward_workspace(M, F, K) bytes, 16-byte aligned, under the
- * rules of hkq_gemm_a8w8_ws; it holds dg and du. At most four launches, no
+ * 4 (< 2^23); dH, X, W, Y 16-byte, dX, dW 8-byte aligned. Either gradient may lie
+ * over dH or Y, dX over X or dW over W (not both of these); dX over W, dW over X,
+ * one over the other or the workspace over any of them is refused. workspace: at
+ * least hkq_gated_ffn_backward_workspace(M, F, K) bytes, 16-byte aligned, under
+ * the rules of hkq_gemm_a8w8_ws; it holds dg and du. At most four launches, no
  * synchronisation, sums in a fixed order. */
 size_t hkq_gated_ffn_backward_workspace(int64_t M, int64_t F, int64_t K);
 int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const void* Y, void* dX, void* dW, int64_t M,

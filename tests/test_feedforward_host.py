@@ -160,3 +160,24 @@ def test_modules_offer_the_operators():
 def test_norm_rows_of_one_launch(M):
     """Four rows per workgroup of 256 threads: 2^26 - 3 rows round up to 2^24 workgroups, 2^32 threads."""
     refused(*norm(M=M, D=8, ldx=8, ldr=8, ldh=8, ldq=8, lds=1, group=0), match="M must")
+
+
+def places(**kw):
+    """A backward call whose operands lie 1 MiB apart but for those given."""
+    at = {n: (i + 1) << 20 for i, n in enumerate(("dH", "X", "W", "Y", "dX", "dW", "ws"))}
+    return backward(**{**at, "n": 1 << 19, **kw})
+
+
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(dX=3 * MB), "dX must not overlap W"), (dict(dX=3 * MB + 128 * 127 * 2 + 128), "dX must not overlap W"),
+    (dict(dW=2 * MB), "dW must not overlap X"), (dict(dW=2 * MB, dX=2 * MB), "dW must not overlap X"),
+    (dict(dX=6 * MB), "dX and dW must not overlap"), (dict(dX=2 * MB, dW=3 * MB), "dX over X and dW over W"),
+    (dict(dX=7 * MB), "workspace"), (dict(dW=7 * MB - 64), "workspace"), (dict(X=7 * MB + 2048), "workspace"),
+    # rows of one pitch: columns that meet by their last and first four; rows of two pitches
+    (dict(dX=3 * MB + 248, lddx=256, ldw=256), "dX must not overlap W"),
+    (dict(dX=3 * MB + 264, lddx=260, ldw=256), "dX must not overlap W")])
+def test_backward_overlap_refusals(kw, match):
+    refused(*places(**kw), match=match)

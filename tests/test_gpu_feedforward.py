@@ -852,3 +852,38 @@ def test_modules_give_the_same_bytes():
     hk.ffn.gated.gated_ffn_backward(H, x, wb, Y, dX, dW)
     want = hkq.gated_ffn_backward(H, x, wb, Y)
     assert torch.equal(dX, want[0]) and torch.equal(dW, want[1])
+
+
+# ------------------------------------------------------------- outputs over operands
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("M,F,K", [(5, 32, 64), (1001, 1408, 1024), (600, 8200, 3328)])
+def test_backward_outputs_over_operands(interleaved, M, F, K):
+    """dX in X's place, dW in W's, dX in Y's memory: the bits of outputs of their own."""
+    require_gpu()
+    ops = bf16((M, F), 4, 0.3), bf16((M, K), 1), bf16((2 * F, K), 2, 0.05), bf16((M, 2 * F), 3, 1.5)
+    dH, X, W, Y = (t.cuda() for t in ops)
+    dX, dW = hkq.gated_ffn_backward(dH, X, W, Y, interleaved=interleaved)
+    x = X.clone()
+    got = hkq.gated_ffn_backward(dH, x, W, Y, interleaved=interleaved, dX=x)
+    assert torch.equal(got[0], dX) and torch.equal(got[1], dW), "dX over X"
+    w = W.clone()
+    got = hkq.gated_ffn_backward(dH, X, w, Y, interleaved=interleaved, dW=w)
+    assert torch.equal(got[0], dX) and torch.equal(got[1], dW), "dW over W"
+    both = torch.cat((Y, X), 1)  # rows of Y followed by rows of X: dX goes over Y's
+    if K <= 2 * F:
+        got = hkq.gated_ffn_backward(dH, both[:, 2 * F:], W, both[:, :2 * F], interleaved=interleaved, dX=both[:, :K])
+        assert torch.equal(got[0], dX) and torch.equal(got[1], dW), "dX over Y"
+        assert torch.equal(both[:, 2 * F:], X)
+
+
+def test_backward_outputs_beside_operands():
+    """Columns of one buffer side by side share no element: not refused."""
+    require_gpu()
+    M, F, K = 70, 72, 64
+    dH, X, W, Y = bf16((M, F), 4, 0.3).cuda(), bf16((M, K), 1).cuda(), bf16((2 * F, K), 2, 0.05).cuda(), bf16((M, 2 * F), 3).cuda()
+    dX, dW = hkq.gated_ffn_backward(dH, X, W, Y)
+    xs, ws = torch.cat((X, X), 1), torch.cat((W, W), 1)
+    got = hkq.gated_ffn_backward(dH, xs[:, K:], ws[:, :K], Y, dX=xs[:, :K], dW=ws[:, K:])
+    assert torch.equal(got[0], dX) and torch.equal(got[1], dW)
+    assert torch.equal(xs[:, K:], X) and torch.equal(ws[:, :K], W)
