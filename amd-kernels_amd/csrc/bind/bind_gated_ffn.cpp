@@ -73,7 +73,7 @@ void gated_ffn_backward(py::object dH, py::object X, py::object W, py::object Y,
     if (!dX.is_none()) pdx = (void*)matrix(dX, "dX", M, K, &lddx).ptr;
     if (!dW.is_none()) pdw = (void*)matrix(dW, "dW", 2 * F, K, &lddw).ptr;
     const int id = activation(act);
-    Workspace ws = workspace(hkq_gated_ffn_backward_workspace(M, F, K), X);
+    Workspace ws = workspace(pdx || pdw ? hkq_gated_ffn_backward_workspace(M, F, K) : 0, X);
     check(hkq_gated_ffn_backward((const void*)dh.ptr, (const void*)x.ptr, (const void*)w.ptr, (const void*)y.ptr, pdx, pdw,
                                  M, F, K, lddh, ldx, ldw, ldy, lddx, lddw, id, alpha, interleaved ? 1 : 0, ws.ptr, ws.bytes,
                                  current_stream()),

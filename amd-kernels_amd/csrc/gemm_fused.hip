@@ -456,6 +456,7 @@ int hkq_gated_ffn_backward(const void* dH, const void* X, const void* W, const v
     HKQ_CHECK_ARG(!dW || (lddw >= K && lddw % 4 == 0 && lddw < (1 << 23)), "lddw must be >= K, a multiple of 4 and < 2^23");
     ActParams a;
     if (int e = check_act(act, alpha, a)) return e;
+    if (!dX && !dW) return 0;
     if (F == 0 && (M == 0 || !dX)) return 0;
     HKQ_CHECK_ARG(M == 0 || F == 0 || (dH && Y), "dH and Y are required");
     HKQ_CHECK_ARG(M == 0 || F == 0 || ((!dW || X) && (!dX || W)), "X is required for dW, W for dX");

@@ -534,7 +534,7 @@ def gated_ffn_backward(dH, X, W, Y, act: str = "silu", alpha: float = 1.0, inter
             dX = torch.empty((M, K), dtype=torch.bfloat16, device=X.device)
         if need_dw and dW is None:
             dW = torch.empty((2 * F, K), dtype=torch.bfloat16, device=X.device)
-        ws = _workspace(int(lib().hkq_gated_ffn_backward_workspace(M, F, K)), X)
+        ws = _workspace(int(lib().hkq_gated_ffn_backward_workspace(M, F, K)) if need_dx or need_dw else 0, X)
         call("hkq_gated_ffn_backward", _ptr(dH), _ptr(X), _ptr(W), _ptr(Y), _opt_ptr(dX), _opt_ptr(dW), M, F, K,
              _pitch(dH), _pitch(X), _pitch(W), _pitch(Y), _pitch(dX), _pitch(dW), a, alpha, int(interleaved),
              _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))

@@ -304,7 +304,8 @@ int hkq_gated_ffn_bf16(const void* X, const void* W, void* H, void* Y, int64_t M
  *   dg = dH * u * act'(g), du = dH * act(g)  (fp32, rounded to bf16),
  *   dX [M, K] = dg . Wg + du . Wu,  dW [2F, K] = [dg, du]^T . X in W's row order
  * (overwritten, not accumulated; either may be NULL: not computed, and then its
- * own other operand, W or X, may be NULL). act'(0) of ReLU is 0. M < 2^29,
+ * own other operand, W or X, may be NULL; both: nothing runs and no workspace is
+ * needed). act'(0) of ReLU is 0. M < 2^29,
  * F <= 2^20; lddh, ldx, ldw, ldy multiples of 8 (ldx, ldw < 2^24), lddx, lddw of
  * 4 (< 2^23); dH, X, W, Y 16-byte, dX, dW 8-byte aligned. Either gradient may lie
  * over dH or Y, dX over X or dW over W (not both of these); dX over W, dW over X,

@@ -181,3 +181,10 @@ MB = 1 << 20
     (dict(dX=3 * MB + 264, lddx=260, ldw=256), "dX must not overlap W")])
 def test_backward_overlap_refusals(kw, match):
     refused(*places(**kw), match=match)
+
+
+def test_backward_of_neither_gradient():
+    """Nothing to compute: no workspace, no operand, no launch."""
+    hkq.call(*backward(dX=None, dW=None, ws=None, n=0))
+    hkq.call(*backward(dX=None, dW=None, ws=None, n=0, dH=None, X=None, W=None, Y=None))
+    refused(*backward(dX=None, dW=None, ws=None, n=0, act=5), match="act")

@@ -887,3 +887,14 @@ def test_backward_outputs_beside_operands():
     got = hkq.gated_ffn_backward(dH, xs[:, K:], ws[:, :K], Y, dX=xs[:, :K], dW=ws[:, K:])
     assert torch.equal(got[0], dX) and torch.equal(got[1], dW)
     assert torch.equal(xs[:, K:], X) and torch.equal(ws[:, :K], W)
+
+
+def test_backward_of_neither_gradient():
+    """No workspace is taken where nothing is asked for."""
+    require_gpu()
+    M, F, K = 512, 1024, 512
+    dH, X, W, Y = bf16((M, F), 4).cuda(), bf16((M, K), 1).cuda(), bf16((2 * F, K), 2).cuda(), bf16((M, 2 * F), 3).cuda()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    assert hkq.gated_ffn_backward(dH, X, W, Y, need_dx=False, need_dw=False) == (None, None)
+    assert torch.cuda.max_memory_allocated() == before
