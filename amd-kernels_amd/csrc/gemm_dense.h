@@ -1796,6 +1796,9 @@ static bool use_narrow(int mode, const DenseParams& p, int64_t batch, int64_t co
     return !one_round && mode == MODE_A8W8 && S >= 24 && p.M <= (wgs >= 3 * ncu ? 4 : wgs >= 2 * ncu ? 1 : 0);
 }
 
+constexpr char PITCH_REFUSAL[] = "row pitches too large: 32 rows of each operand (or all of its rows) and of its scales "
+                                 "must span less than 2^31 bytes";
+
 template <class Op, int MODE>
 static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipStream_t stream) {
     p.c16 = (p.ldc % 8 == 0) && (reinterpret_cast<uintptr_t>(p.C) % 16 == 0);
@@ -1869,8 +1872,7 @@ static int launch_dense(typename Op::Params& p, void* ws, size_t ws_bytes, hipSt
             }
             break;
         case DT_NONE:
-            HKQ_CHECK_ARG(false, "row pitches too large: 32 rows of each operand (or all of its rows) and of its scales "
-                                 "must span less than 2^31 bytes");
+            HKQ_CHECK_ARG(false, PITCH_REFUSAL);
     }
     // 128-byte K-tiles of this kernel need whole ones in every row: a partial
     // last K-tile would read the next row's bytes instead of zeros

@@ -327,6 +327,15 @@ static int check_act(int act, float alpha, ActParams& a) {
     return 0;
 }
 
+// The refusal of a call whose output shares memory with an operand; pitches that
+// no kernel reaches are named as such.
+template <int MODE>
+static int check_overlap(const FusedParams& p, bool gated, const char* clash) {
+    HKQ_CHECK_ARG(!clash || dense_tile_plan(MODE, p, 1, nullptr, gated, !gated) != DT_NONE, PITCH_REFUSAL);
+    HKQ_CHECK_ARG(!clash, clash);
+    return 0;
+}
+
 template <int MODE>
 static int gemm_epilogue(const void* A, const void* B, const float* sa, const float* sb, const void* bias,
                          const void* residual, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldr,
@@ -364,6 +373,19 @@ static int gemm_epilogue(const void* A, const void* B, const float* sa, const fl
     p.lda = lda * ES; p.ldb = ldb * ES; p.ldc = ldc;
     p.residual = static_cast<const uint16_t*>(residual);
     p.ldr = ldr;
+    const MemRows mc{C, M, 2 * N, 2 * ldc};
+    const size_t need = MODE == MODE_BF16 ? hkq_gemm_bf16_workspace(M, N, K) : hkq_gemm_a8w8_workspace(M, N, K);
+    const MemRows mws{workspace_bytes >= need ? workspace : nullptr, 1, (int64_t)need, 0};
+    const char* clash = nullptr;
+    if (overlap(mc, {A, M, K * ES, lda * ES}) || overlap(mc, {B, N, K * ES, ldb * ES}) || overlap(mc, {sa, 1, 4 * M, 0}) ||
+        overlap(mc, {sb, 1, 4 * N, 0}) || overlap(mc, {bias, 1, 2 * N, 0}))
+        clash = "C must not overlap A, B, the scales or the bias";
+    else if (residual != C && overlap(mc, {residual, M, 2 * N, 2 * ldr}))
+        clash = "the residual must be C itself or not overlap it";
+    else if (overlap(mws, mc) || overlap(mws, {residual, M, 2 * N, 2 * ldr}) || overlap(mws, {A, M, K * ES, lda * ES}) ||
+             overlap(mws, {B, N, K * ES, ldb * ES}))
+        clash = "the workspace must not overlap an operand";
+    if (int e = check_overlap<MODE>(p, false, clash)) return e;
     return launch_dense<FusedOp, MODE>(p, workspace, workspace_bytes, stream);
 }
 
@@ -403,6 +425,13 @@ static int gated_ffn(const void* X, const void* W, const float* sx, const float*
     p.Y = static_cast<uint16_t*>(Y);
     p.ldy = ldy;
     p.y16 = ldy % 8 == 0 && reinterpret_cast<uintptr_t>(Y) % 16 == 0;
+    const MemRows mh{H, M, 2 * F, 2 * ldh}, my{Y, M, 4 * F, 2 * ldy}, mx{X, M, K * ES, ldx * ES}, mw{W, 2 * F, K * ES, ldw * ES};
+    const char* clash = nullptr;
+    if (overlap(mh, mx) || overlap(mh, mw) || overlap(mh, {sx, 1, 4 * M, 0}) || overlap(mh, {sw, 1, 8 * F, 0}))
+        clash = "H must not overlap X, W or the scales";
+    else if (overlap(my, mx) || overlap(my, mw) || overlap(my, mh))
+        clash = "Y must not overlap X, W or H";
+    if (int e = check_overlap<MODE>(p, true, clash)) return e;
     return launch_dense<GatedOp, MODE>(p, nullptr, 0, stream);
 }
 

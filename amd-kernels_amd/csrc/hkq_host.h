@@ -23,7 +23,8 @@ struct MemRows {
 inline bool overlap(const MemRows& a, const MemRows& b) {
     if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
     const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
-    if (d >= (a.rows - 1) * a.pitch + a.width || -d >= (b.rows - 1) * b.pitch + b.width) return false;
+    auto extent = [](const MemRows& r) { return (__int128)(r.rows - 1) * r.pitch + r.width; };  // any pitch
+    if (d >= extent(a) || -(__int128)d >= extent(b)) return false;
     const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
     if (b.rows > 1 && b.pitch != pitch) return true;
     if (a.rows == 1 && b.rows == 1) return true;

@@ -507,6 +507,13 @@ extern "C" int hkq_add_rmsnorm_quant(const void* x, const void* res, const void*
     HKQ_CHECK_ALIGN(h, 16);
     HKQ_CHECK_ALIGN(q, 8);
     HKQ_CHECK_ALIGN(s, 4);
+    const MemRows mx{x, M, 2 * D, 2 * ldx}, mr{res, M, 2 * D, 2 * ldr}, mw{w, 1, 2 * D, 0}, mh{h, M, 2 * D, 2 * ldh},
+        mq{q, M, D, ldq}, ms{s, M, group ? D / 128 * 4 : 4, 4 * lds};
+    HKQ_CHECK_ARG((h == x || !overlap(mh, mx)) && (h == res || !overlap(mh, mr)) && !overlap(mh, mw),
+                  "h must be x or res itself or overlap neither, and not overlap w");
+    HKQ_CHECK_ARG(!overlap(mq, mx) && !overlap(mq, mr) && !overlap(mq, mw) && !overlap(mq, mh), "q must not overlap x, res, w or h");
+    HKQ_CHECK_ARG(!overlap(ms, mx) && !overlap(ms, mr) && !overlap(ms, mw) && !overlap(ms, mh) && !overlap(ms, mq),
+                  "s must not overlap another operand");
     auto run = [&](auto k, auto g) {
         return add_rmsnorm_nc<decltype(k)::value, decltype(g)::value>(
             (int)D, (const uint16_t*)x, (const uint16_t*)res, (const uint16_t*)w, (uint16_t*)h, (uint8_t*)q, s, (int)M,

@@ -116,12 +116,12 @@ int hkq_swiglu_quant(const void* y, void* q, float* s, int64_t M, int64_t F, int
  * (group 0: s[m * lds]) or per 128 columns (group 128: s[m * lds + k / 128]);
  * kind HKQ_KIND_FP8 (E4M3FN, QMAX 448) or HKQ_KIND_INT8 (round half even,
  * QMAX 127). The sum is fp32 in an order fixed by D; a NaN among the values of
- * a scale makes that scale NaN. h may be x or res (same pitch). D a multiple of
- * 8 (128 with groups) in [8, 16384]; pitches multiples of 8; M < 2^24 (up to
- * 2^26 - 4 for D <= 1024). No counterpart in the reference (its
- * fused_rmsnorm_fp8_quant_fwd has no residual and 1x128 scales only): what feeds
- * the layer's first product, hkq_gemm_a8w8 / hkq_gated_ffn_a8w8 (group 0) or
- * hkq_gemm_blockscale (group 128). */
+ * a scale makes that scale NaN. h may be x or res (same pitch); outputs share no
+ * other memory with an operand or each other (refused). D a multiple of 8 (128
+ * with groups) in [8, 16384]; pitches multiples of 8; M < 2^24 (up to 2^26 - 4 for
+ * D <= 1024). No counterpart in the reference (its fused_rmsnorm_fp8_quant_fwd has
+ * no residual and 1x128 scales only): what feeds the layer's first product,
+ * hkq_gemm_a8w8 / hkq_gated_ffn_a8w8 (group 0) or hkq_gemm_blockscale (group 128). */
 int hkq_add_rmsnorm_quant(const void* x, const void* res, const void* w, void* h, void* q, float* s, int64_t M,
                           int64_t D, int64_t ldx, int64_t ldr, int64_t ldh, int64_t ldq, int64_t lds, float eps,
                           int group, int kind, hkq_stream_t stream);
@@ -268,10 +268,11 @@ int hkq_batched_gemm_bf16(const void* A, const void* B, const void* bias, void* 
  * C = bf16(act((A . B^T) * sa[m] * sb[n] + bias[n]) + residual[m, n]), formed in
  * fp32 and rounded once. bias bf16 [N] and residual bf16 rows of ldr >= N
  * elements (a multiple of 4; ldr, ldc < 2^24) may be NULL; the residual may be C
- * itself (same pitch). Shapes, strides and alignment as the plain GEMMs; the
- * workspace is that of hkq_gemm_a8w8_workspace / hkq_gemm_bf16_workspace (NULL:
- * no split of K over workgroups) under the rules of hkq_gemm_a8w8_ws. No
- * counterpart in the reference beyond its block-scale multiply-add. */
+ * itself (same pitch), which shares no other memory with an operand (refused).
+ * Shapes, strides and alignment as the plain GEMMs; the workspace is that of
+ * hkq_gemm_a8w8_workspace / hkq_gemm_bf16_workspace (NULL: no split of K over
+ * workgroups) under the rules of hkq_gemm_a8w8_ws. No counterpart in the
+ * reference beyond its block-scale multiply-add. */
 int hkq_gemm_a8w8_epilogue(const void* A, const void* B, const float* sa, const float* sb, const void* bias,
                            const void* residual, void* C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
                            int64_t ldr, int64_t ldc, int act, float alpha, void* workspace, size_t workspace_bytes,
@@ -289,9 +290,10 @@ int hkq_gemm_bf16_epilogue(const void* A, const void* B, const void* bias, const
  * in W's row order, K % 64 == 0. bf16: no scales, K % 32 == 0; Y (NULL: not
  * kept) gets bf16(g), bf16(u) as [M, 2F] rows of ldy in W's row order, what
  * hkq_gated_ffn_backward needs. F % 8 == 0; ldh, ldy multiples of 4 below 2^24;
- * X, W, sw 16-byte, H, Y 8-byte aligned. 32 rows of W of one half (ldw, or 2 ldw
- * interleaved, apart) and of X must span less than 2^31 bytes. No counterpart
- * in the reference, whose gate/up product writes both halves to memory
+ * X, W, sw 16-byte, H, Y 8-byte aligned, H and Y sharing no memory with each other
+ * or an operand (refused). 32 rows of W of one half (ldw, or 2 ldw interleaved,
+ * apart) and of X must span less than 2^31 bytes. No counterpart in the
+ * reference, whose gate/up product writes both halves to memory
  * (kernels/moe-gemm/moe_op_silu_fused/kernel.cpp:1-13). */
 int hkq_gated_ffn_a8w8(const void* X, const void* W, const float* sx, const float* sw, void* H, int64_t M, int64_t F,
                        int64_t K, int64_t ldx, int64_t ldw, int64_t ldh, int act, float alpha, int interleaved,

@@ -188,3 +188,52 @@ def test_backward_of_neither_gradient():
     hkq.call(*backward(dX=None, dW=None, ws=None, n=0))
     hkq.call(*backward(dX=None, dW=None, ws=None, n=0, dH=None, X=None, W=None, Y=None))
     refused(*backward(dX=None, dW=None, ws=None, n=0, act=5), match="act")
+
+
+def apart(names):
+    """Operands 1 MiB apart, in order."""
+    return {n: (i + 1) << 20 for i, n in enumerate(names)}
+
+
+NORM = apart(("x", "res", "w", "h", "q", "s"))
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(h=NORM["x"] + 512), "h must be x or res"), (dict(h=NORM["res"] + 16), "h must be x or res"), (dict(h=NORM["w"]), "h must"),
+    (dict(q=NORM["x"]), "q must not"), (dict(q=NORM["res"] + 64), "q must not"), (dict(q=NORM["w"]), "q must not"),
+    (dict(q=NORM["h"]), "q must not"), (dict(s=NORM["x"] + 2032), "s must not"), (dict(s=NORM["w"]), "s must not"),
+    (dict(s=NORM["h"]), "s must not"), (dict(s=NORM["q"] + 1020), "s must not"), (dict(s=NORM["q"], group=0, lds=1), "s must not"),
+    (dict(q=NORM["x"], res=None, h=None), "q must not")])
+def test_norm_overlap_refusals(kw, match):
+    refused(*norm(**{**NORM, **kw}), match=match)
+
+
+@pytest.mark.parametrize("kind", ["a8w8", "bf16"])
+@pytest.mark.parametrize("kw,match", [
+    (dict(C="A"), "C must not"), (dict(C="B"), "C must not"), (dict(C="bias"), "C must not"), (dict(C="res", off=128), "C itself"),
+    (dict(C="res", off=64), "C itself"), (dict(C="sa"), "C must not"), (dict(C="sb"), "C must not"), (dict(C="ws"), "workspace"),
+    (dict(C="res", off=-8), "C itself"), (dict(C="A", off=-128, ldc=128), "C must not")])
+def test_epilogue_overlap_refusals(kind, kw, match):
+    names = ("A", "B", *(("sa", "sb") if kind == "a8w8" else ()), "bias", "res", "C", "ws")
+    at = apart(names)
+    if kw["C"] not in at:
+        return  # bf16 has no scales
+    # 128 x 1024 x 8192: K split over workgroups, with a workspace in use
+    big = dict(M=128, N=1024, K=8192, lda=8192, ldb=8192, ldr=1024, ldc=1024) if kw["C"] == "ws" else {}
+    n = int(getattr(hkq.lib(), f"hkq_gemm_{kind}_workspace")(128, 1024, 8192))
+    at = {k: v * 64 for k, v in at.items()} if big else at
+    more = {k: v for k, v in kw.items() if k not in ("C", "off")}
+    refused(*epilogue(kind, **{**at, "n": n, **big, "C": at[kw["C"]] + kw.get("off", 0), **more}), match=match)
+
+
+@pytest.mark.parametrize("kind", ["a8w8", "bf16"])
+@pytest.mark.parametrize("kw,match", [
+    (dict(H="X"), "H must not"), (dict(H="W"), "H must not"), (dict(H="W", off=64 * 128), "H must not"), (dict(H="sx"), "H must not"),
+    (dict(H="sw"), "H must not"), (dict(Y="X"), "Y must not"), (dict(Y="W"), "Y must not"), (dict(Y="H"), "Y must not"),
+    (dict(Y="H", off=64, ldy=256, ldh=256), "Y must not")])
+def test_gated_overlap_refusals(kind, kw, match):
+    at = apart(("X", "W", *(("sx", "sw", "H") if kind == "a8w8" else ("H", "Y"))))
+    (out, over), more = list(kw.items())[0], {k: v for k, v in kw.items() if k.startswith("ld")}
+    if out not in at or over not in at:
+        return  # FP8 keeps no projections, bf16 has no scales
+    refused(*gated(kind, **{**at, out: at[over] + kw.get("off", 0), **more}), match=match)

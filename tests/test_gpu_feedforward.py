@@ -898,3 +898,24 @@ def test_backward_of_neither_gradient():
     before = torch.cuda.max_memory_allocated()
     assert hkq.gated_ffn_backward(dH, X, W, Y, need_dx=False, need_dw=False) == (None, None)
     assert torch.cuda.max_memory_allocated() == before
+
+
+def test_outputs_beside_operands():
+    """Outputs in the columns beside their operands' share no element: not refused, and nothing else is written."""
+    require_gpu()
+    M, K, F = 70, 64, 64
+    x, res, w = bf16((M, K), 1).cuda(), bf16((M, K), 2).cuda(), bf16((K,), 3).cuda()
+    W = bf16((2 * F, K), 4, 0.1).cuda()
+    q, s, h = hkq.add_rmsnorm_quant(x, w, res)
+    both = torch.cat((x, res, res), 1)
+    q2, s2, _ = hkq.add_rmsnorm_quant(both[:, :K], w, both[:, K:2 * K], h=both[:, 2 * K:])
+    assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
+    assert torch.equal(both, torch.cat((x, res, h), 1))
+    H, Y = hkq.gated_ffn_bf16(x, W, save=True)
+    both = torch.cat((x, torch.zeros_like(H), torch.zeros_like(Y)), 1)
+    hkq.gated_ffn_bf16(both[:, :K], W, H=both[:, K:K + F], Y=both[:, K + F:])
+    assert torch.equal(both, torch.cat((x, H, Y), 1))
+    C = hkq.gemm_bf16_epilogue(x, W, act="silu", residual=Y)
+    both = torch.cat((x, Y, torch.zeros_like(Y)), 1)
+    hkq.gemm_bf16_epilogue(both[:, :K], W, act="silu", residual=both[:, K:K + 2 * F], C=both[:, K + 2 * F:])
+    assert torch.equal(both, torch.cat((x, Y, C), 1))
