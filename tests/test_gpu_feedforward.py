@@ -919,3 +919,93 @@ def test_outputs_beside_operands():
     both = torch.cat((x, Y, torch.zeros_like(Y)), 1)
     hkq.gemm_bf16_epilogue(both[:, :K], W, act="silu", residual=both[:, K:K + 2 * F], C=both[:, K + 2 * F:])
     assert torch.equal(both, torch.cat((x, Y, C), 1))
+
+
+# ------------------------------------------------------------- operands past 32 bits
+
+def sampled(n, k, *marks):
+    """k indices of n: the first, the last, those around each mark, others."""
+    at = {0, n - 1, *(i for m in marks for i in (m - 1, m) if 0 <= i < n)}
+    at |= set(torch.randint(0, n, (k,), generator=gen(n)).tolist())
+    return torch.tensor(sorted(at), device="cuda")
+
+
+def gpu_bf16(shape, seed, std=1.0):
+    """Normal values made on the GPU, a block of rows at a time."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    out = torch.empty(shape, dtype=BF16, device="cuda")
+    step = max(1, (1 << 28) // shape[1])
+    for i in range(0, shape[0], step):
+        n = min(step, shape[0] - i)
+        out[i:i + n] = torch.randn((n, shape[1]), generator=g, device="cuda") * std
+    return out
+
+
+def columns(t, f, F):
+    """Columns f of both halves of [.., 2F]."""
+    return torch.cat((t[:, f], t[:, F + f]), 1)
+
+
+# dW's sums over tokens whose gradients (the K-tiles' memory rows) pass 4 GiB: on
+# K groups of 128 x 64 tiles, the streaming kernel (K-tiles in eights) and the
+# one-tile kernel; dX's over 4 GiB of weights, in parts of K
+@pytest.mark.parametrize("M,F,K", [(70001, 16384, 64), (66048, 16384, 512), (66049, 16384, 512), (300, 1 << 20, 1056)])
+def test_gated_operands_past_32_bits(M, F, K):
+    """Forward with the projections kept, and both gradients: rows and columns on
+    either side of 2^31 and 2^32 bytes into each tensor, and random ones."""
+    require_gpu()
+    torch.cuda.empty_cache()
+    X, W, dH = gpu_bf16((M, K), 1), gpu_bf16((2 * F, K), 2, 1 / math.sqrt(K)), gpu_bf16((M, F), 3, 0.3)
+    H, Y = hkq.gated_ffn_bf16(X, W, save=True)
+    assert max(Y.numel(), W.numel()) * 2 > 1 << 32
+    marks = [(1 << b) // (2 * w) for b in (31, 32) for w in (F, 2 * F, K)]
+    m, f = sampled(M, 12, *marks), sampled(F, 12, *(x for k in marks for x in (k, k - F)))
+    w = torch.cat((W[f], W[F + f]))
+    y = X[m].double() @ w.double().t()
+    err = (K + 4) * E * (X[m].double().abs() @ w.double().abs().t())
+    close(columns(Y[m], f, F), y, err + U * y.abs(), "Y")
+    close(H[m][:, f], *gated_ref(y, err, "silu", 1.0, False), "H")
+    del H
+    dX, dW = hkq.gated_ffn_backward(dH, X, W, Y)
+    _, rw = backward_ref(dH[:, f], X, w, columns(Y, f, F), "silu", 1.0, False)
+    close(torch.cat((dW[f], dW[F + f])), *rw, "dW", 2)
+    want = torch.zeros((len(m), K), dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(want)
+    step = 1 << 16
+    for i in range(0, F, step):  # a range of features at a time
+        n = torch.arange(i, min(F, i + step), device="cuda")
+        (dx, tx), _ = backward_ref(dH[m][:, n], X[m][:, :32], torch.cat((W[n], W[F + n])), columns(Y[m], n, F), "silu", 1.0, False)
+        want += dx
+        # the bound of 2n summed products, scaled to that of all 2F
+        tol += (tx - U * dx.abs()) * ((2 * F + 4) / (2 * len(n) + 4))
+    close(dX[m], want, tol + U * want.abs(), "dX", 2)
+
+
+@pytest.mark.parametrize("kind", ["a8w8", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(70001, 32768, 64), (66049, 32776, 1024)])
+def test_epilogue_operands_past_32_bits(kind, M, N, K):
+    """C and the residual of more than 4 GiB, the residual also in C's place."""
+    require_gpu()
+    torch.cuda.empty_cache()
+    A, B, sa, sb = (t if t is None else t.cuda() for t in operands(kind, M, N, K, 3))
+    res, bias = gpu_bf16((M, N), 4, 2.0), bf16((N,), 5).cuda()
+    C = epilogue(kind, A, B, sa, sb, bias=bias, act="silu", residual=res)
+    marks = [(1 << b) // (2 * N) for b in (31, 32)]
+    m, n = sampled(M, 40, *marks), sampled(N, 40)
+    a, b = (t.view(torch.uint8)[i].view(t.dtype) for t, i in ((A, m), (B, n)))
+    v, err = sums(kind, a, b, *(() if sa is None else (sa[m], sb[n])))
+    close(C[m][:, n], *epilogue_ref(v, err, bias[n], "silu", 1.0, res[m][:, n]), kind)
+    assert torch.equal(epilogue(kind, A, B, sa, sb, bias=bias, act="silu", residual=res, C=res), C)
+
+
+# a row of 8 columns per wave, at the most rows of one launch, and rows whose
+# offsets pass 2^32 bytes
+@pytest.mark.parametrize("kind,M,D,group", [(hkq.KIND_INT8, (1 << 26) - 4, 8, 0), (hkq.KIND_FP8, 270001, 8192, 128)])
+def test_add_rmsnorm_quant_most_rows(kind, M, D, group):
+    require_gpu()
+    torch.cuda.empty_cache()
+    x, res, w = gpu_bf16((M, D), 1), gpu_bf16((M, D), 2, 2.0), bf16((D,), 3)
+    q, s, h = hkq.add_rmsnorm_quant(x, w.cuda(), res, 1e-6, kind, group)
+    m = sampled(M, 200, *((1 << b) // (2 * D) for b in (31, 32)), *((1 << b) // D for b in (31, 32)))
+    q = q.view(torch.uint8)[m].view(q.dtype)
+    check_norm(x[m].cpu(), res[m].cpu(), w, 1e-6, group, kind, q, s[m], h[m])
