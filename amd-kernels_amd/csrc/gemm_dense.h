@@ -278,8 +278,8 @@ __device__ __forceinline__ void store_staged(const HKQ_LDS uint8_t* ep, int lane
 
 // Residual of a wave's sub-tile, in registers from before the K loop, so that
 // nothing waits on it after the sums (no residual: an empty buffer, whose loads
-// give zeros). Tiles of one or two accumulator blocks HOLD it in the
-// accumulators' layout; larger ones as whole row pieces (16 bytes per lane, full
+// give zeros). Sub-tiles of one row of accumulator blocks, or of two blocks, HOLD
+// it in the accumulators' layout; larger ones as whole row pieces (16 bytes per lane, full
 // lines), which reach that layout through the staging area: read straight, 32 rows
 // x 8 bytes per load, they would cost a line request per row and load. FP8
 // 128x5632x2048 with a residual 10.2 us, 10.6 with the pieces fetched after the
@@ -1604,6 +1604,13 @@ static DensePlan dense_plan(int mode, int64_t M, int64_t N, int64_t kbytes) {
 // 13.0, 128 x 128 15.9, 64 x 64 19.2; FP8 64x28672x4096 26.0, 28.3, 34.9; bf16
 // with up to 64 rows is bound by the weights' way from memory, where 64 x 64
 // tiles keep more of them in flight (33x28672x4096 58, 64 x 64 49).
+// Their estimates rank the sizes and are no times: those of 256-row tiles were
+// fitted where a last round runs as M halves, and 192 x 256 stands beside them, so
+// whole tiles take about twice as long (epilogue bf16 601x14336x4096 with SiLU and
+// a residual, estimated and measured: 192 x 256 44 and 89, 256 x 256 46 and 98,
+// 128 x 256 82 and 106, 128 x 128 71 and 114). By these constants 192 x 256 comes
+// before 256 x 256 where its own tiles are one round, and only where 128 x 256
+// tiles take a second one, which is where it was measured to be the better one.
 enum DenseTile {
     DT_32x32, DT_32x64, DT_32x128, DT_32x256, DT_64x64, DT_128x64, DT_128x128, DT_128x256,
     DT_128x128_PAIR,  // two workgroups per CU (dense_tile_kernel)

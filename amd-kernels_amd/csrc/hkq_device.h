@@ -140,10 +140,12 @@ __device__ __forceinline__ float butterfly_partner(float v) {
 }
 
 // Maximum over groups of W adjacent lanes (W a power of two <= 64, all lanes
-// active, the result in every lane of the group) of values that are +0 or
-// positive and never NaN (absolute maxima accumulated from 0 with max_num):
-// their bit patterns order as unsigned integers, so each butterfly step is one
-// integer max of the DPP-moved value, with no NaN quieting around it.
+// active, the result in every lane of the group) of values without a sign bit
+// (absolute values): their bit patterns order as unsigned integers, so each
+// butterfly step is one integer max of the DPP-moved value, with no NaN quieting
+// around it. A NaN orders above every number and is the result, on which
+// add_rmsnorm_quant_kernel relies (a scale over a NaN is NaN); maxima accumulated
+// from 0 with max_num hold none.
 template <int W>
 __device__ __forceinline__ float group_max_abs(float v) {
     uint32_t x = __float_as_uint(v);
