@@ -89,9 +89,11 @@ struct KgSrc {
     uint32_t bs_step;
     int sc_shift;
     int KT;       // K-tiles
-    // the last K-tile holds 64 bytes of K per row (linear operands): the lanes
-    // that carry its upper four chunks read nothing, so the LDS holds zeros there
+    // the last K-tile holds fewer than 128 bytes of K per row (linear operands): the
+    // lanes that carry its chunks from tail_chunk on read nothing, so the LDS holds
+    // zeros there
     bool half_tail = false;
+    int tail_chunk = 4;
 };
 
 __device__ __forceinline__ uint32_t clamp_bytes(int64_t n) {
@@ -148,12 +150,12 @@ __device__ __forceinline__ void kgroup_kloop(const KgSrc<Cfg, GATHER>& src, HKQ_
     // this group's K-tiles
     const int k0 = kg * src.KT / KG, mine = (kg + 1) * src.KT / KG - k0;
 
-    // OOB in the lanes that carry chunks 4 .. 7 of a row
+    // OOB in the lanes that carry the chunks past a short last K-tile's end
     uint32_t upper[GATHER ? 1 : Cfg::SWP];
     if constexpr (!GATHER) {
 #pragma unroll
         for (int i = 0; i < Cfg::SWP; ++i)
-            upper[i] = KT::load_chunk(lane, kg_row<Cfg>(i, wg, lane)) >= 4 ? OOB : 0u;
+            upper[i] = KT::load_chunk(lane, kg_row<Cfg>(i, wg, lane)) >= src.tail_chunk ? OOB : 0u;
     }
     // the loads of round t (K-tile k0 + t); past the group's last they read
     // nothing. A scale block goes out before the first K-tile that uses it, so

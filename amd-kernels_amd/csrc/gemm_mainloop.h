@@ -117,6 +117,7 @@ struct LoopSrc {
     // GATED: first row of the up half; `b` is that of the gate half, b_bytes the
     // extent of either
     const uint8_t* b2 = nullptr;
+    int tail_chunk = 8;  // KTAIL: 16-byte chunks of K per row in the last K-tile
 };
 
 // GATED tiles: the 32-column n-tiles of each wave are gate columns in the first
@@ -277,8 +278,10 @@ __device__ __forceinline__ v4i read_t16(uint32_t base, int row) {
 //
 // BT / AT: B N-contiguous (FP8, FP4: KTileT; bf16: KTileT16) / A M-contiguous
 // (bf16); GATED: B rows from the two halves of a gate/up weight (src.b, src.b2).
+// KTAIL: rows of K-contiguous operands end inside the last K-tile (src.tail_chunk);
+// the lanes that carry the chunks past the end read zeros.
 template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, int KTB, int NS, bool BT = false, bool AT = false,
-          bool GATED = false, typename AOff, typename BOff>
+          bool GATED = false, bool KTAIL = false, typename AOff, typename BOff>
 __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_off, const BOff& b_off,
                                               HKQ_LDS uint8_t* smem, int lane, int wave, v16f (&acc)[TN][TM]) {
     using Cfg = DenseCfg<MODE, WAVES_M, WAVES_N, TM, TN, KTB>;
@@ -371,9 +374,12 @@ __device__ __forceinline__ void gemm_mainloop(const LoopSrc& src, const AOff& a_
     // For kt >= KTN the scale buffers are empty, so those loads read zero (the
     // loop needs no branches).
     // kslot: (kt + SB_KT - 1) % SB_KT, the slot of the scale unit (SBLK)
+    // KTAIL: a lane carries the same chunk of every row that it loads
+    static_assert(!KTAIL || (NW * Cfg::RPL % 16 == 0 && !FP4), "one chunk per lane");
+    const int ktl = KTAIL && KT::load_chunk(lane, wave * Cfg::RPL + lane / KT::CHUNKS) >= src.tail_chunk ? KTN - 1 : KTN;
     auto load_piece = [&](int kt, int stage, int idx, auto kslot) {
         const int kb = kt * KTB;
-        const bool live = kt < KTN;
+        const bool live = kt < (KTAIL ? ktl : KTN);
         if constexpr (Cfg::SBLK) {
             if (idx == LA + LB) {
                 load_scale_unit(kt + Cfg::SB_KT - 1, kslot);

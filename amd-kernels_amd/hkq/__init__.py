@@ -61,6 +61,8 @@ SIGNATURES = {
     "hkq_gated_ffn_bf16": (_I, [_P] * 4 + [_I64] * 7 + [_I, ctypes.c_float, _I, _P]),
     "hkq_gated_ffn_backward_workspace": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "hkq_gated_ffn_backward": (_I, [_P] * 6 + [_I64] * 9 + [_I, ctypes.c_float, _I, _P, ctypes.c_size_t, _P]),
+    "hkq_grouped_gemm_bf16": (_I, [_P] * 4 + [_I64] * 8 + [_P]),
+    "hkq_grouped_gemm_backward": (_I, [_P] * 6 + [_I64] * 11 + [_P]),
     "hkq_swiglu_quant": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float, _I, _I, _P]),
     "hkq_moe_mxfp4": (_I, [_P] * 10 + [_I64, _I64, _I64, _I64, _I] + [_I64] * 10 + [_P]),
     "hkq_moe_mxfp4_kn": (_I, [_P] * 10 + [_I64, _I64, _I64, _I64, _I] + [_I64] * 10 + [_P]),
@@ -538,6 +540,63 @@ def gated_ffn_backward(dH, X, W, Y, act: str = "silu", alpha: float = 1.0, inter
         call("hkq_gated_ffn_backward", _ptr(dH), _ptr(X), _ptr(W), _ptr(Y), _opt_ptr(dX), _opt_ptr(dW), M, F, K,
              _pitch(dH), _pitch(X), _pitch(W), _pitch(Y), _pitch(dX), _pitch(dW), a, alpha, int(interleaved),
              _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+    return dX, dW
+
+
+def _stride3(t) -> tuple[int, int]:
+    """(group stride, row pitch) of an [E, N, K] operand; what is not stepped over counts as contiguous."""
+    E, N, K = t.shape
+    pitch = K if N <= 1 or t.numel() == 0 else t.stride(1)
+    return (N * pitch if E <= 1 or t.numel() == 0 else t.stride(0)), pitch
+
+
+def grouped_gemm_bf16(X, W, offs, Y=None, stream=None):
+    """Products over ragged groups of rows: Y[r] = X[r] . W[e]^T for offs[e] <= r <
+    offs[e + 1]. X bf16 [M, K], W bf16 [E, N, K], offs int32 [E + 1] on the GPU
+    (moe_routing's) -> Y bf16 [M, N]. Rows of no group are left as they were: pass
+    a Y that holds something there."""
+    import torch
+
+    M, K = X.shape
+    E, N = W.shape[:2]
+    bf16 = (torch.bfloat16,)
+    _expect(X, "X", (M, K), bf16, X.device)
+    _expect(W, "W", (E, N, K), bf16, X.device)
+    _expect(offs, "offs", (E + 1,), (torch.int32,), X.device)
+    if Y is not None:
+        _expect(Y, "Y", (M, N), bf16, X.device)
+    with _on(X.device, stream):
+        if Y is None:
+            Y = torch.empty((M, N), dtype=torch.bfloat16, device=X.device)
+        se, lw = _stride3(W)
+        call("hkq_grouped_gemm_bf16", _ptr(X), _ptr(W), _ptr(Y), _ptr(offs), M, E, N, K, _pitch(X), lw, se, _pitch(Y),
+             _stream(stream))
+    return Y
+
+
+def grouped_gemm_backward(dY, X, W, offs, dX=None, dW=None, need_dx: bool = True, need_dw: bool = True, stream=None):
+    """Gradients (dX bf16 [M, K], dW bf16 [E, N, K]) of grouped_gemm_bf16 from dY
+    bf16 [M, N] and its inputs; one that is not needed is None. Both are
+    overwritten, not accumulated: dW is zero for a group without rows, rows of
+    dX of no group are left as they were."""
+    import torch
+
+    M, K = X.shape
+    E, N = W.shape[:2]
+    bf16 = (torch.bfloat16,)
+    dX, dW = dX if need_dx else None, dW if need_dw else None
+    for t, name, shape in ((X, "X", (M, K)), (W, "W", (E, N, K)), (dY, "dY", (M, N)), (dX, "dX", (M, K)), (dW, "dW", (E, N, K))):
+        if t is not None:
+            _expect(t, name, shape, bf16, X.device)
+    _expect(offs, "offs", (E + 1,), (torch.int32,), X.device)
+    with _on(X.device, stream):
+        if need_dx and dX is None:
+            dX = torch.empty((M, K), dtype=torch.bfloat16, device=X.device)
+        if need_dw and dW is None:
+            dW = torch.empty((E, N, K), dtype=torch.bfloat16, device=X.device)
+        (se, lw), (sd, ldw) = _stride3(W), (0, 0) if dW is None else _stride3(dW)
+        call("hkq_grouped_gemm_backward", _ptr(dY), _ptr(X), _ptr(W), _opt_ptr(dX), _opt_ptr(dW), _ptr(offs), M, E, N, K,
+             _pitch(dY), _pitch(X), lw, se, _pitch(dX), ldw, sd, _stream(stream))
     return dX, dW
 
 

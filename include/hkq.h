@@ -453,6 +453,31 @@ int hkq_moe_mxfp4_kn(const void* A, const void* B, void* C, const void* A_mx_sca
                      int64_t stride_bmxe, int64_t stride_bmxk, int64_t num_tokens, int64_t num_experts,
                      int64_t grid_m, hkq_stream_t stream);
 
+/* ---- matrix products over ragged groups of rows ---------------------------- */
+/* Group e (an expert) owns rows offs[e] <= r < offs[e + 1] of the [M, ..] operands;
+ * offs int32 [E + 1], on the GPU, nondecreasing within [0, M] (the TokenStart of
+ * hkq_expt_data_compute). Groups may be empty; rows before offs[0] and from
+ * offs[E] on belong to none and are left as they were. Bounds outside [0, M]
+ * count as the nearest inside. No host synchronization; sums in fp32, one
+ * rounding to bf16. Rows of K (N) contiguous values, pitches < 2^22 values and
+ * multiples of 8, base pointers 16-byte aligned; N and K multiples of 8; M < 2^28.
+ * An output shares no memory with an operand or another output (refused). No
+ * counterpart in the reference, whose MoE products are quantized, over rows
+ * padded to routing blocks, and have no gradients. */
+
+/* Y[r, n] = bf16(sum_k X[r, k] W[e][n, k]): X bf16 [M, K], W[e] bf16 [N, K] at
+ * W + e * stride_we, Y bf16 [M, N]. */
+int hkq_grouped_gemm_bf16(const void* X, const void* W, void* Y, const int32_t* offs, int64_t M, int64_t E, int64_t N,
+                          int64_t K, int64_t ldx, int64_t ldw, int64_t stride_we, int64_t ldy, hkq_stream_t stream);
+
+/* Its gradients: dX[r, k] = bf16(sum_n dY[r, n] W[e][n, k]) and dW[e][n, k] =
+ * bf16(sum over group e's rows of dY[r, n] X[r, k]), zeros for a group without
+ * rows. dX NULL (then W is not read) or dW NULL (X): not asked for. Both are
+ * overwritten, dW[e] at dW + e * stride_dwe. */
+int hkq_grouped_gemm_backward(const void* dY, const void* X, const void* W, void* dX, void* dW, const int32_t* offs,
+                              int64_t M, int64_t E, int64_t N, int64_t K, int64_t lddy, int64_t ldx, int64_t ldw,
+                              int64_t stride_we, int64_t lddx, int64_t lddw, int64_t stride_dwe, hkq_stream_t stream);
+
 /* ---- MoE routing metadata producers --------------------------------------- */
 /* All index outputs are deterministic: gates of one expert keep their input
  * order (the order of the reference's test formulas, tests/test_moe.py:97-128,
