@@ -41,7 +41,7 @@ HIP_FLAGS = [
 ]
 
 HIP_SOURCES = ["gemm_fused.hip", "quant.hip", "gemm.hip", "gemm_blockscale.hip", "moe.hip", "moe_blockscale.hip", "routing.hip",
-               "norm_quant.hip", "grouped.hip"]
+               "norm_quant.hip", "grouped.hip", "w4.hip"]
 CPP_SOURCES = ["hkq_error.cpp"]
 # Per-source code generation options. The block-scale GEMM promotes every
 # K group on the VALU (acc += P * scale): its MFMAs must write the partial P

@@ -1,0 +1,463 @@
+// w4.hip -- 4-bit weights: their quantizer, and products of bf16 rows with them.
+//
+//   hkq_w4_quant / hkq_w4_dequant   bf16 weights <-> codes with group scales
+//   hkq_gemm_w4a16                  C = X . W^T
+//   hkq_grouped_gemm_w4a16          the same over ragged groups of rows, a weight each
+//
+// A weight is (code - zero) * scale (HKQ_W4_INT4: bf16 scales, and zero points or 8,
+// per 32, 64 or 128 values of K) or an E2M1 value times a power of two
+// (HKQ_W4_MXFP4). Neither is rounded on its way: code - zero and the MXFP4 values are
+// exact in bf16, as the matrix instruction's operand, and an INT4 scale multiplies the
+// fp32 sums of its group.
+#include <algorithm>
+#include <type_traits>
+
+#include "gemm_core.h"
+#include "ragged.h"
+
+namespace hkq {
+
+struct W4Params {
+    const uint8_t* X;  // bf16
+    const uint8_t* Q;
+    const uint8_t* S;  // bf16 or e8m0
+    const uint8_t* Z;  // zero points (nullptr: 8)
+    uint16_t* C;
+    const int32_t* offs;    // nullptr: one group of M rows
+    const int32_t* gather;  // row r is X row gather[r] / topk (nullptr: r itself)
+    int M, T, E, N, K;      // T: rows of X
+    int64_t ldx, ldq, lds, ldc;    // bytes, bytes, scales, values
+    int64_t stride_q, stride_s;    // group to group: bytes, scales
+    int glog2, topk;
+    int tiles_m, tiles_n, group_m;
+};
+
+// ---------------------------------------------------------------------------
+// Quantizer: a lane holds 8 values, G / 8 lanes a group. HBM-bound: 2 bytes read
+// and half a byte written per value.
+// ---------------------------------------------------------------------------
+template <int W, typename F>
+__device__ __forceinline__ float group_fold(float v, F f) {
+    if constexpr (W >= 2) v = f(v, butterfly_partner<1>(v));
+    if constexpr (W >= 4) v = f(v, butterfly_partner<2>(v));
+    if constexpr (W >= 8) v = f(v, butterfly_partner<4>(v));
+    if constexpr (W >= 16) v = f(v, butterfly_partner<8>(v));
+    return v;
+}
+
+template <int G>
+__global__ __launch_bounds__(256) void w4_quant_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ q,
+                                                       uint16_t* __restrict__ s, uint8_t* __restrict__ z, int64_t N, int K,
+                                                       int64_t ldw, int64_t ldq, int64_t lds) {
+    constexpr int L = G / 8;
+    const int64_t per = K / 8, total = N * per;
+    for (int64_t b = (int64_t)blockIdx.x * 256; b < total; b += (int64_t)gridDim.x * 256) {
+        const int64_t at = b + threadIdx.x;  // whole groups: K is a multiple of G, 256 lanes of L
+        if (at >= total) return;
+        const int64_t row = at / per;
+        const int k = (int)(at - row * per) * 8;
+        const v4i raw = *reinterpret_cast<const v4i*>(w + row * ldw + k);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = bf16_to_f32((uint32_t)raw[i] & 0xFFFF);
+            v[2 * i + 1] = bf16_to_f32((uint32_t)raw[i] >> 16);
+        }
+        // largest magnitude; a NaN orders above every number and is the scale then
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        const float amax = group_max_abs<L>(__uint_as_float(top));
+        float scale, zero = 8.0f;
+        if (z) {
+            float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) lo = min_num(lo, v[i]), hi = max_num(hi, v[i]);
+            lo = group_fold<L>(lo, min_num);
+            hi = group_fold<L>(hi, max_num);
+            scale = hi / 15.0f - lo / 15.0f;
+            if (amax != amax) scale = amax;
+            scale = bf16_to_f32(f32_to_bf16(scale));
+            zero = -lo;
+        } else {
+            scale = bf16_to_f32(f32_to_bf16(amax / 7.0f));
+        }
+        // no reciprocal of zero, of a subnormal (it may overflow) or of a NaN: codes of zero
+        const float inv = scale >= 0x1p-126f ? 1.0f / scale : 0.0f;
+        if (z) zero = min_num(max_num(__builtin_rintf(zero * inv), 0.0f), 15.0f);
+        const float lo = z ? 0.0f : -8.0f, hi = z ? 15.0f : 7.0f, off = z ? zero : 0.0f;
+        uint32_t code = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float c = min_num(max_num(__builtin_rintf(v[i] * inv) + off, lo), hi);
+            code |= (uint32_t)(int)(c + (z ? 0.0f : 8.0f)) << (4 * i);
+        }
+        *reinterpret_cast<uint32_t*>(q + row * ldq + k / 2) = code;
+        if (threadIdx.x % L == 0) {
+            s[row * lds + k / G] = (uint16_t)f32_to_bf16(scale);
+            if (z) z[row * lds + k / G] = (uint8_t)(int)zero;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void w4_dequant_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ s,
+                                                         const uint8_t* __restrict__ z, uint16_t* __restrict__ out, int64_t N,
+                                                         int K, int64_t ldq, int64_t lds, int64_t ldo, int glog2) {
+    const int64_t per = K / 8, total = N * per;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+        const int64_t row = at / per;
+        const int k = (int)(at - row * per) * 8;
+        const uint32_t code = *reinterpret_cast<const uint32_t*>(q + row * ldq + k / 2);
+        const int64_t g = row * lds + (k >> glog2);
+        const float scale = bf16_to_f32(s[g]), zero = z ? (float)z[g] : 8.0f;
+        v4i o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = (int)pk_bf16(((float)(code >> (8 * i) & 15) - zero) * scale, ((float)(code >> (8 * i + 4) & 15) - zero) * scale);
+        *reinterpret_cast<v4i*>(out + row * ldo + k) = o;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Operands from codes.
+// ---------------------------------------------------------------------------
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// 8 codes (value j in nibble j) -> 8 bf16 values code - zero, exactly: a byte that
+// holds 0 .. 15 is, as E4M3, that number times 2^-9, so one conversion with scale 2^9
+// gives two codes as fp32; the difference has at most 4 significant bits, and the
+// upper half of its fp32 pattern is its bf16.
+__device__ __forceinline__ v4i int4_operand(uint32_t w, float zero) {
+    const uint32_t ev = w & 0x0F0F0F0Fu, od = w >> 4 & 0x0F0F0F0Fu;
+    v4i o;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const f32x2_t e = h ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(ev, 512.0f, true)
+                            : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(ev, 512.0f, false);
+        const f32x2_t d = h ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(od, 512.0f, true)
+                            : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(od, 512.0f, false);
+        o[2 * h] = (int)__builtin_amdgcn_perm(__float_as_uint(d[0] - zero), __float_as_uint(e[0] - zero), 0x07060302u);
+        o[2 * h + 1] = (int)__builtin_amdgcn_perm(__float_as_uint(d[1] - zero), __float_as_uint(e[1] - zero), 0x07060302u);
+    }
+    return o;
+}
+// 8 E2M1 codes times 2^(e8m0 - 127), the scale as the fp32 of that exponent.
+__device__ __forceinline__ v4i fp4_operand(uint32_t w, float scale) {
+    v4i o;
+    o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    o[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    o[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+    return o;
+}
+
+__device__ __forceinline__ v4f mfma_bf16_16(const v4i& a, const v4i& b, const v4f& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf16, a), __builtin_bit_cast(v8bf16, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+    const v2u r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the weights' way from memory. A workgroup owns 16 MT rows of one group
+// and 16 NT columns; its waves split K in units of 128 values and load their operands
+// straight into registers, D units ahead. Lane c + 16 q of a unit loads 16 bytes (32
+// codes) of column c, values 32 q .. 32 q + 31; INT4 words are then transposed over q,
+// so that each matrix instruction (16 x 16 x 32) takes 32 consecutive values, which
+// lie in one group, and a group's sums are multiplied by its scale. MXFP4 scales go
+// into the operands. The sums of the waves meet in LDS.
+//
+// D[m][n]: rows of X are the instruction's first operand, so that a lane holds one
+// column's sums and needs one scale per group.
+// ---------------------------------------------------------------------------
+template <bool MX, int MT, int NT, int NW, int D>
+__global__ __launch_bounds__(64 * NW) void w4_stream_kernel(const W4Params p) {
+    __shared__ v4f red[NW > 1 ? NW - 1 : 1][MT * NT][64];
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    RaggedTile t;
+    if (p.offs) {
+        if (!ragged_tile<16 * MT>(p, t)) return;
+    } else {
+        t.e = 0;
+        tile_coords(blockIdx.x, p.tiles_m, p.tiles_n, p.group_m, t.m0, t.tn);
+        t.m0 *= 16 * MT;
+        t.rows = p.M - t.m0;
+    }
+    const int n0 = t.tn * 16 * NT, cols = min(p.N - n0, 16 * NT);
+    const auto qr = make_rsrc(p.Q + t.e * p.stride_q + n0 * p.ldq, (uint32_t)((cols - 1) * p.ldq + p.K / 2));
+    constexpr int SB = MX ? 1 : 2;  // bytes per scale
+    const int groups = p.K >> p.glog2;
+    const auto sr = make_rsrc(p.S + (t.e * p.stride_s + n0 * p.lds) * SB, (uint32_t)(((cols - 1) * p.lds + groups) * SB));
+    const auto zr = make_rsrc(p.Z + (t.e * p.stride_s + n0 * p.lds), p.Z ? (uint32_t)((cols - 1) * p.lds + groups) : 0u);
+    // rows: 32-bit offsets from the tile's first, or (gathered) from X
+    uint32_t x_off[MT];
+    const uint8_t* x0 = p.X;
+    uint32_t x_bytes;
+    if (p.gather) {
+        x_bytes = (uint32_t)((p.T - 1) * p.ldx + p.K * 2);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int r = 16 * i + c;
+            const int id = r < t.rows ? p.gather[t.m0 + r] : -1;
+            const int row = id < 0 ? -1 : id / p.topk;
+            x_off[i] = row >= 0 && row < p.T ? (uint32_t)(row * p.ldx) : OOB;
+        }
+    } else {
+        x0 += t.m0 * p.ldx;
+        x_bytes = (uint32_t)((min(t.rows, 16 * MT) - 1) * p.ldx + p.K * 2);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x_off[i] = 16 * i + c < t.rows ? (uint32_t)((16 * i + c) * p.ldx) : OOB;
+    }
+    const auto xr = make_rsrc(x0, x_bytes);
+
+    const int units = (p.K + 127) / 128, u0 = wave * units / NW, u1 = (wave + 1) * units / NW;
+    struct Unit {
+        v4i w[NT], x[MT][4];
+        uint32_t s[NT][MX ? 1 : 4], z[NT][MX ? 1 : 4];
+    };
+    auto load = [&](int u, Unit& f) {
+        const int k = u * 128 + 32 * q;  // the lane's first value
+        const bool live = u < u1;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int n = 16 * i + c;
+            f.w[i] = __builtin_amdgcn_raw_buffer_load_b128(qr, live && k < p.K ? (uint32_t)(n * p.ldq + k / 2) : OOB, 0, 0);
+            if constexpr (MX) {
+                f.s[i][0] = __builtin_amdgcn_raw_buffer_load_b8(sr, live && k < p.K ? (uint32_t)(n * p.lds + k / 32) : OOB, 0, 0);
+            } else {
+                // the scale of each matrix instruction's 32 values: one load per group
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int g = u * 128 + 32 * j;
+                    if (j > 0 && (p.glog2 == 7 || (p.glog2 == 6 && (j & 1)))) {
+                        f.s[i][j] = f.s[i][j - 1], f.z[i][j] = f.z[i][j - 1];
+                        continue;
+                    }
+                    const uint32_t at = live && g < p.K ? (uint32_t)(n * p.lds + (g >> p.glog2)) : OOB;
+                    f.s[i][j] = __builtin_amdgcn_raw_buffer_load_b16(sr, at == OOB ? OOB : at * 2, 0, 0);
+                    f.z[i][j] = p.Z ? __builtin_amdgcn_raw_buffer_load_b8(zr, at, 0, 0) : 8;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int kx = u * 128 + (MX ? 32 * q + 8 * j : 32 * j + 8 * q);
+                f.x[i][j] = __builtin_amdgcn_raw_buffer_load_b128(
+                    xr, live && kx < p.K && x_off[i] != OOB ? x_off[i] + (uint32_t)(kx * 2) : OOB, 0, 0);
+            }
+    };
+    v4f acc[MT][NT] = {};
+    auto work = [&](const Unit& f) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            uint32_t w[4] = {(uint32_t)f.w[i][0], (uint32_t)f.w[i][1], (uint32_t)f.w[i][2], (uint32_t)f.w[i][3]};
+            if constexpr (MX) {
+                const float s = exp2i((int)f.s[i][0] - 127);
+                const float s0 = f.s[i][0] == 255 ? __builtin_nanf("") : s;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const v4i b = fp4_operand(w[j], s0);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[m][i] = mfma_bf16_16(f.x[m][j], b, acc[m][i]);
+                }
+            } else {
+                swap32(w[0], w[2]);
+                swap32(w[1], w[3]);
+                swap16(w[0], w[1]);
+                swap16(w[2], w[3]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const v4i b = int4_operand(w[j], (float)f.z[i][j]);
+                    const float s = bf16_to_f32(f.s[i][j]);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const v4f P = mfma_bf16_16(f.x[m][j], b, v4f{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[m][i][e] = __builtin_fmaf(P[e], s, acc[m][i][e]);
+                    }
+                }
+            }
+        }
+    };
+    Unit ring[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(u0 + d, ring[d]);
+    for (int u = u0; u < u1; u += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (u + d < u1) work(ring[d]);
+            load(u + d + D, ring[d]);
+        }
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) red[wave - 1][m * NT + i][lane] = acc[m][i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            v4f v = acc[m][i];
+#pragma unroll
+            for (int o = 0; o < NW - 1; ++o) v = v + red[o][m * NT + i][lane];
+            const int n = 16 * i + c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 16 * m + 4 * q + e;
+                if (r < t.rows && n < cols) p.C[(int64_t)(t.m0 + r) * p.ldc + n0 + n] = (uint16_t)f32_to_bf16(v[e]);
+            }
+        }
+}
+
+template <bool MX, int MT, int NT, int NW, int D>
+static int launch_w4_stream(W4Params& p, hipStream_t stream) {
+    p.tiles_m = (int)ragged_most(p.M, p.E, 16 * MT);
+    p.tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
+    p.group_m = 8;
+    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
+    HKQ_CHECK_ARG(blocks < (1 << 23), "too many tiles for one launch");
+    w4_stream_kernel<MX, MT, NT, NW, D><<<(unsigned)blocks, 64 * NW, 0, stream>>>(p);
+    return hkq_launch_status();
+}
+
+template <bool MX>
+static int run_w4(W4Params& p, hipStream_t stream) {
+    const int64_t r = p.M / std::min(p.M, p.E);
+    if (r <= 4) return launch_w4_stream<MX, 1, 1, 8, 2>(p, stream);
+    if (r <= 16) return launch_w4_stream<MX, 1, 2, 8, 2>(p, stream);
+    return launch_w4_stream<MX, 4, 2, 4, 1>(p, stream);
+}
+
+static int check_w4_weights(int64_t N, int64_t K, int64_t ldq, int64_t lds, int64_t group) {
+    HKQ_CHECK_ARG(N >= 0 && K >= 0, "N and K must be >= 0");
+    HKQ_CHECK_ARG(N < (1 << 22) && K < (1 << 22), "N and K must be < 2^22");
+    HKQ_CHECK_ARG(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
+    HKQ_CHECK_ARG(K % group == 0, "K must be a multiple of group");
+    HKQ_CHECK_ARG(ldq >= K / 2 && ldq < (1 << 22), "ldq must be >= K / 2 and < 2^22");
+    HKQ_CHECK_ARG(lds >= K / group && lds < (1 << 22), "lds must be >= K / group and < 2^22");
+    return 0;
+}
+
+}  // namespace hkq
+
+using namespace hkq;
+
+extern "C" int hkq_w4_quant(const void* w, void* q, void* s, void* z, int64_t N, int64_t K, int64_t ldw, int64_t ldq, int64_t lds,
+                            int64_t group, hipStream_t stream) {
+    if (int e = check_w4_weights(N, K, ldq, lds, group)) return e;
+    HKQ_CHECK_ARG(ldw >= K && ldw % 8 == 0 && ldw < (1 << 22), "ldw must be >= K, a multiple of 8 and < 2^22");
+    HKQ_CHECK_ARG(ldq % 4 == 0, "ldq must be a multiple of 4");
+    if (N == 0 || K == 0) return 0;
+    HKQ_CHECK_ARG(w && q && s, "w, q and s are required");
+    HKQ_CHECK_ALIGN(w, 16);
+    HKQ_CHECK_ALIGN(q, 4);
+    HKQ_CHECK_ALIGN(s, 2);
+    const int64_t G = K / group;
+    const MemRows mw{w, N, 2 * K, 2 * ldw}, mq{q, N, K / 2, ldq}, ms{s, N, 2 * G, 2 * lds}, mz{z, N, G, lds};
+    HKQ_CHECK_ARG(!overlap(mq, mw) && !overlap(ms, mw) && !overlap(mz, mw) && !overlap(mq, ms) && !overlap(mq, mz) && !overlap(ms, mz),
+                  "q, s and z must not overlap w or each other");
+    const unsigned blocks = (unsigned)std::min<int64_t>((N * (K / 8) + 255) / 256, 1 << 16);
+    auto kern = group == 32 ? w4_quant_kernel<32> : group == 64 ? w4_quant_kernel<64> : w4_quant_kernel<128>;
+    kern<<<blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(w), static_cast<uint8_t*>(q), static_cast<uint16_t*>(s),
+                                     static_cast<uint8_t*>(z), N, (int)K, ldw, ldq, lds);
+    return hkq_launch_status();
+}
+
+extern "C" int hkq_w4_dequant(const void* q, const void* s, const void* z, void* out, int64_t N, int64_t K, int64_t ldq,
+                              int64_t lds, int64_t ldo, int64_t group, hipStream_t stream) {
+    if (int e = check_w4_weights(N, K, ldq, lds, group)) return e;
+    HKQ_CHECK_ARG(ldo >= K && ldo % 8 == 0 && ldo < (1 << 22), "ldo must be >= K, a multiple of 8 and < 2^22");
+    HKQ_CHECK_ARG(ldq % 4 == 0, "ldq must be a multiple of 4");
+    if (N == 0 || K == 0) return 0;
+    HKQ_CHECK_ARG(q && s && out, "q, s and out are required");
+    HKQ_CHECK_ALIGN(q, 4);
+    HKQ_CHECK_ALIGN(s, 2);
+    HKQ_CHECK_ALIGN(out, 16);
+    const int64_t G = K / group;
+    const MemRows mo{out, N, 2 * K, 2 * ldo};
+    HKQ_CHECK_ARG(!overlap(mo, {q, N, K / 2, ldq}) && !overlap(mo, {s, N, 2 * G, 2 * lds}) && !overlap(mo, {z, N, G, lds}),
+                  "out must not overlap q, s or z");
+    const unsigned blocks = (unsigned)std::min<int64_t>((N * (K / 8) + 255) / 256, 1 << 16);
+    w4_dequant_kernel<<<blocks, 256, 0, stream>>>(static_cast<const uint8_t*>(q), static_cast<const uint16_t*>(s),
+                                                  static_cast<const uint8_t*>(z), static_cast<uint16_t*>(out), N, (int)K, ldq, lds,
+                                                  ldo, group == 32 ? 5 : group == 64 ? 6 : 7);
+    return hkq_launch_status();
+}
+
+static int w4_product(const void* X, const void* Q, const void* S, const void* Z, void* C, const int32_t* offs, const int32_t* gather,
+                      int64_t M, int64_t T, int64_t E, int64_t N, int64_t K, int64_t topk, int64_t ldx, int64_t ldq, int64_t stride_q,
+                      int64_t lds, int64_t stride_s, int64_t ldc, int64_t group, int kind, bool grouped, hipStream_t stream) {
+    HKQ_CHECK_ARG(kind == HKQ_W4_INT4 || kind == HKQ_W4_MXFP4, "kind must be HKQ_W4_INT4 or HKQ_W4_MXFP4");
+    HKQ_CHECK_ARG(M >= 0 && E >= 0 && T >= 0, "M, E and the rows of X must be >= 0");
+    HKQ_CHECK_ARG(M < (1 << 28) && T < (1 << 28) && E < (1 << 16), "M and the rows of X must be < 2^28, E < 2^16");
+    if (int e = check_w4_weights(N, K, ldq, lds, group)) return e;
+    const bool mx = kind == HKQ_W4_MXFP4;
+    HKQ_CHECK_ARG(!mx || (group == 32 && !Z), "MXFP4 weights have groups of 32 and no zero points");
+    HKQ_CHECK_ARG(ldx >= K && ldx % 8 == 0 && ldx < (1 << 22), "ldx must be >= K, a multiple of 8 and < 2^22");
+    HKQ_CHECK_ARG(ldq % 16 == 0, "ldq must be a multiple of 16");
+    HKQ_CHECK_ARG(ldc >= N && ldc < (1 << 22), "ldc must be >= N and < 2^22");
+    HKQ_CHECK_ARG(stride_q >= 0 && stride_q % 16 == 0 && stride_q < (1ll << 40), "stride_q must be >= 0, a multiple of 16 and < 2^40");
+    HKQ_CHECK_ARG(stride_s >= 0 && stride_s < (1ll << 40), "stride_s must be >= 0 and < 2^40");
+    HKQ_CHECK_ARG(!gather || (topk >= 1 && topk <= 65535), "topk must be in [1, 65535]");
+    HKQ_CHECK_ARG(!gather || 2 * (int64_t)(T * ldx) < (1ll << 31), "with a gather, X must span less than 2^31 bytes");
+    HKQ_CHECK_ARG(gather || !grouped || T >= M, "without a gather, X must have M rows");
+    if (M == 0 || E == 0 || N == 0) return 0;
+    HKQ_CHECK_ARG(C && (!grouped || offs) && (K == 0 || (Q && S && (X || T == 0))), "X, Q, S, the output and (grouped) offs are required");
+    HKQ_CHECK_ALIGN(X, 16);
+    HKQ_CHECK_ALIGN(Q, 16);
+    HKQ_CHECK_ALIGN(S, 2);
+    HKQ_CHECK_ALIGN(C, 2);
+    HKQ_CHECK_ALIGN(offs, 4);
+    HKQ_CHECK_ALIGN(gather, 4);
+    const int64_t G = K / group, sb = mx ? 1 : 2;
+    const MemRows mc{C, M, 2 * N, 2 * ldc};
+    HKQ_CHECK_ARG(!overlap(mc, {X, T, 2 * K, 2 * ldx}) && !overlap(mc, grouped_mem(Q, E, N, K / 2, ldq, stride_q)) &&
+                      !overlap(mc, grouped_mem(S, E, N, G * sb, lds * sb, stride_s * sb)) &&
+                      !overlap(mc, grouped_mem(Z, E, N, G, lds, stride_s)) && !overlap(mc, {offs, 1, 4 * (E + 1), 0}) &&
+                      !overlap(mc, {gather, 1, 4 * M, 0}),
+                  "the output must not overlap an operand");
+    W4Params p{};
+    p.X = static_cast<const uint8_t*>(X);
+    p.Q = static_cast<const uint8_t*>(Q);
+    p.S = static_cast<const uint8_t*>(S);
+    p.Z = static_cast<const uint8_t*>(Z);
+    p.C = static_cast<uint16_t*>(C);
+    p.offs = offs;
+    p.gather = gather;
+    p.M = (int)M; p.T = (int)T; p.E = (int)E; p.N = (int)N; p.K = (int)K;
+    p.ldx = 2 * ldx; p.ldq = ldq; p.lds = lds; p.ldc = ldc;
+    p.stride_q = stride_q; p.stride_s = stride_s;
+    p.glog2 = group == 32 ? 5 : group == 64 ? 6 : 7;
+    p.topk = gather ? (int)topk : 1;
+    return mx ? run_w4<true>(p, stream) : run_w4<false>(p, stream);
+}
+
+extern "C" size_t hkq_gemm_w4a16_workspace(int64_t, int64_t, int64_t) { return 0; }
+
+extern "C" int hkq_gemm_w4a16(const void* X, const void* Q, const void* S, const void* Z, void* C, int64_t M, int64_t N, int64_t K,
+                              int64_t ldx, int64_t ldq, int64_t lds, int64_t ldc, int64_t group, int kind, void*, size_t,
+                              hipStream_t stream) {
+    return w4_product(X, Q, S, Z, C, nullptr, nullptr, M, M, 1, N, K, 1, ldx, ldq, 0, lds, 0, ldc, group, kind, false, stream);
+}
+
+extern "C" size_t hkq_grouped_gemm_w4a16_workspace(int64_t, int64_t, int64_t, int64_t) { return 0; }
+
+extern "C" int hkq_grouped_gemm_w4a16(const void* X, const void* Q, const void* S, const void* Z, void* Y, const int32_t* offs,
+                                      const int32_t* gather, int64_t M, int64_t T, int64_t E, int64_t N, int64_t K, int64_t topk,
+                                      int64_t ldx, int64_t ldq, int64_t stride_q, int64_t lds, int64_t stride_s, int64_t ldy,
+                                      int64_t group, int kind, void*, size_t, hipStream_t stream) {
+    return w4_product(X, Q, S, Z, Y, offs, gather, M, T, E, N, K, topk, ldx, ldq, stride_q, lds, stride_s, ldy, group, kind, true, stream);
+}

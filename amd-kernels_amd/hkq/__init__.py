@@ -17,6 +17,10 @@ LIB_PATH = os.path.join(_PKG, "lib", "libhkq.so")
 KIND_FP8 = 0
 KIND_INT8 = 1
 
+# kinds of 4-bit weights (HKQ_W4_*)
+W4_INT4 = 0
+W4_MXFP4 = 1
+
 # activations of the fused epilogues and the gated feed-forward (HKQ_ACT_*)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu": 4}
 
@@ -63,6 +67,12 @@ SIGNATURES = {
     "hkq_gated_ffn_backward": (_I, [_P] * 6 + [_I64] * 9 + [_I, ctypes.c_float, _I, _P, ctypes.c_size_t, _P]),
     "hkq_grouped_gemm_bf16": (_I, [_P] * 4 + [_I64] * 8 + [_P]),
     "hkq_grouped_gemm_backward": (_I, [_P] * 6 + [_I64] * 11 + [_P]),
+    "hkq_w4_quant": (_I, [_P] * 4 + [_I64] * 6 + [_P]),
+    "hkq_w4_dequant": (_I, [_P] * 4 + [_I64] * 6 + [_P]),
+    "hkq_gemm_w4a16_workspace": (ctypes.c_size_t, [_I64] * 3),
+    "hkq_gemm_w4a16": (_I, [_P] * 5 + [_I64] * 8 + [_I, _P, ctypes.c_size_t, _P]),
+    "hkq_grouped_gemm_w4a16_workspace": (ctypes.c_size_t, [_I64] * 4),
+    "hkq_grouped_gemm_w4a16": (_I, [_P] * 7 + [_I64] * 13 + [_I, _P, ctypes.c_size_t, _P]),
     "hkq_swiglu_quant": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float, _I, _I, _P]),
     "hkq_moe_mxfp4": (_I, [_P] * 10 + [_I64, _I64, _I64, _I64, _I] + [_I64] * 10 + [_P]),
     "hkq_moe_mxfp4_kn": (_I, [_P] * 10 + [_I64, _I64, _I64, _I64, _I] + [_I64] * 10 + [_P]),
@@ -598,6 +608,142 @@ def grouped_gemm_backward(dY, X, W, offs, dX=None, dW=None, need_dx: bool = True
         call("hkq_grouped_gemm_backward", _ptr(dY), _ptr(X), _ptr(W), _opt_ptr(dX), _opt_ptr(dW), _ptr(offs), M, E, N, K,
              _pitch(dY), _pitch(X), lw, se, _pitch(dX), ldw, sd, _stream(stream))
     return dX, dW
+
+
+def w4_quant(w, group: int = 128, zeros: bool = False, q=None, s=None, z=None, stream=None):
+    """INT4 codes of weights w bf16 [N, K] or [E, N, K] with one scale per `group` (32,
+    64 or 128) values: (q u8 [.., K / 2], s bf16 [.., K / group]), and with zeros the
+    zero points z u8 of s's shape: w ~ (code - z) * s, z = 8 without them."""
+    import torch
+
+    if group not in (32, 64, 128):
+        raise ValueError(f"group must be 32, 64 or 128, got {group}")
+    *lead, K = w.shape
+    if len(lead) not in (1, 2) or K % group:
+        raise ValueError(f"w must be [N, K] or [E, N, K] with K a multiple of {group}, got {list(w.shape)}")
+    if len(lead) == 2:  # one call for all experts
+        w = w.reshape(-1, K)
+    N = w.shape[0]
+    _expect(w, "w", (N, K), (torch.bfloat16,), w.device)
+    flat = []
+    for t, name, cols, dtype in ((q, "q", K // 2, torch.uint8), (s, "s", K // group, torch.bfloat16), (z, "z", K // group, torch.uint8)):
+        if t is not None:
+            _expect(t, name, (*lead, cols), (dtype,), w.device)
+            t = t.view(N, cols)
+        flat.append(t)
+    q, s, z = flat
+    with _on(w.device, stream):
+        if q is None:
+            q = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
+        if s is None:
+            s = torch.empty((N, K // group), dtype=torch.bfloat16, device=w.device)
+        if z is None and zeros:
+            z = torch.empty((N, K // group), dtype=torch.uint8, device=w.device)
+        if z is not None and _pitch(z) != _pitch(s):
+            raise ValueError("s and z must have one pitch")
+        call("hkq_w4_quant", _ptr(w), _ptr(q), _ptr(s), _opt_ptr(z), N, K, _pitch(w), _pitch(q), _pitch(s), group,
+             _stream(stream))
+    return tuple(t.view(*lead, t.shape[1]) for t in (q, s, z) if t is not None)
+
+
+def _w4_weights(Q, S, Z, device):
+    """(kind, group) of 4-bit weights, [N, ..] or [E, N, ..]."""
+    import torch
+
+    *lead, half = Q.shape
+    K = 2 * half
+    mx = S.dtype == torch.uint8
+    groups = S.shape[-1] if S.dim() == Q.dim() else 0
+    group = 32 if mx else K // groups if groups and K % groups == 0 else 0
+    if not mx and K == 0:
+        group = 32
+    if group not in (32, 64, 128):
+        raise ValueError(f"scales of {list(S.shape)} for codes of {list(Q.shape)}: groups of 32, 64 or 128 values are wanted")
+    _expect(Q, "Q", (*lead, half), (torch.uint8,), device)
+    _expect(S, "S", (*lead, K // group), (torch.uint8, torch.bfloat16), device)
+    if Z is not None:
+        if mx:
+            raise ValueError("MXFP4 weights have no zero points")
+        _expect(Z, "Z", (*lead, K // group), (torch.uint8,), device)
+        if Z.numel() and any(n > 1 and a != b for n, a, b in zip(S.shape, S.stride(), Z.stride())):
+            raise ValueError("S and Z must have the same strides")
+    return (W4_MXFP4 if mx else W4_INT4), group
+
+
+def w4_dequant(q, s, z=None, out=None, stream=None):
+    """bf16((code - z) * s) of w4_quant's outputs, [N, K] or [E, N, K]."""
+    import torch
+
+    kind, group = _w4_weights(q, s, z, q.device)
+    if kind != W4_INT4:
+        raise TypeError("s must be bf16 (MXFP4: mx_dequant)")
+    *lead, half = q.shape
+    K = 2 * half
+    if out is not None:
+        _expect(out, "out", (*lead, K), (torch.bfloat16,), q.device)
+    with _on(q.device, stream):
+        if out is None:
+            out = torch.empty((*lead, K), dtype=torch.bfloat16, device=q.device)
+        n = 1
+        for d in lead:
+            n *= d
+        q2, s2, o2 = q.view(n, half), s.view(n, K // group), out.view(n, K)
+        z2 = None if z is None else z.view(n, K // group)
+        call("hkq_w4_dequant", _ptr(q2), _ptr(s2), _opt_ptr(z2), _ptr(o2), n, K, _pitch(q2), _pitch(s2), _pitch(o2), group,
+             _stream(stream))
+    return out
+
+
+def gemm_w4a16(X, Q, S, Z=None, C=None, stream=None):
+    """C = X . W^T of bf16 rows X [M, K] and 4-bit weights: codes Q u8 [N, K / 2] with
+    scales S bf16 [N, K / group] (and zero points Z u8, w4_quant's) or MXFP4 codes
+    with e8m0 scales S u8 [N, K / 32] (mx_quant's) -> bf16 [M, N]."""
+    import torch
+
+    M, K = X.shape
+    N = Q.shape[0]
+    _expect(X, "X", (M, K), (torch.bfloat16,), X.device)
+    _expect(Q, "Q", (N, K // 2), (torch.uint8,), X.device)
+    kind, group = _w4_weights(Q, S, Z, X.device)
+    if C is not None:
+        _expect(C, "C", (M, N), (torch.bfloat16,), X.device)
+    with _on(X.device, stream):
+        if C is None:
+            C = torch.empty((M, N), dtype=torch.bfloat16, device=X.device)
+        ws = _workspace(int(lib().hkq_gemm_w4a16_workspace(M, N, K)), X)
+        call("hkq_gemm_w4a16", _ptr(X), _ptr(Q), _ptr(S), _opt_ptr(Z), _ptr(C), M, N, K, _pitch(X), _pitch(Q), _pitch(S),
+             _pitch(C), group, kind, _opt_ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+    return C
+
+
+def grouped_gemm_w4a16(X, Q, S, offs, Z=None, gather=None, topk: int = 1, Y=None, stream=None):
+    """gemm_w4a16 over ragged groups of rows: Y[r] = X[x(r)] . W[e]^T for offs[e] <= r <
+    offs[e + 1], 4-bit weights Q [E, N, K / 2], S (and Z) [E, N, K / group]. x(r) = r,
+    or gather[r] // topk with moe_routing's gather int32 [M] (a row outside X counts
+    as zeros). offs int32 [E + 1] and gather are on the GPU -> bf16 [M, N]; rows of no
+    group are left as they were: pass a Y that holds something there."""
+    import torch
+
+    T, K = X.shape
+    E, N = Q.shape[:2]
+    M = T if gather is None else gather.shape[0]
+    _expect(X, "X", (T, K), (torch.bfloat16,), X.device)
+    _expect(Q, "Q", (E, N, K // 2), (torch.uint8,), X.device)
+    kind, group = _w4_weights(Q, S, Z, X.device)
+    _expect(offs, "offs", (E + 1,), (torch.int32,), X.device)
+    if gather is not None:
+        _expect(gather, "gather", (M,), (torch.int32,), X.device)
+    if Y is not None:
+        _expect(Y, "Y", (M, N), (torch.bfloat16,), X.device)
+    (sq, lq), (ss, ls) = _stride3(Q), _stride3(S)
+    with _on(X.device, stream):
+        if Y is None:
+            Y = torch.empty((M, N), dtype=torch.bfloat16, device=X.device)
+        ws = _workspace(int(lib().hkq_grouped_gemm_w4a16_workspace(M, E, N, K)), X)
+        call("hkq_grouped_gemm_w4a16", _ptr(X), _ptr(Q), _ptr(S), _opt_ptr(Z), _ptr(Y), _ptr(offs), _opt_ptr(gather), M, T, E,
+             N, K, topk, _pitch(X), lq, sq, ls, ss, _pitch(Y), group, kind, _opt_ptr(ws),
+             ws.numel() if ws is not None else 0, _stream(stream))
+    return Y
 
 
 def moe_a8w8(X, W, hist, offs, expt_data, topk, gather=None, x_scale=None, w_scale=None, bias=None, Y=None,

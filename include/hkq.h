@@ -478,6 +478,54 @@ int hkq_grouped_gemm_backward(const void* dY, const void* X, const void* W, void
                               int64_t M, int64_t E, int64_t N, int64_t K, int64_t lddy, int64_t ldx, int64_t ldw,
                               int64_t stride_we, int64_t lddx, int64_t lddw, int64_t stride_dwe, hkq_stream_t stream);
 
+/* ---- 4-bit weights ---------------------------------------------------------- */
+/* Weights W [N, K] as codes Q [N, ldq] bytes (two per byte, the even K index in the
+ * low nibble) with one scale per `group` values of K:
+ *   HKQ_W4_INT4   (code - zero) * scale, S bf16 [N, lds], Z u8 [N, lds] values 0 .. 15
+ *                 (NULL: 8 throughout); group 32, 64 or 128;
+ *   HKQ_W4_MXFP4  E2M1 codes times 2^(e - 127), S e8m0 [N, lds] (255: NaN), no Z,
+ *                 group 32: what hkq_mx_quant writes.
+ * K is a multiple of group; N, K and every pitch < 2^22; ldq a multiple of 4 (of 16,
+ * with Q 16-byte aligned, in the products). */
+#define HKQ_W4_INT4 0
+#define HKQ_W4_MXFP4 1
+
+/* INT4 codes of w bf16 [N, ldw]. z NULL: s = bf16(amax / 7), code = clamp(rint(w *
+ * (1 / s)), -8, 7) + 8; else, with lo and hi the group's extremes or 0, s =
+ * bf16(hi / 15 - lo / 15), zero = clamp(rint(-lo * (1 / s)), 0, 15), code =
+ * clamp(rint(w * (1 / s)) + zero, 0, 15). fp32, ties to even; a scale below 2^-126
+ * takes codes of zero, a NaN makes its group's scale NaN, an infinity makes it
+ * infinite. ldw a multiple of 8, w 16-byte aligned. No counterpart in the
+ * reference (its 4-bit codes are MXFP4). */
+int hkq_w4_quant(const void* w, void* q, void* s, void* z, int64_t N, int64_t K, int64_t ldw, int64_t ldq, int64_t lds,
+                 int64_t group, hkq_stream_t stream);
+
+/* out bf16 [N, ldo] = bf16((code - zero) * scale), INT4 (MXFP4: hkq_mx_dequant). */
+int hkq_w4_dequant(const void* q, const void* s, const void* z, void* out, int64_t N, int64_t K, int64_t ldq,
+                   int64_t lds, int64_t ldo, int64_t group, hkq_stream_t stream);
+
+/* C[m, n] = bf16(sum_k X[m, k] W[n, k]), X bf16 [M, K] (pitch ldx a multiple of 8,
+ * 16-byte aligned), C bf16 [M, ldc] (any pitch >= N). The weights are not rounded:
+ * an INT4 scale multiplies the fp32 sums of its group. workspace: unused where the
+ * query gives 0 (16-byte aligned, calls that overlap need one each). C shares no
+ * memory with an operand (refused). No counterpart in the reference, whose 4-bit
+ * products take 4-bit activations or dequantized weights. */
+size_t hkq_gemm_w4a16_workspace(int64_t M, int64_t N, int64_t K);
+int hkq_gemm_w4a16(const void* X, const void* Q, const void* S, const void* Z, void* C, int64_t M, int64_t N, int64_t K,
+                   int64_t ldx, int64_t ldq, int64_t lds, int64_t ldc, int64_t group, int kind, void* workspace,
+                   size_t workspace_bytes, hkq_stream_t stream);
+
+/* The same over ragged groups of rows (offs as in hkq_grouped_gemm_bf16), group e
+ * with the weight at Q + e * stride_q, S (and Z) + e * stride_s scales: Y[r, n] =
+ * bf16(sum_k X[x(r), k] W[e][n, k]), x(r) = r, or with gather int32 [M] on the GPU
+ * gather[r] / topk (the token of a routed gate); a row outside X's T rows counts as
+ * zeros. With a gather X spans less than 2^31 bytes. */
+size_t hkq_grouped_gemm_w4a16_workspace(int64_t M, int64_t E, int64_t N, int64_t K);
+int hkq_grouped_gemm_w4a16(const void* X, const void* Q, const void* S, const void* Z, void* Y, const int32_t* offs,
+                           const int32_t* gather, int64_t M, int64_t T, int64_t E, int64_t N, int64_t K, int64_t topk,
+                           int64_t ldx, int64_t ldq, int64_t stride_q, int64_t lds, int64_t stride_s, int64_t ldy,
+                           int64_t group, int kind, void* workspace, size_t workspace_bytes, hkq_stream_t stream);
+
 /* ---- MoE routing metadata producers --------------------------------------- */
 /* All index outputs are deterministic: gates of one expert keep their input
  * order (the order of the reference's test formulas, tests/test_moe.py:97-128,
