@@ -41,13 +41,14 @@ HIP_FLAGS = [
 ]
 
 HIP_SOURCES = ["gemm_fused.hip", "quant.hip", "gemm.hip", "gemm_blockscale.hip", "moe.hip", "moe_blockscale.hip", "routing.hip",
-               "norm_quant.hip", "grouped.hip", "w4.hip"]
+               "norm_quant.hip", "grouped.hip", "w4.hip", "w4_tile.hip"]
 CPP_SOURCES = ["hkq_error.cpp"]
 # Per-source code generation options. The block-scale GEMM promotes every
 # K group on the VALU (acc += P * scale): its MFMAs must write the partial P
 # to arch VGPRs, which the compiler's default register-class choice does not
 # do (it writes AGPRs and then copies every element out).
-SRC_FLAGS = {"gemm_blockscale.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+SRC_FLAGS = {"gemm_blockscale.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+             "w4_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}  # likewise: INT4 group sums
 
 # pybind11 module name -> binding source (module names are the reference's)
 MODULES = {
