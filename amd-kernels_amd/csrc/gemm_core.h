@@ -102,14 +102,6 @@ __device__ __forceinline__ void lds_load4(const void* base, uint32_t bytes, HKQ_
                  : "memory", "m0");
 }
 
-__device__ __forceinline__ void lds_load4_d(const v4i& desc, HKQ_LDS void* dst, uint32_t off) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :
-                 : "s"(m0), "v"(off), "s"(desc)
-                 : "memory", "m0");
-}
-
 __device__ __forceinline__ v4i lds_read16(const HKQ_LDS uint8_t* p) { return *reinterpret_cast<const HKQ_LDS v4i*>(p); }
 
 // N-contiguous ("transposed") B tiles: the weights of a K-tile stored as they

@@ -25,32 +25,49 @@ struct W4Params {
 // ---------------------------------------------------------------------------
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-// 8 codes (value j in nibble j) -> 8 bf16 values code - zero, exactly: a byte that
-// holds 0 .. 15 is, as E4M3, that number times 2^-9, so one conversion with scale 2^9
-// gives two codes as fp32; the difference has at most 4 significant bits, and the
-// upper half of its fp32 pattern is its bf16.
-__device__ __forceinline__ v4i int4_operand(uint32_t w, float zero) {
-    const uint32_t ev = w & 0x0F0F0F0Fu, od = w >> 4 & 0x0F0F0F0Fu;
-    v4i o;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const f32x2_t e = h ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(ev, 512.0f, true)
-                            : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(ev, 512.0f, false);
-        const f32x2_t d = h ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(od, 512.0f, true)
-                            : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(od, 512.0f, false);
-        o[2 * h] = (int)__builtin_amdgcn_perm(__float_as_uint(d[0] - zero), __float_as_uint(e[0] - zero), 0x07060302u);
-        o[2 * h + 1] = (int)__builtin_amdgcn_perm(__float_as_uint(d[1] - zero), __float_as_uint(e[1] - zero), 0x07060302u);
-    }
-    return o;
+// Codes (value j in nibble j) 4 H .. 4 H + 3 -> bf16 values code - zero, exactly: a
+// byte that holds 0 .. 15 is, as E4M3, that number times 2^-9, so one conversion with
+// scale 2^9 gives two codes as fp32; the difference has at most 4 significant bits,
+// and the upper half of its fp32 pattern is its bf16. 19 instructions per 8 codes.
+template <int H>
+__device__ __forceinline__ v2i int4_operand2(uint32_t w, float zero) {
+    const f32x2_t e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w & 0x0F0F0F0Fu, 512.0f, H != 0);
+    const f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w >> 4 & 0x0F0F0F0Fu, 512.0f, H != 0);
+    return v2i{(int)__builtin_amdgcn_perm(__float_as_uint(d[0] - zero), __float_as_uint(e[0] - zero), 0x07060302u),
+               (int)__builtin_amdgcn_perm(__float_as_uint(d[1] - zero), __float_as_uint(e[1] - zero), 0x07060302u)};
 }
-// 8 E2M1 codes times 2^(e8m0 - 127), the scale as the fp32 of that exponent.
+__device__ __forceinline__ v4i int4_operand(uint32_t w, float zero) {
+    const v2i a = int4_operand2<0>(w, zero), b = int4_operand2<1>(w, zero);
+    return v4i{a[0], a[1], b[0], b[1]};
+}
+// The same for zero = 8, as sixteenths (code - 8) / 16: with its upper bit inverted a
+// code is a signed nibble, which v_cvt_off_f32_i4 converts from the low half of any
+// byte. 14 instructions per 8 codes.
+template <int BYTE>
+__device__ __forceinline__ float signed_nibble(uint32_t w) {
+    float v;
+    if constexpr (BYTE == 0) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(v) : "v"(w));
+    if constexpr (BYTE == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(v) : "v"(w));
+    if constexpr (BYTE == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(v) : "v"(w));
+    if constexpr (BYTE == 3) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(v) : "v"(w));
+    return v;
+}
+template <int H>
+__device__ __forceinline__ v2i int4_sixteenths(uint32_t w) {
+    const uint32_t ev = w ^ 0x88888888u, od = ev >> 4;
+    return v2i{(int)__builtin_amdgcn_perm(__float_as_uint(signed_nibble<2 * H>(od)), __float_as_uint(signed_nibble<2 * H>(ev)), 0x07060302u),
+               (int)__builtin_amdgcn_perm(__float_as_uint(signed_nibble<2 * H + 1>(od)), __float_as_uint(signed_nibble<2 * H + 1>(ev)),
+                                          0x07060302u)};
+}
+// E2M1 codes 4 H .. 4 H + 3 times 2^(e8m0 - 127), the scale as the fp32 of that exponent.
+template <int H>
+__device__ __forceinline__ v2i fp4_operand2(uint32_t w, float scale) {
+    return v2i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2 * H)),
+               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2 * H + 1))};
+}
 __device__ __forceinline__ v4i fp4_operand(uint32_t w, float scale) {
-    v4i o;
-    o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
-    o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
-    o[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
-    o[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
-    return o;
+    const v2i a = fp4_operand2<0>(w, scale), b = fp4_operand2<1>(w, scale);
+    return v4i{a[0], a[1], b[0], b[1]};
 }
 
 __device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {

@@ -10,20 +10,22 @@
 // group. MXFP4 scales go into the operands.
 #include <type_traits>
 
+#include "gemm_kgroup.h"
 #include "w4_core.h"
 
 namespace hkq {
 
-// G: values per group, 0 for MXFP4 (32)
-template <int G_, int TM_, int TN_, int NS_>
+// G: values per group, 0 for MXFP4 (32); Z: zero points
+template <int G_, bool Z_, int TM_, int TN_, int NS_>
 struct W4Tile {
+    static constexpr bool Z = Z_;
     static constexpr int G = G_, TM = TM_, TN = TN_, NS = NS_, NW = 4;
     static constexpr bool MX = G == 0;
     static constexpr int BM = 32 * TM, BN = NW * TN * 32, SB = MX ? 1 : 2;
     static constexpr int NG = MX ? 4 : 128 / G;  // groups in a unit
     // A row's scales of a unit start at any multiple of SB bytes (its zero points at
     // any byte): the aligned dwords that hold them
-    static constexpr int SD = (NG * SB + 4 - SB + 3) / 4, ZD = MX ? 0 : (NG + 3 + 3) / 4;
+    static constexpr int SD = (NG * SB + 4 - SB + 3) / 4, ZD = Z ? (NG + 3 + 3) / 4 : 0;
     static constexpr int XB = 2 * BM * 128, WB = BN * 64, STAGE = XB + WB + NW * (SD + ZD) * 256;
     static constexpr int LX = 2 * BM / 8 / NW, LW = BN / 16 / NW, NLD = LX + LW + SD + ZD;
     static constexpr int EP_PITCH = TN * 64 + 16, EP = NW * BM * EP_PITCH;
@@ -31,6 +33,18 @@ struct W4Tile {
     static_assert(LDS <= 160 * 1024 && NS >= 3 && (NS - 2) * NLD <= 63, "LDS and vmcnt budget");
     static constexpr int PARTS = MX ? 1 : NG, CH = 8 / PARTS;  // chains of matrix instructions per n-tile and m-tile
 };
+
+template <int I, int N, class F>
+__device__ __forceinline__ void for_each_from(F& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        for_each_from<I + 1, N>(f);
+    }
+}
+template <int N, class F>
+__device__ __forceinline__ void for_each_int(F& f) {
+    for_each_from<0, N>(f);
+}
 
 template <class T>
 __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
@@ -83,50 +97,49 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
     const int64_t s_at = t.e * p.stride_s + n0 * p.lds, s_n = (cols - 1) * p.lds + groups;
     const v4i ds = dwords(p.S + s_at * SB, (int)(s_n * SB), s_rem);
     v4i dz{};
-    if constexpr (!MX) dz = dwords(p.Z ? p.Z + s_at : nullptr, p.Z ? (int)s_n : 0, z_rem);
+    if constexpr (T::Z) dz = dwords(p.Z + s_at, (int)s_n, z_rem);
     const uint32_t s_col = (uint32_t)((wave * TN * 32 + lane % (TN * 32)) * p.lds);  // the lane's column, in scales
 
     const int units = (p.K + 127) / 128;
+    // the lane's chunk of the last unit's halves: past K it reads nothing
+    const int last_k = (units - 1) * 128 + xc * 8;
+    const uint32_t x_tail[2] = {last_k < p.K ? 0u : OOB, last_k + 64 < p.K ? 0u : OOB};
     // a unit's loads into a stage; past the last they read nothing
     auto issue = [&](int u, int stage) {
         HKQ_LDS uint8_t* st = smem + stage * T::STAGE;
-        const bool live = u < units;
+        const uint32_t dead = u < units ? 0u : OOB;
 #pragma unroll
-        for (int i = 0; i < T::LX; ++i) {
-            const int half = i / (T::LX / 2), r = i % (T::LX / 2);
-            const bool in = live && u * 128 + half * 64 + xc * 8 < p.K && x_off[r] != OOB;
-            lds_load16_d(dx, st + half * BM * 128 + (r * NW + wave) * 1024, in ? x_off[r] + (uint32_t)(u * 256 + half * 128) : OOB);
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t none = u + 1 < units ? 0u : x_tail[half] | dead;
+#pragma unroll
+            for (int r = 0; r < T::LX / 2; ++r)
+                lds_load16_s(dx, st + half * BM * 128 + (r * NW + wave) * 1024, x_off[r] | none,
+                             dead ? 0u : (uint32_t)(u * 256 + half * 128));
         }
 #pragma unroll
         for (int i = 0; i < T::LW; ++i)
-            lds_load16_d(dq, st + T::XB + (i * NW + wave) * 1024, live ? w_off[i] + (uint32_t)(u * 64) : OOB);
+            lds_load16_s(dq, st + T::XB + (i * NW + wave) * 1024, w_off[i] | dead, dead ? 0u : (uint32_t)(u * 64));
         HKQ_LDS uint8_t* sc = st + T::XB + T::WB + wave * (T::SD + T::ZD) * 256;
+        const uint32_t s0 = ((s_rem + (s_col + (uint32_t)(u * NG)) * SB) & ~3u) | dead;
 #pragma unroll
-        for (int d = 0; d < T::SD; ++d)
-            lds_load4_d(ds, sc + d * 256, live ? ((s_rem + (s_col + (uint32_t)(u * NG)) * SB) & ~3u) + 4 * d : OOB);
+        for (int d = 0; d < T::SD; ++d) lds_load4_s(ds, sc + d * 256, s0, 4 * d);
+        const uint32_t z0 = ((z_rem + s_col + (uint32_t)(u * NG)) & ~3u) | dead;
 #pragma unroll
-        for (int d = 0; d < T::ZD; ++d)
-            lds_load4_d(dz, sc + (T::SD + d) * 256, live && p.Z ? ((z_rem + s_col + (uint32_t)(u * NG)) & ~3u) + 4 * d : OOB);
+        for (int d = 0; d < T::ZD; ++d) lds_load4_s(dz, sc + (T::SD + d) * 256, z0, 4 * d);
     };
 
-    // an n-tile's codes of a unit, and its operands
+    // an n-tile's codes of a unit
     struct Raw {
-        uint32_t w[8];                // word s: values 16 s + 8 h .. of the unit (MXFP4: 64 (s / 4) + 32 h + 8 (s % 4))
-        float s[NG], z[MX ? 1 : NG];  // MXFP4: s[half]: the lane's block
+        uint32_t w[8];                   // word s: values 16 s + 8 h .. of the unit (MXFP4: 64 (s / 4) + 32 h + 8 (s % 4))
+        float s[NG], z[T::Z ? NG : 1];   // MXFP4: s[half]: the lane's block
     };
     auto read_raw = [&](int u, int stage, int i, Raw& r) {
         const HKQ_LDS uint8_t* st = smem + stage * T::STAGE;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const v4i v = lds_read16(st + T::XB + KW::swz((wave * TN + i) * 32 + ln, 2 * half + h));
-            uint32_t a = (uint32_t)v[0], b = (uint32_t)v[1], c = (uint32_t)v[2], d = (uint32_t)v[3];
-            if constexpr (!MX) {
-                swap32(a, b);  // a: words 0 and 1 of the 64 values' first 32, b: 4 and 5
-                swap32(c, d);
-                r.w[4 * half] = a, r.w[4 * half + 1] = c, r.w[4 * half + 2] = b, r.w[4 * half + 3] = d;
-            } else {
-                r.w[4 * half] = a, r.w[4 * half + 1] = b, r.w[4 * half + 2] = c, r.w[4 * half + 3] = d;
-            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) r.w[4 * half + q] = (uint32_t)v[q];
         }
         // scales: bytes at any offset in the staged dwords of the lane's column
         const int cl = i * 32 + ln;
@@ -144,24 +157,38 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
                 const bool live = u * NG + g < groups;
                 const float v = __uint_as_float(bits(sc, ((s_rem + col * 2) & 3) + 2 * g) << 16);
                 r.s[g] = live ? v : 0.0f;
-                r.z[g] = p.Z ? (float)(bits(sc + T::SD * 256, ((z_rem + col) & 3) + g) & 255) : 8.0f;
+                if constexpr (T::Z) r.z[g] = (float)(bits(sc + T::SD * 256, ((z_rem + col) & 3) + g) & 255);
             }
         }
     };
-    auto operand = [&](const Raw& r, int s) {
-        if constexpr (MX) return fp4_operand(r.w[s], r.s[s / 4]);
-        else return int4_operand(r.w[s], r.z[s / CH]);
+    // Values 4 half .. 4 half + 3 of word s as a matrix operand's (INT4 without zero
+    // points: a sixteenth of each). The words of INT4 change places between the lane
+    // halves first (turn), so that an instruction's 16 values lie in one group.
+    auto turn = [&](Raw& r) {
+        if constexpr (!MX) {
+#pragma unroll
+            for (int q = 0; q < 8; q += 4) {
+                swap32(r.w[q], r.w[q + 1]);  // words 0 and 1 of the first 32 values | of the next
+                swap32(r.w[q + 2], r.w[q + 3]);
+                const uint32_t v = r.w[q + 1];
+                r.w[q + 1] = r.w[q + 2], r.w[q + 2] = v;
+            }
+        }
     };
-    // fragment s of m-tile j
+    auto operand_half = [&](const Raw& r, int s, int half, v4i& b) {
+        v2i o;
+        if constexpr (MX) o = half ? fp4_operand2<1>(r.w[s], r.s[s / 4]) : fp4_operand2<0>(r.w[s], r.s[s / 4]);
+        else if constexpr (T::Z) o = half ? int4_operand2<1>(r.w[s], r.z[s / CH]) : int4_operand2<0>(r.w[s], r.z[s / CH]);
+        else o = half ? int4_sixteenths<1>(r.w[s]) : int4_sixteenths<0>(r.w[s]);
+        b[2 * half] = o[0], b[2 * half + 1] = o[1];
+    };
+    // fragment f of a step: values 16 (f % 8) of the unit, m-tile f / 8 (chains of CH: the same order)
     uint32_t a_at[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        a_at[s] = (uint32_t)(uintptr_t)smem + (uint32_t)KT::swz(ln, MX ? 4 * h + s : 2 * s + h);
-        asm volatile("" : "+v"(a_at[s]));
-    }
-    auto read_a = [&](int stage, int j, int s) {
+    for (int s = 0; s < 4; ++s) a_at[s] = (uint32_t)(uintptr_t)smem + (uint32_t)KT::swz(ln, MX ? 4 * h + s : 2 * s + h);
+    auto read_a = [&](const uint32_t (&at)[4], int f) {
         return lds_read16(reinterpret_cast<const HKQ_LDS uint8_t*>(
-            (uintptr_t)(a_at[s & 3] + (uint32_t)(stage * T::STAGE + (s / 4) * BM * 128 + j * 32 * 128))));
+            (uintptr_t)(at[f & 3] + (uint32_t)(f % 8 / 4 * BM * 128 + f / 8 * 32 * 128))));
     };
 
     v16f acc[TN][TM];
@@ -170,83 +197,93 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = v16f{};
 
-    auto bmfma = [](const v4i& a, const v4i& b, const v16f& c) { return mfma_bf16(a, b, c); };
-
 #pragma unroll
     for (int u = 0; u < NS - 1; ++u) issue(u, u);
     tile_barrier<(NS - 2) * T::NLD>();
-    v4i B[2][8];
-    Raw raw[2];
-    read_raw(0, 0, 0, raw[0]);
+    constexpr int SLOTS = 8 * TM, RING = 8, AHEAD = 6;
+    v4i B[2][8], A[RING];
+    Raw raw;
+    float sc[2][NG];  // the scales of the operands in B
+    read_raw(0, 0, 0, raw);
+    turn(raw);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) B[0][s] = operand(raw[0], s);
+    for (int s = 0; s < 8; ++s) operand_half(raw, s, 0, B[0][s]), operand_half(raw, s, 1, B[0][s]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sc[0][g] = raw.s[g];
     int stage = 0;
-    constexpr int CHUNKS = TM * T::PARTS;
-    v16f Pq{};  // the chain before this one's sums, and their scale
+    uint32_t at[4], at_next[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) at[s] = at_next[s] = a_at[s];
+#pragma unroll
+    for (int f = 0; f < AHEAD; ++f) A[f] = read_a(at, f);
+    v16f P{}, Pq{};  // a chain's sums; the chain's before, and their scale
     float sq = 0.0f;
-    // n-tile i of unit u: matrix instructions on B[cur] while the next n-tile's
-    // operands are formed in B[cur ^ 1]
+    // n-tile i of unit u: matrix instructions on B[cur], one per slot, and between them
+    // the fragment reads AHEAD slots on, the sums of the chain before into acc, and the
+    // next n-tile's operands into B[cur ^ 1]
     auto step = [&](int u, auto ii, auto par) {
         constexpr int i = decltype(ii)::value, cur = decltype(par)::value;
+        constexpr bool LAST = i == TN - 1;
         const int next_stage = stage + 1 == NS ? 0 : stage + 1;
-        if constexpr (i == TN - 1) {
-            // unit u + 1 resident; every wave past unit u - 1, whose stage takes unit u + NS - 1
-            tile_barrier<(NS - 3) * T::NLD>();
+        if constexpr (LAST) {
+            // unit u + 1 resident; every wave past unit u - 1, whose stage takes unit u + NS - 1.
+            // (Reads of unit u may be on their way: nothing writes there.)
+            __builtin_amdgcn_s_waitcnt(waitcnt_imm((NS - 3) * T::NLD, 15));
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
             issue(u + NS - 1, stage == 0 ? NS - 1 : stage - 1);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                at_next[s] = a_at[s] + (uint32_t)(next_stage * T::STAGE);
+                asm volatile("" : "+v"(at_next[s]));
+            }
         }
-        read_raw(i == TN - 1 ? u + 1 : u, i == TN - 1 ? next_stage : stage, (i + 1) % TN, raw[cur ^ 1]);
-        v4i A[2][CH];
-#pragma unroll
-        for (int s = 0; s < CH; ++s) A[0][s] = read_a(stage, 0, s);
+        read_raw(LAST ? u + 1 : u, LAST ? next_stage : stage, (i + 1) % TN, raw);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int j = c / T::PARTS, part = c % T::PARTS;
-            if (c + 1 < CHUNKS) {
-#pragma unroll
-                for (int s = 0; s < CH; ++s) A[(c + 1) & 1][s] = read_a(stage, (c + 1) / T::PARTS, (c + 1) % T::PARTS * CH + s);
-            }
-            v16f P = MX ? acc[i][j] : v16f{};
-#pragma unroll
-            for (int s = 0; s < CH; ++s) P = bmfma(A[c & 1][s], B[cur][part * CH + s], P);
-#pragma unroll
-            for (int s = c * 8 / CHUNKS; s < (c + 1) * 8 / CHUNKS; ++s) B[cur ^ 1][s] = operand(raw[cur ^ 1], s);
+        constexpr int FIRST = 4;  // slots before the codes have arrived
+        auto slot = [&](auto fi) {
+            constexpr int f = decltype(fi)::value, j = f / 8, s = f % 8, part = s / CH;
+            constexpr int g = f + AHEAD;
+            A[g % RING] = g < SLOTS ? read_a(at, g) : read_a(LAST ? at_next : at, g - SLOTS);
             if constexpr (MX) {
-                acc[i][j] = P;
+                acc[i][j] = mfma_bf16(A[f % RING], B[cur][s], acc[i][j]);
             } else {
-                // the chain before: its matrix instructions are done by now
-                const int pc = c == 0 ? CHUNKS - 1 : c - 1, pi = c == 0 ? (i + TN - 1) % TN : i;
+                P = mfma_bf16(A[f % RING], B[cur][s], s % CH == 0 ? v16f{} : P);
+                // 16 / CH sums of the chain before
+                constexpr int pc = f < CH ? SLOTS - 1 : f / CH * CH - 1, pi = f < CH ? (i + TN - 1) % TN : i, pj = pc / 8;
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    acc[pi][pc / T::PARTS][e] = __builtin_fmaf(Pq[e], sq, acc[pi][pc / T::PARTS][e]);
-                Pq = P;
-                sq = raw[cur].s[part];
+                for (int e = s % CH * 16 / CH; e < (s % CH + 1) * 16 / CH; ++e)
+                    acc[pi][pj][e] = __builtin_fmaf(Pq[e], sq, acc[pi][pj][e]);
             }
+            if constexpr (f == FIRST) turn(raw);
+            constexpr int N = SLOTS - FIRST, p0 = f < FIRST ? 0 : (f - FIRST) * 16 / N, p1 = f < FIRST ? 0 : (f - FIRST + 1) * 16 / N;
 #pragma unroll
-            for (int s = 0; s < CH; ++s) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one matrix instruction,
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // one LDS read,
-                __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // eight vector instructions
-            }
+            for (int q = p0; q < p1; ++q) operand_half(raw, q / 2, q % 2, B[cur ^ 1][q / 2]);
+            if constexpr (!MX && s % CH == CH - 1) Pq = P, sq = sc[cur][part];
             __builtin_amdgcn_sched_barrier(0);
+        };
+        for_each_int<SLOTS>(slot);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) sc[cur ^ 1][g] = raw.s[g];
+        if constexpr (LAST) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) at[s] = at_next[s];
+            stage = next_stage;
         }
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
-    auto advance = [&] { stage = stage + 1 == NS ? 0 : stage + 1; };
     if constexpr (TN == 2) {
         for (int u = 0; u < units; ++u) {
             step(u, I0{}, I0{});
             step(u, I1{}, I1{});
-            advance();
         }
     } else {
         int u = 0;
         for (; u + 1 < units; u += 2) {
             step(u, I0{}, I0{});
-            advance();
             step(u + 1, I0{}, I1{});
-            advance();
         }
         if (u < units) step(u, I0{}, I0{});
     }
@@ -265,7 +302,8 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
         for (int j = 0; j < TM; ++j)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const uint32_t v = pk_bf16(acc[i][j][e], acc[i][j][e + 1]);
+                constexpr float unit = MX || T::Z ? 1.0f : 16.0f;  // (sixteenths of the codes)
+                const uint32_t v = pk_bf16(acc[i][j][e] * unit, acc[i][j][e + 1] * unit);
                 const int m = j * 32 + 8 * (e / 4) + 4 * h + e % 4;
                 *reinterpret_cast<HKQ_LDS uint16_t*>(ep + m * T::EP_PITCH + (i * 32 + ln) * 2) = (uint16_t)v;
                 *reinterpret_cast<HKQ_LDS uint16_t*>(ep + (m + 1) * T::EP_PITCH + (i * 32 + ln) * 2) = (uint16_t)(v >> 16);
@@ -310,15 +348,19 @@ static int launch_tile(W4Params& p, hipStream_t stream) {
     return hkq_launch_status();
 }
 
+template <int G, bool Z>
+static int launch_rows(W4Params& p, hipStream_t stream) {
+    const int64_t r = p.M / std::min(p.M, p.E);
+    if (r <= 64) return launch_tile<W4Tile<G, Z, 2, 1, 4>>(p, stream);
+    return launch_tile<W4Tile<G, Z, 4, 2, 3>>(p, stream);
+}
 template <int G>
 static int launch_group(W4Params& p, hipStream_t stream) {
-    const int64_t r = p.M / std::min(p.M, p.E);
-    if (r <= 64) return launch_tile<W4Tile<G, 2, 1, 4>>(p, stream);
-    return launch_tile<W4Tile<G, 4, 2, 3>>(p, stream);
+    return p.Z ? launch_rows<G, true>(p, stream) : launch_rows<G, false>(p, stream);
 }
 
 int launch_w4_tile(W4Params& p, bool mx, hipStream_t stream) {
-    if (mx) return launch_group<0>(p, stream);
+    if (mx) return launch_rows<0, false>(p, stream);
     return p.glog2 == 5 ? launch_group<32>(p, stream) : p.glog2 == 6 ? launch_group<64>(p, stream) : launch_group<128>(p, stream);
 }
 
