@@ -43,21 +43,25 @@ __device__ __forceinline__ v4i int4_operand(uint32_t w, float zero) {
 // The same for zero = 8, as sixteenths (code - 8) / 16: with its upper bit inverted a
 // code is a signed nibble, which v_cvt_off_f32_i4 converts from the low half of any
 // byte. 14 instructions per 8 codes.
-template <int BYTE>
-__device__ __forceinline__ float signed_nibble(uint32_t w) {
-    float v;
-    if constexpr (BYTE == 0) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(v) : "v"(w));
-    if constexpr (BYTE == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(v) : "v"(w));
-    if constexpr (BYTE == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(v) : "v"(w));
-    if constexpr (BYTE == 3) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(v) : "v"(w));
-    return v;
-}
 template <int H>
 __device__ __forceinline__ v2i int4_sixteenths(uint32_t w) {
     const uint32_t ev = w ^ 0x88888888u, od = ev >> 4;
-    return v2i{(int)__builtin_amdgcn_perm(__float_as_uint(signed_nibble<2 * H>(od)), __float_as_uint(signed_nibble<2 * H>(ev)), 0x07060302u),
-               (int)__builtin_amdgcn_perm(__float_as_uint(signed_nibble<2 * H + 1>(od)), __float_as_uint(signed_nibble<2 * H + 1>(ev)),
-                                          0x07060302u)};
+    // (one block: the compiler has no byte select for this conversion, and pads asm
+    // results with wait states that whole-register writes do not need)
+#define HKQ_NIBBLES(B0, B1)                                                           \
+    "v_cvt_off_f32_i4_sdwa %0, %4 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B0 "\n\t" \
+    "v_cvt_off_f32_i4_sdwa %2, %5 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B0 "\n\t" \
+    "v_cvt_off_f32_i4_sdwa %1, %4 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B1 "\n\t" \
+    "v_cvt_off_f32_i4_sdwa %3, %5 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B1 "\n\t" \
+    "v_perm_b32 %0, %2, %0, %6\n\t"                                                   \
+    "v_perm_b32 %1, %3, %1, %6"
+    uint32_t o0, o1, t0, t1;
+    if constexpr (H == 0)
+        asm(HKQ_NIBBLES("BYTE_0", "BYTE_1") : "=&v"(o0), "=&v"(o1), "=&v"(t0), "=&v"(t1) : "v"(ev), "v"(od), "s"(0x07060302u));
+    else
+        asm(HKQ_NIBBLES("BYTE_2", "BYTE_3") : "=&v"(o0), "=&v"(o1), "=&v"(t0), "=&v"(t1) : "v"(ev), "v"(od), "s"(0x07060302u));
+#undef HKQ_NIBBLES
+    return v2i{(int)o0, (int)o1};
 }
 // E2M1 codes 4 H .. 4 H + 3 times 2^(e8m0 - 127), the scale as the fp32 of that exponent.
 template <int H>

@@ -35,14 +35,14 @@ struct W4Tile {
 };
 
 template <int I, int N, class F>
-__device__ __forceinline__ void for_each_from(F& f) {
+__device__ __forceinline__ void for_each_from(F&& f) {
     if constexpr (I < N) {
         f(std::integral_constant<int, I>{});
         for_each_from<I + 1, N>(f);
     }
 }
 template <int N, class F>
-__device__ __forceinline__ void for_each_int(F& f) {
+__device__ __forceinline__ void for_each_int(F&& f) {
     for_each_from<0, N>(f);
 }
 
@@ -104,34 +104,36 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
     // the lane's chunk of the last unit's halves: past K it reads nothing
     const int last_k = (units - 1) * 128 + xc * 8;
     const uint32_t x_tail[2] = {last_k < p.K ? 0u : OOB, last_k + 64 < p.K ? 0u : OOB};
-    // a unit's loads into a stage; past the last they read nothing
-    auto issue = [&](int u, int stage) {
+    // load l of a unit's into a stage; past the last unit they read nothing
+    auto issue = [&](int u, int stage, int l) {
         HKQ_LDS uint8_t* st = smem + stage * T::STAGE;
         const uint32_t dead = u < units ? 0u : OOB;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint32_t none = u + 1 < units ? 0u : x_tail[half] | dead;
-#pragma unroll
-            for (int r = 0; r < T::LX / 2; ++r)
-                lds_load16_s(dx, st + half * BM * 128 + (r * NW + wave) * 1024, x_off[r] | none,
-                             dead ? 0u : (uint32_t)(u * 256 + half * 128));
-        }
-#pragma unroll
-        for (int i = 0; i < T::LW; ++i)
+        if (l < T::LX) {
+            const int half = l / (T::LX / 2), r = l % (T::LX / 2);
+            lds_load16_s(dx, st + half * BM * 128 + (r * NW + wave) * 1024, x_off[r] | (u + 1 < units ? 0u : x_tail[half] | dead),
+                         dead ? 0u : (uint32_t)(u * 256 + half * 128));
+        } else if (l < T::LX + T::LW) {
+            const int i = l - T::LX;
             lds_load16_s(dq, st + T::XB + (i * NW + wave) * 1024, w_off[i] | dead, dead ? 0u : (uint32_t)(u * 64));
-        HKQ_LDS uint8_t* sc = st + T::XB + T::WB + wave * (T::SD + T::ZD) * 256;
-        const uint32_t s0 = ((s_rem + (s_col + (uint32_t)(u * NG)) * SB) & ~3u) | dead;
-#pragma unroll
-        for (int d = 0; d < T::SD; ++d) lds_load4_s(ds, sc + d * 256, s0, 4 * d);
-        const uint32_t z0 = ((z_rem + s_col + (uint32_t)(u * NG)) & ~3u) | dead;
-#pragma unroll
-        for (int d = 0; d < T::ZD; ++d) lds_load4_s(dz, sc + (T::SD + d) * 256, z0, 4 * d);
+        } else {
+            const int d = l - T::LX - T::LW;
+            HKQ_LDS uint8_t* sc = st + T::XB + T::WB + (wave * (T::SD + T::ZD) + d) * 256;
+            if (d < T::SD) lds_load4_s(ds, sc, ((s_rem + (s_col + (uint32_t)(u * NG)) * SB) & ~3u) | dead, 4 * d);
+            else lds_load4_s(dz, sc, ((z_rem + s_col + (uint32_t)(u * NG)) & ~3u) | dead, 4 * (d - T::SD));
+        }
     };
 
     // an n-tile's codes of a unit
+    constexpr int NS_ = MX ? 2 : NG;  // scales of a lane (MXFP4: its block of each half)
     struct Raw {
-        uint32_t w[8];                   // word s: values 16 s + 8 h .. of the unit (MXFP4: 64 (s / 4) + 32 h + 8 (s % 4))
-        float s[NG], z[T::Z ? NG : 1];   // MXFP4: s[half]: the lane's block
+        uint32_t w[8];  // word s: values 16 s + 8 h .. of the unit (MXFP4: 64 (s / 4) + 32 h + 8 (s % 4))
+        uint32_t sb[NS_], zb[T::Z ? NG : 1];  // dwords that hold them
+        float s[NS_], z[T::Z ? NG : 1];
+    };
+    // scales and zero points are bytes at any offset in the staged dwords of the lane's
+    // column: the first group's, of n-tile i and unit u
+    auto scale_at = [&](int u, int i, uint32_t rem, int bytes) {
+        return (rem + ((uint32_t)((wave * TN * 32 + i * 32 + ln) * p.lds) + (uint32_t)(u * NG)) * bytes) & 3;
     };
     auto read_raw = [&](int u, int stage, int i, Raw& r) {
         const HKQ_LDS uint8_t* st = smem + stage * T::STAGE;
@@ -141,30 +143,32 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) r.w[4 * half + q] = (uint32_t)v[q];
         }
-        // scales: bytes at any offset in the staged dwords of the lane's column
-        const int cl = i * 32 + ln;
-        const uint32_t col = (uint32_t)((wave * TN * 32 + cl) * p.lds) + (uint32_t)(u * NG);
-        const HKQ_LDS uint8_t* sc = st + T::XB + T::WB + wave * (T::SD + T::ZD) * 256 + cl * 4;
-        auto bits = [&](const HKQ_LDS uint8_t* at, uint32_t b) {
-            return *reinterpret_cast<const HKQ_LDS uint32_t*>(at + (b >> 2) * 256) >> (8 * (b & 3));
-        };
+        const HKQ_LDS uint8_t* sc = st + T::XB + T::WB + wave * (T::SD + T::ZD) * 256 + (i * 32 + ln) * 4;
+        const uint32_t s0 = scale_at(u, i, s_rem, SB) + (MX ? h : 0), z0 = T::Z ? scale_at(u, i, z_rem, 1) : 0;
 #pragma unroll
-        for (int g = 0; g < (MX ? 2 : NG); ++g) {
-            if constexpr (MX) {
-                const uint32_t e = u * NG + 2 * g + h < groups ? bits(sc, ((s_rem + col) & 3) + 2 * g + h) & 255 : 0u;
-                r.s[g] = e == 255 ? __builtin_nanf("") : exp2i((int)e - 127);
-            } else {
-                const bool live = u * NG + g < groups;
-                const float v = __uint_as_float(bits(sc, ((s_rem + col * 2) & 3) + 2 * g) << 16);
-                r.s[g] = live ? v : 0.0f;
-                if constexpr (T::Z) r.z[g] = (float)(bits(sc + T::SD * 256, ((z_rem + col) & 3) + g) & 255);
-            }
+        for (int g = 0; g < NS_; ++g) r.sb[g] = *reinterpret_cast<const HKQ_LDS uint32_t*>(sc + ((s0 + 2 * g) >> 2) * 256);
+        if constexpr (T::Z) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                r.zb[g] = *reinterpret_cast<const HKQ_LDS uint32_t*>(sc + T::SD * 256 + ((z0 + g) >> 2) * 256);
         }
     };
-    // Values 4 half .. 4 half + 3 of word s as a matrix operand's (INT4 without zero
-    // points: a sixteenth of each). The words of INT4 change places between the lane
-    // halves first (turn), so that an instruction's 16 values lie in one group.
-    auto turn = [&](Raw& r) {
+    // the scales as numbers; the words of INT4 change places between the lane halves, so
+    // that an instruction's 16 values lie in one group
+    auto finish_raw = [&](int u, int i, Raw& r) {
+        const uint32_t s0 = scale_at(u, i, s_rem, SB) + (MX ? h : 0), z0 = T::Z ? scale_at(u, i, z_rem, 1) : 0;
+#pragma unroll
+        for (int g = 0; g < NS_; ++g) {
+            const uint32_t v = r.sb[g] >> (8 * ((s0 + 2 * g) & 3));
+            if constexpr (MX) {
+                const uint32_t e = u * NG + 2 * g + h < groups ? v & 255 : 0u;
+                // 2^(e - 127): the conversion takes the exponent, 0 of a subnormal, 255 of a NaN
+                r.s[g] = __uint_as_float(e << 23 | (e == 255 ? 0x400000u : 0u));
+            } else {
+                r.s[g] = u * NG + g < groups ? __uint_as_float(v << 16) : 0.0f;
+                if constexpr (T::Z) r.z[g] = (float)(r.zb[g] >> (8 * ((z0 + g) & 3)) & 255);
+            }
+        }
         if constexpr (!MX) {
 #pragma unroll
             for (int q = 0; q < 8; q += 4) {
@@ -175,6 +179,8 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
             }
         }
     };
+    // Values 4 half .. 4 half + 3 of word s as a matrix operand's (INT4 without zero
+    // points: a sixteenth of each).
     auto operand_half = [&](const Raw& r, int s, int half, v4i& b) {
         v2i o;
         if constexpr (MX) o = half ? fp4_operand2<1>(r.w[s], r.s[s / 4]) : fp4_operand2<0>(r.w[s], r.s[s / 4]);
@@ -182,7 +188,8 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
         else o = half ? int4_sixteenths<1>(r.w[s]) : int4_sixteenths<0>(r.w[s]);
         b[2 * half] = o[0], b[2 * half + 1] = o[1];
     };
-    // fragment f of a step: values 16 (f % 8) of the unit, m-tile f / 8 (chains of CH: the same order)
+    // fragment f of the rows: values 16 (f % 8) of the unit (chains of CH: the same order),
+    // m-tile f / 8
     uint32_t a_at[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) a_at[s] = (uint32_t)(uintptr_t)smem + (uint32_t)KT::swz(ln, MX ? 4 * h + s : 2 * s + h);
@@ -198,29 +205,27 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
         for (int j = 0; j < TM; ++j) acc[i][j] = v16f{};
 
 #pragma unroll
-    for (int u = 0; u < NS - 1; ++u) issue(u, u);
+    for (int u = 0; u < NS - 1; ++u)
+#pragma unroll
+        for (int l = 0; l < T::NLD; ++l) issue(u, u, l);
     tile_barrier<(NS - 2) * T::NLD>();
-    constexpr int SLOTS = 8 * TM, RING = 8, AHEAD = 6;
-    v4i B[2][8], A[RING];
+    constexpr int SLOTS = 8 * TM;
+    v4i B[2][8], A[SLOTS];
     Raw raw;
-    float sc[2][NG];  // the scales of the operands in B
+    float sc[2][MX ? 2 : NG];  // the scales of the operands in B
     read_raw(0, 0, 0, raw);
-    turn(raw);
+    finish_raw(0, 0, raw);
 #pragma unroll
     for (int s = 0; s < 8; ++s) operand_half(raw, s, 0, B[0][s]), operand_half(raw, s, 1, B[0][s]);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) sc[0][g] = raw.s[g];
+    for (int g = 0; g < NS_; ++g) sc[0][g] = raw.s[g];
     int stage = 0;
-    uint32_t at[4], at_next[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) at[s] = at_next[s] = a_at[s];
-#pragma unroll
-    for (int f = 0; f < AHEAD; ++f) A[f] = read_a(at, f);
+    for_each_int<SLOTS>([&](auto f) { A[decltype(f)::value] = read_a(a_at, decltype(f)::value); });
     v16f P{}, Pq{};  // a chain's sums; the chain's before, and their scale
     float sq = 0.0f;
     // n-tile i of unit u: matrix instructions on B[cur], one per slot, and between them
-    // the fragment reads AHEAD slots on, the sums of the chain before into acc, and the
-    // next n-tile's operands into B[cur ^ 1]
+    // the sums of the chain before into acc, the next n-tile's operands into B[cur ^ 1]
+    // and, at the last n-tile, the next unit's rows in place of those just used
     auto step = [&](int u, auto ii, auto par) {
         constexpr int i = decltype(ii)::value, cur = decltype(par)::value;
         constexpr bool LAST = i == TN - 1;
@@ -232,31 +237,35 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            issue(u + NS - 1, stage == 0 ? NS - 1 : stage - 1);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                at_next[s] = a_at[s] + (uint32_t)(next_stage * T::STAGE);
-                asm volatile("" : "+v"(at_next[s]));
-            }
         }
+        const int refill = stage == 0 ? NS - 1 : stage - 1;
+        uint32_t at[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) at[s] = a_at[s] + (uint32_t)(next_stage * T::STAGE);
         read_raw(LAST ? u + 1 : u, LAST ? next_stage : stage, (i + 1) % TN, raw);
         __builtin_amdgcn_sched_barrier(0);
+        constexpr int LPS = (T::NLD + SLOTS / 2 - 1) / (SLOTS / 2);  // loads per slot, in the step's first half
         constexpr int FIRST = 4;  // slots before the codes have arrived
         auto slot = [&](auto fi) {
             constexpr int f = decltype(fi)::value, j = f / 8, s = f % 8, part = s / CH;
-            constexpr int g = f + AHEAD;
-            A[g % RING] = g < SLOTS ? read_a(at, g) : read_a(LAST ? at_next : at, g - SLOTS);
             if constexpr (MX) {
-                acc[i][j] = mfma_bf16(A[f % RING], B[cur][s], acc[i][j]);
+                acc[i][j] = mfma_bf16(A[f], B[cur][s], acc[i][j]);
             } else {
-                P = mfma_bf16(A[f % RING], B[cur][s], s % CH == 0 ? v16f{} : P);
-                // 16 / CH sums of the chain before
+                P = mfma_bf16(A[f], B[cur][s], s % CH == 0 ? v16f{} : P);
+                // sums of the chain before (whose last instruction is still on its way at s % CH == 0)
                 constexpr int pc = f < CH ? SLOTS - 1 : f / CH * CH - 1, pi = f < CH ? (i + TN - 1) % TN : i, pj = pc / 8;
 #pragma unroll
-                for (int e = s % CH * 16 / CH; e < (s % CH + 1) * 16 / CH; ++e)
+                for (int e = (s % CH - 1) * 16 / (CH - 1); e < s % CH * 16 / (CH - 1); ++e)
                     acc[pi][pj][e] = __builtin_fmaf(Pq[e], sq, acc[pi][pj][e]);
             }
-            if constexpr (f == FIRST) turn(raw);
+            if constexpr (LAST) {
+                A[f] = read_a(at, f);
+#pragma unroll
+                for (int l = f * LPS; l < (f + 1) * LPS && l < T::NLD; ++l) issue(u + NS - 1, refill, l);
+            }
+            // rows live in the accumulation registers: the others are full
+            asm volatile("" : "+a"(A[(f + 1) % SLOTS]));
+            if constexpr (f == FIRST) finish_raw(LAST ? u + 1 : u, (i + 1) % TN, raw);
             constexpr int N = SLOTS - FIRST, p0 = f < FIRST ? 0 : (f - FIRST) * 16 / N, p1 = f < FIRST ? 0 : (f - FIRST + 1) * 16 / N;
 #pragma unroll
             for (int q = p0; q < p1; ++q) operand_half(raw, q / 2, q % 2, B[cur ^ 1][q / 2]);
@@ -265,12 +274,8 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
         };
         for_each_int<SLOTS>(slot);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sc[cur ^ 1][g] = raw.s[g];
-        if constexpr (LAST) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) at[s] = at_next[s];
-            stage = next_stage;
-        }
+        for (int g = 0; g < NS_; ++g) sc[cur ^ 1][g] = raw.s[g];
+        if constexpr (LAST) stage = next_stage;
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
