@@ -107,38 +107,55 @@ __device__ __forceinline__ v4f mfma_bf16_16(const v4i& a, const v4i& b, const v4
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: the weights' way from memory. A workgroup owns 16 MT rows of one group
-// and 16 NT columns; its waves split K in units of 128 values and load their operands
-// straight into registers, D units ahead. Lane c + 16 q of a unit loads 16 bytes (32
-// codes) of column c, values 32 q .. 32 q + 31; INT4 words are then transposed over q,
-// so that each matrix instruction (16 x 16 x 32) takes 32 consecutive values, which
-// lie in one group, and a group's sums are multiplied by its scale. MXFP4 scales go
-// into the operands. The sums of the waves meet in LDS.
+// Few rows: the weights' way from memory. A workgroup owns 16 MT rows (4 XL with MT 1)
+// of one group and 16 NT columns; its waves split K in units of 128 values, of which
+// they hold D (codes) and XD (rows) in registers on their way. The sums of the waves
+// meet in LDS.
+//
+// Loads are made for the memory path and turned in LDS (the wave's own, in order, no
+// barrier): neighbouring lanes load neighbouring 16 bytes, a column's 64 bytes of codes
+// four lanes, where the matrix instruction (16 x 16 x 32) wants lane c + 16 q to hold
+// column c. Loaded as the instruction wants them, 16 columns side by side, each lane's
+// 16 bytes were an access of their own, about 70 cycles a load (1x28672x4096 18.7 us,
+// 16 rows 25.9).
 //
 // D[m][n]: rows of X are the instruction's first operand, so that a lane holds one
-// column's sums and needs one scale per group.
+// column's sums. An instruction takes 32 consecutive values, which lie in one group:
+// INT4 sums are multiplied by the group's scale, MXFP4 scales go into the operands. A
+// wave's scales: one load for four units (lane c + 16 q: column c of unit q), handed to
+// the lanes as each unit is worked on.
 // ---------------------------------------------------------------------------
-template <bool MX, int MT, int NT, int NW, int D>
-__global__ __launch_bounds__(64 * NW) void w4_stream_kernel(const W4Params p) {
-    __shared__ v4f red[NW > 1 ? NW - 1 : 1][MT * NT][64];
+// G: values per group, 0 for MXFP4 (32); Z: zero points
+template <int G, bool Z, int MT, int XL, int NT, int NW, int D, int XD, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void w4_stream_kernel(const W4Params p) {
+    constexpr bool MX = G == 0;
+    constexpr int NG = MX ? 4 : 128 / G, SB = MX ? 1 : 2;  // scales of a unit, bytes of each
+    constexpr int SL = MX ? 1 : NG;                        // registers that hold them (MXFP4: one, four bytes)
+    constexpr int XR = 4 * XL, ROWS = MT == 1 ? XR : 16 * MT;
+    static_assert(MT == 1 || XL == 4, "whole row tiles");
+    constexpr int BUF = (NT + MT * XL) * 1024, RED = MT * NT * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[NW][BUF > RED ? BUF : RED];
     const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     RaggedTile t;
     if (p.offs) {
-        if (!ragged_tile<16 * MT>(p, t)) return;
+        if (!ragged_tile<ROWS>(p, t)) return;
     } else {
         t.e = 0;
         tile_coords(blockIdx.x, p.tiles_m, p.tiles_n, p.group_m, t.m0, t.tn);
-        t.m0 *= 16 * MT;
+        t.m0 *= ROWS;
         t.rows = p.M - t.m0;
     }
     const int n0 = t.tn * 16 * NT, cols = min(p.N - n0, 16 * NT);
     const auto qr = make_rsrc(p.Q + t.e * p.stride_q + n0 * p.ldq, (uint32_t)((cols - 1) * p.ldq + p.K / 2));
-    constexpr int SB = MX ? 1 : 2;  // bytes per scale
     const int groups = p.K >> p.glog2;
-    const auto sr = make_rsrc(p.S + (t.e * p.stride_s + n0 * p.lds) * SB, (uint32_t)(((cols - 1) * p.lds + groups) * SB));
-    const auto zr = make_rsrc(p.Z + (t.e * p.stride_s + n0 * p.lds), p.Z ? (uint32_t)((cols - 1) * p.lds + groups) : 0u);
-    // rows: 32-bit offsets from the tile's first, or (gathered) from X
+    const uint8_t* s_base = p.S + (t.e * p.stride_s + n0 * p.lds) * SB;
+    const auto sr = make_rsrc(s_base, (uint32_t)(((cols - 1) * p.lds + groups) * SB));
+    const auto zr = make_rsrc(p.Z + (t.e * p.stride_s + n0 * p.lds), Z ? (uint32_t)((cols - 1) * p.lds + groups) : 0u);
+    // rows: load l of XL brings pieces (16 bytes) 16 / XL l .. of the unit's 16 of XR rows;
+    // 32-bit offsets from the tile's first row, or (gathered) from X
+    constexpr int PL = 16 / XL;
+    const int xrow = lane / PL, xpiece = lane % PL;
     uint32_t x_off[MT];
     const uint8_t* x0 = p.X;
     uint32_t x_bytes;
@@ -146,142 +163,242 @@ __global__ __launch_bounds__(64 * NW) void w4_stream_kernel(const W4Params p) {
         x_bytes = (uint32_t)((p.T - 1) * p.ldx + p.K * 2);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const int r = 16 * i + c;
+            const int r = 16 * i + xrow;
             const int id = r < t.rows ? p.gather[t.m0 + r] : -1;
             const int row = id < 0 ? -1 : id / p.topk;
             x_off[i] = row >= 0 && row < p.T ? (uint32_t)(row * p.ldx) : OOB;
         }
     } else {
         x0 += t.m0 * p.ldx;
-        x_bytes = (uint32_t)((min(t.rows, 16 * MT) - 1) * p.ldx + p.K * 2);
+        x_bytes = (uint32_t)((min(t.rows, ROWS) - 1) * p.ldx + p.K * 2);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) x_off[i] = 16 * i + c < t.rows ? (uint32_t)((16 * i + c) * p.ldx) : OOB;
+        for (int i = 0; i < MT; ++i) x_off[i] = 16 * i + xrow < t.rows ? (uint32_t)((16 * i + xrow) * p.ldx) : OOB;
     }
     const auto xr = make_rsrc(x0, x_bytes);
 
+    // LDS: codes piece k of column r in 16-byte slot 4 r + (k ^ r / 4), rows' piece 4 j + kg
+    // of row r in slot 4 (XR j + r) + (kg ^ r / 4): the 16 lanes of a read fall on all banks
+    HKQ_LDS uint8_t* lw = (HKQ_LDS uint8_t*)smem[wave];
+    HKQ_LDS uint8_t* lx = lw + NT * 1024;
+    HKQ_LDS uint8_t* w_put = lw + (lane / 4 * 4 + ((lane & 3) ^ (lane >> 4))) * 16;
+    HKQ_LDS uint8_t *w_get[4], *x_put[XL], *x_get;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w_get[j] = lw + (c * 4 + (j ^ (c >> 2))) * 16 + q * 4;
+#pragma unroll
+    for (int l = 0; l < XL; ++l) {
+        const int piece = l * PL + xpiece;
+        x_put[l] = lx + ((piece / 4 * XR + xrow) * 4 + (piece % 4 ^ (xrow >> 2))) * 16;
+    }
+    x_get = lx + (c % XR * 4 + (q ^ (c % XR >> 2))) * 16;
+
     const int units = (p.K + 127) / 128, u0 = wave * units / NW, u1 = (wave + 1) * units / NW;
-    struct Unit {
-        v4i w[NT], x[MT][4];
-        uint32_t s[NT][MX ? 1 : 4], z[NT][MX ? 1 : 4];
+    struct Codes {
+        v4i w[NT];
     };
-    auto load = [&](int u, Unit& f) {
-        const int k = u * 128 + 32 * q;  // the lane's first value
-        const bool live = u < u1;
+    struct Rows {
+        v4i x[MT][XL];
+    };
+    const uint32_t w_lane = (uint32_t)(lane / 4 * p.ldq + (lane & 3) * 16);
+    auto load_codes = [&](int u, Codes& f, int i) {  // of n-tile i
+        const bool live = u < u1 && u * 128 + 32 * (lane & 3) < p.K;
+        f.w[i] = __builtin_amdgcn_raw_buffer_load_b128(qr, live ? w_lane + (uint32_t)(16 * i * p.ldq + u * 64) : OOB, 0, 0);
+    };
+    auto load_rows = [&](int u, Rows& f) {
+#pragma unroll
+        for (int l = 0; l < XL; ++l) {
+            const int kx = u * 128 + 8 * (l * PL + xpiece);
+            const bool live = u < u1 && kx < p.K;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                f.x[i][l] = __builtin_amdgcn_raw_buffer_load_b128(xr, live && x_off[i] != OOB ? x_off[i] + (uint32_t)(kx * 2) : OOB, 0, 0);
+        }
+    };
+    // scales and zero points of units u .. u + 3: lane c + 16 q those of unit u + q
+    struct Four {
+        uint32_t s[NT][SL], z[Z ? NT : 1][Z ? NG : 1];
+    };
+    const bool dwords = MX && ((reinterpret_cast<uintptr_t>(s_base) | (uintptr_t)p.lds | (uintptr_t)groups) & 3) == 0;
+    auto load_scales = [&](int u, Four& f) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const int n = 16 * i + c;
-            f.w[i] = __builtin_amdgcn_raw_buffer_load_b128(qr, live && k < p.K ? (uint32_t)(n * p.ldq + k / 2) : OOB, 0, 0);
-            if constexpr (MX) {
-                f.s[i][0] = __builtin_amdgcn_raw_buffer_load_b8(sr, live && k < p.K ? (uint32_t)(n * p.lds + k / 32) : OOB, 0, 0);
-            } else {
-                // the scale of each matrix instruction's 32 values: one load per group
+            const int at = (u + q) * NG, col = (16 * i + c) * (int)p.lds;
+            if (MX && dwords) {
+                f.s[i][0] = __builtin_amdgcn_raw_buffer_load_b32(sr, u + q < u1 ? (uint32_t)(col + at) : OOB, 0, 0);
+                continue;
+            }
+            if constexpr (MX) f.s[i][0] = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int g = u * 128 + 32 * j;
-                    if (j > 0 && (p.glog2 == 7 || (p.glog2 == 6 && (j & 1)))) {
-                        f.s[i][j] = f.s[i][j - 1], f.z[i][j] = f.z[i][j - 1];
-                        continue;
-                    }
-                    const uint32_t at = live && g < p.K ? (uint32_t)(n * p.lds + (g >> p.glog2)) : OOB;
-                    f.s[i][j] = __builtin_amdgcn_raw_buffer_load_b16(sr, at == OOB ? OOB : at * 2, 0, 0);
-                    f.z[i][j] = p.Z ? __builtin_amdgcn_raw_buffer_load_b8(zr, at, 0, 0) : 8;
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t off = u + q < u1 && at + g < groups ? (uint32_t)(col + at + g) : OOB;
+                if constexpr (MX) {
+                    f.s[i][0] |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(sr, off, 0, 0) << (8 * g);
+                } else {
+                    f.s[i][g] = __builtin_amdgcn_raw_buffer_load_b16(sr, off == OOB ? OOB : off * 2, 0, 0);
+                    if constexpr (Z) f.z[i][g] = __builtin_amdgcn_raw_buffer_load_b8(zr, off, 0, 0);
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int kx = u * 128 + (MX ? 32 * q + 8 * j : 32 * j + 8 * q);
-                f.x[i][j] = __builtin_amdgcn_raw_buffer_load_b128(
-                    xr, live && kx < p.K && x_off[i] != OOB ? x_off[i] + (uint32_t)(kx * 2) : OOB, 0, 0);
-            }
     };
     v4f acc[MT][NT] = {};
-    auto work = [&](const Unit& f) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            uint32_t w[4] = {(uint32_t)f.w[i][0], (uint32_t)f.w[i][1], (uint32_t)f.w[i][2], (uint32_t)f.w[i][3]};
-            if constexpr (MX) {
-                const float s = exp2i((int)f.s[i][0] - 127);
-                const float s0 = f.s[i][0] == 255 ? __builtin_nanf("") : s;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const v4i b = fp4_operand(w[j], s0);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[m][i] = mfma_bf16_16(f.x[m][j], b, acc[m][i]);
-                }
-            } else {
-                swap32(w[0], w[2]);
-                swap32(w[1], w[3]);
-                swap16(w[0], w[1]);
-                swap16(w[2], w[3]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const v4i b = int4_operand(w[j], (float)f.z[i][j]);
-                    const float s = bf16_to_f32(f.s[i][j]);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const v4f P = mfma_bf16_16(f.x[m][j], b, v4f{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[m][i][e] = __builtin_fmaf(P[e], s, acc[m][i][e]);
-                    }
-                }
-            }
-        }
-    };
-    Unit ring[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(u0 + d, ring[d]);
-    for (int u = u0; u < u1; u += D) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            if (u + d < u1) work(ring[d]);
-            load(u + d + D, ring[d]);
-        }
-    }
-    if (wave > 0) {
+    // unit u, place d in its four; the registers take unit u + D's codes and u + XD's rows
+    // once they are in LDS
+    auto work = [&](int u, Codes& f, Rows& xs, const Four& sc, int d) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) red[wave - 1][m * NT + i][lane] = acc[m][i];
+            for (int l = 0; l < XL; ++l) *reinterpret_cast<HKQ_LDS v4i*>(x_put[l] + m * XL * 1024) = xs.x[m][l];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) *reinterpret_cast<HKQ_LDS v4i*>(w_put + i * 1024) = f.w[i];
+        load_rows(u + XD, xs);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) load_codes(u + D, f, i);
+        v4i x[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[m][j] = lds_read16(x_get + m * XL * 1024 + j * XR * 64);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const HKQ_LDS uint32_t*>(w_get[j] + i * 1024);
+            v4f P[MT];
+            float s[NG], z[NG];
+            uint32_t v[SL];
+#pragma unroll
+            for (int g = 0; g < SL; ++g) {
+                v[g] = MX ? sc.s[i][g] : sc.s[i][g] << 16;
+                if constexpr (Z) v[g] |= sc.z[i][g];
+                v[g] = (uint32_t)__builtin_amdgcn_ds_bpermute((c + 16 * d) * 4, (int)v[g]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if constexpr (MX) {
+                    const uint32_t e = v[0] >> (8 * g) & 255;
+                    s[g] = __uint_as_float(e << 23 | (e == 255 ? 0x400000u : 0u));
+                } else {
+                    if constexpr (Z) z[g] = (float)(v[g] & 255);
+                    s[g] = __uint_as_float(Z ? v[g] & 0xFFFF0000u : v[g]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v4i b;
+                if constexpr (MX) {
+                    b = fp4_operand(w[j], s[j]);
+                } else if constexpr (Z) {
+                    b = int4_operand(w[j], z[j * NG / 4]);
+                } else {
+                    const v2i lo = int4_sixteenths<0>(w[j]), hi = int4_sixteenths<1>(w[j]);
+                    b = v4i{lo[0], lo[1], hi[0], hi[1]};
+                }
+                const bool first = !MX && j % (4 / NG) == 0, last = !MX && (j + 1) % (4 / NG) == 0;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if constexpr (MX) {
+                        acc[m][i] = mfma_bf16_16(x[m][j], b, acc[m][i]);
+                    } else {
+                        P[m] = mfma_bf16_16(x[m][j], b, first ? v4f{0.f, 0.f, 0.f, 0.f} : P[m]);
+                        if (last) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[m][i][e] = __builtin_fmaf(P[m][e], s[j * NG / 4], acc[m][i][e]);
+                        }
+                    }
+                }
+            }
+        }
+    };
+    static_assert(4 % D == 0 && 4 % XD == 0, "whole rings per four units");
+    Codes codes[D];
+    Rows rows[XD];
+    Four sc;
+    load_scales(u0, sc);
+#pragma unroll
+    for (int d = 0; d < (D > XD ? D : XD); ++d) {
+        if (d < XD) load_rows(u0 + d, rows[d]);
+        if (d < D) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) load_codes(u0 + d, codes[d], i);
+        }
     }
-    __syncthreads();
-    if (wave > 0) return;
+    for (int u = u0; u < u1; u += 4) {
+        Four next;
+        load_scales(u + 4, next);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            if (u + d >= u1) break;
+            work(u + d, codes[d % D], rows[d % XD], sc, d);
+        }
+        sc = next;
+    }
+    // the waves' sums: each in its own area, added in wave order; tile o by wave o % NW
+    v4f* red = reinterpret_cast<v4f*>(smem[wave]);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            v4f v = acc[m][i];
+        for (int i = 0; i < NT; ++i) red[(m * NT + i) * 64 + lane] = acc[m][i];
+    __syncthreads();
+    constexpr float unit = MX || Z ? 1.0f : 16.0f;  // (sixteenths of the codes)
+    for (int o = wave; o < MT * NT; o += NW) {
+        v4f v = reinterpret_cast<const v4f*>(smem[0])[o * 64 + lane];
 #pragma unroll
-            for (int o = 0; o < NW - 1; ++o) v = v + red[o][m * NT + i][lane];
-            const int n = 16 * i + c;
+        for (int w = 1; w < NW; ++w) v = v + reinterpret_cast<const v4f*>(smem[w])[o * 64 + lane];
+        const int m = o / NT, n = 16 * (o % NT) + c;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 16 * m + 4 * q + e;
-                if (r < t.rows && n < cols) p.C[(int64_t)(t.m0 + r) * p.ldc + n0 + n] = (uint16_t)f32_to_bf16(v[e]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int r = 16 * m + 4 * q + e;
+            if (4 * q + e < XR && r < t.rows && n < cols)
+                p.C[(int64_t)(t.m0 + r) * p.ldc + n0 + n] = (uint16_t)f32_to_bf16(v[e] * unit);
         }
+    }
 }
 
-template <bool MX, int MT, int NT, int NW, int D>
+template <int G, bool Z, int MT, int XL, int NT, int NW, int D, int XD, int OCC>
 static int launch_w4_stream(W4Params& p, hipStream_t stream) {
-    p.tiles_m = (int)ragged_most(p.M, p.E, 16 * MT);
+    p.tiles_m = (int)ragged_most(p.M, p.E, MT == 1 ? 4 * XL : 16 * MT);
     p.tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
     p.group_m = 8;
     const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
     HKQ_CHECK_ARG(blocks < (1 << 23), "too many tiles for one launch");
-    w4_stream_kernel<MX, MT, NT, NW, D><<<(unsigned)blocks, 64 * NW, 0, stream>>>(p);
+    w4_stream_kernel<G, Z, MT, XL, NT, NW, D, XD, OCC><<<(unsigned)blocks, 64 * NW, 0, stream>>>(p);
     return hkq_launch_status();
 }
 
-template <bool MX>
-static int run_w4(W4Params& p, hipStream_t stream) {
-    const int64_t r = p.M / std::min(p.M, p.E);
-    if (r <= 4) return launch_w4_stream<MX, 1, 1, 8, 2>(p, stream);
-    if (r <= 16) return launch_w4_stream<MX, 1, 2, 8, 2>(p, stream);
-    if (r <= 32) return launch_w4_stream<MX, 2, 2, 8, 1>(p, stream);
-    return launch_w4_tile(p, MX, stream);
+// Rows per group r (the mean) and columns. A row tile of r rows; more columns per
+// workgroup once there are workgroups enough, so that a unit's rows are fetched for more
+// columns: us at M x N x K, zero points, 1 | 2 | 4 column tiles: 16x4096x4096 6.1 | 7.8 |
+// 11.4, 16x28672x4096 28.2 | 25.0 | 21.5, 6x28672x4096 23.9 | 20.2; MXFP4 16x28672x4096
+// 27.8 | 22.8 | 17.9. Up to four rows, one column tile: eight waves 1x4096x14336 10.5,
+// 1x28672x4096 20.7, four waves 13.1 and 17.4.
+template <int G, bool Z>
+static int run_w4_stream(W4Params& p, int64_t r, hipStream_t stream) {
+    const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
+    const bool many = std::min(p.M, p.E) * ((p.N + 15) / 16) > 3 * ncu;
+    if (r <= 4)
+        return many ? launch_w4_stream<G, Z, 1, 1, 1, 4, 4, 4, 4>(p, stream) : launch_w4_stream<G, Z, 1, 1, 1, 8, 4, 4, 4>(p, stream);
+    if (r <= 8)
+        return many ? launch_w4_stream<G, Z, 1, 2, 2, 8, 2, 2, 4>(p, stream) : launch_w4_stream<G, Z, 1, 2, 1, 8, 2, 2, 4>(p, stream);
+    if (r <= 16)
+        return many ? launch_w4_stream<G, Z, 1, 4, 4, 8, 1, 1, 4>(p, stream) : launch_w4_stream<G, Z, 1, 4, 1, 8, 2, 2, 4>(p, stream);
+    return launch_w4_stream<G, Z, 2, 4, 1, 8, 2, 1, 4>(p, stream);
+}
+template <int G>
+static int run_w4_group(W4Params& p, int64_t r, hipStream_t stream) {
+    return p.Z ? run_w4_stream<G, true>(p, r, stream) : run_w4_stream<G, false>(p, r, stream);
+}
+
+// Streamed or tiled. Up to 16 rows per group the stream reads a weight once; beyond, it
+// does so once per 32 rows, in 5.8 us per 8192 units of K (128 values of 16 columns), and
+// the tiles of 64 rows and 128 columns take 0.8 us per unit and round of them over the
+// CUs, a unit's chain of waits (32x4096x4096 8.7 and 26, 64x28672x4096 85 and 28.7).
+static int run_w4(W4Params& p, bool mx, hipStream_t stream) {
+    const int64_t live = std::min(p.M, p.E), r = p.M / live, ncu = cu_count() > 0 ? cu_count() : 256, units = (p.K + 127) / 128;
+    const int64_t streams = live * ((r + 31) / 32) * ((p.N + 15) / 16), tiles = live * ((r + 63) / 64) * ((p.N + 127) / 128);
+    const double us_stream = 3.0 + (double)std::max(streams, ncu) * units * (5.8 / 8192),
+                 us_tile = 3.0 + (double)((tiles + ncu - 1) / ncu) * units * 0.8;
+    if (r > 16 && us_tile < us_stream) return launch_w4_tile(p, mx, stream);
+    if (mx) return run_w4_stream<0, false>(p, r, stream);
+    return p.glog2 == 5 ? run_w4_group<32>(p, r, stream) : p.glog2 == 6 ? run_w4_group<64>(p, r, stream) : run_w4_group<128>(p, r, stream);
 }
 
 static int check_w4_weights(int64_t N, int64_t K, int64_t ldq, int64_t lds, int64_t group) {
@@ -385,7 +502,7 @@ static int w4_product(const void* X, const void* Q, const void* S, const void* Z
     p.stride_q = stride_q; p.stride_s = stride_s;
     p.glog2 = group == 32 ? 5 : group == 64 ? 6 : 7;
     p.topk = gather ? (int)topk : 1;
-    return mx ? run_w4<true>(p, stream) : run_w4<false>(p, stream);
+    return run_w4(p, mx, stream);
 }
 
 extern "C" size_t hkq_gemm_w4a16_workspace(int64_t, int64_t, int64_t) { return 0; }
