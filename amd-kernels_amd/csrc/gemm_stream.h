@@ -38,9 +38,16 @@ struct StreamSrc {
 //   the tile's epilogue scales; loads it issues are waited for by the loop's
 //   next barrier), end(t, acc) after tile t's last MFMA has drained; it must
 //   not touch the LDS ring. On return every wave is past a vmcnt(0) barrier.
+// A Seq with VARIES gives each tile its own K: kt(t) K-tiles (even, at least 4), of
+// which kt_live(t) hold something and the rest read zeros (AT and bf16 BT operands).
 // BT: B tiles N-contiguous (KTileT layout, transposed fragment reads; the
 // sequence then provides b_kstep, the bytes from one K-tile of B to the next).
 // GATED, AT, bf16 BT: as in gemm_mainloop.
+template <class S, class = void>
+struct SeqVaries : std::false_type {};
+template <class S>
+struct SeqVaries<S, std::void_t<decltype(S::VARIES)>> : std::true_type {};
+
 template <int MODE, int WAVES_M, int WAVES_N, int TM, int TN, bool BT = false, bool AT = false, bool GATED = false,
           typename AOff, typename BOff, typename Seq, typename Epi>
 __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const BOff& b_off, HKQ_LDS uint8_t* smem,
@@ -60,7 +67,10 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
     static_assert(!BT || BT16 || (Cfg::BN == KTileT::ROW && MODE == MODE_A8W8), "N-contiguous B: FP8 tiles of 256 columns");
     static_assert(!AT || MODE == MODE_BF16, "M-contiguous A: bf16");
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-    const int KTN = seq.KT;
+    constexpr bool VARIES = SeqVaries<Seq>::value;
+    int KTN, ld_kt = 0;  // VARIES: K-tiles of the tile that `ld` reads that hold something
+    if constexpr (VARIES) KTN = seq.kt(0), ld_kt = seq.kt_live(0);
+    else KTN = seq.KT;
 
     // Loads run NS K-tiles (data) and NS + SB_KT - 1 scale units (MXFP4) ahead
     // of the compute, so near the end of a tile they read the next tile: `ld`
@@ -117,8 +127,9 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
     v4i t16_a, t16_b;
     T16Cursor cur_a{ld.ta.base}, cur_b{ld.tb.base};
     auto t16_next = [&](int kl) {
-        if constexpr (AT) t16_a = cur_a.next(ld.ta, kl, ld_live ? KTN : 0);
-        if constexpr (BT16) t16_b = cur_b.next(ld.tb, kl, ld_live ? KTN : 0);
+        const int kt = VARIES ? ld_kt : KTN;
+        if constexpr (AT) t16_a = cur_a.next(ld.ta, kl, ld_live ? kt : 0);
+        if constexpr (BT16) t16_b = cur_b.next(ld.tb, kl, ld_live ? kt : 0);
     };
 
     // load instruction idx of K-tile kl of `ld` into `stage`; MXFP4: scale
@@ -336,6 +347,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
     using F0 = std::false_type;
     for (int t = 0; t < seq.tiles; ++t) {
         cur = t;
+        if constexpr (VARIES) KTN = seq.kt(t);
         if (t > 0) {
             epi.begin(t);
             // K-tile 1's loads went out before the previous tile's epilogue:
@@ -374,6 +386,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         ld = seq.src(min(t + 1, seq.tiles - 1));
         cur_a.at = ld.ta.base;
         cur_b.at = ld.tb.base;
+        if constexpr (VARIES) ld_kt = seq.kt_live(min(t + 1, seq.tiles - 1));
         if constexpr (Seq::GATHER) seq.a_rows(min(t + 1, seq.tiles - 1), a_off);
         ktile(KTN - 2, Q2{}, F0{}, F0{});
         ktile(KTN - 1, Q3{}, F0{}, std::true_type{});

@@ -141,25 +141,25 @@ __global__ __launch_bounds__(256, 1) void grouped_whole_kernel(const GroupedPara
 struct DwTile {
     int e, m0, n0, start, rows;
 };
-template <int BM, int BN>
-__device__ __forceinline__ DwTile dw_tile(const GroupedParams& p) {
-    const int per = p.tiles_m * p.tiles_n, id = xcd_order(blockIdx.x, per * p.E);
+template <int BM, int BN, class Rows>
+__device__ __forceinline__ DwTile dw_tile(const GroupedParams& p, int id, Rows group) {
+    const int per = p.tiles_m * p.tiles_n;
     DwTile t;
     t.e = id / per;
-    const int in = id - t.e * per, group = p.group_m * p.tiles_n, first = in / group * p.group_m,
-              size = min(p.tiles_m - first, p.group_m), at = in % group;
-    t.m0 = (first + at % size) * BM;
-    t.n0 = at / size * BN;
-    const int2 r = group_rows(p, t.e);
-    t.start = r.x;
-    t.rows = r.y - r.x;
+    // every group's tiles over all XCDs: groups differ in rows
+    tile_coords(id - t.e * per, p.tiles_m, p.tiles_n, p.group_m, t.m0, t.n0);
+    t.m0 *= BM;
+    t.n0 *= BN;
+    const int2 r = group(t.e);
+    t.start = __builtin_amdgcn_readfirstlane(r.x);
+    t.rows = __builtin_amdgcn_readfirstlane(r.y) - t.start;
     return t;
 }
 template <class Cfg, int MINB>
 __global__ __launch_bounds__(Cfg::THREADS, MINB) void grouped_dw_small_kernel(const GroupedParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
     HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
-    const DwTile t = dw_tile<Cfg::BM, Cfg::BN>(p);
+    const DwTile t = dw_tile<Cfg::BM, Cfg::BN>(p, blockIdx.x, [&](int e) { return group_rows(p, e); });
     v16f acc[Cfg::TN][Cfg::TM];
     small_tile<true, true, Cfg>(p.A + t.start * p.lda + t.m0 * 2, p.B + t.start * p.ldb + t.n0 * 2, p.lda, p.ldb,
                                 min(p.K - t.m0, Cfg::BM), min(p.N - t.n0, Cfg::BN), t.rows, smem, acc);
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(Cfg::THREADS, MINB) void grouped_dw_small_kernel(co
 __global__ __launch_bounds__(256, 1) void grouped_dw_whole_kernel(const GroupedParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
     HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
-    const DwTile t = dw_tile<DENSE_BM, DENSE_BN>(p);
+    const DwTile t = dw_tile<DENSE_BM, DENSE_BN>(p, blockIdx.x, [&](int e) { return group_rows(p, e); });
     v16f acc[DENSE_TN][DENSE_TM];
     whole_tile<true, true>(p.A + t.start * p.lda + t.m0 * 2, p.B + t.start * p.ldb + t.n0 * 2, p.lda, p.ldb,
                            min(p.K - t.m0, DENSE_BM), min(p.N - t.n0, DENSE_BN), t.rows, smem, acc);
@@ -180,6 +180,217 @@ __global__ __launch_bounds__(256, 1) void grouped_dw_whole_kernel(const GroupedP
     store_tile_bf16<DENSE_TM, DENSE_TN>(acc, smem, wave, threadIdx.x & 63, p.C + t.e * p.stride_e, p.ldc, p.K, p.N,
                                         t.m0 + wave / DENSE_WAVES_N * DENSE_TM * 32, t.n0 + wave % DENSE_WAVES_N * DENSE_TN * 32,
                                         p.c16 != 0, NoScale{}, NoScale{}, NoBias{});
+}
+
+// ---------------------------------------------------------------------------
+// Large groups: one workgroup per CU computes its 256 x 256 tiles as one stream of
+// K-tiles (gemm_stream.h), so that a tile's stores run under the next one's loads. The
+// groups' tile counts go to LDS at the start, where each tile's group is looked up.
+// ---------------------------------------------------------------------------
+constexpr int STREAM_GROUPS = 512;  // groups that the LDS table holds
+constexpr int STREAM_TABLE = stream_stg_off<PlainOp, MODE_BF16>() + DENSE_WAVES_M * DENSE_WAVES_N * STREAM_STG;
+constexpr int STREAM_LDS = STREAM_TABLE + 3 * STREAM_GROUPS * 4 + 16;
+static_assert(STREAM_LDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
+
+struct GroupTable {
+    HKQ_LDS int *end, *row0, *row1;  // row tiles up to the group's end, its rows
+    int E;
+    // fills the table; the tiles of all groups (every wave; ends in a barrier)
+    __device__ int fill(const GroupedParams& p, HKQ_LDS uint8_t* at) {
+        end = reinterpret_cast<HKQ_LDS int*>(at);
+        row0 = end + STREAM_GROUPS;
+        row1 = row0 + STREAM_GROUPS;
+        E = p.E;
+        HKQ_LDS int* total = row1 + STREAM_GROUPS;
+        if (threadIdx.x < 64) {
+            const int lane = threadIdx.x;
+            int before = 0;
+            for (int e0 = 0; e0 < E; e0 += 64) {
+                const int e = e0 + lane;
+                int2 r = make_int2(0, 0);
+                if (e < E) r = group_rows(p, e);
+                int s = (r.y - r.x + DENSE_BM - 1) / DENSE_BM;
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) {
+                    const int o = __shfl_up(s, d, 64);
+                    if (lane >= d) s += o;
+                }
+                if (e < E) end[e] = before + s, row0[e] = r.x, row1[e] = r.y;
+                before += __builtin_amdgcn_readlane(s, 63);
+            }
+            if (lane == 0) *total = min(before, p.tiles_m);  // bounds that count a row twice: the most there can be
+        }
+        __syncthreads();
+        return __builtin_amdgcn_readfirstlane(*total);
+    }
+    // tile id of total * tiles_n: its group, first row and the group's rows from there on,
+    // and its column tile
+    __device__ __forceinline__ void find(const GroupedParams& p, int id, int total, int& e, int& m0, int& rows, int& tn) const {
+        const int lane = threadIdx.x & 63;
+        id = xcd_order(id, total * p.tiles_n);
+        const int at = id / p.tiles_n;
+        e = 0;
+        for (int e0 = 0; e0 < E; e0 += 64) {
+            const uint64_t past = __ballot(e0 + lane < E && end[min(e0 + lane, E - 1)] > at);
+            if (past) {
+                e = e0 + __builtin_ctzll(past);
+                break;
+            }
+        }
+        const int r0 = __builtin_amdgcn_readfirstlane(row0[e]), r1 = __builtin_amdgcn_readfirstlane(row1[e]);
+        const int tiles = max(1, (r1 - r0 + DENSE_BM - 1) / DENSE_BM), first = __builtin_amdgcn_readfirstlane(end[e]) - tiles;
+        int tm;
+        group_tile(id - first * p.tiles_n, tiles, p.tiles_n, p.group_m, tm, tn);
+        m0 = r0 + tm * DENSE_BM;
+        rows = r1 - m0;
+    }
+};
+
+template <bool BT>
+struct RaggedSeq {
+    static constexpr bool GATHER = false;
+    const GroupedParams* p;
+    GroupTable table;
+    int tiles, KT;
+    uint32_t lsa, lsb;
+    int total, first, stride;
+    __device__ void at(int k, int& e, int& m0, int& rows, int& n0) const {
+        table.find(*p, first + k * stride, total, e, m0, rows, n0);
+        n0 *= DENSE_BN;
+    }
+    __device__ StreamSrc src(int k) const {
+        int e, m0, rows, n0;
+        at(k, e, m0, rows, n0);
+        const int cols = min(p->N - n0, DENSE_BN);
+        StreamSrc s{};
+        s.a = p->A + m0 * p->lda;
+        s.a_bytes = clamp_bytes((int64_t)(min(rows, DENSE_BM) - 1) * p->lda + p->K * 2);
+        s.b = p->B + e * p->stride_e + (BT ? n0 * 2 : n0 * p->ldb);
+        s.b_bytes = clamp_bytes((int64_t)(cols - 1) * p->ldb + p->K * 2);
+        if constexpr (BT) s.tb = T16Src::of(s.b, p->ldb, cols, 0, p->K, KT);
+        return s;
+    }
+};
+struct DwSeq {
+    static constexpr bool GATHER = false, VARIES = true;
+    const GroupedParams* p;
+    GroupTable table;
+    int tiles, KT;
+    uint32_t lsa, lsb;
+    int first, stride;
+    __device__ DwTile at(int k) const {
+        return dw_tile<DENSE_BM, DENSE_BN>(*p, first + k * stride, [&](int e) { return make_int2(table.row0[e], table.row1[e]); });
+    }
+    __device__ int kt_live(int k) const { return (at(k).rows + 63) / 64; }
+    __device__ int kt(int k) const { return max(4, (kt_live(k) + 1) / 2 * 2); }
+    __device__ StreamSrc src(int k) const {
+        const DwTile t = at(k);
+        const int n = (t.rows + 63) / 64;
+        StreamSrc s{};
+        s.ta = T16Src::of(p->A + t.start * p->lda + t.m0 * 2, p->lda, min(p->K - t.m0, DENSE_BM), 0, t.rows, n);
+        s.tb = T16Src::of(p->B + t.start * p->ldb + t.n0 * 2, p->ldb, min(p->N - t.n0, DENSE_BN), 0, t.rows, n);
+        return s;
+    }
+};
+template <bool DW, class Seq>
+struct GroupedEpi {
+    static constexpr int TM = DENSE_TM, TN = DENSE_TN, VM_ISSUED = TN * TM * 2;
+    const Seq* seq;
+    HKQ_LDS uint8_t* stg;
+    int lane, wave;
+    __device__ void begin(int) {}
+    __device__ void end(int k, v16f (&acc)[TN][TM]) {
+        const GroupedParams& p = *seq->p;
+        const int mw = wave / DENSE_WAVES_N * TM * 32, nw = wave % DENSE_WAVES_N * TN * 32;
+        uint16_t* c;
+        int rows, cols;
+        if constexpr (DW) {
+            const DwTile t = seq->at(k);
+            c = p.C + t.e * p.stride_e + t.m0 * p.ldc + t.n0;
+            rows = p.K - t.m0, cols = p.N - t.n0;
+        } else {
+            int e, m0, n0;
+            seq->at(k, e, m0, rows, n0);
+            c = p.C + m0 * p.ldc + n0;
+            cols = p.N - n0;
+        }
+        float one[TM];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) one[j] = 1.0f;
+        stream_store_tile<TM, TN>(acc, stg, c + mw * p.ldc + nw, p.ldc, rows - mw, cols - nw, one,
+                                  [](int, int) { return v4f{1.f, 1.f, 1.f, 1.f}; }, lane);
+    }
+};
+
+// The M half `half` of row tile (e, m0), column tile n0.
+template <bool BT>
+__device__ __forceinline__ void grouped_half(const GroupedParams& p, int e, int m0, int rows, int n0, int half, HKQ_LDS uint8_t* smem) {
+    using Op = TransOp<false, BT>;
+    using Half = DenseCfg<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM / 2, DENSE_TN, 128>;
+    DenseParams d{};
+    d.A = p.A + m0 * p.lda;
+    d.B = p.B + e * p.stride_e;
+    d.C = p.C + m0 * p.ldc;
+    d.M = rows; d.N = p.N; d.K = p.K; d.kbytes = p.K * 2;
+    d.lda = p.lda; d.ldb = p.ldb; d.ldc = p.ldc;
+    d.c16 = p.c16;
+    dense_rows<Op, MODE_BF16, DENSE_TM / 2, 128, HALF_NS, Half::lds_bytes(HALF_NS)>(d, half * Half::BM, n0, smem);
+}
+
+// Where the last round of tiles would leave half of the CUs idle or more, its tiles run
+// as M halves, by workgroups b with b / 16 * 8 + b % 8 the tile and b / 8 % 2 the half
+// (both on one XCD); every second one takes its half first, so that the tiles' ends fall
+// between the others'.
+template <bool BT>
+__global__ __launch_bounds__(256, 1) void grouped_stream_kernel(const GroupedParams p) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
+    HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    GroupTable table;
+    const int total = table.fill(p, smem + STREAM_TABLE);
+    const int b = blockIdx.x, G = gridDim.x, tiles = total * p.tiles_n, last = tiles % G;
+    const int split = last > 0 && (last + 7) / 8 * 16 <= G ? last : 0, whole = tiles - split;
+    const int mine = b < whole ? (whole - 1 - b) / G + 1 : 0;
+    const int t = 8 * (b >> 4) + (b & 7);
+    const bool half_first = (b >> 4) & 1, has_half = t < split;
+    auto run_half = [&] {
+        int e, m0, rows, tn;
+        table.find(p, whole + t, total, e, m0, rows, tn);
+        grouped_half<BT>(p, e, m0, rows, tn * DENSE_BN, (b >> 3) & 1, smem);
+    };
+    if (half_first && has_half) {
+        run_half();
+        lds_barrier();  // every wave's LDS reads are done before the stream's first loads
+    }
+    if (mine > 0) {
+        using Cfg = DenseCfg<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM, DENSE_TN, 128>;
+        RaggedSeq<BT> seq{&p, table, mine, p.K / 64, 0, 0, total, b, G};
+        GroupedEpi<false, RaggedSeq<BT>> epi{&seq, smem + stream_stg_off<PlainOp, MODE_BF16>() + wave * STREAM_STG, lane, wave};
+        auto a_off = dense_offs<Cfg::NW, 128, Cfg::LA>(wave, lane, p.lda);
+        auto b_off = dense_offs<Cfg::NW, 128, Cfg::LB>(wave, lane, p.ldb);
+        if constexpr (BT) b_off = dense_offs_t16<Cfg::NW, Cfg::LB, Cfg::BN>(wave, lane, p.ldb);
+        v16f acc[DENSE_TN][DENSE_TM];
+        gemm_stream<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM, DENSE_TN, BT>(seq, a_off, b_off, smem, lane, wave, acc, epi);
+    }
+    if (!half_first && has_half) run_half();
+}
+__global__ __launch_bounds__(256, 1) void grouped_dw_stream_kernel(const GroupedParams p) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
+    HKQ_LDS uint8_t* smem = (HKQ_LDS uint8_t*)smem_raw;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    using Cfg = DenseCfg<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM, DENSE_TN, 128>;
+    const int b = blockIdx.x, G = gridDim.x, tiles = p.tiles_m * p.tiles_n * p.E;
+    GroupTable table;
+    table.fill(p, smem + STREAM_TABLE);
+    if (b >= tiles) return;
+    DwSeq seq{&p, table, (tiles - 1 - b) / G + 1, 0, 0, 0, b, G};
+    GroupedEpi<true, DwSeq> epi{&seq, smem + stream_stg_off<PlainOp, MODE_BF16>() + wave * STREAM_STG, lane, wave};
+    auto a_off = dense_offs_t16<Cfg::NW, Cfg::LA, Cfg::BM>(wave, lane, p.lda);
+    auto b_off = dense_offs_t16<Cfg::NW, Cfg::LB, Cfg::BN>(wave, lane, p.ldb);
+    v16f acc[DENSE_TN][DENSE_TM];
+    gemm_stream<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM, DENSE_TN, true, true>(seq, a_off, b_off, smem, lane, wave, acc, epi);
 }
 
 template <class Kern>
@@ -201,6 +412,19 @@ static int launch_small(GroupedParams& p, hipStream_t stream) {
 }
 template <bool BT>
 static int launch_whole(GroupedParams& p, hipStream_t stream) {
+    const int ncu = cu_count();
+    if (ncu > 0 && p.E <= STREAM_GROUPS && p.K % 128 == 0 && p.K >= 256 && p.c16) {
+        p.tiles_m = (int)ragged_most(p.M, p.E, DENSE_BM);
+        p.tiles_n = (p.N + DENSE_BN - 1) / DENSE_BN;
+        p.group_m = 8;
+        if ((int64_t)p.tiles_m * p.tiles_n < (1 << 23)) {
+            auto kern = grouped_stream_kernel<BT>;
+            static bool attr = false;
+            if (int e = set_lds(kern, STREAM_LDS, attr)) return e;
+            kern<<<ncu, 256, STREAM_LDS, stream>>>(p);
+            return hkq_launch_status();
+        }
+    }
     static bool attr = false;
     return launch_grouped(grouped_whole_kernel<BT>, attr, WHOLE_LDS, DENSE_BM, DENSE_BN, 256, p, stream);
 }
@@ -249,6 +473,15 @@ static int run_dw(GroupedParams& p, hipStream_t stream) {
     p.c16 = p.ldc % 8 == 0 && p.stride_e % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     const int64_t tiles = (int64_t)((p.K + 255) / 256) * ((p.N + 255) / 256) * p.E;
+    if (tiles >= ncu && p.E <= STREAM_GROUPS && p.c16 && tiles < (1 << 23)) {
+        p.tiles_m = (p.K + DENSE_BM - 1) / DENSE_BM;
+        p.tiles_n = (p.N + DENSE_BN - 1) / DENSE_BN;
+        p.group_m = 8;
+        static bool attr = false;
+        if (int e = set_lds(grouped_dw_stream_kernel, STREAM_LDS, attr)) return e;
+        grouped_dw_stream_kernel<<<(unsigned)ncu, 256, STREAM_LDS, stream>>>(p);
+        return hkq_launch_status();
+    }
     if (tiles >= ncu) {
         static bool attr = false;
         return launch_dw(grouped_dw_whole_kernel, attr, WHOLE_LDS, DENSE_BM, DENSE_BN, 256, p, stream);

@@ -17,11 +17,19 @@ __device__ __forceinline__ int2 group_rows(const P& p, int e) {
     return make_int2(start, min(max(p.offs[e + 1], start), p.M));
 }
 
-// The id-th workgroup in the order in which an XCD's workgroups, dealt out round
-// robin, are neighbours.
+// The bid-th workgroup's place in the order in which an XCD's workgroups, which are
+// dealt out round robin, are neighbours.
 __device__ __forceinline__ int xcd_order(int bid, int n) {
     const int q = n >> 3, rem = n & 7, xcd = bid & 7, idx = bid >> 3;
     return xcd < rem ? xcd * (q + 1) + idx : rem * (q + 1) + (xcd - rem) * q + idx;
+}
+// Tile `in` of a group with tiles_m x tiles_n of them, group_m row tiles at a time, rows
+// first: neighbours share a group's weight columns and rows in their XCD's L2.
+__device__ __forceinline__ void group_tile(int in, int tiles_m, int tiles_n, int group_m, int& tm, int& tn) {
+    const int band = in / (group_m * tiles_n), first = band * group_m, size = min(tiles_m - first, group_m);
+    const int at = in - band * group_m * tiles_n;
+    tm = first + at % size;
+    tn = at / size;
 }
 
 struct RaggedTile {
@@ -53,16 +61,17 @@ __device__ __forceinline__ bool ragged_tile(const P& p, RaggedTile& t) {
     for (int e0 = 64; e0 < p.E; e0 += 64) total += __builtin_amdgcn_readlane(scan(count(e0 + lane)), 63);
     total = min(total, p.tiles_m);  // bounds that count a row twice: the tiles that the grid holds
     if ((int)blockIdx.x >= total * p.tiles_n) return false;
-    int tm;
-    tile_coords(blockIdx.x, total, p.tiles_n, p.group_m, tm, t.tn);
+    const int id = xcd_order(blockIdx.x, total * p.tiles_n), at = id / p.tiles_n;
     int before = 0;  // tiles of the groups before this round's
     for (int e0 = 0; e0 < p.E; e0 += 64) {
         if (e0 > 0) n = count(e0 + lane), s = scan(n);
-        const uint64_t past = __ballot(before + s > tm);
+        const uint64_t past = __ballot(before + s > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             t.e = e0 + l;
-            tm -= before + __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(n, l);
+            const int tiles = __builtin_amdgcn_readlane(n, l), first = before + __builtin_amdgcn_readlane(s, l) - tiles;
+            int tm;
+            group_tile(id - first * p.tiles_n, tiles, p.tiles_n, p.group_m, tm, t.tn);
             const int2 r = group_rows(p, t.e);
             t.m0 = __builtin_amdgcn_readfirstlane(r.x + tm * BM);
             t.rows = __builtin_amdgcn_readfirstlane(r.y) - t.m0;
