@@ -66,6 +66,8 @@ MODULES = {
     "fused_gemm_a8w8_epilogue_tk": "bind_fused_gemm_a8w8_epilogue.cpp",
     "fused_gemm_a16w16_epilogue_tk": "bind_fused_gemm_a16w16_epilogue.cpp",
     "gated_ffn_tk": "bind_gated_ffn.cpp",
+    "grouped_gemm_tk": "bind_grouped_gemm.cpp",
+    "w4_tk": "bind_w4.cpp",
     "moe_op_gemm_a8w8_tk": "bind_moe_op_gemm_a8w8.cpp",
     "moe_op_gemm_a8w8_blockscale_tk": "bind_moe_op_gemm_a8w8_blockscale.cpp",
     "moe_op_mxfp4_tk": "bind_moe_op_mxfp4.cpp",

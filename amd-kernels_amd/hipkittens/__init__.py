@@ -14,6 +14,8 @@ the modules this build provides:
                                                            # (also .a8w8_blockscale_a16w16)
     hk.fused_gemm.a8w8_epilogue.dispatch(A, B, a_s, b_s, C, bias, residual, act)   # (also .a16w16_epilogue)
     hk.ffn.gated.gated_ffn_a8w8(X, W, x_s, w_s, H, act)    # (also gated_ffn_bf16, gated_ffn_backward)
+    hk.moe.grouped.grouped_gemm_bf16(X, W, Y, offs)        # (also grouped_gemm_backward)
+    hk.w4.gemm_w4a16(X, Q, S, C, Z)                        # (also w4_quant, w4_dequant, grouped_gemm_w4a16)
     hk.moe_routing.quant.downcast_to_mxfp(...)             # quant_moe_tk
     hk.moe_routing.topk.moe_topk(X, ...)                   # moe_topk_tk (also bitmatrix,
                                                            # expt_data, align_block_size)
@@ -203,6 +205,8 @@ class _MoeGemmNamespace:
     a8w8 = _SubModule("moe_op_gemm_a8w8_tk")
     a8w8_blockscale = _SubModule("moe_op_gemm_a8w8_blockscale_tk")
     mxfp4 = _SubModule("moe_op_mxfp4_tk")
+    # extension: bf16 products over ragged groups of rows, and their gradients
+    grouped = _SubModule("grouped_gemm_tk")
 
 
 class _MoeRoutingNamespace:
@@ -221,3 +225,4 @@ fused_gemm = _FusedGemmNamespace()
 ffn = _FeedForwardNamespace()
 moe = _MoeGemmNamespace()
 moe_routing = _MoeRoutingNamespace()
+w4 = _SubModule("w4_tk")  # extension: 4-bit weights, their quantizer and products

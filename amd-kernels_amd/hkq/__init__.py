@@ -563,7 +563,7 @@ def _stride3(t) -> tuple[int, int]:
 def grouped_gemm_bf16(X, W, offs, Y=None, stream=None):
     """Products over ragged groups of rows: Y[r] = X[r] . W[e]^T for offs[e] <= r <
     offs[e + 1]. X bf16 [M, K], W bf16 [E, N, K], offs int32 [E + 1] on the GPU
-    (moe_routing's) -> Y bf16 [M, N]. Rows of no group are left as they were: pass
+    (moe_routing's token_start) -> Y bf16 [M, N]. Rows of no group are left as they were: pass
     a Y that holds something there."""
     import torch
 
@@ -720,8 +720,8 @@ def grouped_gemm_w4a16(X, Q, S, offs, Z=None, gather=None, topk: int = 1, Y=None
     """gemm_w4a16 over ragged groups of rows: Y[r] = X[x(r)] . W[e]^T for offs[e] <= r <
     offs[e + 1], 4-bit weights Q [E, N, K / 2], S (and Z) [E, N, K / group]. x(r) = r,
     or gather[r] // topk with moe_routing's gather int32 [M] (a row outside X counts
-    as zeros). offs int32 [E + 1] and gather are on the GPU -> bf16 [M, N]; rows of no
-    group are left as they were: pass a Y that holds something there."""
+    as zeros). offs int32 [E + 1] (moe_routing's token_start) and gather are on the GPU
+    -> bf16 [M, N]; rows of no group are left as they were: pass a Y that holds something there."""
     import torch
 
     T, K = X.shape

@@ -185,9 +185,11 @@ def test_dense_short_and_ragged_k(kind, group, zeros):
 
 @pytest.mark.parametrize("kind,group,zeros", KINDS)
 @pytest.mark.parametrize("M,N,K", [(1, 4096, 14336), (16, 14336, 4096), (48, 4096, 4096), (200, 4096, 2048), (600, 2816, 2048),
-                                   (1030, 1408, 4096)])
+                                   (1030, 1408, 4096), (3, 13001, 544), (7, 13001, 544), (12, 13001, 544), (29, 13001, 544)])
 def test_dense_layer_sizes(M, N, K, kind, group, zeros):
+    """Many columns (the last four: ragged ones) take more of them per workgroup."""
     require_gpu()
+    K = K // group * group
     check_dense(M, N, K, kind, group, zeros, seed=3)
 
 
@@ -257,3 +259,175 @@ def test_mxfp4_scales():
             fin = torch.isfinite(torch.tensor(6.0) * torch.pow(2.0, torch.arange(255).double() - 127).float())
             assert ok[:, fin].all(), (k, M, (~ok[:, fin]).nonzero()[:4])
             assert C[:, 255].isnan().all()
+
+
+def test_weights_of_other_layouts():
+    """Groups side by side in each row, one weight for all groups, scales of odd pitch."""
+    require_gpu()
+    E, N, K, rows = 3, 40, 160, [5, 0, 70]
+    q, s, z, val = weights((N, E, K), "int4", 32, True, 1)
+    offs = torch.tensor([0, 5, 5, 75], dtype=torch.int32, device="cuda")
+    X = rows_of(75, K, 2)
+    Y = hkq.grouped_gemm_w4a16(X, q.transpose(0, 1), s.transpose(0, 1), offs, z.transpose(0, 1))
+    ref = hkq.grouped_gemm_w4a16(X, q.transpose(0, 1).contiguous(), s.transpose(0, 1).contiguous(), offs, z.transpose(0, 1).contiguous())
+    assert torch.equal(Y, ref)
+    one = [t[:, 0].contiguous()[None].expand(E, N, -1) for t in (q, s, z)]
+    Y = hkq.grouped_gemm_w4a16(X, one[0], one[1], offs, one[2])
+    close(Y, X.double() @ val[:, 0].t(), X.double().abs() @ val[:, 0].abs().t(), K, "one weight")
+
+
+@pytest.mark.parametrize("kind,group,zeros", KINDS)
+@pytest.mark.parametrize("M", [1, 7, 16, 30, 100])
+def test_nan_infinity_and_zero_weights(M, kind, group, zeros):
+    """An infinity in X gives what the weight at its place makes of it: a signed infinity, or NaN where that is zero; it and
+    a NaN stay in their rows. Weights of zero give zeros, whatever X."""
+    require_gpu()
+    N, K = 70, 4 * group
+    q, s, z, val = weights((N, K), kind, group, zeros, 5)
+    q[9] = 0 if kind == "mx" else 0x88
+    if z is not None:
+        z[9] = 8
+    val[9] = 0
+    X = rows_of(M, K, 6)
+    clean = hkq.gemm_w4a16(X, q, s, z)
+    assert (clean[:, 9] == 0).all()
+    at = group + 3
+    X[M - 1, at] = float("inf")
+    C = hkq.gemm_w4a16(X, q, s, z)
+    assert torch.equal(C[:-1], clean[:-1])
+    v = val[:, at]
+    assert torch.equal(C[-1].isnan(), v == 0) and torch.equal(C[-1][v != 0] > 0, v[v != 0] > 0) and not C[-1].isfinite().any()
+    X[M - 1, at] = NAN
+    assert hkq.gemm_w4a16(X, q, s, z)[-1].isnan().all()
+    # a NaN scale reaches the outputs of its column only (test_mxfp4_scales: MXFP4's)
+    if kind == "int4":
+        X[M - 1, at] = 1.0
+        s[3, 1] = NAN
+        C = hkq.gemm_w4a16(X, q, s, z)
+        assert C[:, 3].isnan().all() and C[:, :3].isfinite().all() and C[:, 4:].isfinite().all()
+
+
+def test_no_rows_no_sums():
+    require_gpu()
+    q, s, z, _ = weights((24, 64), "int4", 32, True, 1)
+    X = torch.empty((0, 64), dtype=BF16, device="cuda")
+    assert hkq.gemm_w4a16(X, q, s, z).shape == (0, 24)
+    offs = torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert hkq.grouped_gemm_w4a16(X, q[None], s[None], offs, z[None]).shape == (0, 24)
+    empty = [t[:, :0] for t in (q, s)]
+    for M in (1, 20, 100):
+        C = hkq.gemm_w4a16(torch.empty((M, 0), dtype=BF16, device="cuda"), *empty, C=torch.full((M, 24), 7.0, dtype=BF16, device="cuda"))
+        assert (C == 0).all()
+
+
+@pytest.mark.parametrize("kind,group,zeros", [("int4", 64, True), ("mx", 32, False)])
+def test_offsets_past_32_bits(kind, group, zeros):
+    """Codes of 5.4 GB, rows and outputs of 2.4 GB."""
+    require_gpu()
+    E, N, K = 80, 16384, 8192
+    q, s, z, val = weights((64, K), kind, group, zeros, 1)
+    Q = torch.zeros((E, N, K // 2), dtype=torch.uint8, device="cuda")
+    S = torch.zeros((E, N, K // group), dtype=s.dtype, device="cuda")
+    Z = torch.zeros((E, N, K // group), dtype=torch.uint8, device="cuda") if zeros else None
+    for e in (0, E - 1):
+        Q[e, -64:], S[e, -64:] = q, s
+        if zeros:
+            Z[e, -64:] = z
+    for rows in ([1] + [0] * (E - 2) + [3], [70] + [0] * (E - 2) + [130]):
+        M = sum(rows)
+        offs = torch.tensor([0] + [rows[0]] * (E - 1) + [M], dtype=torch.int32, device="cuda")
+        X = rows_of(M, K, 2)
+        Y = hkq.grouped_gemm_w4a16(X, Q, S, offs, Z)
+        close(Y[:, -64:], X.double() @ val.t(), X.double().abs() @ val.abs().t(), K, "last columns")
+    del Q, S, Z
+    M, K, N = 300000, 4096, 4096
+    q, s, z, val = weights((N, K), kind, group, zeros, 3)
+    X = torch.zeros((M, K), dtype=BF16, device="cuda")
+    X[-300:] = bf16((300, K), 4)
+    C = hkq.gemm_w4a16(X, q, s, z)
+    x = X[-300:].double()
+    close(C[-300:], x @ val.t(), x.abs() @ val.abs().t(), K, "last rows")
+    assert (C[:-300] == 0).all()
+
+
+def test_streams_and_graphs():
+    """On a stream of the caller's, several at once, and captured: every replay as the eager call, with eager work between."""
+    require_gpu()
+    sets = []
+    for i, (M, N, K, (kind, group, zeros)) in enumerate([(1, 512, 1024, KINDS[1]), (13, 300, 640, KINDS[4]), (40, 256, 384, KINDS[5]),
+                                                         (200, 520, 512, KINDS[0])]):
+        q, s, z, _ = weights((2, N, K), kind, group, zeros, i)
+        offs = torch.tensor([0, M // 3, M], dtype=torch.int32, device="cuda")
+        sets.append((rows_of(M, K, i + 9), q, s, z, offs))
+    w = bf16((96, 256), 30).cuda()
+
+    def run(x, q, s, z, offs, stream=None):
+        a = hkq.gemm_w4a16(x, q[0], s[0], z[0] if z is not None else None, stream=stream)
+        b = hkq.grouped_gemm_w4a16(x, q, s, offs, z, stream=stream)
+        c = hkq.w4_quant(w, 64, True, stream=stream)
+        return (a, b, *c, hkq.w4_dequant(*c, stream=stream))
+
+    eager = [run(*t) for t in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        out = [run(*t, stream=st) for t, st in zip(sets, streams)]
+        torch.cuda.synchronize()
+        for a, b in zip(eager, out):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        out = [run(*t) for t in sets]
+    for _ in range(3):
+        for o in out:
+            for t in o:
+                t.fill_(3)
+        g.replay()
+        run(*sets[0])
+        torch.cuda.synchronize()
+        for a, b in zip(eager, out):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_hipkittens_module():
+    require_gpu()
+    import hipkittens as hk
+
+    w, X = bf16((48, 256), 1).cuda(), rows_of(20, 256, 2)
+    q, s, z = (torch.empty((48, n), dtype=t, device="cuda") for n, t in ((128, torch.uint8), (4, BF16), (4, torch.uint8)))
+    hk.w4.w4_quant(w, q, s, z)
+    ref = hkq.w4_quant(w, 64, True)
+    assert all(torch.equal(a, b) for a, b in zip((q, s, z), ref))
+    out, C = torch.empty_like(w), torch.empty((20, 48), dtype=BF16, device="cuda")
+    hk.w4.w4_dequant(q, s, out, z)
+    hk.w4.gemm_w4a16(X, q, s, C, z)
+    assert torch.equal(out, hkq.w4_dequant(q, s, z)) and torch.equal(C, hkq.gemm_w4a16(X, q, s, z))
+    offs = torch.tensor([0, 7, 20], dtype=torch.int32, device="cuda")
+    Q, S = torch.stack((q, q.flip(0))), torch.stack((s, s.flip(0)))
+    gather = torch.randperm(20, generator=gen(3)).to(torch.int32).cuda()
+    Y = torch.empty((20, 48), dtype=BF16, device="cuda")
+    hk.w4.grouped_gemm_w4a16(X[:10], Q, S, Y, offs, gather=gather, topk=2)
+    assert torch.equal(Y, hkq.grouped_gemm_w4a16(X[:10], Q, S, offs, None, gather, 2))
+    mq, ms = hkq.mx_quant(w, True)
+    hk.w4.gemm_w4a16(X, mq, ms, C)
+    assert torch.equal(C, hkq.gemm_w4a16(X, mq, ms))
+    with pytest.raises(ValueError, match="scale per"):
+        hk.w4.gemm_w4a16(X, q, s[:, :1].contiguous(), C)
+    with pytest.raises(TypeError, match="Q"):
+        hk.w4.gemm_w4a16(X, q.float(), s, C)
+    with pytest.raises(ValueError, match="zero points"):
+        hk.w4.gemm_w4a16(X, mq, ms, C, ms)
+
+
+def test_quantized_weights_through_the_products():
+    """w4_quant's and mx_quant's outputs as the products take them."""
+    require_gpu()
+    w, X = bf16((200, 512), 1, 0.05).cuda(), rows_of(37, 512, 2)
+    for group, zeros in ((32, True), (64, False), (128, True), (128, False)):
+        t = hkq.w4_quant(w, group, zeros)
+        c = unpack(t[0]).double().view(200, -1, group)
+        val = ((c - (t[2].double()[..., None] if zeros else 8.0)) * t[1].double()[..., None]).view(200, 512)
+        close(hkq.gemm_w4a16(X, *t), X.double() @ val.t(), X.double().abs() @ val.abs().t(), 512, f"{group} {zeros}")
+    q, s = hkq.mx_quant(w, True)
+    val = hkq.mx_dequant(q, s, 512, True).double()
+    close(hkq.gemm_w4a16(X, q, s), X.double() @ val.t(), X.double().abs() @ val.abs().t(), 512, "mx")
