@@ -388,15 +388,17 @@ static int run_w4_group(W4Params& p, int64_t r, hipStream_t stream) {
 }
 
 // Streamed or tiled. Up to 16 rows per group the stream reads a weight once; beyond, it
-// does so once per 32 rows, in 5.8 us per 8192 units of K (128 values of 16 columns), and
-// the tiles of 64 rows and 128 columns take 0.8 us per unit and round of them over the
-// CUs, a unit's chain of waits (32x4096x4096 8.7 and 26, 64x28672x4096 85 and 28.7).
+// does so once per 32 rows, in 5.8 us per 8192 units of K (128 values of 16 columns)
+// (32x4096x4096 8.7 us, on 32-row tiles 22; 64x4096x4096 13.3 and 22; 24x28672x4096 57,
+// 22.7).
 static int run_w4(W4Params& p, bool mx, hipStream_t stream) {
     const int64_t live = std::min(p.M, p.E), r = p.M / live, ncu = cu_count() > 0 ? cu_count() : 256, units = (p.K + 127) / 128;
-    const int64_t streams = live * ((r + 31) / 32) * ((p.N + 15) / 16), tiles = live * ((r + 63) / 64) * ((p.N + 127) / 128);
-    const double us_stream = 3.0 + (double)std::max(streams, ncu) * units * (5.8 / 8192),
-                 us_tile = 3.0 + (double)((tiles + ncu - 1) / ncu) * units * 0.8;
-    if (r > 16 && us_tile < us_stream) return launch_w4_tile(p, mx, stream);
+    if (r > 16) {
+        const int64_t wgs = live * ((r + 31) / 32) * ((p.N + 15) / 16);
+        const double us_stream = 3.0 + (double)(std::max(wgs, ncu) * units) * (5.8 / 8192);
+        int tile;
+        if (w4_tile_plan(p, tile) < us_stream) return launch_w4_tile(p, mx, tile, stream);
+    }
     if (mx) return run_w4_stream<0, false>(p, r, stream);
     return p.glog2 == 5 ? run_w4_group<32>(p, r, stream) : p.glog2 == 6 ? run_w4_group<64>(p, r, stream) : run_w4_group<128>(p, r, stream);
 }

@@ -83,7 +83,8 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
     a = r[0], b = r[1];
 }
 
-// The tile kernel of w4_tile.hip.
-int launch_w4_tile(W4Params& p, bool mx, hipStream_t stream);
+// The tiles of w4_tile.hip: the size with the least estimated time (us), and its launch.
+float w4_tile_plan(const W4Params& p, int& tile);
+int launch_w4_tile(W4Params& p, bool mx, int tile, hipStream_t stream);
 
 }  // namespace hkq

@@ -30,6 +30,7 @@ struct W4Tile {
     static constexpr int LX = 2 * BM / 8 / NW, LW = BN / 16 / NW, NLD = LX + LW + SD + ZD;
     static constexpr int EP_PITCH = TN * 64 + 16, EP = NW * BM * EP_PITCH;
     static constexpr int LDS = NS * STAGE > EP ? NS * STAGE : EP;
+    static constexpr int OCC = TM == 1 && 2 * LDS <= 160 * 1024 ? 2 : 1;  // workgroups per CU (larger ones would spill)
     static_assert(LDS <= 160 * 1024 && NS >= 3 && (NS - 2) * NLD <= 63, "LDS and vmcnt budget");
     static constexpr int PARTS = MX ? 1 : NG, CH = 8 / PARTS;  // chains of matrix instructions per n-tile and m-tile
 };
@@ -47,7 +48,7 @@ __device__ __forceinline__ void for_each_int(F&& f) {
 }
 
 template <class T>
-__global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
+__global__ __launch_bounds__(256, T::OCC) void w4_tile_kernel(const W4Params p) {
     constexpr int TM = T::TM, TN = T::TN, NS = T::NS, BM = T::BM, NW = T::NW, SB = T::SB, NG = T::NG, CH = T::CH;
     constexpr bool MX = T::MX;
     using KT = KTile<128>;
@@ -263,8 +264,8 @@ __global__ __launch_bounds__(256, 1) void w4_tile_kernel(const W4Params p) {
 #pragma unroll
                 for (int l = f * LPS; l < (f + 1) * LPS && l < T::NLD; ++l) issue(u + NS - 1, refill, l);
             }
-            // rows live in the accumulation registers: the others are full
-            asm volatile("" : "+a"(A[(f + 1) % SLOTS]));
+            // one wave per SIMD: rows live in the accumulation registers, the others are full
+            if constexpr (T::OCC == 1) asm volatile("" : "+a"(A[(f + 1) % SLOTS]));
             if constexpr (f == FIRST) finish_raw(LAST ? u + 1 : u, (i + 1) % TN, raw);
             constexpr int N = SLOTS - FIRST, p0 = f < FIRST ? 0 : (f - FIRST) * 16 / N, p1 = f < FIRST ? 0 : (f - FIRST + 1) * 16 / N;
 #pragma unroll
@@ -353,20 +354,54 @@ static int launch_tile(W4Params& p, hipStream_t stream) {
     return hkq_launch_status();
 }
 
-template <int G, bool Z>
-static int launch_rows(W4Params& p, hipStream_t stream) {
-    const int64_t r = p.M / std::min(p.M, p.E);
-    if (r <= 64) return launch_tile<W4Tile<G, Z, 2, 1, 4>>(p, stream);
-    return launch_tile<W4Tile<G, Z, 4, 2, 3>>(p, stream);
-}
-template <int G>
-static int launch_group(W4Params& p, hipStream_t stream) {
-    return p.Z ? launch_rows<G, true>(p, stream) : launch_rows<G, false>(p, stream);
+// Tile sizes, and us per unit and per tile on MI355X: a wave's instructions, one wave per
+// SIMD (4.8 cycles each beside 9.5 per matrix instruction), so that converting the codes
+// counts as much as multiplying. Two workgroups of the smallest share a CU. Measured at
+// 32, 64 x 128, 64, 96, 128 x 256 and 128 x 128 (us): 24x28672x4096 22.7, 26.7, 42, 47, 56,
+// 35; 300x4096x14336 109, 82, 140, 153, 184, 107; 2048x4096x14336 486, 362, 317, 334, 238,
+// 271; 6006 rows of 64 groups 2048x1408 84, 91, 74, 66, 75, 90.
+static const struct {
+    int bm, bn;
+    float us, e;
+} W4_TILES[] = {{32, 128, 0.62f, 2.0f}, {64, 128, 0.76f, 2.0f}, {64, 256, 1.27f, 2.0f}, {96, 256, 1.42f, 2.0f}, {128, 256, 1.70f, 2.0f},
+                {128, 128, 1.00f, 2.0f}};
+
+float w4_tile_plan(const W4Params& p, int& tile) {
+    const int64_t ncu = cu_count() > 0 ? cu_count() : 256, units = (p.K + 127) / 128;
+    const double live = (double)std::min(p.M, p.E), r = p.M / live;
+    float best = 0.f;
+    for (int t = 0; t < 6; ++t) {
+        const auto& c = W4_TILES[t];
+        const double rows = p.offs ? live * std::max(1.0, r / c.bm + 0.5) : (double)((p.M + c.bm - 1) / c.bm);
+        const int64_t tiles = (int64_t)(rows * (double)((p.N + c.bn - 1) / c.bn) + 0.999);
+        const bool pairs = t == 0 && tiles > ncu;  // two on a CU slow each other down
+        const int64_t rounds = (tiles + (pairs ? 2 * ncu : ncu) - 1) / (pairs ? 2 * ncu : ncu);
+        const float us = (float)rounds * ((float)units * (pairs ? 1.0f : c.us) + c.e);
+        if (best == 0.f || us < best) best = us, tile = t;
+    }
+    return best;
 }
 
-int launch_w4_tile(W4Params& p, bool mx, hipStream_t stream) {
-    if (mx) return launch_rows<0, false>(p, stream);
-    return p.glog2 == 5 ? launch_group<32>(p, stream) : p.glog2 == 6 ? launch_group<64>(p, stream) : launch_group<128>(p, stream);
+template <int G, bool Z>
+static int launch_rows(W4Params& p, int tile, hipStream_t stream) {
+    switch (tile) {
+        case 0: return launch_tile<W4Tile<G, Z, 1, 1, 4>>(p, stream);
+        case 1: return launch_tile<W4Tile<G, Z, 2, 1, 4>>(p, stream);
+        case 2: return launch_tile<W4Tile<G, Z, 2, 2, 3>>(p, stream);
+        case 3: return launch_tile<W4Tile<G, Z, 3, 2, 3>>(p, stream);
+        case 4: return launch_tile<W4Tile<G, Z, 4, 2, 3>>(p, stream);
+    }
+    return launch_tile<W4Tile<G, Z, 4, 1, 3>>(p, stream);
+}
+template <int G>
+static int launch_group(W4Params& p, int tile, hipStream_t stream) {
+    return p.Z ? launch_rows<G, true>(p, tile, stream) : launch_rows<G, false>(p, tile, stream);
+}
+
+int launch_w4_tile(W4Params& p, bool mx, int tile, hipStream_t stream) {
+    if (mx) return launch_rows<0, false>(p, tile, stream);
+    return p.glog2 == 5 ? launch_group<32>(p, tile, stream)
+                        : p.glog2 == 6 ? launch_group<64>(p, tile, stream) : launch_group<128>(p, tile, stream);
 }
 
 }  // namespace hkq
