@@ -9,6 +9,7 @@
 // K loops and tiles are the dense GEMMs'; in dX and dW the operands whose K runs
 // across memory rows are read transposed from LDS, so that nothing is copied.
 #include <algorithm>
+#include <cmath>
 
 #include "gemm_dense.h"
 #include "ragged.h"
@@ -440,25 +441,36 @@ static int launch_dw(Kern kern, bool& attr, int lds, int bm, int bn, int threads
     return hkq_launch_status();
 }
 
-// Tile size by the mean rows of a group: the least of rounds over the CUs * (K-tiles
-// * us + e).
+// Tile size by the mean rows of a group: the least estimated time. A K-tile takes
+// us + c * share with c workgroups on a CU; groups need about half a row tile more than
+// their rows fill. Fitted to 5 sizes x 62 shapes (1 to 1024 rows in each of 8 or 64
+// groups, N and K 1408 to 28672, Y and dX): 1.03 of the best size's time on average, 1.20
+// at the most. What a size is for, Y in us:
+//   64 groups 2816x2048, 4 rows:    64x64 127, 64x128 133, 128x256 142, 256x256 158
+//   8 groups 4096x14336, 64 rows:   128x128 190, 64x128 240, 128x256 249, 256x256 235
+//   8 groups 28672x4096, 1024 rows: 256x256 1546, 128x256 1806, 128x128 2226, 64x64 3560
 struct RaggedSize {
     int bm, bn, slots;  // slots: workgroups per CU
-    float us, e;
+    float us, share, e;  // e: start and epilogue
 };
 template <bool BT>
 static int run_ragged(GroupedParams& p, hipStream_t stream) {
     p.c16 = p.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
-    static const RaggedSize S[] = {{256, 256, 1, 1.37f, 5.7f}, {128, 256, 1, 0.85f, 3.2f}, {128, 128, 1, 0.57f, 2.2f},
-                                   {64, 128, 2, 0.60f, 2.0f}, {64, 64, 3, 0.55f, 2.0f}};
-    const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
+    static const RaggedSize S[] = {{256, 256, 1, 0.43f, 0.63f, 13.2f}, {128, 256, 1, 0.40f, 0.50f, 5.2f},
+                                   {128, 128, 1, 0.28f, 0.32f, 1.4f}, {64, 128, 2, 0.15f, 0.34f, 1.6f},
+                                   {64, 64, 3, 0.38f, 0.14f, 0.3f}};
+    const double ncu = cu_count() > 0 ? cu_count() : 256;
     const double KT = (p.K + 63) / 64, live = (double)std::min(p.M, p.E), r = p.M / live;
     int best = 0;
     double best_us = 0;
     for (int i = 0; i < 5; ++i) {
-        const double tiles = live * std::max(1.0, r / S[i].bm + 0.5) * ((p.N + S[i].bn - 1) / S[i].bn);
-        const double rounds = std::max(1.0, tiles / (double)(ncu * S[i].slots));
-        const double us = rounds * (KT * S[i].us + S[i].e);
+        const RaggedSize& s = S[i];
+        const double tiles = live * std::max(1.0, r / s.bm + 0.5) * ((p.N + s.bn - 1) / s.bn);
+        auto round = [&](int c) { return c == 0 ? 0.0 : KT * (s.us + s.share * c) + s.e; };
+        const double per = tiles / ncu;  // tiles of a CU
+        const int full = (int)std::min(per / s.slots, 2.0);
+        const double us = full == 2 ? (per / s.slots + 0.5) * round(s.slots)
+                                    : full * round(s.slots) + round((int)std::ceil(per - full * s.slots - 1e-9));
         if (best_us == 0 || us < best_us) best = i, best_us = us;
     }
     switch (best) {

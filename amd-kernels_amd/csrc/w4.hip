@@ -29,6 +29,11 @@ __device__ __forceinline__ float group_fold(float v, F f) {
     return v;
 }
 
+// at / per, in 32 bits where all of them fit
+__device__ __forceinline__ int64_t row_of(int64_t at, int64_t per, int64_t total) {
+    return total >> 32 == 0 ? (int64_t)((uint32_t)at / (uint32_t)per) : at / per;
+}
+
 template <int G>
 __global__ __launch_bounds__(256) void w4_quant_kernel(const uint16_t* __restrict__ w, uint8_t* __restrict__ q,
                                                        uint16_t* __restrict__ s, uint8_t* __restrict__ z, int64_t N, int K,
@@ -38,7 +43,7 @@ __global__ __launch_bounds__(256) void w4_quant_kernel(const uint16_t* __restric
     for (int64_t b = (int64_t)blockIdx.x * 256; b < total; b += (int64_t)gridDim.x * 256) {
         const int64_t at = b + threadIdx.x;  // whole groups: K is a multiple of G, 256 lanes of L
         if (at >= total) return;
-        const int64_t row = at / per;
+        const int64_t row = row_of(at, per, total);
         const int k = (int)(at - row * per) * 8;
         const v4i raw = *reinterpret_cast<const v4i*>(w + row * ldw + k);
         float v[8];
@@ -89,7 +94,7 @@ __global__ __launch_bounds__(256) void w4_dequant_kernel(const uint8_t* __restri
                                                          int K, int64_t ldq, int64_t lds, int64_t ldo, int glog2) {
     const int64_t per = K / 8, total = N * per;
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
-        const int64_t row = at / per;
+        const int64_t row = row_of(at, per, total);
         const int k = (int)(at - row * per) * 8;
         const uint32_t code = *reinterpret_cast<const uint32_t*>(q + row * ldq + k / 2);
         const int64_t g = row * lds + (k >> glog2);

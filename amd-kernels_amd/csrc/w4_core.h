@@ -78,10 +78,6 @@ __device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
     const v2u r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     a = r[0], b = r[1];
 }
-__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
-    const v2u r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0], b = r[1];
-}
 
 // The tiles of w4_tile.hip: the size with the least estimated time (us), and its launch.
 float w4_tile_plan(const W4Params& p, int& tile);
