@@ -23,8 +23,8 @@ struct GroupedParams {
     const int32_t* offs;
     int M, E, N, K;  // C has N columns; K: the length of the sums (Y, dX), the columns of A (dW)
     int64_t lda, ldb, stride_e;  // bytes; stride_e: group to group, of B (Y, dX) or C (dW, values)
-    int64_t ldc;                 // values
-    int tiles_m, tiles_n, group_m, c16;  // tiles_m: Y, dX: the most there can be
+    int64_t ldc;                 // values; 16-byte pieces of C are aligned (pitch, stride and base are checked)
+    int tiles_m, tiles_n, group_m;  // tiles_m: Y, dX: the most there can be
 };
 
 struct NoScale {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(Cfg::THREADS, MINB) void grouped_small_kernel(const
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wg = wave % Cfg::GW;
     if (wave >= Cfg::GW) return;
     store_tile_bf16<Cfg::TM, Cfg::TN>(acc, smem, wg, threadIdx.x & 63, p.C + t.m0 * p.ldc, p.ldc, t.rows, p.N,
-                                      wg / Cfg::WN * Cfg::TM * 32, n0 + wg % Cfg::WN * Cfg::TN * 32, p.c16 != 0, NoScale{},
+                                      wg / Cfg::WN * Cfg::TM * 32, n0 + wg % Cfg::WN * Cfg::TN * 32, true, NoScale{},
                                       NoScale{}, NoBias{});
 }
 template <bool BT>
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256, 1) void grouped_whole_kernel(const GroupedPara
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     store_tile_bf16<DENSE_TM, DENSE_TN>(acc, smem, wave, threadIdx.x & 63, p.C + t.m0 * p.ldc, p.ldc, t.rows, p.N,
                                         wave / DENSE_WAVES_N * DENSE_TM * 32, n0 + wave % DENSE_WAVES_N * DENSE_TN * 32,
-                                        p.c16 != 0, NoScale{}, NoScale{}, NoBias{});
+                                        true, NoScale{}, NoScale{}, NoBias{});
 }
 
 // dW: tile (tm, tn) of group e's [K columns of dY] x [N columns of X], summed over
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(Cfg::THREADS, MINB) void grouped_dw_small_kernel(co
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wg = wave % Cfg::GW;
     if (wave >= Cfg::GW) return;
     store_tile_bf16<Cfg::TM, Cfg::TN>(acc, smem, wg, threadIdx.x & 63, p.C + t.e * p.stride_e, p.ldc, p.K, p.N,
-                                      t.m0 + wg / Cfg::WN * Cfg::TM * 32, t.n0 + wg % Cfg::WN * Cfg::TN * 32, p.c16 != 0,
+                                      t.m0 + wg / Cfg::WN * Cfg::TM * 32, t.n0 + wg % Cfg::WN * Cfg::TN * 32, true,
                                       NoScale{}, NoScale{}, NoBias{});
 }
 __global__ __launch_bounds__(256, 1) void grouped_dw_whole_kernel(const GroupedParams p) {
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, 1) void grouped_dw_whole_kernel(const GroupedP
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     store_tile_bf16<DENSE_TM, DENSE_TN>(acc, smem, wave, threadIdx.x & 63, p.C + t.e * p.stride_e, p.ldc, p.K, p.N,
                                         t.m0 + wave / DENSE_WAVES_N * DENSE_TM * 32, t.n0 + wave % DENSE_WAVES_N * DENSE_TN * 32,
-                                        p.c16 != 0, NoScale{}, NoScale{}, NoBias{});
+                                        true, NoScale{}, NoScale{}, NoBias{});
 }
 
 // ---------------------------------------------------------------------------
@@ -334,7 +334,7 @@ __device__ __forceinline__ void grouped_half(const GroupedParams& p, int e, int 
     d.C = p.C + m0 * p.ldc;
     d.M = rows; d.N = p.N; d.K = p.K; d.kbytes = p.K * 2;
     d.lda = p.lda; d.ldb = p.ldb; d.ldc = p.ldc;
-    d.c16 = p.c16;
+    d.c16 = 1;
     dense_rows<Op, MODE_BF16, DENSE_TM / 2, 128, HALF_NS, Half::lds_bytes(HALF_NS)>(d, half * Half::BM, n0, smem);
 }
 
@@ -395,8 +395,8 @@ __global__ __launch_bounds__(256, 1) void grouped_dw_stream_kernel(const Grouped
 }
 
 template <class Kern>
-static int launch_grouped(Kern kern, bool& attr, int lds, int bm, int bn, int threads, GroupedParams& p, hipStream_t stream) {
-    if (int e = set_lds(kern, lds, attr)) return e;
+static int launch_grouped(Kern kern, std::atomic<uint64_t>& attr, int lds, int bm, int bn, int threads, GroupedParams& p, hipStream_t stream) {
+    if (int e = set_device_lds(kern, lds, attr)) return e;
     p.tiles_m = (int)ragged_most(p.M, p.E, bm);
     p.tiles_n = (p.N + bn - 1) / bn;
     p.group_m = 8;
@@ -408,30 +408,30 @@ static int launch_grouped(Kern kern, bool& attr, int lds, int bm, int bn, int th
 template <bool BT, class Cfg, int MINB = 1>
 static int launch_small(GroupedParams& p, hipStream_t stream) {
     static_assert(Cfg::LDS * MINB <= 160 * 1024, "LDS budget of a CDNA4 CU");
-    static bool attr = false;
+    static std::atomic<uint64_t> attr{0};
     return launch_grouped(grouped_small_kernel<BT, Cfg, MINB>, attr, Cfg::LDS, Cfg::BM, Cfg::BN, Cfg::THREADS, p, stream);
 }
 template <bool BT>
 static int launch_whole(GroupedParams& p, hipStream_t stream) {
     const int ncu = cu_count();
-    if (ncu > 0 && p.E <= STREAM_GROUPS && p.K % 128 == 0 && p.K >= 256 && p.c16) {
+    if (ncu > 0 && p.E <= STREAM_GROUPS && p.K % 128 == 0 && p.K >= 256) {
         p.tiles_m = (int)ragged_most(p.M, p.E, DENSE_BM);
         p.tiles_n = (p.N + DENSE_BN - 1) / DENSE_BN;
         p.group_m = 8;
         if ((int64_t)p.tiles_m * p.tiles_n < (1 << 23)) {
             auto kern = grouped_stream_kernel<BT>;
-            static bool attr = false;
-            if (int e = set_lds(kern, STREAM_LDS, attr)) return e;
+            static std::atomic<uint64_t> attr{0};
+            if (int e = set_device_lds(kern, STREAM_LDS, attr)) return e;
             kern<<<ncu, 256, STREAM_LDS, stream>>>(p);
             return hkq_launch_status();
         }
     }
-    static bool attr = false;
+    static std::atomic<uint64_t> attr{0};
     return launch_grouped(grouped_whole_kernel<BT>, attr, WHOLE_LDS, DENSE_BM, DENSE_BN, 256, p, stream);
 }
 template <class Kern>
-static int launch_dw(Kern kern, bool& attr, int lds, int bm, int bn, int threads, GroupedParams& p, hipStream_t stream) {
-    if (int e = set_lds(kern, lds, attr)) return e;
+static int launch_dw(Kern kern, std::atomic<uint64_t>& attr, int lds, int bm, int bn, int threads, GroupedParams& p, hipStream_t stream) {
+    if (int e = set_device_lds(kern, lds, attr)) return e;
     p.tiles_m = (p.K + bm - 1) / bm;
     p.tiles_n = (p.N + bn - 1) / bn;
     p.group_m = 8;
@@ -455,7 +455,6 @@ struct RaggedSize {
 };
 template <bool BT>
 static int run_ragged(GroupedParams& p, hipStream_t stream) {
-    p.c16 = p.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
     static const RaggedSize S[] = {{256, 256, 1, 0.43f, 0.63f, 13.2f}, {128, 256, 1, 0.40f, 0.50f, 5.2f},
                                    {128, 128, 1, 0.28f, 0.32f, 1.4f}, {64, 128, 2, 0.15f, 0.34f, 1.6f},
                                    {64, 64, 3, 0.38f, 0.14f, 0.3f}};
@@ -482,24 +481,23 @@ static int run_ragged(GroupedParams& p, hipStream_t stream) {
     return launch_small<BT, KgCfg<MODE_BF16, 2, 2, 1, 1, 1, 3>, 3>(p, stream);
 }
 static int run_dw(GroupedParams& p, hipStream_t stream) {
-    p.c16 = p.ldc % 8 == 0 && p.stride_e % 8 == 0 && reinterpret_cast<uintptr_t>(p.C) % 16 == 0;
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     const int64_t tiles = (int64_t)((p.K + 255) / 256) * ((p.N + 255) / 256) * p.E;
-    if (tiles >= ncu && p.E <= STREAM_GROUPS && p.c16 && tiles < (1 << 23)) {
+    if (tiles >= ncu && p.E <= STREAM_GROUPS && tiles < (1 << 23)) {
         p.tiles_m = (p.K + DENSE_BM - 1) / DENSE_BM;
         p.tiles_n = (p.N + DENSE_BN - 1) / DENSE_BN;
         p.group_m = 8;
-        static bool attr = false;
-        if (int e = set_lds(grouped_dw_stream_kernel, STREAM_LDS, attr)) return e;
+        static std::atomic<uint64_t> attr{0};
+        if (int e = set_device_lds(grouped_dw_stream_kernel, STREAM_LDS, attr)) return e;
         grouped_dw_stream_kernel<<<(unsigned)ncu, 256, STREAM_LDS, stream>>>(p);
         return hkq_launch_status();
     }
     if (tiles >= ncu) {
-        static bool attr = false;
+        static std::atomic<uint64_t> attr{0};
         return launch_dw(grouped_dw_whole_kernel, attr, WHOLE_LDS, DENSE_BM, DENSE_BN, 256, p, stream);
     }
     using Cfg = KgCfg<MODE_BF16, 4, 2, 1, 1, 2, 4>;
-    static bool attr = false;
+    static std::atomic<uint64_t> attr{0};
     return launch_dw(grouped_dw_small_kernel<Cfg, 1>, attr, Cfg::LDS, Cfg::BM, Cfg::BN, Cfg::THREADS, p, stream);
 }
 

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "hkq.h"
 
 namespace hkq {
@@ -30,6 +32,23 @@ inline bool overlap(const MemRows& a, const MemRows& b) {
     if (a.rows == 1 && b.rows == 1) return true;
     const int64_t col = (d % pitch + pitch) % pitch;  // b's first byte in a's rows
     return col < a.width || col + b.width > pitch;
+}
+
+// The dynamic LDS that a kernel takes, set once on each device (bit of `done`; a device
+// past 63 every time).
+template <class Kern>
+inline int set_device_lds(Kern kern, int lds, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (e == hipSuccess && (done.load(std::memory_order_relaxed) & bit)) return 0;
+    if (e == hipSuccess) e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) {
+        set_error("hipFuncSetAttribute(MaxDynamicSharedMemorySize=%d) failed: %s", lds, hipGetErrorString(e));
+        return (int)e;
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
 }
 }  // namespace hkq
 

@@ -505,7 +505,8 @@ static int w4_product(const void* X, const void* Q, const void* S, const void* Z
     p.offs = offs;
     p.gather = gather;
     p.M = (int)M; p.T = (int)T; p.E = (int)E; p.N = (int)N; p.K = (int)K;
-    p.ldx = 2 * ldx; p.ldq = ldq; p.lds = lds; p.ldc = ldc;
+    // without rows X's span, (T - 1) ldx + 2 K bytes, has to be 0
+    p.ldx = T > 0 ? 2 * ldx : 2 * K; p.ldq = ldq; p.lds = lds; p.ldc = ldc;
     p.stride_q = stride_q; p.stride_s = stride_s;
     p.glog2 = group == 32 ? 5 : group == 64 ? 6 : 7;
     p.topk = gather ? (int)topk : 1;

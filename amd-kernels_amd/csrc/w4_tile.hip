@@ -336,15 +336,8 @@ __global__ __launch_bounds__(256, T::OCC) void w4_tile_kernel(const W4Params p) 
 template <class T>
 static int launch_tile(W4Params& p, hipStream_t stream) {
     auto kern = w4_tile_kernel<T>;
-    static bool attr = false;
-    if (!attr) {
-        hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-        if (e != hipSuccess) {
-            set_error("hipFuncSetAttribute(MaxDynamicSharedMemorySize=%d) failed: %s", T::LDS, hipGetErrorString(e));
-            return (int)e;
-        }
-        attr = true;
-    }
+    static std::atomic<uint64_t> attr{0};
+    if (int e = set_device_lds(kern, T::LDS, attr)) return e;
     p.tiles_m = (int)ragged_most(p.M, p.E, T::BM);
     p.tiles_n = (p.N + T::BN - 1) / T::BN;
     p.group_m = 8;

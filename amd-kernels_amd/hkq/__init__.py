@@ -621,29 +621,39 @@ def w4_quant(w, group: int = 128, zeros: bool = False, q=None, s=None, z=None, s
     *lead, K = w.shape
     if len(lead) not in (1, 2) or K % group:
         raise ValueError(f"w must be [N, K] or [E, N, K] with K a multiple of {group}, got {list(w.shape)}")
-    if len(lead) == 2:  # one call for all experts
-        w = w.reshape(-1, K)
-    N = w.shape[0]
-    _expect(w, "w", (N, K), (torch.bfloat16,), w.device)
-    flat = []
-    for t, name, cols, dtype in ((q, "q", K // 2, torch.uint8), (s, "s", K // group, torch.bfloat16), (z, "z", K // group, torch.uint8)):
+    for t, name, cols, dtype in ((w, "w", K, torch.bfloat16), (q, "q", K // 2, torch.uint8), (s, "s", K // group, torch.bfloat16),
+                                 (z, "z", K // group, torch.uint8)):
         if t is not None:
             _expect(t, name, (*lead, cols), (dtype,), w.device)
-            t = t.view(N, cols)
-        flat.append(t)
-    q, s, z = flat
     with _on(w.device, stream):
         if q is None:
-            q = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
+            q = torch.empty((*lead, K // 2), dtype=torch.uint8, device=w.device)
         if s is None:
-            s = torch.empty((N, K // group), dtype=torch.bfloat16, device=w.device)
+            s = torch.empty((*lead, K // group), dtype=torch.bfloat16, device=w.device)
         if z is None and zeros:
-            z = torch.empty((N, K // group), dtype=torch.uint8, device=w.device)
-        if z is not None and _pitch(z) != _pitch(s):
-            raise ValueError("s and z must have one pitch")
-        call("hkq_w4_quant", _ptr(w), _ptr(q), _ptr(s), _opt_ptr(z), N, K, _pitch(w), _pitch(q), _pitch(s), group,
-             _stream(stream))
-    return tuple(t.view(*lead, t.shape[1]) for t in (q, s, z) if t is not None)
+            z = torch.empty((*lead, K // group), dtype=torch.uint8, device=w.device)
+        out = tuple(t for t in (q, s, z) if t is not None)
+        # one call for all experts where their rows follow each other, else one for each
+        for rows in zip(*_experts(w, *out)):
+            if z is not None and _pitch(rows[3]) != _pitch(rows[2]):
+                raise ValueError("s and z must have one pitch")
+            call("hkq_w4_quant", _ptr(rows[0]), _ptr(rows[1]), _ptr(rows[2]), _ptr(rows[3]) if z is not None else 0, rows[0].shape[0],
+                 K, _pitch(rows[0]), _pitch(rows[1]), _pitch(rows[2]), group, _stream(stream))
+    return out
+
+
+def _experts(*tensors):
+    """[N, ..] or [E, N, ..] tensors as lists of 2-D ones: all rows if each tensor's
+    experts follow at its row pitch, else an item for each expert."""
+    def together(t):
+        E, N, _ = t.shape
+        return E <= 1 or N <= 1 or t.stride(0) == N * t.stride(1)
+
+    if tensors[0].dim() == 2:
+        return [[t] for t in tensors]
+    if all(together(t) for t in tensors):
+        return [[t.flatten(0, 1)] for t in tensors]
+    return [list(t) for t in tensors]
 
 
 def _w4_weights(Q, S, Z, device):
@@ -679,18 +689,16 @@ def w4_dequant(q, s, z=None, out=None, stream=None):
         raise TypeError("s must be bf16 (MXFP4: mx_dequant)")
     *lead, half = q.shape
     K = 2 * half
+    if len(lead) not in (1, 2):
+        raise ValueError(f"q must be [N, K / 2] or [E, N, K / 2], got {list(q.shape)}")
     if out is not None:
         _expect(out, "out", (*lead, K), (torch.bfloat16,), q.device)
     with _on(q.device, stream):
         if out is None:
             out = torch.empty((*lead, K), dtype=torch.bfloat16, device=q.device)
-        n = 1
-        for d in lead:
-            n *= d
-        q2, s2, o2 = q.view(n, half), s.view(n, K // group), out.view(n, K)
-        z2 = None if z is None else z.view(n, K // group)
-        call("hkq_w4_dequant", _ptr(q2), _ptr(s2), _opt_ptr(z2), _ptr(o2), n, K, _pitch(q2), _pitch(s2), _pitch(o2), group,
-             _stream(stream))
+        for rows in zip(*_experts(q, s, out, *(() if z is None else (z,)))):
+            call("hkq_w4_dequant", _ptr(rows[0]), _ptr(rows[1]), 0 if z is None else _ptr(rows[3]), _ptr(rows[2]), rows[0].shape[0], K,
+                 _pitch(rows[0]), _pitch(rows[1]), _pitch(rows[2]), group, _stream(stream))
     return out
 
 

@@ -112,6 +112,27 @@ KINDS = [("int4", 128, False), ("int4", 128, True), ("int4", 64, True), ("int4",
 MIDS = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0], dtype=torch.float64)
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantizer_of_experts_apart(zeros):
+    """Halves of experts' rows in one buffer, quantized on another stream: what the experts
+    give one by one, and nothing between them written."""
+    both = bf16((3, 10, 256), 12).cuda()
+    q = torch.full((3, 10, 128), 0xA5, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    for half in (slice(0, 5), slice(5, 10)):
+        got = hkq.w4_quant(both[:, half], 128, zeros, q=q[:, half], stream=stream)
+        back = hkq.w4_dequant(*got, stream=stream)
+        stream.synchronize()
+        assert got[0].data_ptr() == q[:, half].data_ptr()
+        for e in range(3):
+            one = hkq.w4_quant(both[e, half].contiguous(), 128, zeros)
+            assert all(torch.equal(a[e].view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, one))
+            assert torch.equal(back[e], hkq.w4_dequant(*one))
+        if half.start == 0:
+            assert (q[:, 5:] == 0xA5).all()
+
+
 def weights(shape, kind, group, zeros, seed, pad=0):
     """Random codes, scales and zero points on the GPU, `pad` scales (NaN), and 16 pad bytes, past each row; and the values."""
     *lead, K = shape
@@ -318,6 +339,24 @@ def test_no_rows_no_sums():
     for M in (1, 20, 100):
         C = hkq.gemm_w4a16(torch.empty((M, 0), dtype=BF16, device="cuda"), *empty, C=torch.full((M, 24), 7.0, dtype=BF16, device="cuda"))
         assert (C == 0).all()
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_gather_from_no_rows(M):
+    """An X without rows, whatever its pitch: every gathered row counts as zeros."""
+    N, K = 64, 256
+    Q = torch.full((1, N, K // 2), 0x21, dtype=torch.uint8, device="cuda")
+    S = torch.ones((1, N, K // 128), dtype=torch.bfloat16, device="cuda")
+    X = torch.ones((4, 2 * K), dtype=torch.bfloat16, device="cuda")
+    offs = torch.tensor([0, M], dtype=torch.int32, device="cuda")
+    gather = torch.arange(M, dtype=torch.int32, device="cuda") - 1
+    for pitch in (K, 2 * K, 1 << 20):
+        Y = torch.full((M, N), 7.0, dtype=torch.bfloat16, device="cuda")
+        hkq.call("hkq_grouped_gemm_w4a16", X.data_ptr(), Q.data_ptr(), S.data_ptr(), 0, Y.data_ptr(), offs.data_ptr(), gather.data_ptr(),
+                 M, 0, 1, N, K, 1, pitch, K // 2, N * K // 2, K // 128, N * K // 128, N, 128, hkq.W4_INT4, 0, 0,
+                 torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert (Y == 0).all()
 
 
 @pytest.mark.parametrize("kind,group,zeros", [("int4", 64, True), ("mx", 32, False)])
