@@ -62,7 +62,7 @@ __device__ __forceinline__ bool ragged_tile(const P& p, RaggedTile& t) {
     total = min(total, p.tiles_m);  // bounds that count a row twice: the tiles that the grid holds
     if ((int)blockIdx.x >= total * p.tiles_n) return false;
     const int id = xcd_order(blockIdx.x, total * p.tiles_n), at = id / p.tiles_n;
-    int before = 0;  // tiles of the groups before this round's
+    int before = 0;  // tiles of the groups before e0
     for (int e0 = 0; e0 < p.E; e0 += 64) {
         if (e0 > 0) n = count(e0 + lane), s = scan(n);
         const uint64_t past = __ballot(before + s > at);
