@@ -385,11 +385,16 @@ static int launch_w4_stream(W4Params& p, hipStream_t stream) {
 // columns: us at M x N x K, zero points, 1 | 2 | 4 column tiles: 16x4096x4096 6.1 | 7.8 |
 // 11.4, 16x28672x4096 28.2 | 25.0 | 21.5, 6x28672x4096 23.9 | 20.2; MXFP4 16x28672x4096
 // 27.8 | 22.8 | 17.9. Up to four rows, one column tile: eight waves 1x4096x14336 10.5,
-// 1x28672x4096 20.7, four waves 13.1 and 17.4.
+// 1x28672x4096 20.7, four waves 13.1 and 17.4. Groups of unlike length: beyond a mean of
+// two, tiles of 16 rows, where most groups have one, which reads their weights once (mean
+// 8, tiles of 8 | 16 rows: 64 groups 2816x2048 103 | 71, 8 groups 28672x4096 150 | 115,
+// 4096x4096 22.9 | 21.0; mean 3, 4 | 16: 63 | 68, 126 | 102, 21.0 | 20.4).
+static bool ragged(const W4Params& p) { return p.offs && p.E > 1; }
 template <int G, bool Z>
 static int run_w4_stream(W4Params& p, int64_t r, hipStream_t stream) {
     const int64_t ncu = cu_count() > 0 ? cu_count() : 256;
     const bool many = std::min(p.M, p.E) * ((p.N + 15) / 16) > 3 * ncu;
+    if (ragged(p) && r > 2) r = 16;
     if (r <= 4)
         return many ? launch_w4_stream<G, Z, 1, 1, 1, 4, 4, 4, 4>(p, stream) : launch_w4_stream<G, Z, 1, 1, 1, 8, 4, 4, 4>(p, stream);
     if (r <= 8)
@@ -403,17 +408,18 @@ static int run_w4_group(W4Params& p, int64_t r, hipStream_t stream) {
     return p.Z ? run_w4_stream<G, true>(p, r, stream) : run_w4_stream<G, false>(p, r, stream);
 }
 
-// Streamed or tiled. Up to 16 rows per group the stream reads a weight once; beyond, it
-// does so once per 32 rows, in 5.8 us per 8192 units of K (128 values of 16 columns)
-// (32x4096x4096 8.7 us, on 32-row tiles 22; 64x4096x4096 13.3 and 22; 24x28672x4096 57,
-// 22.7).
+// Streamed or tiled. Up to 16 rows per group the stream reads a weight once. Beyond, a
+// single weight may still stream, once per 32 rows, in 5.8 us per 8192 units of K (128
+// values of 16 columns) (32x4096x4096 8.7 us, on 32-row tiles 22; 64x4096x4096 13.3 and 22;
+// 24x28672x4096 57, 22.7); groups do not (20 rows of each of 8 groups 4096x4096 32.4 us,
+// tiles 27.8; of 64 groups 2816x2048 109 and 69).
 static int run_w4(W4Params& p, bool mx, hipStream_t stream) {
     const int64_t live = std::min(p.M, p.E), r = p.M / live, ncu = cu_count() > 0 ? cu_count() : 256, units = (p.K + 127) / 128;
     if (r > 16) {
-        const int64_t wgs = live * ((r + 31) / 32) * ((p.N + 15) / 16);
+        const int64_t wgs = (r + 31) / 32 * ((p.N + 15) / 16);
         const double us_stream = 3.0 + (double)(std::max(wgs, ncu) * units) * (5.8 / 8192);
         int tile;
-        if (w4_tile_plan(p, tile) < us_stream) return launch_w4_tile(p, mx, tile, stream);
+        if (w4_tile_plan(p, tile) < us_stream || ragged(p)) return launch_w4_tile(p, mx, tile, stream);
     }
     if (mx) return run_w4_stream<0, false>(p, r, stream);
     return p.glog2 == 5 ? run_w4_group<32>(p, r, stream) : p.glog2 == 6 ? run_w4_group<64>(p, r, stream) : run_w4_group<128>(p, r, stream);
