@@ -10,6 +10,7 @@
 // exact in bf16, as the matrix instruction's operand, and an INT4 scale multiplies the
 // fp32 sums of its group.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "w4_core.h"
@@ -408,18 +409,30 @@ static int run_w4_group(W4Params& p, int64_t r, hipStream_t stream) {
     return p.Z ? run_w4_stream<G, true>(p, r, stream) : run_w4_stream<G, false>(p, r, stream);
 }
 
-// Streamed or tiled. Up to 16 rows per group the stream reads a weight once. Beyond, a
-// single weight may still stream, once per 32 rows, in 5.8 us per 8192 units of K (128
-// values of 16 columns) (32x4096x4096 8.7 us, on 32-row tiles 22; 64x4096x4096 13.3 and 22;
-// 24x28672x4096 57, 22.7); groups do not (20 rows of each of 8 groups 4096x4096 32.4 us,
-// tiles 27.8; of 64 groups 2816x2048 109 and 69).
+// Streamed or tiled, by estimated time. Up to 16 rows the stream reads a single weight once;
+// beyond, once per 32 rows, in 5.8 us per 8192 units of K (128 values of 16 columns)
+// (32x4096x4096 8.7 us, on 32-row tiles 22; 64x4096x4096 13.3 and 22; 24x28672x4096 57, 22.7).
+// Groups on row tiles of 16: a workgroup's 64 columns take 1.2 us and 0.18 (MXFP4) to 0.4 us
+// (scales per 32 values) per unit (stream and 32-row tiles, us: 3 rows of each of 64 groups
+// 2816x2048, scales per 64, 68 and 60, 10 rows 73 and 61; 8 groups 4096x14336 58 and 66, 79 and
+// 67; MXFP4 28672x4096 102 and 135, 127 and 138); beyond 16 rows they are tiled (20 rows of each
+// of 8 groups 4096x4096 32.4 us, tiles 27.8).
 static int run_w4(W4Params& p, bool mx, hipStream_t stream) {
     const int64_t live = std::min(p.M, p.E), r = p.M / live, ncu = cu_count() > 0 ? cu_count() : 256, units = (p.K + 127) / 128;
-    if (r > 16) {
-        const int64_t wgs = (r + 31) / 32 * ((p.N + 15) / 16);
-        const double us_stream = 3.0 + (double)(std::max(wgs, ncu) * units) * (5.8 / 8192);
+    const bool groups = ragged(p);
+    if (r > (groups ? 2 : 16)) {
         int tile;
-        if (w4_tile_plan(p, tile) < us_stream || ragged(p)) return launch_w4_tile(p, mx, tile, stream);
+        const float us_tile = w4_tile_plan(p, tile);
+        double us_stream;
+        if (!groups) {
+            const int64_t wgs = (r + 31) / 32 * ((p.N + 15) / 16);
+            us_stream = 3.0 + (double)(std::max(wgs, ncu) * units) * (5.8 / 8192);
+        } else {
+            const double wgs = (double)live * std::max(1.0, (double)p.M / live / 16 + 0.5) * ((p.N + 63) / 64);
+            const double unit = mx ? 0.18 : p.glog2 == 7 ? 0.21 : p.glog2 == 6 ? 0.29 : 0.40;
+            us_stream = std::ceil(wgs / ncu) * (units * unit + 1.2);
+        }
+        if (us_tile < us_stream || (groups && r > 16)) return launch_w4_tile(p, mx, tile, stream);
     }
     if (mx) return run_w4_stream<0, false>(p, r, stream);
     return p.glog2 == 5 ? run_w4_group<32>(p, r, stream) : p.glog2 == 6 ? run_w4_group<64>(p, r, stream) : run_w4_group<128>(p, r, stream);
