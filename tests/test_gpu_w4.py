@@ -261,6 +261,14 @@ def test_grouped_layer_sizes(rows, N, K, topk, kind, group, zeros):
     check_grouped(rows, N, K, kind, group, zeros, topk=topk, seed=4)
 
 
+@pytest.mark.parametrize("kind,group,zeros", KINDS)
+def test_grouped_short_groups_of_many_columns(kind, group, zeros):
+    """Means of 3 to 16 rows, where streams and tiles take over from each other."""
+    require_gpu()
+    check_grouped([3, 9, 0, 5, 33, 1, 2, 17, 4, 0, 6, 8, 3, 1, 40, 2], 5632, 1024, kind, group, zeros, first=2, tail=3, topk=3, seed=21)
+    check_grouped([3, 2, 4, 0, 5, 17, 1, 3], 4104, 1152, kind, group, zeros, tail=1, seed=22)
+
+
 def test_mxfp4_scales():
     """Every e8m0 code, 255 as NaN; products with one value of X, so that nothing cancels."""
     require_gpu()
