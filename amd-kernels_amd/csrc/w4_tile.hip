@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "gemm_kgroup.h"
+#include "w4_chain.h"
 #include "w4_core.h"
 
 namespace hkq {
@@ -259,10 +260,10 @@ __global__ __launch_bounds__(256, T::OCC) void w4_tile_kernel(const W4Params p) 
                 acc[i][j] = mfma_bf16(A[f], B[cur][s], acc[i][j]);
             } else {
                 P = mfma_bf16(A[f], B[cur][s], s % CH == 0 ? v16f{} : P);
-                // sums of the chain before (whose last instruction is still on its way at s % CH == 0)
+                // sums of the chain before
                 constexpr int pc = f < CH ? SLOTS - 1 : f / CH * CH - 1, pi = f < CH ? (i + TN - 1) % TN : i, pj = pc / 8;
 #pragma unroll
-                for (int e = (s % CH - 1) * 16 / (CH - 1); e < s % CH * 16 / (CH - 1); ++e)
+                for (int e = chain_added(s % CH, CH); e < chain_added(s % CH + 1, CH); ++e)
                     acc[pi][pj][e] = __builtin_fmaf(Pq[e], sq, acc[pi][pj][e]);
             }
             if constexpr (LAST) {
