@@ -1,0 +1,38 @@
+"""GPU tests of the 4-bit weights at the edges of what their calls take: the largest
+values, expert stacks past one call's rows, scales at any address, ends of the e8m0
+range, more tiles than one launch holds."""
+import pytest
+import torch
+
+import hkq
+from gpu_util import require_gpu
+from test_gpu_w4 import BF16, MIDS, bf16, close, quant_ref, unpack
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantizer_of_the_largest_values(group, zeros):
+    """Near the largest bf16: codes, scales and zero points as the formulas give them, and values bf16((code - zero) * scale),
+    an infinity exactly where that passes the largest bf16."""
+    require_gpu()
+    top = 3.3895e38
+    w = bf16((6, 2 * group), 3)
+    w[0, :group], w[1, group:] = top, -top
+    w[2, :group // 2], w[2, group // 2:group] = top, -top
+    w[3, 5], w[4, group + 1] = top, -top
+    w[5, ::3], w[5, 1::3] = top, -0.5 * top
+    assert w.isfinite().all()
+    c, s, z = quant_ref(w, group, zeros)
+    assert s.isfinite().all() and int(c.max()) == 15
+    got = hkq.w4_quant(w.cuda(), group, zeros)
+    assert torch.equal(unpack(got[0].cpu()), c), "codes"
+    assert torch.equal(got[1].cpu().view(torch.int16), s.view(torch.int16)), "scales"
+    assert not zeros or torch.equal(got[2].cpu(), z), "zero points"
+    off = z.float()[..., None] if zeros else 8.0
+    ref = ((c.float().view(*s.shape, group) - off) * s.float()[..., None]).to(BF16).flatten(-2)
+    back = hkq.w4_dequant(*got).cpu()
+    assert torch.equal(back.view(torch.int16), ref.view(torch.int16)), "values"
+    fin = ref.isfinite()
+    assert ((back.float() - w.float()).abs()[fin] <= (s.float().repeat_interleave(group, -1) * (0.5 + 2 * 15 * 2.0 ** -8))[fin]).all()
