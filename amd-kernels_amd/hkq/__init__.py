@@ -644,14 +644,15 @@ def w4_quant(w, group: int = 128, zeros: bool = False, q=None, s=None, z=None, s
 
 def _experts(*tensors):
     """[N, ..] or [E, N, ..] tensors as lists of 2-D ones: all rows if each tensor's
-    experts follow at its row pitch, else an item for each expert."""
+    experts follow at its row pitch and one call takes them, else an item for each expert."""
     def together(t):
-        E, N, _ = t.shape
-        return E <= 1 or N <= 1 or t.stride(0) == N * t.stride(1)
+        E, N, cols = t.shape
+        pitch = t.stride(0) if N <= 1 < E else t.stride(1)
+        return E * N < 1 << 22 and (min(E, N) <= 1 or t.stride(0) == N * pitch) and (E * N <= 1 or cols <= pitch < 1 << 22)
 
     if tensors[0].dim() == 2:
         return [[t] for t in tensors]
-    if all(together(t) for t in tensors):
+    if all(t.numel() == 0 or together(t) for t in tensors):
         return [[t.flatten(0, 1)] for t in tensors]
     return [list(t) for t in tensors]
 

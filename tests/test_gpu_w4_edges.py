@@ -36,3 +36,30 @@ def test_quantizer_of_the_largest_values(group, zeros):
     assert torch.equal(back.view(torch.int16), ref.view(torch.int16)), "values"
     fin = ref.isfinite()
     assert ((back.float() - w.float()).abs()[fin] <= (s.float().repeat_interleave(group, -1) * (0.5 + 2 * 15 * 2.0 ** -8))[fin]).all()
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantizer_of_more_rows_than_a_call_takes(zeros):
+    """2^22 rows of two experts: past one call's limit, so one for each."""
+    require_gpu()
+    w = torch.zeros((2, 1 << 21, 32), dtype=BF16, device="cuda")
+    rows = [0, 1, 77777, (1 << 21) - 1]
+    w[:, rows] = bf16((2, 4, 32), 1).cuda()
+    got = hkq.w4_quant(w, 32, zeros)
+    c, s, z = quant_ref(w[:, rows].cpu(), 32, zeros)
+    assert torch.equal(unpack(got[0][:, rows].cpu()), c) and torch.equal(got[1][:, rows].cpu(), s)
+    assert not zeros or torch.equal(got[2][:, rows].cpu(), z)
+    back = hkq.w4_dequant(*got)
+    assert torch.equal(back[:, rows], torch.stack([hkq.w4_dequant(*(t[e][rows].contiguous() for t in got)) for e in range(2)]))
+    assert (back[:, 2:77777] == 0).all()
+
+
+def test_quantizer_of_one_row_of_each_expert():
+    """A row of each expert's matrix, the experts 2^22 values apart, and one row for all of them."""
+    require_gpu()
+    whole = bf16((3, 4, 1 << 20), 2).cuda()
+    for w in (whole[:, 1:2, :256], whole[:1, :1, :256].expand(3, 1, 256)):
+        got = hkq.w4_quant(w, 64, True)
+        ref = hkq.w4_quant(w.contiguous(), 64, True)
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+        assert torch.equal(hkq.w4_dequant(*got), hkq.w4_dequant(*ref))
