@@ -517,7 +517,7 @@ static int w4_product(const void* X, const void* Q, const void* S, const void* Z
     HKQ_CHECK_ARG(C && (!grouped || offs) && (K == 0 || (Q && S && (X || T == 0))), "X, Q, S, the output and (grouped) offs are required");
     HKQ_CHECK_ALIGN(X, 16);
     HKQ_CHECK_ALIGN(Q, 16);
-    HKQ_CHECK_ALIGN(S, 2);
+    HKQ_CHECK_ARG(mx || reinterpret_cast<uintptr_t>(S) % 2 == 0, "S (bf16) must be 2-byte aligned");
     HKQ_CHECK_ALIGN(C, 2);
     HKQ_CHECK_ALIGN(offs, 4);
     HKQ_CHECK_ALIGN(gather, 4);

@@ -63,3 +63,26 @@ def test_quantizer_of_one_row_of_each_expert():
         ref = hkq.w4_quant(w.contiguous(), 64, True)
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
         assert torch.equal(hkq.w4_dequant(*got), hkq.w4_dequant(*ref))
+
+
+@pytest.mark.parametrize("M", [1, 7, 16, 30, 100, 300])
+def test_mxfp4_scales_at_any_address(M):
+    """e8m0 scales are bytes: rows of any pitch from any address."""
+    require_gpu()
+    N, K = 133, 416
+    g = torch.Generator().manual_seed(M)
+    code = torch.randint(0, 16, (2, N, K), generator=g, dtype=torch.uint8)
+    sc = torch.randint(118, 124, (2, N, K // 32), generator=g, dtype=torch.uint8)
+    q = (code[..., 0::2] | (code[..., 1::2] << 4)).cuda()
+    val = (MIDS[code.long()].view(2, N, -1, 32) * torch.pow(2.0, sc.double() - 127)[..., None]).view(2, N, K).cuda()
+    X = bf16((M, K), M + 1).cuda()
+    x, offs = X.double(), torch.tensor([0, M // 3, M], dtype=torch.int32, device="cuda")
+    for at in (1, 2, 3):
+        for pitch in (13, 14, 16):
+            buf = torch.full((at + 2 * N * pitch,), 255, dtype=torch.uint8, device="cuda")
+            S = buf.as_strided((2, N, K // 32), (N * pitch, pitch, 1), at)
+            S.copy_(sc)
+            close(hkq.gemm_w4a16(X, q[0], S[0]), x @ val[0].t(), x.abs() @ val[0].abs().t(), K, f"{at} {pitch}")
+            Y = hkq.grouped_gemm_w4a16(X, q, S, offs)
+            for e, r in enumerate((slice(0, M // 3), slice(M // 3, M))):
+                close(Y[r], x[r] @ val[e].t(), x[r].abs() @ val[e].abs().t(), K, f"group {e}, {at} {pitch}")
