@@ -199,7 +199,7 @@ constexpr int STREAM_LDS = STREAM_TABLE + 3 * STREAM_GROUPS * 4 + 16;
 static_assert(STREAM_LDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
 
 struct GroupTable {
-    HKQ_LDS int *end, *row0, *row1;  // row tiles up to the group's end, its rows
+    HKQ_LDS int *end, *row0, *row1;  // row tiles up to the group's end (512 x 2^20 at the most), its rows
     int E;
     // fills the table; the tiles of all groups (every wave; ends in a barrier)
     __device__ int fill(const GroupedParams& p, HKQ_LDS uint8_t* at) {

@@ -32,6 +32,10 @@ __device__ __forceinline__ void group_tile(int in, int tiles_m, int tiles_n, int
     tn = at / size;
 }
 
+// Sums of tile counts, held at the largest int: bounds that count rows many times (65535
+// groups of all rows) would pass it.
+__device__ __forceinline__ int add_sat(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+
 struct RaggedTile {
     int e, m0, rows;  // group, the tile's first row among all rows, the group's rows from there on
     int tn;
@@ -53,19 +57,19 @@ __device__ __forceinline__ bool ragged_tile(const P& p, RaggedTile& t) {
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const int o = __shfl_up(v, d, 64);
-            if (lane >= d) v += o;
+            if (lane >= d) v = add_sat(v, o);
         }
         return v;
     };
     int n = count(lane), s = scan(n), total = __builtin_amdgcn_readlane(s, 63);
-    for (int e0 = 64; e0 < p.E; e0 += 64) total += __builtin_amdgcn_readlane(scan(count(e0 + lane)), 63);
+    for (int e0 = 64; e0 < p.E; e0 += 64) total = add_sat(total, __builtin_amdgcn_readlane(scan(count(e0 + lane)), 63));
     total = min(total, p.tiles_m);  // bounds that count a row twice: the tiles that the grid holds
     if ((int)blockIdx.x >= total * p.tiles_n) return false;
     const int id = xcd_order(blockIdx.x, total * p.tiles_n), at = id / p.tiles_n;
     int before = 0;  // tiles of the groups before e0
     for (int e0 = 0; e0 < p.E; e0 += 64) {
         if (e0 > 0) n = count(e0 + lane), s = scan(n);
-        const uint64_t past = __ballot(before + s > at);
+        const uint64_t past = __ballot(add_sat(before, s) > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             t.e = e0 + l;
@@ -77,7 +81,7 @@ __device__ __forceinline__ bool ragged_tile(const P& p, RaggedTile& t) {
             t.rows = __builtin_amdgcn_readfirstlane(r.y) - t.m0;
             return true;
         }
-        before += __builtin_amdgcn_readlane(s, 63);
+        before = add_sat(before, __builtin_amdgcn_readlane(s, 63));
     }
     return false;
 }
