@@ -395,23 +395,21 @@ __global__ __launch_bounds__(256, 1) void grouped_dw_stream_kernel(const Grouped
     gemm_stream<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM, DENSE_TN, true, true>(seq, a_off, b_off, smem, lane, wave, acc, epi);
 }
 
-template <class Kern>
+template <bool BT, class Kern>
 static int launch_grouped(Kern kern, std::atomic<uint64_t>& attr, int lds, int bm, int bn, int threads, GroupedParams& p,
                           hipStream_t stream) {
     if (int e = set_device_lds(kern, lds, attr)) return e;
     p.tiles_m = (int)ragged_most(p.M, p.E, bm);
-    p.tiles_n = (p.N + bn - 1) / bn;
     p.group_m = 8;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-    HKQ_CHECK_ARG(blocks < (1 << 23), "too many tiles for one launch");
-    kern<<<(unsigned)blocks, threads, lds, stream>>>(p);
-    return hkq_launch_status();
+    return launch_columns(
+        p, bn, threads, [](GroupedParams& q, int64_t n) { q.B += BT ? 2 * n : n * q.ldb, q.C += n; },
+        [&](const GroupedParams& q, unsigned blocks) { kern<<<blocks, threads, lds, stream>>>(q); });
 }
 template <bool BT, class Cfg, int MINB = 1>
 static int launch_small(GroupedParams& p, hipStream_t stream) {
     static_assert(Cfg::LDS * MINB <= 160 * 1024, "LDS budget of a CDNA4 CU");
     static std::atomic<uint64_t> attr{0};
-    return launch_grouped(grouped_small_kernel<BT, Cfg, MINB>, attr, Cfg::LDS, Cfg::BM, Cfg::BN, Cfg::THREADS, p, stream);
+    return launch_grouped<BT>(grouped_small_kernel<BT, Cfg, MINB>, attr, Cfg::LDS, Cfg::BM, Cfg::BN, Cfg::THREADS, p, stream);
 }
 template <bool BT>
 static int launch_whole(GroupedParams& p, hipStream_t stream) {
@@ -429,19 +427,28 @@ static int launch_whole(GroupedParams& p, hipStream_t stream) {
         }
     }
     static std::atomic<uint64_t> attr{0};
-    return launch_grouped(grouped_whole_kernel<BT>, attr, WHOLE_LDS, DENSE_BM, DENSE_BN, 256, p, stream);
+    return launch_grouped<BT>(grouped_whole_kernel<BT>, attr, WHOLE_LDS, DENSE_BM, DENSE_BN, 256, p, stream);
 }
+// (a launch takes as many groups as keep it below 2^32 threads; one group's tiles do, as its
+// gradient fits the memory)
 template <class Kern>
-static int launch_dw(Kern kern, std::atomic<uint64_t>& attr, int lds, int bm, int bn, int threads, GroupedParams& p,
+static int launch_dw(Kern kern, std::atomic<uint64_t>& attr, int lds, int bm, int bn, int threads, const GroupedParams& p,
                      hipStream_t stream) {
     if (int e = set_device_lds(kern, lds, attr)) return e;
-    p.tiles_m = (p.K + bm - 1) / bm;
-    p.tiles_n = (p.N + bn - 1) / bn;
-    p.group_m = 8;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.E;
-    HKQ_CHECK_ARG(blocks < (1 << 23), "too many tiles for one launch");
-    kern<<<(unsigned)blocks, threads, lds, stream>>>(p);
-    return hkq_launch_status();
+    GroupedParams q = p;
+    q.tiles_m = (p.K + bm - 1) / bm;
+    q.tiles_n = (p.N + bn - 1) / bn;
+    q.group_m = 8;
+    const int64_t per = (int64_t)q.tiles_m * q.tiles_n, most = 0xFFFFFFFFll / threads / per;
+    HKQ_CHECK_ARG(most > 0, "too many tiles for one launch");
+    for (int64_t e = 0; e < p.E; e += most) {
+        q.E = (int)std::min<int64_t>(p.E - e, most);
+        q.offs = p.offs + e;
+        q.C = p.C + e * p.stride_e;
+        kern<<<(unsigned)(per * q.E), threads, lds, stream>>>(q);
+        if (int err = hkq_launch_status()) return err;
+    }
+    return 0;
 }
 
 // Tile size by the mean rows of a group: the least estimated time. A K-tile takes

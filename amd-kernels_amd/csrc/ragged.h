@@ -93,6 +93,24 @@ inline int64_t ragged_most(int64_t M, int64_t E, int64_t bm) {
     return (M - live) / bm + live;
 }
 
+// Launches of a product with p.N columns in tiles of bn: one, or as many as keep each below
+// 2^32 threads (a grid's limit), of whole column tiles each. at(q, n) moves a copy's operands to
+// column n. One column of row tiles always fits: below 2^28 rows make at most 2^22 + 2^16 of
+// 64 rows with 512 threads, 2^23 + 2^16 of 32 with 256; shorter ones take below 2^27 rows.
+template <class P, class At, class Launch>
+inline int launch_columns(const P& p, int bn, int threads, At at, Launch launch) {
+    const int64_t most = std::max<int64_t>(1, 0xFFFFFFFFll / threads / p.tiles_m);
+    for (int64_t n = 0; n < p.N; n += most * bn) {
+        P q = p;
+        q.N = (int)std::min<int64_t>(p.N - n, most * bn);
+        q.tiles_n = (q.N + bn - 1) / bn;
+        at(q, n);
+        launch(q, (unsigned)((int64_t)q.tiles_m * q.tiles_n));
+        if (int e = hkq_launch_status()) return e;
+    }
+    return 0;
+}
+
 // E groups of R rows of `width` bytes, `pitch` apart, groups `stride` apart: one
 // operand's memory for overlap().
 inline MemRows grouped_mem(const void* p, int64_t E, int64_t R, int64_t width, int64_t pitch, int64_t stride) {

@@ -373,12 +373,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void w4_stream_kernel(const W4Params 
 template <int G, bool Z, int MT, int XL, int NT, int NW, int D, int XD, int OCC>
 static int launch_w4_stream(W4Params& p, hipStream_t stream) {
     p.tiles_m = (int)ragged_most(p.M, p.E, MT == 1 ? 4 * XL : 16 * MT);
-    p.tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
     p.group_m = 8;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-    HKQ_CHECK_ARG(blocks < (1 << 23), "too many tiles for one launch");
-    w4_stream_kernel<G, Z, MT, XL, NT, NW, D, XD, OCC><<<(unsigned)blocks, 64 * NW, 0, stream>>>(p);
-    return hkq_launch_status();
+    return launch_columns(p, 16 * NT, 64 * NW, w4_from_column<G == 0>, [&](const W4Params& q, unsigned blocks) {
+        w4_stream_kernel<G, Z, MT, XL, NT, NW, D, XD, OCC><<<blocks, 64 * NW, 0, stream>>>(q);
+    });
 }
 
 // Rows per group r (the mean) and columns. A row tile of r rows; more columns per
@@ -432,7 +430,8 @@ static int run_w4(W4Params& p, bool mx, hipStream_t stream) {
             const double unit = mx ? 0.18 : p.glog2 == 7 ? 0.21 : p.glog2 == 6 ? 0.29 : 0.40;
             us_stream = std::ceil(wgs / ncu) * (units * unit + 1.2);
         }
-        if (us_tile < us_stream || (groups && r > 16)) return launch_w4_tile(p, mx, tile, stream);
+        // (from 2^27 rows on a grid of the stream's row tiles, of 512 threads, may be too large)
+        if (us_tile < us_stream || (groups && r > 16) || p.M >= 1 << 27) return launch_w4_tile(p, mx, tile, stream);
     }
     if (mx) return run_w4_stream<0, false>(p, r, stream);
     return p.glog2 == 5 ? run_w4_group<32>(p, r, stream) : p.glog2 == 6 ? run_w4_group<64>(p, r, stream) : run_w4_group<128>(p, r, stream);

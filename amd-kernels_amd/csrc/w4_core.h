@@ -79,6 +79,15 @@ __device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
     a = r[0], b = r[1];
 }
 
+// The weights, and the output, from column n on (launch_columns).
+template <bool MX>
+inline void w4_from_column(W4Params& q, int64_t n) {
+    q.Q += n * q.ldq;
+    q.S += n * q.lds * (MX ? 1 : 2);
+    if (q.Z) q.Z += n * q.lds;
+    q.C += n;
+}
+
 // The tiles of w4_tile.hip: the size with the least estimated time (us), and its launch.
 float w4_tile_plan(const W4Params& p, int& tile);
 int launch_w4_tile(W4Params& p, bool mx, int tile, hipStream_t stream);

@@ -346,12 +346,9 @@ static int launch_tile(W4Params& p, hipStream_t stream) {
     static std::atomic<uint64_t> attr{0};
     if (int e = set_device_lds(kern, T::LDS, attr)) return e;
     p.tiles_m = (int)ragged_most(p.M, p.E, T::BM);
-    p.tiles_n = (p.N + T::BN - 1) / T::BN;
     p.group_m = 8;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-    HKQ_CHECK_ARG(blocks < (1 << 23), "too many tiles for one launch");
-    kern<<<(unsigned)blocks, 256, T::LDS, stream>>>(p);
-    return hkq_launch_status();
+    return launch_columns(p, T::BN, 256, w4_from_column<T::MX>,
+                          [&](const W4Params& q, unsigned blocks) { kern<<<blocks, 256, T::LDS, stream>>>(q); });
 }
 
 // Tile sizes, and us per unit and per tile on MI355X: a wave's instructions, one wave per
