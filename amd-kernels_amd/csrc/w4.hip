@@ -6,9 +6,10 @@
 //
 // A weight is (code - zero) * scale (HKQ_W4_INT4: bf16 scales, and zero points or 8,
 // per 32, 64 or 128 values of K) or an E2M1 value times a power of two
-// (HKQ_W4_MXFP4). Neither is rounded on its way: code - zero and the MXFP4 values are
-// exact in bf16, as the matrix instruction's operand, and an INT4 scale multiplies the
-// fp32 sums of its group.
+// (HKQ_W4_MXFP4). Neither is rounded on its way: code - zero and the MXFP4 values from
+// 2^-128 to below 2^128 are exact in bf16, as the matrix instruction's operand (which
+// keeps values below the smallest normal number), and an INT4 scale multiplies the fp32
+// sums of its group. MXFP4 values of 2^128 and more are infinities in the operand.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

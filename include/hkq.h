@@ -484,7 +484,10 @@ int hkq_grouped_gemm_backward(const void* dY, const void* X, const void* W, void
  *   HKQ_W4_INT4   (code - zero) * scale, S bf16 [N, lds], Z u8 [N, lds] values 0 .. 15
  *                 (NULL: 8 throughout); group 32, 64 or 128;
  *   HKQ_W4_MXFP4  E2M1 codes times 2^(e - 127), S e8m0 [N, lds] (255: NaN), no Z,
- *                 group 32: what hkq_mx_quant writes.
+ *                 group 32: what hkq_mx_quant writes. A value of 2^128 or more (codes of 4
+ *                 and 6 with e = 253, of 2 and more with 254) is an infinity, as
+ *                 hkq_mx_dequant writes it; every other one is exact, down to 2^-128.
+ * S bf16 is 2-byte aligned, e8m0 and Z are at any address.
  * K is a multiple of group; N, K and every pitch < 2^22; ldq a multiple of 4 (of 16,
  * with Q 16-byte aligned, in the products). */
 #define HKQ_W4_INT4 0
@@ -506,10 +509,10 @@ int hkq_w4_dequant(const void* q, const void* s, const void* z, void* out, int64
 
 /* C[m, n] = bf16(sum_k X[m, k] W[n, k]), X bf16 [M, K] (pitch ldx a multiple of 8,
  * 16-byte aligned), C bf16 [M, ldc] (any pitch >= N). The weights are not rounded:
- * an INT4 scale multiplies the fp32 sums of its group. workspace: unused where the
- * query gives 0 (16-byte aligned, calls that overlap need one each). C shares no
- * memory with an operand (refused). No counterpart in the reference, whose 4-bit
- * products take 4-bit activations or dequantized weights. */
+ * an INT4 scale multiplies the fp32 sums of its group. workspace: the query's bytes,
+ * 16-byte aligned, one for each of calls that overlap; no plan takes one so far, and
+ * the query gives 0. C shares no memory with an operand (refused). No counterpart in
+ * the reference, whose 4-bit products take 4-bit activations or dequantized weights. */
 size_t hkq_gemm_w4a16_workspace(int64_t M, int64_t N, int64_t K);
 int hkq_gemm_w4a16(const void* X, const void* Q, const void* S, const void* Z, void* C, int64_t M, int64_t N, int64_t K,
                    int64_t ldx, int64_t ldq, int64_t lds, int64_t ldc, int64_t group, int kind, void* workspace,

@@ -86,3 +86,32 @@ def test_mxfp4_scales_at_any_address(M):
             Y = hkq.grouped_gemm_w4a16(X, q, S, offs)
             for e, r in enumerate((slice(0, M // 3), slice(M // 3, M))):
                 close(Y[r], x[r] @ val[e].t(), x[r].abs() @ val[e].abs().t(), K, f"group {e}, {at} {pitch}")
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 300])
+def test_mxfp4_ends_of_the_scales(M):
+    """A code by itself in its row, under each scale byte: exact down to the smallest (2^-128, below bf16's normal numbers),
+    up to where a value is 2^128 or more and the weight an infinity, as mx_dequant has it. Powers of two as X."""
+    require_gpu()
+    N, K = 255 * 16, 64
+    e, c = torch.arange(255).repeat_interleave(16), torch.arange(16, dtype=torch.uint8).repeat(255)
+    val = MIDS[c.long()] * torch.pow(2.0, e.double() - 127)
+    over = val.abs() >= 2.0 ** 128
+    assert sorted(set(e[over].tolist())) == [253, 254] and int(over.sum()) == 4 + 8
+    s = e.to(torch.uint8)[:, None].expand(N, 2).contiguous().cuda()
+    for k in (0, 13, 39, 63):
+        q = torch.zeros((N, K // 2), dtype=torch.uint8)
+        q[:, k // 2] = c << (4 * (k % 2))
+        q = q.cuda()
+        w = hkq.mx_dequant(q, s, K).cpu().double()
+        assert torch.equal(w[:, k], torch.where(over, val.sign() * float("inf"), val))
+        for x in (1.0, -2.0 ** -20, 2.0 ** 60, 2.0 ** -3):
+            X = torch.full((M, K), x, dtype=BF16, device="cuda")
+            # one rounding of the exact product (fp32 holds it or rounds as bf16 does: two significant bits)
+            ref = torch.where(over, val.sign() * x * float("inf"), val * x).float().to(BF16)
+            C = hkq.gemm_w4a16(X, q, s).cpu()
+            Y = hkq.grouped_gemm_w4a16(X, q[None], s[None], torch.tensor([0, M], dtype=torch.int32, device="cuda")).cpu()
+            assert torch.equal(C, ref.expand(M, N)) and torch.equal(Y, C), (k, x)
+    X[:] = 0.0
+    C = hkq.gemm_w4a16(X, q, s).cpu()
+    assert torch.equal(C.isnan(), over.expand(M, N)) and (C[:, ~over] == 0).all()
