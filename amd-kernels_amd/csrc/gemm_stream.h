@@ -7,10 +7,10 @@
 // starts its accumulators from zero (a literal-zero MFMA accumulator input),
 // so no accumulator is cleared.
 //
-// Restrictions (the caller checks them): 128-byte K-tiles in a 2-stage ring,
-// and a K-tile count per tile that is a multiple of 8, so that tiles start at
-// stage 0 with the fragment parity 0 and (MXFP4) the scale blocks of 4 K-tiles
-// never straddle two tiles and alternate their ring slot across tiles.
+// Restrictions (the caller checks them): 128-byte K-tiles in a 2-stage ring, and a
+// K-tile count per tile that is even and at least 4, so that tiles start at stage 0
+// with the fragment parity 0; MXFP4: a multiple of 8, so that the scale blocks of 4
+// K-tiles never straddle two tiles and alternate their ring slot across tiles.
 #pragma once
 #include <type_traits>
 
@@ -299,8 +299,8 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
     // VM: vector-memory operations younger than K-tile kt+1's loads when the
     // body waits for them (the C stores and scale loads of an epilogue that ran
     // after those loads were issued may stay in flight)
-    // Q: kt % SB_KT (MXFP4's scale slots; K-tiles per tile are a multiple of
-    // 8, so it also fixes the stage and the fragment parity)
+    // Q: kt % SB_KT (MXFP4's scale slots; K-tiles per tile are a multiple of 8
+    // there), whose lowest bit is the stage and the fragment parity
     auto ktile_vm = [&](int kt, auto qslot, auto first, auto last, auto vm) {
         constexpr int Q = decltype(qslot)::value;
         constexpr int P = Q & 1;

@@ -197,6 +197,9 @@ constexpr int STREAM_GROUPS = 512;  // groups that the LDS table holds
 constexpr int STREAM_TABLE = stream_stg_off<PlainOp, MODE_BF16>() + DENSE_WAVES_M * DENSE_WAVES_N * STREAM_STG;
 constexpr int STREAM_LDS = STREAM_TABLE + 3 * STREAM_GROUPS * 4 + 16;
 static_assert(STREAM_LDS <= 160 * 1024, "LDS budget of a CDNA4 CU");
+// a wave may load its half tile's K-tiles while another still looks its own up in the table
+static_assert(DenseCfg<MODE_BF16, DENSE_WAVES_M, DENSE_WAVES_N, DENSE_TM / 2, DENSE_TN, 128>::lds_bytes(HALF_NS) <= STREAM_TABLE,
+              "a half tile's ring ends before the table");
 
 struct GroupTable {
     HKQ_LDS int *end, *row0, *row1;  // row tiles up to the group's end (512 x 2^20 at the most), its rows

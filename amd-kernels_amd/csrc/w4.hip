@@ -307,8 +307,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void w4_stream_kernel(const W4Params 
                 } else if constexpr (Z) {
                     b = int4_operand(w[j], z[j * NG / 4]);
                 } else {
-                    const v2i lo = int4_sixteenths<0>(w[j]), hi = int4_sixteenths<1>(w[j]);
-                    b = v4i{lo[0], lo[1], hi[0], hi[1]};
+                    b = int4_sixteenths_operand(w[j]);
                 }
                 const bool first = !MX && j % (4 / NG) == 0, last = !MX && (j + 1) % (4 / NG) == 0;
 #pragma unroll

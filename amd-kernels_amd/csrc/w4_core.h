@@ -42,7 +42,9 @@ __device__ __forceinline__ v4i int4_operand(uint32_t w, float zero) {
 }
 // The same for zero = 8, as sixteenths (code - 8) / 16: with its upper bit inverted a
 // code is a signed nibble, which v_cvt_off_f32_i4 converts from the low half of any
-// byte. 14 instructions per 8 codes.
+// byte. 14 instructions per 8 codes. A matrix instruction may read the result two wait
+// states later; the compiler keeps that distance for instructions that it knows, not for
+// these (int4_sixteenths_settle).
 template <int H>
 __device__ __forceinline__ v2i int4_sixteenths(uint32_t w) {
     const uint32_t ev = w ^ 0x88888888u, od = ev >> 4;
@@ -62,6 +64,14 @@ __device__ __forceinline__ v2i int4_sixteenths(uint32_t w) {
         asm(HKQ_NIBBLES("BYTE_2", "BYTE_3") : "=&v"(o0), "=&v"(o1), "=&v"(t0), "=&v"(t1) : "v"(ev), "v"(od), "s"(0x07060302u));
 #undef HKQ_NIBBLES
     return v2i{(int)o0, (int)o1};
+}
+// Those two wait states: an operand that a matrix instruction reads next.
+__device__ __forceinline__ void int4_sixteenths_settle(v4i& b) { asm("s_nop 1" : "+v"(b)); }
+__device__ __forceinline__ v4i int4_sixteenths_operand(uint32_t w) {
+    const v2i lo = int4_sixteenths<0>(w), hi = int4_sixteenths<1>(w);
+    v4i b = v4i{lo[0], lo[1], hi[0], hi[1]};
+    int4_sixteenths_settle(b);
+    return b;
 }
 // E2M1 codes 4 H .. 4 H + 3 times 2^(e8m0 - 127), the scale as the fp32 of that exponent.
 template <int H>

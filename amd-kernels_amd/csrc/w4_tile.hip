@@ -224,7 +224,11 @@ __global__ __launch_bounds__(256, T::OCC) void w4_tile_kernel(const W4Params p) 
     read_raw(0, 0, 0, raw);
     finish_raw(0, 0, raw);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) operand_half(raw, s, 0, B[0][s]), operand_half(raw, s, 1, B[0][s]);
+    for (int s = 0; s < 8; ++s) {
+        operand_half(raw, s, 0, B[0][s]), operand_half(raw, s, 1, B[0][s]);
+        // (inside the loop a step's conversions are a step ahead of its matrix instructions)
+        if constexpr (!MX && !T::Z) int4_sixteenths_settle(B[0][s]);
+    }
 #pragma unroll
     for (int g = 0; g < NS_; ++g) sc[0][g] = raw.s[g];
     int stage = 0;
