@@ -94,9 +94,14 @@ __device__ __forceinline__ void lds_load16_u(const void* base, uint32_t bytes, H
     const uint32_t n = __builtin_amdgcn_readfirstlane(bytes);
     lds_load16(reinterpret_cast<const void*>(((uint64_t)hi << 32) | lo), n, dst, off);
 }
+// Between a vector instruction's write to a scalar register and a memory instruction that
+// reads it there have to be five wait states, which the compiler does not keep for inline
+// assembly (the built library's code is checked for it). The descriptors of the loads above
+// come from scalar instructions; these, of scales and bias, are the ones that are spilled to
+// vector registers and read back right before, so the block holds the wait states.
 __device__ __forceinline__ void lds_load4(const void* base, uint32_t bytes, HKQ_LDS void* dst, uint32_t off) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(m0), "v"(off), "s"(buffer_desc(base, bytes))
                  : "memory", "m0");

@@ -78,7 +78,13 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
     // the last tile), `ls` the one the scale units read. Each switches to the
     // next tile at the top of a K-tile body, before its MFMAs (a branch there
     // leaves the body's MFMA/load interleave in one basic block).
-    StreamSrc ld = seq.src(0), ls = ld;
+    // (the extents' range stays hidden: with it left()'s difference would turn unsigned)
+    auto source = [&](int t) {
+        StreamSrc s = seq.src(t);
+        asm("" : "+s"(s.a_bytes), "+s"(s.b_bytes));
+        return s;
+    };
+    StreamSrc ld = source(0), ls = ld;
     bool ld_live = true, ls_live = true;
 
     HKQ_LDS uint8_t* sblk = smem + NS * STAGE;
@@ -112,6 +118,11 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         su_off[k] = (su_a[k] ? (uint32_t)r * seq.lsa : (uint32_t)(r - BM) * seq.lsb) + half * 16u;
         asm volatile("" : "+v"(su_off[k]));
     }
+    // The bytes from `at` on of an operand of `bytes` (both below 2^31), 0 past its end or of a
+    // dead one: a signed difference, in scalar instructions (an unsigned one held at 0 is a
+    // vector instruction, and the load would have to wait for its copy in the descriptor).
+    auto left = [](bool live, uint32_t bytes, uint32_t at) { return live ? (uint32_t)max((int)bytes - (int)at, 0) : 0u; };
+
     // scale unit u (slot K = u % SB_KT) of the tile `ls`
     auto load_scale_unit = [&](int u, auto kslot) {
         constexpr int K = decltype(kslot)::value;
@@ -119,7 +130,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         const bool live = ls_live && blk * Cfg::SB_KT < KTN;
         const uint8_t* base = (su_a[K] ? ls.as : ls.bs) + blk * 32;
         const uint32_t ext = su_a[K] ? ls.as_bytes : ls.bs_bytes, kb = (uint32_t)blk * 32u;
-        lds_load16_u(base, live && ext > kb ? ext - kb : 0u, sblk + (blk & 1) * Cfg::SB_SLOT + su_g[K] * 1024,
+        lds_load16_u(base, left(live, ext, kb), sblk + (blk & 1) * Cfg::SB_SLOT + su_g[K] * 1024,
                      su_off[K]);
     };
 
@@ -148,7 +159,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
         } else if (BT16 && idx >= LA) {
             lds_load16_d(t16_b, wave_dst(Cfg::b_stage(NS, stage) + (idx - LA) * NW * 1024), b_off.v[idx - LA]);
         } else if (idx < LA) {
-            lds_load16_u(ld.a + kb, ld_live && ld.a_bytes > kb ? ld.a_bytes - kb : 0u,
+            lds_load16_u(ld.a + kb, left(ld_live, ld.a_bytes, kb),
                          wave_dst(Cfg::a_stage(NS, stage) + idx * NW * 1024), a_off.v[idx]);
         } else {
             const int i = idx - LA;
@@ -156,7 +167,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
             if constexpr (BT && !BT16) kbb = (uint32_t)kl * seq.b_kstep;
             const uint8_t* b = ld.b;
             if constexpr (GATED) b = gated_up<Cfg, TN>(i) ? ld.b2 : ld.b;
-            lds_load16_u(b + kbb, ld_live && ld.b_bytes > kbb ? ld.b_bytes - kbb : 0u,
+            lds_load16_u(b + kbb, left(ld_live, ld.b_bytes, kbb),
                          wave_dst(Cfg::b_stage(NS, stage) + i * NW * 1024), b_off.v[i]);
         }
     };
@@ -372,7 +383,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
             }
             ktile(KTN - 6, Q2{}, F0{}, F0{});
             ls_live = t + 1 < seq.tiles;
-            ls = seq.src(min(t + 1, seq.tiles - 1));
+            ls = source(min(t + 1, seq.tiles - 1));
             ktile(KTN - 5, Q3{}, F0{}, F0{});
             ktile(KTN - 4, Q0{}, F0{}, F0{});
             ktile(KTN - 3, Q1{}, F0{}, F0{});
@@ -383,7 +394,7 @@ __device__ __forceinline__ void gemm_stream(const Seq& seq, AOff& a_off, const B
             }
         }
         ld_live = t + 1 < seq.tiles;
-        ld = seq.src(min(t + 1, seq.tiles - 1));
+        ld = source(min(t + 1, seq.tiles - 1));
         cur_a.at = ld.ta.base;
         cur_b.at = ld.tb.base;
         if constexpr (VARIES) ld_kt = seq.kt_live(min(t + 1, seq.tiles - 1));
