@@ -9,10 +9,11 @@
 // K loops and tiles are the dense GEMMs'; in dX and dW the operands whose K runs
 // across memory rows are read transposed from LDS, so that nothing is copied.
 //
-// Few rows are bound by the weights' way from memory (48 rows of 8 groups 4096x14336: 177
-// us, 5.3 TB/s; 6006 rows of 64 groups 2816x2048: 172 us, 4.6 TB/s), many by the matrix
-// cores (8192 rows of 8 groups 28672x4096: 1555 us, 1.24 PFLOP/s, dX 1760, dW 1630; the
-// dense product of one group 1347).
+// Few rows are bound by the weights' way from memory (48 rows of 8 groups 4096x14336: 175
+// us, 5.3 TB/s; 6006 rows of 64 groups 2816x2048: 165 to 174 us, 4.6 TB/s), many by the
+// matrix cores (8192 rows of 8 groups 28672x4096: 1550 to 1610 us, 1.2 PFLOP/s, dX 1760 to
+// 1790, dW 1640; the dense product of one group 1340). Few outputs with long sums leave CUs
+// idle, as a workgroup walks its whole sum (dX of 3 rows, N 8160, K 640: 37 us).
 #include <algorithm>
 #include <cmath>
 
@@ -190,7 +191,8 @@ __global__ __launch_bounds__(256, 1) void grouped_dw_whole_kernel(const GroupedP
 
 // ---------------------------------------------------------------------------
 // Large groups: one workgroup per CU computes its 256 x 256 tiles as one stream of
-// K-tiles (gemm_stream.h), so that a tile's stores run under the next one's loads. The
+// K-tiles (gemm_stream.h), so that a tile's stores run under the next one's loads (dW's,
+// 128 KB from each CU after 16 K-tiles of a group of 1024 rows, in part only). The
 // groups' tile counts go to LDS at the start, where each tile's group is looked up.
 // ---------------------------------------------------------------------------
 constexpr int STREAM_GROUPS = 512;  // groups that the LDS table holds
@@ -350,8 +352,8 @@ __device__ __forceinline__ void grouped_half(const GroupedParams& p, int e, int 
 // as M halves, by workgroups b with b / 16 * 8 + b % 8 the tile and b / 8 % 2 the half
 // (both on one XCD). All of them last: an XCD's workgroups stay side by side in K and
 // share their rows and columns in its L2. With every second half first, so that the tiles'
-// ends fall between the others', 8192 rows of 8 groups 28672x4096 took 1606 us (now 1555)
-// and their dX, 448 K-tiles a tile, 1960 with 7.7 GB fetched (now 1760 to 1825).
+// ends fall between the others', 8192 rows of 8 groups 28672x4096 took 1606 us (1555 in the
+// same run) and their dX, 448 K-tiles a tile, 1960 with 7.7 GB fetched (1760 to 1790).
 template <bool BT>
 __global__ __launch_bounds__(256, 1) void grouped_stream_kernel(const GroupedParams p) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[];
@@ -458,7 +460,8 @@ static int launch_dw(Kern kern, std::atomic<uint64_t>& attr, int lds, int bm, in
 // us + c * share with c workgroups on a CU; groups need about half a row tile more than
 // their rows fill. Fitted to 5 sizes x 62 shapes (1 to 1024 rows in each of 8 or 64
 // groups, N and K 1408 to 28672, Y and dX): 1.03 of the best size's time on average, 1.20
-// at the most. What a size is for, Y in us:
+// at the most; smaller N and K and fewer groups lie outside the fit. What a size is for,
+// Y in us:
 //   64 groups 2816x2048, 4 rows:    64x64 127, 64x128 133, 128x256 142, 256x256 158
 //   8 groups 4096x14336, 64 rows:   128x128 190, 64x128 240, 128x256 249, 256x256 235
 //   8 groups 28672x4096, 1024 rows: 256x256 1546, 128x256 1806, 128x128 2226, 64x64 3560

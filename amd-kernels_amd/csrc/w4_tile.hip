@@ -10,9 +10,10 @@
 // group. MXFP4 scales go into the operands.
 //
 // Bound by the issue port that conversion and matrix instructions share, one wave per
-// SIMD, up to the matrix cores' rate at 128 rows: 2048x4096x14336, groups of 128, 220 us
-// (bf16 weights 208), with zero points 237; 6006 rows of 64 groups 2816x2048, groups of
-// 64, 142 us, 1.5 tiles for a group's 94 rows.
+// SIMD: 2048x4096x14336, groups of 128, 214 to 220 us (bf16 weights 206 to 209), with zero
+// points 232; 6006 rows of 64 groups 2816x2048, groups of 64, 129 to 147 us, 1.5 tiles of 96
+// rows for a group's 94. Fewer tiles than CUs leave the rest idle, K is not split:
+// 128x4096x14336 59 us on 128 CUs (bf16 weights 38).
 #include <cmath>
 #include <type_traits>
 

@@ -729,7 +729,7 @@ def grouped_gemm_w4a16(X, Q, S, offs, Z=None, gather=None, topk: int = 1, Y=None
     """gemm_w4a16 over ragged groups of rows: Y[r] = X[x(r)] . W[e]^T for offs[e] <= r <
     offs[e + 1], 4-bit weights Q [E, N, K / 2], S (and Z) [E, N, K / group]. x(r) = r,
     or gather[r] // topk with moe_routing's gather int32 [M] (a row outside X counts
-    as zeros). offs int32 [E + 1] (moe_routing's token_start) and gather are on the GPU
+    as zeros; X then spans less than 2^31 bytes). offs int32 [E + 1] (moe_routing's token_start) and gather are on the GPU
     -> bf16 [M, N]; rows of no group are left as they were: pass a Y that holds something there."""
     import torch
 
